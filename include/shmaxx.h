@@ -148,6 +148,30 @@ int mx_gemm_i8_reduce(hipStream_t st, const int32_t* P, int nsplit, long p_split
 long mx_gemm_ws_elems(int cfg, int splits, int M, int N);
 long mx_gemm_ws_counters(int cfg, int splits, int M, int N);
 
+/* ============================================================================================ MXFP4
+ * 4-bit e2m1 codes with one power-of-two scale (E8M0 byte: exponent + 127, 255 = NaN) per 32 columns of a row, OCP MX
+ * v1.0's conversion: e = max(floor(log2(max |x|)) - 2, -127), code = e2m1(x 2^-e) to nearest even, saturating at 6; a
+ * block with an infinity or NaN is NaN. No reference counterpart (its narrowest Linear is W8A8).
+ * Codes and scales are stored in the order of the matrix instruction's operands (csrc/mxfp4.h): sizes from
+ * mx_mxfp4_code_bytes / mx_mxfp4_scale_bytes (rows M, columns K), codes 16-byte and scales 4-byte aligned. Any M, K. */
+long mx_mxfp4_code_bytes(int M, int K);
+long mx_mxfp4_scale_bytes(int M, int K);
+/* bf16 rows (row stride ldx, any alignment; 16-byte aligned rows are read fastest) to MXFP4, and the values that the
+ * codes stand for as bf16 (exact). */
+int mx_quant_mxfp4(hipStream_t st, const uint16_t* x, long ldx, uint8_t* codes, uint8_t* scales, int M, int K);
+int mx_mxfp4_values(hipStream_t st, const uint8_t* codes, const uint8_t* scales, uint16_t* y, long ldy, int M, int K);
+/* C[m, n] = act(sum_k x[m, k] W[n, k] + bias[n]) + R[m % r_rows or m, n], both operands in MXFP4, fp32 throughout and
+ * rounded to bf16 once. act: 0 none, 1 GELU-tanh, 2 GELU-erf, on columns >= act_from. bias, R nullable; any M, N, K.
+ * mx_gemm_mxfp4 takes quantised rows; mx_gemv_mxfp4 takes at most mx_gemv_mxfp4_rows() rows in bf16 and quantises them
+ * on the way (the same result). */
+int mx_gemv_mxfp4_rows(void);
+int mx_gemv_mxfp4(hipStream_t st, const uint16_t* x, long ldx, const uint8_t* wc, const uint8_t* ws, const float* bias,
+                  const uint16_t* R, long ldr, int r_rows, uint16_t* C, long ldc, int M, int N, int K, int act,
+                  int act_from);
+int mx_gemm_mxfp4(hipStream_t st, const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws,
+                  const float* bias, const uint16_t* R, long ldr, int r_rows, uint16_t* C, long ldc, int M, int N, int K,
+                  int act, int act_from);
+
 /* ============================================================================================ attention
  * O[b, i, h*D + d] = softmax(scale * Q K^T) V over visible keys; key j visible to query i iff j < Tk and
  * (j < causal_from || j <= qpos0 + i). D in {64, 72}. Q/K/V/O addressed as base + b*s_b + h*s_h + t*s_t + d.
@@ -163,6 +187,34 @@ int mx_sdpa_check(const void* Q, long sq_t, const void* K, long sk_t, const void
  * (the kernel is attn_fwd_kernel<D, t0, t1, t2, t3>). The reference picks its tile from a fixed table by head dim
  * (moondream/gpu/hattn.py:21); this one also looks at the grid size. */
 void mx_sdpa_tiling(int B, int H, int Tq, int D, int* t);
+
+/* ============================================================================================ 8-bit KV cache
+ * e4m3 codes with a power-of-two scale for each block of 64 tokens of one head, K and V apart (layout: csrc/kv8.h):
+ * kc, vc [nslots][H][blocks][64 D] bytes, ks, vs [nslots][H][blocks], blocks = ceil(ctx / 64), all zero at first; D 64 or
+ * 128. No reference counterpart (its cache is bf16).
+ * Positions: base + pos[b * pos_s] (pos null: base), lengths alike; device values outside the cache write nothing /
+ * are clamped to it. */
+/* Rows t < n of B sequences (k, v: strides per sequence, head, row; unit column stride) to positions pos_b + t of slot b
+ * (bcast: B = 1, to every slot). count (nullable): only the first count[b] rows of sequence b. A block's exponent is the
+ * smallest e with max |x| <= 448 2^e (at least -127) over the new rows, and not less than before if it holds earlier
+ * rows, whose codes are rounded to it; what the last block holds behind the new rows is undefined. Infinities and NaN are stored as NaN. cs (nullable, D = 64): the (ncs, 16, 2)
+ * rotary table of mx_rope_kv, applied to k and to the Hq query heads q -> q_out [B][Hq][n][D] (q nullable). */
+int mx_kv8_append(hipStream_t st, const uint16_t* k, long sk_b, long sk_h, long sk_t, const uint16_t* v, long sv_b,
+                  long sv_h, long sv_t, uint8_t* kc, uint8_t* vc, uint8_t* ks, uint8_t* vs, int B, int H, int n, int D,
+                  int ctx, int nslots, int bcast, const int* pos, long pos_s, int base, const int* count, long count_s,
+                  const float* cs, int ncs, const uint16_t* q, long sq_b, long sq_h, long sq_t, int Hq, uint16_t* q_out);
+/* Rows 0 .. n - 1 of every slot and head as bf16 (exact): k, v [nslots][H][n][D]. */
+int mx_kv8_read(hipStream_t st, const uint8_t* kc, const uint8_t* vc, const uint8_t* ks, const uint8_t* vs, uint16_t* k,
+                uint16_t* v, int nslots, int H, int n, int D, int ctx);
+/* o[b, i, h D ..] = softmax(scale q[b, h, i] K^T) V over the visible keys of slot b, key head h / G, for H G query heads:
+ * j < len_b and (j < causal_from or j <= qpos + i) (qend: qpos = len_b - Tq; causal_from = INT_MAX: no mask); a row that
+ * sees none is zero. scale > 0. q rows and strides 16-byte aligned, o 8-byte. part: mx_kv8_sdpa_ws() floats, 16-byte
+ * aligned, free again once the call's kernels have run (null where that is 0). */
+long mx_kv8_sdpa_ws(int B, int H, int G, int Tq, int ctx, int D);
+int mx_kv8_sdpa(hipStream_t st, const uint16_t* q, long sq_b, long sq_h, long sq_t, const uint8_t* kc, const uint8_t* vc,
+                const uint8_t* ks, const uint8_t* vs, uint16_t* o, long so_b, long so_t, int B, int H, int G, int Tq,
+                int D, int ctx, const int* len, long len_s, int base, int qpos, int qend, int causal_from, float scale,
+                float* part, long part_elems);
 
 /* ============================================================================================ norms
  * LayerNorm over rows of D (fp32 statistics, one rounding). Replaces F.layer_norm in _ln (md2fast.py:43-44) and the

@@ -672,6 +672,289 @@ def resize_patchify(img_u8, size, patch, ldo=None, out=None):
     return y
 
 
+# ------------------------------------------------------------------------------------------------ MXFP4, 8-bit KV cache
+def _call_on(dev, name, *args):
+    """call() on the current stream of the tensors' own device."""
+    if dev.type != "cuda":
+        raise ValueError(f"{name} needs tensors on the GPU, got {dev}")
+    if dev.index == torch.cuda.current_device():
+        return call(name, stream(), *args)
+    with torch.cuda.device(dev):
+        return call(name, stream(), *args)
+
+
+def _need(t, name, dev, dtype=BF):
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, not on {dev}")
+
+
+class MxFp4:
+    """A matrix (rows, K) in MXFP4: 4-bit e2m1 codes and a power-of-two scale for each 32 columns of a row, held in the
+    order of the matrix instruction's operands (codes, scales: uint8 buffers of their own layout)."""
+
+    def __init__(self, codes, scales, rows, K):
+        self.codes, self.scales, self.rows, self.K = codes, scales, rows, K
+
+    def values(self, out=None):
+        """(rows, K) bf16: the values the codes stand for, exact."""
+        dev = self.codes.device
+        y = out if out is not None else torch.empty(self.rows, self.K, device=dev, dtype=BF)
+        _need(y, "out", dev)
+        if y.shape != (self.rows, self.K) or y.stride(1) != 1:
+            raise ValueError(f"out must be ({self.rows}, {self.K}) with unit column stride")
+        if y.numel():
+            _call_on(dev, "mx_mxfp4_values", self.codes.data_ptr(), self.scales.data_ptr(), y.data_ptr(), y.stride(0),
+                     self.rows, self.K)
+        return y
+
+
+def quant_mxfp4(x):
+    """x (..., K) bf16 -> MxFp4 of its rows. Per block of 32 columns e = max(floor(log2 max|x|) - 2, -127), codes
+    e2m1(x 2^-e) to nearest even, saturating at 6 (OCP MX v1.0); a block with an infinity or NaN becomes NaN."""
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("x needs at least one column")
+    _need(x, "x", x.device)
+    K = x.shape[-1]
+    x2 = x.reshape(-1, K)
+    if x2.stride(1) != 1 and K > 1:
+        x2 = x2.contiguous()
+    M = x2.shape[0]
+    nkt = (K + 127) // 128
+    rt = (M + 15) // 16
+    codes = torch.empty(rt * nkt * 1024, device=x.device, dtype=torch.uint8)
+    scales = torch.empty(rt * ((nkt + 3) // 4) * 256, device=x.device, dtype=torch.uint8)
+    if M:
+        _call_on(x.device, "mx_quant_mxfp4", x2.data_ptr(), x2.stride(0), codes.data_ptr(), scales.data_ptr(), M, K)
+    return MxFp4(codes, scales, M, K)
+
+
+class MxFp4Lin:
+    """MXFP4 Linear: y = act(x W^T + b) [+ res] with W quantised once and x per call (quant_mxfp4's rule for both), on the
+    scaled MFMA; fp32 throughout, rounded to bf16 once. `pre` takes an already quantised input (MxFp4), so layers that
+    read the same activation share one quantisation. Any (N, K). act: None / "tanh" / "erf", on columns >= act_from.
+    Few rows are quantised inside the product's launch; the results are the same."""
+    fused_gelu = True
+    fused_res = True
+
+    def __init__(self, weight, bias, dtype=BF, device="cuda"):
+        if dtype != BF:
+            raise ValueError("bf16 activations only")
+        self._set(quant_mxfp4(weight.detach().to(device=device, dtype=BF)), bias)
+
+    @classmethod
+    def from_quantized(cls, w, bias):
+        """A Linear over an already quantised (N, K) weight (MxFp4)."""
+        self = cls.__new__(cls)
+        self._set(w, bias)
+        return self
+
+    def _set(self, w, bias):
+        self.wq, self.N, self.K = w, w.rows, w.K
+        self.dev = w.codes.device
+        if self.N < 1:
+            raise ValueError("the weight needs at least one row")
+        if bias is not None and bias.shape != (self.N,):
+            raise ValueError(f"bias must be ({self.N},)")
+        self.b = None if bias is None else bias.detach().to(device=self.dev, dtype=torch.float32).contiguous()
+        self.rows = _lib.load().mx_gemv_mxfp4_rows()
+
+    def quant(self, x):
+        return quant_mxfp4(x)
+
+    def __call__(self, x, gelu=False, res=None, pre=None, act=None, out=None, act_from=0):
+        a = ACT[act if act is not None else gelu]
+        if a == 3:
+            raise ValueError("no gated GELU in the MXFP4 path")
+        if act_from < 0:
+            raise ValueError("act_from must not be negative")
+        N, K = self.N, self.K
+        if pre is None:
+            if x.shape[-1] != K:
+                raise ValueError(f"input width {x.shape[-1]} != {K}")
+            _need(x, "x", self.dev)
+            x2 = x.reshape(-1, K)
+            if x2.stride(1) != 1 and K > 1:
+                x2 = x2.contiguous()
+            M = x2.shape[0]
+        else:
+            if pre.K != K or pre.codes.device != self.dev:
+                raise ValueError(f"pre: width {pre.K} on {pre.codes.device}, need {K} on {self.dev}")
+            M = pre.rows
+            if x is not None and x.numel() != M * x.shape[-1]:
+                raise ValueError("x and pre have different rows")
+        y = out if out is not None else torch.empty(M, N, device=self.dev, dtype=BF)
+        y2 = y if y.dim() == 2 else y.view(-1, N)
+        if y2.shape != (M, N) or (y2.stride(1) != 1 and N > 1):
+            raise ValueError(f"out must be ({M}, {N}) with unit column stride")
+        _need(y2, "out", self.dev)
+        r2, r_rows, ldr = None, 0, 0
+        if res is not None:
+            _need(res, "res", self.dev)
+            if res.shape[-1] != N:
+                raise ValueError(f"residual width {res.shape[-1]} != {N}")
+            r2 = res.reshape(-1, N)
+            if r2.stride(1) != 1 and N > 1:
+                r2 = r2.contiguous()
+            ldr = r2.stride(0)
+            if r2.shape[0] != M:
+                if not r2.shape[0] or M % r2.shape[0]:
+                    raise ValueError("residual rows must equal or divide the output rows")
+                r_rows = r2.shape[0]
+        if M:
+            w = self.wq
+            tail = (w.codes.data_ptr(), w.scales.data_ptr(), ptr(self.b), ptr(r2), ldr, r_rows, y2.data_ptr(),
+                    y2.stride(0), M, N, K, a, act_from)
+            if pre is None and M <= self.rows:
+                _call_on(self.dev, "mx_gemv_mxfp4", x2.data_ptr(), x2.stride(0), *tail)
+            else:
+                q = quant_mxfp4(x2) if pre is None else pre
+                _call_on(self.dev, "mx_gemm_mxfp4", q.codes.data_ptr(), q.scales.data_ptr(), *tail)
+        if out is not None:
+            return y
+        return y2 if x is None else y2.view(*x.shape[:-1], N)
+
+
+def _where(v, B, dev, name):
+    """(pointer, stride, base) of a position or length: an int, or an int32 tensor of B values."""
+    if isinstance(v, torch.Tensor):
+        if v.dim() != 1 or v.shape[0] != B:
+            raise ValueError(f"{name} must be an int or a tensor of {B} values")
+        _need(v, name, dev, torch.int32)
+        return v.data_ptr(), v.stride(0), 0
+    return None, 0, int(v)
+
+
+def _rows4(t):
+    """t with unit column stride (copied if it has another)."""
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+class KV8Cache:
+    """A KV cache in 8 bits: e4m3 codes, one power-of-two scale for each block of 64 tokens of a head, K and V apart.
+    `slots` sequences of at most `ctx` tokens, `heads` key heads of dim 64 or 128, contiguous per sequence. What the cache
+    holds is exact in bf16 (read(); but for what rounds to 2^128); the codes are stored in the order of the matrix instruction's operands.
+    Calls on one cache belong on one stream (or must be ordered by the caller), as with any tensor that is written."""
+    BLOCK = 64
+
+    def __init__(self, slots, heads, ctx, hd, device="cuda"):
+        if min(slots, heads, ctx) < 1 or hd not in (64, 128):
+            raise ValueError(f"slots {slots}, heads {heads}, ctx {ctx} must be positive and hd {hd} be 64 or 128")
+        self.slots, self.heads, self.ctx, self.hd = slots, heads, ctx, hd
+        nb = -(-ctx // self.BLOCK)
+        z = lambda *s: torch.zeros(*s, device=device, dtype=torch.uint8)
+        self.kc, self.vc = z(slots, heads, nb, 64 * hd), z(slots, heads, nb, 64 * hd)
+        self.ks, self.vs = z(slots, heads, nb), z(slots, heads, nb)
+        self.dev = self.kc.device
+
+    def _ptrs(self):
+        return self.kc.data_ptr(), self.vc.data_ptr(), self.ks.data_ptr(), self.vs.data_ptr()
+
+    def append(self, k, v, pos=0, base=0, count=None, bcast=False, cs=None, q=None):
+        """Writes k, v (B, heads, n, hd) at positions base + pos_b + t of slot b (bcast: B = 1, into every slot). pos: an
+        int, or an int32 tensor (B,) read on the device, so that a captured graph follows it; rows whose position then
+        falls outside the cache are dropped (with an int that raises). count (int32 tensor (B,)): only the first
+        count[b] rows of sequence b. A block that already holds rows before pos_b keeps its exponent or raises it (its
+        codes are rounded to the new one). The sequence then ends behind the new rows: what their last block holds after
+        them is undefined, other blocks and slots stay as they are.
+        cs: the rotary table (positions, 16, 2) of synth.freqs_cis, hd = 64 only: k is rotated first, and q (B, Hq, n, hd)
+        with it, which is returned as (B, Hq, n, hd)."""
+        if k.dim() != 4 or k.shape != v.shape or k.shape[1] != self.heads or k.shape[3] != self.hd:
+            raise ValueError(f"k, v must be (B, {self.heads}, n, {self.hd}), got {tuple(k.shape)}, {tuple(v.shape)}")
+        B, H, n, D = k.shape
+        if (B != 1) if bcast else (B > self.slots):
+            raise ValueError(f"{B} sequences for {'a broadcast' if bcast else self.slots}")
+        _need(k, "k", self.dev)
+        _need(v, "v", self.dev)
+        pp, ps, p0 = _where(pos, B, self.dev, "pos")
+        base = int(base) + p0
+        if pp is None and not 0 <= base <= self.ctx - n:
+            raise ValueError(f"positions {base} .. {base + n - 1} outside the {self.ctx}-entry cache")
+        cp, cstr, _ = (None, 0, 0) if count is None else _where(count, B, self.dev, "count")
+        if count is not None and cp is None:
+            raise ValueError("count must be a tensor")
+        q_out, qa = None, (None, 0, 0, 0, 0, None)
+        if q is not None and cs is None:
+            raise ValueError("q goes with cs")
+        if cs is not None:
+            _need(cs, "cs", self.dev, torch.float32)
+            if D != 64 or cs.dim() != 3 or cs.shape[1:] != (16, 2) or cs.shape[0] < 1 or not cs.is_contiguous():
+                raise ValueError("cs must be a contiguous (positions, 16, 2) table and hd 64")
+            if pp is None and base + n > cs.shape[0]:
+                raise ValueError(f"position {base + n - 1} is past the {cs.shape[0]}-entry rotary table")
+            if q is not None:
+                if q.dim() != 4 or q.shape[0] != B or q.shape[2:] != k.shape[2:]:
+                    raise ValueError(f"q must be ({B}, Hq, {n}, {D}), got {tuple(q.shape)}")
+                _need(q, "q", self.dev)
+                q = _rows4(q)
+                q_out = torch.empty(q.shape, device=self.dev, dtype=BF)
+                qa = (q.data_ptr(), *q.stride()[:3], q.shape[1], q_out.data_ptr())
+        if k.numel():
+            k, v = _rows4(k), _rows4(v)
+            _call_on(self.dev, "mx_kv8_append", k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3],
+                     *self._ptrs(), B, H, n, D, self.ctx, self.slots, int(bcast), pp, ps, base, cp, cstr, ptr(cs),
+                     0 if cs is None else cs.shape[0], *qa)
+        return q_out
+
+    def read(self, n=None):
+        """(k, v), each (slots, heads, n, hd) bf16: what positions 0 .. n - 1 (default: all) hold, exact."""
+        n = self.ctx if n is None else int(n)
+        if not 0 <= n <= self.ctx:
+            raise ValueError(f"n {n} outside 0 .. {self.ctx}")
+        k = torch.empty(self.slots, self.heads, n, self.hd, device=self.dev, dtype=BF)
+        v = torch.empty_like(k)
+        if n:
+            _call_on(self.dev, "mx_kv8_read", *self._ptrs(), k.data_ptr(), v.data_ptr(), self.slots, self.heads, n, self.hd,
+                     self.ctx)
+        return k, v
+
+
+def sdpa_kv8(q, cache, kv_len, base=0, out=None, scale=None, qpos0=None, causal_from=None):
+    """Attention of q (B, Hq, Tq, D) over the first base + kv_len_b tokens of slots 0 .. B - 1 of a KV8Cache, Hq a multiple
+    of its heads (query head h reads key head h / (Hq / heads)); out (B, Tq, Hq * D).
+
+    kv_len: an int, or an int32 tensor (B,) read on the device (values outside 0 .. ctx are clamped). Mask, as in sdpa:
+    key j is visible to query i iff j < len_b and (j < causal_from or j <= qpos0 + i); causal_from=None: no mask;
+    qpos0=None: the queries are the last Tq tokens of their sequence, qpos0 = len_b - Tq. Rows that see no key are 0."""
+    if q.dim() != 4 or q.shape[3] != cache.hd or q.shape[1] < 1 or q.shape[1] % cache.heads or q.shape[0] > cache.slots:
+        raise ValueError(f"q {tuple(q.shape)} does not fit a cache of {cache.slots} x {cache.heads} heads x {cache.hd}")
+    B, Hq, Tq, D = q.shape
+    dev = cache.dev
+    _need(q, "q", dev)
+    lp, ls, l0 = _where(kv_len, B, dev, "kv_len")
+    base = int(base) + l0
+    if lp is None and not 0 <= base <= cache.ctx:
+        raise ValueError(f"length {base} outside the {cache.ctx}-entry cache")
+    sc = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < sc < float("inf"):
+        raise ValueError(f"scale {sc} must be positive and finite")
+    cf = 0x7fffffff if causal_from is None else int(causal_from)
+    if cf < 0:
+        raise ValueError("causal_from must not be negative")
+    if out is None:
+        out = torch.empty(B, Tq, Hq * D, device=dev, dtype=BF)
+    else:
+        _need(out, "out", dev)
+        if out.shape != (B, Tq, Hq * D) or out.stride(2) != 1 or (out.stride(0) | out.stride(1)) % 4 or out.data_ptr() % 8:
+            raise ValueError(f"out must be ({B}, {Tq}, {Hq * D}) with 8-byte aligned rows of unit stride")
+    if not out.numel():
+        return out
+    s = q.stride()
+    if s[3] != 1 or (s[0] | s[1] | s[2]) % 8 or q.data_ptr() % 16:
+        q = q.contiguous()
+        if q.data_ptr() % 16:
+            q = q.clone()
+        s = q.stride()
+    G = Hq // cache.heads
+    need = _lib.load().mx_kv8_sdpa_ws(B, cache.heads, G, Tq, cache.ctx, D)
+    part = torch.empty(need, device=dev, dtype=torch.float32) if need else None
+    _call_on(dev, "mx_kv8_sdpa", q.data_ptr(), s[0], s[1], s[2], *cache._ptrs(), out.data_ptr(), out.stride(0),
+             out.stride(1), B, cache.heads, G, Tq, D, cache.ctx, lp, ls, base, 0 if qpos0 is None else int(qpos0),
+             int(qpos0 is None), cf, sc, ptr(part), need)
+    return out
+
+
 def gemm_tile(cfg):
     import ctypes
     bm, bn = ctypes.c_int(), ctypes.c_int()

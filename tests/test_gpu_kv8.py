@@ -1,0 +1,317 @@
+"""The 8-bit KV cache and attention over it on the MI355X against the 64-bit oracle: what the cache holds bit for bit, the
+attention within a bound derived from its roundings."""
+import pytest
+import torch
+
+import oracle.lowbit as ol
+import strix_halo_maxx_amd.ops as ops
+from strix_halo_maxx_amd import _lib
+from strix_halo_maxx_amd.synth import freqs_cis
+
+pytestmark = pytest.mark.gpu
+BF, F64 = torch.bfloat16, torch.float64
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def same(a, b):
+    """bf16 a is b, a double that bf16 holds exactly (but 2^128, to which the largest bf16 rounds: infinity)."""
+    a, b = a.to(F64), torch.where(b.abs() == 2.0 ** 128, b * float("inf"), b)
+    return bool(((a == b) | (a.isnan() & b.isnan())).all())
+
+
+def rows(g, *shape, spread=0):
+    x = torch.randn(*shape, generator=g)
+    if spread:
+        x = x * torch.exp2(torch.randint(-spread, spread + 1, shape[:-1] + (1,), generator=g).float())
+    return x.to(BF)
+
+
+def i32(dev, *v):
+    return torch.tensor(v, device=dev, dtype=torch.int32)
+
+
+class Both:
+    """A cache and its oracle, written alike."""
+
+    def __init__(self, dev, slots, H, ctx, D):
+        self.dev, self.c = dev, ops.KV8Cache(slots, H, ctx, D, device=dev)
+        self.k, self.v = ol.KV8(slots, H, ctx, D), ol.KV8(slots, H, ctx, D)
+        self.end = [0] * slots  # where each sequence ends: what its last block holds behind that is undefined
+
+    def append(self, k, v, pos, counts=None, **kw):
+        B = k.shape[0]
+        ps = [pos] * B if isinstance(pos, int) else list(pos)
+        self.c.append(k.to(self.dev), v.to(self.dev), pos if isinstance(pos, int) else i32(self.dev, *pos),
+                      count=None if counts is None else i32(self.dev, *counts), **kw)
+        for b in range(B):
+            n = k.shape[2] if counts is None else max(0, min(counts[b], k.shape[2]))
+            for slot in range(self.c.slots) if kw.get("bcast") else (b,):
+                self.k.append(slot, k[b, :, :n], ps[b])
+                self.v.append(slot, v[b, :, :n], ps[b])
+                if n and ps[b] < self.c.ctx and ps[b] + n > 0:
+                    self.end[slot] = min(ps[b] + n, self.c.ctx)
+
+    def check(self):
+        for got, want in zip(self.c.read(), (self.k, self.v)):
+            for slot, n in enumerate(self.end):
+                rest = -(-n // 64) * 64  # blocks that were never written
+                ok = same(got[slot, :, :n].cpu(), want.val[slot, :, :n]) and same(got[slot, :, rest:].cpu(), want.val[slot, :, rest:])
+                assert ok, slot
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_append_fresh_and_in_steps(dev, D):
+    """A prompt, then single rows with larger and smaller values across a block border: exponents rise, codes follow."""
+    g = gen(D)
+    c = Both(dev, 2, 3, 200, D)
+    c.append(rows(g, 2, 3, 61, D, spread=3), rows(g, 2, 3, 61, D, spread=3), 0)
+    c.check()
+    for t, s in enumerate((0.1, 8.0, 1.0, 300.0, 0.01, 2.0 ** 20, 1.0)):
+        c.append((rows(g, 2, 3, 1, D).float() * s).to(BF), (rows(g, 2, 3, 1, D).float() / s).to(BF), 61 + t)
+        c.check()
+    c.append(rows(g, 2, 3, 100, D, spread=5), rows(g, 2, 3, 100, D), 68)
+    c.check()
+
+
+@pytest.mark.parametrize("D,ctx", [(64, 1), (128, 63), (64, 64), (128, 65), (64, 300)])
+def test_append_positions_on_the_device(dev, D, ctx):
+    """Ragged positions and counts; rows outside the cache are dropped; zero rows; negative and far positions."""
+    g = gen(ctx)
+    c = Both(dev, 6, 2, ctx, D)
+    n = 70
+    k, v = rows(g, 6, 2, n, D), rows(g, 6, 2, n, D)
+    c.append(k, v, (0, ctx // 2, ctx - 1, ctx, -5, -1000), counts=(n, 1, n, n, n, n))
+    c.check()
+    c.append(k * 4, v, (2 ** 31 - 1, -2 ** 31, 0, 3, 1, ctx // 3), counts=(n, n, 0, 2, -3, 2 ** 31 - 1))
+    c.check()
+
+
+def test_append_special_values(dev):
+    """Zeros, subnormals, the largest bf16, 448 and 449 times a power of two, ties, NaN and infinities."""
+    g = gen(3)
+    c = Both(dev, 1, 4, 128, 64)
+    k = torch.zeros(1, 4, 64, 64)
+    k[0, 0, 0, :4] = torch.tensor([448.0, 17.0, 19.0, 2.0 ** -9])     # exponent 0: 17, 19 halfway
+    k[0, 0, 1, :4] = torch.tensor([1.5 * 2.0 ** -10, 2.0 ** -10, 3 * 2.0 ** -10, -27.0])
+    k[0, 1, 5, :2] = torch.tensor([450.0, 17.0])                      # exponent 1
+    k[0, 2] = torch.randn(64, 64, generator=g) * 2.0 ** -131
+    k[0, 3, 7, :3] = torch.tensor([3.3895e38, 1e38, -1e30])
+    v = torch.randn(1, 4, 64, 64, generator=g)
+    v[0, 1, 3, 3], v[0, 2, 9, 9], v[0, 3, 1, 1] = float("nan"), float("inf"), float("-inf")
+    c.append(k[:, :, :40].to(BF), v[:, :, :40].to(BF), 0)
+    c.append(k[:, :, 40:].to(BF) + 1, 100 * v[:, :, 40:].to(BF), 40)  # the kept NaN codes are rounded again
+    c.check()
+
+
+def test_append_strides_and_alignment(dev):
+    """Views of a fused projection, odd addresses and strides, broadcast rows."""
+    g = gen(5)
+    H, n, D = 3, 77, 64
+    qkv = rows(g, 2, n, 3 * H * D + 3)
+    c = Both(dev, 2, H, 128, D)
+    qd = qkv.to(dev)
+    for off in (0, 3):
+        part = lambda x, i: x[:, :, off + i * H * D:off + (i + 1) * H * D].unflatten(2, (H, D)).transpose(1, 2)
+        c.c.append(part(qd, 1), part(qd, 2), 5 + off)
+        for b in range(2):
+            c.k.append(b, part(qkv, 1)[b], 5 + off)
+            c.v.append(b, part(qkv, 2)[b], 5 + off)
+            c.end[b] = 5 + off + n
+        c.check()
+    k, v = rows(g, 1, 1, n, D), rows(g, 1, H, D, n)
+    c.c.append(k.to(dev).expand(2, H, n, D), v.to(dev).transpose(2, 3).expand(2, H, n, D), 0)
+    for b in range(2):
+        c.k.append(b, k[0].expand(H, n, D), 0)
+        c.v.append(b, v[0].transpose(1, 2), 0)
+        c.end[b] = n
+    c.check()
+
+
+def test_append_broadcast_and_rope(dev):
+    """bcast writes every slot; the rotary form equals mx_rope_kv's rounded rows appended, and rotates q as it does."""
+    g = gen(6)
+    H, D, n, pos, ctx = 32, 64, 90, 37, 256
+    cs = freqs_cis(32, ctx).to(dev)
+    qkv = rows(g, n, 3 * H * D).to(dev)
+    q = torch.empty(1, H, n, D, device=dev, dtype=BF)
+    kc, vc = torch.zeros(2, H, ctx, D, device=dev, dtype=BF), torch.zeros(2, H, ctx, D, device=dev, dtype=BF)
+    _lib.call("mx_rope_kv", _lib.stream(), qkv.data_ptr(), qkv.stride(0), cs.data_ptr(), q.data_ptr(), kc.data_ptr(),
+              vc.data_ptr(), 1, n, H, ctx, pos, 2, 1)
+    part = [qkv[:, i * H * D:(i + 1) * H * D].view(1, n, H, D).transpose(1, 2) for i in range(3)]
+    want, got = ops.KV8Cache(2, H, ctx, D, device=dev), ops.KV8Cache(2, H, ctx, D, device=dev)
+    want.append(kc[:1, :, pos:pos + n], vc[:1, :, pos:pos + n], pos, bcast=True)
+    for p, b in ((pos, 0), (i32(dev, pos - 30), 30)):
+        q2 = got.append(part[1], part[2], p, base=b, bcast=True, cs=cs, q=part[0])
+        assert torch.equal(q2, q)
+        for x, y in zip(want.read() + (want.ks, want.vs), got.read() + (got.ks, got.vs)):
+            assert torch.equal(x, y)
+
+
+def test_read_part(dev):
+    g = gen(7)
+    c = Both(dev, 2, 2, 150, 128)
+    c.append(rows(g, 2, 2, 150, 128), rows(g, 2, 2, 150, 128), 0)
+    for n in (1, 64, 65, 149):
+        k, v = c.c.read(n)
+        ok = same(k.cpu(), c.k.val[:, :, :n]) and same(v.cpu(), c.v.val[:, :, :n])
+        assert ok
+    assert c.c.read(0)[0].shape == (2, 2, 0, 128)
+
+
+def check_sdpa(y, q, c, lens, **kw):
+    """The output's rounding, 2^-8 of it; per weight 2^-8 (two e4m3 terms, half a step of 2^-4 each: 2^-4 2^-4) and the
+    error of its score, taken as 2^-12 of the largest sum |q k| scale for the MFMA's sums; the product with V, 2^-12 of
+    the mean |v|. A weight's error moves numerator and denominator: twice."""
+    for b, n in enumerate(lens):
+        ref, avg, size = ol.sdpa(q[b], c.k.val[b], c.v.val[b], n, **kw)
+        out = y[b].to(F64).view(ref.shape)
+        tol = 2.0 ** -8 * ref.abs() + (2.0 ** -8 + 2.0 ** -12 + 2 * 2.0 ** -12 * (1 + size)) * avg
+        bad = (out - ref).abs() > tol
+        assert not bool(bad.any()) and not bool(out.isnan().any()), (b, n, (out - ref).abs().max().item())
+
+
+# slots' lengths, H, G, D, Tq, causal_from
+SDPA = [((1,), 1, 1, 64, 1, None), ((0, 1, 63, 64, 65), 2, 1, 64, 1, None), ((130, 5, 700), 4, 4, 128, 1, None),
+        ((1000,), 32, 1, 64, 1, 0), ((2100, 17), 2, 8, 128, 1, None), ((70, 3), 1, 32, 64, 1, None),
+        ((40, 200), 3, 3, 64, 5, 0), ((33, 90, 0), 2, 1, 64, 40, 0), ((300, 64), 2, 4, 128, 37, 50),
+        ((150,), 2, 2, 64, 150, 100), ((128, 129), 1, 7, 128, 129, 0), ((4500,), 1, 2, 64, 3, 0)]
+
+
+@pytest.mark.parametrize("lens,H,G,D,Tq,cf", SDPA)
+def test_sdpa(dev, lens, H, G, D, Tq, cf):
+    g = gen(sum(lens) + 13 * H + G + D + Tq)
+    B, ctx = len(lens), max(lens) + 11
+    c = Both(dev, B + 1, H, ctx, D)
+    n = max(max(lens), 1)
+    c.append(rows(g, B, H, n, D, spread=1), rows(g, B, H, n, D, spread=1), 0, counts=lens)
+    q = rows(g, B, H * G, Tq, D)
+    print("sdpa_kv8", lens, H, G, D, Tq, cf, flush=True)
+    y = ops.sdpa_kv8(q.to(dev), c.c, i32(dev, *lens), causal_from=cf)
+    check_sdpa(y.cpu(), q, c, lens, causal_from=cf)
+    # lengths from the host, a base with the tensor, positions given
+    if len(set(lens)) == 1:
+        assert torch.equal(ops.sdpa_kv8(q.to(dev), c.c, lens[0], causal_from=cf), y)
+        assert torch.equal(ops.sdpa_kv8(q.to(dev), c.c, lens[0], causal_from=cf, qpos0=lens[0] - Tq), y)
+    assert torch.equal(ops.sdpa_kv8(q.to(dev), c.c, i32(dev, *[n - 7 for n in lens]), base=7, causal_from=cf), y)
+
+
+def test_sdpa_rows_that_see_nothing_are_zero(dev):
+    """Queries before the first key, empty sequences, lengths outside the cache (clamped)."""
+    g = gen(11)
+    c = Both(dev, 4, 2, 100, 64)
+    c.append(rows(g, 4, 2, 100, 64), rows(g, 4, 2, 100, 64), 0)
+    q = rows(g, 4, 2, 6, 64)
+    out = torch.full((4, 6, 128), 9.0, device=dev, dtype=BF)
+    y = ops.sdpa_kv8(q.to(dev), c.c, i32(dev, 0, -7, 100, 10 ** 9), qpos0=-3, causal_from=0, out=out).cpu()
+    assert y is not None and bool((out[:2] == 0).all()) and bool((out[2:, :3] == 0).all())
+    check_sdpa(out.cpu(), q, c, (0, 0, 100, 100), qpos0=-3, causal_from=0)
+
+
+@pytest.mark.parametrize("D,Tq,cf", [(64, 1, None), (128, 20, 0), (64, 70, 64)])
+def test_sdpa_masked_keys_may_hold_nan(dev, D, Tq, cf):
+    """NaN keys and values behind the sequence and behind each query change nothing; a query that sees one is NaN."""
+    g = gen(D + Tq)
+    n, ctx, at = 150, 200, 141
+    k, v, q = rows(g, 1, 2, ctx, D), rows(g, 1, 2, ctx, D), rows(g, 1, 4, Tq, D)
+    clean = Both(dev, 1, 2, ctx, D)
+    clean.append(k, v, 0)
+    k, v = k.clone(), v.clone()
+    k[:, :, n:], v[:, :, n:] = float("nan"), float("inf")
+    c = Both(dev, 1, 2, ctx, D)
+    c.append(k, v, 0)
+    c.k.val[:, :, n:], c.v.val[:, :, n:] = 0, 0
+    y = ops.sdpa_kv8(q.to(dev), c.c, n, causal_from=cf)
+    check_sdpa(y.cpu(), q, c, (n,), causal_from=cf)
+    if Tq == 1:
+        return
+    # one value at position `at` of head 1: queries at .. see it (with the mask), the others do not
+    c.c.append(k[:, :, at:at + 1].to(dev), torch.full((1, 2, 1, D), float("nan"), device=dev, dtype=BF), at)
+    y2 = ops.sdpa_kv8(q.to(dev), c.c, n, causal_from=cf).cpu().float()
+    sees = torch.arange(Tq) + n - Tq >= at
+    assert bool(y2[0, sees].isnan().all()) and not bool(y2[0, ~sees].isnan().any())
+    k2 = k.clone()
+    k2[:, :, at] = float("nan")
+    c.c.append(k2[:, :, at:at + 1].to(dev), v[:, :, at:at + 1].to(dev), at)
+    y3 = ops.sdpa_kv8(q.to(dev), c.c, n, causal_from=cf).cpu().float()
+    assert bool(y3[0, sees].isnan().all()) and not bool(y3[0, ~sees].isnan().any())
+
+
+def test_sdpa_non_finite_queries_and_extreme_scores(dev):
+    """A NaN or infinite query gives a NaN row and no other; one key that outweighs the rest by 2^100 is its value; equal
+    scores average; a long tail of small weights under one large one is kept."""
+    g = gen(21)
+    D, n = 64, 640
+    c = Both(dev, 1, 1, n, D)
+    k, v = rows(g, 1, 1, n, D) * 0.01, rows(g, 1, 1, n, D)
+    k[0, 0, 77] = 0
+    k[0, 0, 77, 0] = 16.0
+    c.append(k, v, 0)
+    q = rows(g, 1, 1, 6, D)
+    q[0, 0, 1, 3], q[0, 0, 2, 5] = float("nan"), float("inf")
+    q[0, 0, 3] = 0
+    q[0, 0, 3, 0] = 64.0   # score 128 against about 0.08
+    q[0, 0, 4] = 0         # equal scores
+    q[0, 0, 5] = 0
+    q[0, 0, 5, 0] = 5.5    # weight e^11 (59874) against 639 of about 1
+    y = ops.sdpa_kv8(q.to(dev), c.c, n).cpu()
+    assert bool(y[0, 1:3].isnan().all()) and not bool(y[0, [0, 3, 4, 5]].isnan().any())
+    keep = [0, 3, 4, 5]
+    check_sdpa(y[:, keep], q[:, :, keep], c, (n,))
+
+
+def test_sdpa_strides_out_and_other_slots(dev):
+    """q as a view of a fused projection, an output inside a larger buffer, fewer sequences than slots, unaligned q."""
+    g = gen(31)
+    B, H, G, D, Tq, n = 2, 2, 2, 64, 9, 100
+    c = Both(dev, 3, H, 128, D)
+    c.append(rows(g, 3, H, n, D), rows(g, 3, H, n, D), 0)
+    fused = rows(g, B, Tq, 3 * H * G * D + 5)
+    for off in (0, 3):
+        q = fused[:, :, off:off + H * G * D].unflatten(2, (H * G, D)).transpose(1, 2)
+        qd = fused.to(dev)[:, :, off:off + H * G * D].unflatten(2, (H * G, D)).transpose(1, 2)
+        big = torch.full((B, Tq + 2, H * G * D + 12), 5.0, device=dev, dtype=BF)
+        out = big[:, 1:-1, 4:4 + H * G * D]
+        ops.sdpa_kv8(qd, c.c, n, out=out, causal_from=0)
+        check_sdpa(out.cpu(), q, c, (n, n), causal_from=0)
+        out.fill_(5.0)
+        assert bool((big == 5.0).all())
+
+
+@pytest.mark.parametrize("n,D,G", [(300, 64, 1), (6000, 128, 4)])
+def test_step_in_a_graph(dev, n, D, G):
+    """Append and attend with the position on the device: a captured graph replayed step by step equals the eager steps,
+    also with two graphs of the same calls replayed in turn."""
+    g = gen(n)
+    H, steps, ctx = 2, 6, n + 20
+    k0, v0 = rows(g, 1, H, n, D).to(dev), rows(g, 1, H, n, D).to(dev)
+    ks, vs = rows(g, steps, 1, H, 1, D, spread=2).to(dev), rows(g, steps, 1, H, 1, D).to(dev)
+    qs = rows(g, steps, 1, H * G, 1, D).to(dev)
+    a, b = ops.KV8Cache(1, H, ctx, D, device=dev), ops.KV8Cache(1, H, ctx, D, device=dev)
+    want = []
+    a.append(k0, v0, 0)
+    for t in range(steps):
+        a.append(ks[t], vs[t], n + t)
+        want.append(ops.sdpa_kv8(qs[t], a, n + t + 1))
+    pos, kb, vb, qb = i32(dev, 0), ks[0].clone(), vs[0].clone(), qs[0].clone()
+    graphs = []
+    for _ in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            b.append(kb, vb, pos, base=n)
+            y = ops.sdpa_kv8(qb, b, pos, base=n + 1)
+            pos.add_(1)
+        graphs.append((gr, y))
+    for _ in range(2):
+        b.kc.zero_(), b.vc.zero_(), b.ks.zero_(), b.vs.zero_(), pos.zero_()
+        b.append(k0, v0, 0)
+        for t in range(steps):
+            kb.copy_(ks[t]), vb.copy_(vs[t]), qb.copy_(qs[t])
+            gr, y = graphs[t % 2]
+            gr.replay()
+            assert torch.equal(y, want[t]), t
+            torch.cuda.synchronize()
+        for x, z in zip(a.read(), b.read()):
+            assert torch.equal(x, z)

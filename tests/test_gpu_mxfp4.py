@@ -1,0 +1,159 @@
+"""MXFP4 quantisation and Linear on the MI355X against the 64-bit oracle: the quantised values bit for bit (every step but
+the rounding of the code is exact), the Linear within its one bf16 rounding plus that of an fp32 sum."""
+import pytest
+import torch
+
+import oracle.lowbit as ol
+import strix_halo_maxx_amd.ops as ops
+
+pytestmark = pytest.mark.gpu
+BF, F64 = torch.bfloat16, torch.float64
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def same(a, b):
+    """Equal values, NaN where NaN."""
+    a, b = a.to(F64), b.to(F64)
+    return bool(((a == b) | (a.isnan() & b.isnan())).all())
+
+
+@pytest.mark.parametrize("M,K", [(1, 1), (1, 2048), (3, 31), (17, 32), (5, 33), (16, 128), (15, 129), (33, 700), (130, 2055)])
+def test_quantised_values_are_exact(dev, M, K):
+    g = gen(M * 10007 + K)
+    x = (torch.randn(M, K, generator=g) * torch.exp2(torch.randint(-20, 20, (M, K), generator=g).float())).to(BF)
+    q = ops.quant_mxfp4(x.to(dev))
+    ok = same(q.values().cpu(), ol.mxfp4(x))
+    assert ok
+
+
+def test_quantised_special_values(dev):
+    """Ties, the saturation between 6 and 8 units, zeros, subnormals, the largest bf16, blocks with NaN and infinities."""
+    rows = torch.zeros(9, 64)
+    rows[0, :12] = torch.tensor([4.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, -0.25, -5.0, -2.5, 4.5])
+    rows[1, :6] = torch.tensor([7.96875, 6.5, 5.0, 6.0, -7.0, 0.2])
+    rows[3] = torch.randn(64, generator=gen(1)) * 2.0 ** -130
+    rows[4, ::2] = 2.0 ** -133
+    rows[5, :3] = torch.tensor([3.3895e38, -1e38, 1e37])
+    rows[6, 3], rows[6, 40] = float("nan"), 1.0
+    rows[7, 3], rows[7, 40] = 1.0, float("-inf")
+    rows[8, :2] = torch.tensor([2.0 ** -126, 2.0 ** -125])
+    x = rows.to(BF)
+    y = ops.quant_mxfp4(x.to(dev)).values().cpu()
+    assert same(y, ol.mxfp4(x))
+    assert y[0, :12].tolist() == [4.0, 0.0, 1.0, 1.0, 2.0, 2.0, 4.0, 4.0, 0.0, -4.0, -2.0, 4.0]
+    assert y[6, :32].isnan().all() and not y[6, 32:].isnan().any() and y[7, 32:].isnan().all()
+
+
+def test_quant_reads_any_rows(dev):
+    """Unaligned starts, odd row strides, a transposed input, repeated rows, more than two dimensions, no rows."""
+    g = gen(4)
+    big = torch.randn(40, 301, generator=g).to(BF)
+    d = big.to(dev)
+    for a, b in ((big[:, 1:290], d[:, 1:290]), (big[3:20, 8:264], d[3:20, 8:264]), (big.t(), d.t()),
+                 (big[:1].expand(20, -1), d[:1].expand(20, -1))):
+        assert same(ops.quant_mxfp4(b).values().cpu(), ol.mxfp4(a.reshape(-1, a.shape[-1])))
+    q = ops.quant_mxfp4(d.view(4, 10, 301))
+    assert (q.rows, q.K) == (40, 301) and same(q.values().cpu(), ol.mxfp4(big))
+    assert ops.quant_mxfp4(d[:0]).values().shape == (0, 301)
+    out = torch.full((42, 310), 7.0, device=dev, dtype=BF)
+    ops.quant_mxfp4(d).values(out=out[1:41, 3:304])
+    assert same(out[1:41, 3:304].cpu(), ol.mxfp4(big))
+    out[1:41, 3:304] = 7.0
+    assert bool((out == 7.0).all())
+
+
+def close(y, ref, mag, act=None):
+    """One rounding to bf16 (2^-8 of the value), the fp32 sum of at most 2^14 exact products (2^-24 of the magnitude for
+    each of the sum's steps, 2^-10 steps' worth: 2^-14 with room to spare over any order), the activation's slope (at
+    most 1.13) and its own few fp32 roundings, 2^-20 of the value and of 1."""
+    err = (y.to(F64) - ref).abs()
+    tol = 2.0 ** -8 * ref.abs() + 1.13 * 2.0 ** -14 * mag + (2.0 ** -20 * (1 + ref.abs()) if act else 0)
+    assert bool((err <= tol).all()), (err - tol).max().item()
+
+
+SHAPES = [(1, 1, 1), (1, 8192, 2048), (1, 2048, 8192), (2, 100, 4304), (7, 37, 100), (16, 64, 129), (17, 768, 768),
+          (33, 130, 1000), (64, 260, 512), (65, 129, 640), (128, 128, 128), (130, 259, 1152), (300, 1000, 385),
+          (520, 516, 2304)]
+
+
+@pytest.mark.parametrize("M,N,K", SHAPES)
+def test_linear(dev, M, N, K):
+    g = gen(M + 3 * N + 7 * K)
+    x, w = torch.randn(M, K, generator=g).to(BF), (torch.randn(N, K, generator=g) * 0.05).to(BF)
+    b, r = (torch.randn(N, generator=g) * 0.1).to(BF), torch.randn(M, N, generator=g).to(BF)
+    lin, plain = ops.MxFp4Lin(w, b, device=dev), ops.MxFp4Lin(w, None, device=dev)
+    xd, rd = x.to(dev), r.to(dev)
+    print(f"mxfp4 linear {M} x {N} x {K}", flush=True)
+    close(plain(xd).cpu(), *ol.mxfp4_linear(x, w))
+    for act in ("tanh", "erf"):
+        close(lin(xd, act=act).cpu(), *ol.mxfp4_linear(x, w, b, act), act=act)
+    close(lin(xd, res=rd).cpu(), *ol.mxfp4_linear(x, w, b, res=r))
+    f = N // 2 + 1
+    close(lin(xd, gelu=True, res=rd, act_from=f).cpu(), *ol.mxfp4_linear(x, w, b, "tanh", r, f), act="tanh")
+    # quantised beforehand: the same codes, another order of the sum at most
+    close(lin(None, pre=lin.quant(xd)).cpu(), *ol.mxfp4_linear(x, w, b))
+
+
+def test_linear_views_and_leading_dims(dev):
+    """Leading dimensions, rows at odd strides and addresses, residual rows that repeat, an output inside a larger buffer
+    whose rest stays."""
+    g = gen(9)
+    w, b = (torch.randn(100, 96, generator=g) * 0.1).to(BF), torch.randn(100, generator=g).to(BF)
+    lin = ops.MxFp4Lin(w, b, device=dev)
+    for M in (6, 150):
+        x = torch.randn(M, 131, generator=g).to(BF)
+        xd = x.to(dev)[:, 5:101]
+        xs = x[:, 5:101]
+        ref, mag = ol.mxfp4_linear(xs, w, b)
+        close(lin(xd).cpu(), ref, mag)
+        assert lin(xd.reshape(2, M // 2, 96)).shape == (2, M // 2, 100)
+        r = torch.randn(3, 100, generator=g).to(BF)
+        close(lin(xd, res=r.to(dev)).cpu(), ref + r.to(F64).repeat(M // 3, 1), mag)
+        for c0 in (4, 7):
+            out = torch.full((M + 2, 120), 3.0, device=dev, dtype=BF)
+            assert lin(xd, out=out[1:-1, c0:c0 + 100]) is not None
+            close(out[1:-1, c0:c0 + 100].cpu(), ref, mag)
+            out[1:-1, c0:c0 + 100] = 3.0
+            assert bool((out == 3.0).all())
+    assert lin(xd[:0]).shape == (0, 100)
+    assert lin(xd[:1].expand(20, -1)).shape == (20, 100)
+
+
+@pytest.mark.parametrize("M", [3, 40, 200])
+def test_linear_nan_stays_in_its_row(dev, M):
+    g = gen(M)
+    x, w = torch.randn(M, 256, generator=g).to(BF), torch.randn(50, 256, generator=g).to(BF)
+    x[1, 70], x[2, 200] = float("nan"), float("inf")
+    y = ops.MxFp4Lin(w, None, device=dev)(x.to(dev)).cpu()
+    bad = y.isnan().any(1)
+    assert bad.nonzero().flatten().tolist() == [1, 2] and bool(y[1:3].isnan().all())
+    keep = [m for m in range(M) if m not in (1, 2)]
+    ref, mag = ol.mxfp4_linear(x[keep], w)
+    close(y[keep], ref, mag)
+
+
+@pytest.mark.parametrize("M", [1, 16, 48, 200])
+def test_linear_in_a_graph_and_on_a_side_stream(dev, M):
+    g = gen(M)
+    w, b = torch.randn(96, 320, generator=g).to(BF), torch.randn(96, generator=g).to(BF)
+    lin = ops.MxFp4Lin(w, b, device=dev)
+    x = torch.randn(M, 320, generator=g).to(BF).to(dev)
+    want = [lin(x * s, act="tanh") for s in (1, 2, 3)]
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        side = lin(x, act="tanh")
+    torch.cuda.current_stream().wait_stream(st)
+    assert torch.equal(side, want[0])
+    buf = x.clone()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        y = lin(buf, act="tanh")
+    for s in (1, 2, 3, 1, 2, 3):
+        buf.copy_(x * s)
+        gr.replay()
+        assert torch.equal(y, want[s - 1])
+        torch.cuda.synchronize()

@@ -1,0 +1,151 @@
+"""Host side of the MXFP4 and 8-bit cache operators, without a GPU: refusals of the C ABI before any launch and of the
+Python entry points before any device work, buffer sizes, and the oracle on values worked out by hand."""
+import math
+
+import pytest
+import torch
+
+import oracle.lowbit as ol
+import strix_halo_maxx_amd.ops as ops
+from strix_halo_maxx_amd import _lib
+
+A16 = 0x10000  # fake device addresses: validation never dereferences them
+BF = torch.bfloat16
+
+
+def test_oracle_mxfp4_by_hand():
+    x = torch.zeros(1, 33)
+    x[0, :8] = torch.tensor([7.0, 5.0, 2.5, 3.5, 1.25, 0.25, 0.75, -0.26])  # unit 1: saturates; ties to even
+    x[0, 32] = 3.0                                                         # a block of one: unit 0.5, code 6
+    assert ol.mxfp4(x)[0, [0, 1, 2, 3, 4, 5, 6, 7, 32]].tolist() == [6, 4, 2, 4, 1, 0, 1, -0.5, 3]
+    assert ol.mxfp4(torch.tensor([[math.inf, 1.0]])).isnan().all()
+
+
+def test_oracle_kv8_by_hand():
+    c = ol.KV8(1, 1, 70, 2)
+    c.append(0, torch.tensor([[[448.0, 17.0]]]), 0)       # exponent 0, 17 lies halfway between 16 and 18
+    assert c.val[0, 0, 0].tolist() == [448, 16] and c.exp[0, 0, 0] == 0
+    c.append(0, torch.tensor([[[449.0, 1.0]]]), 1)        # exponent 1
+    assert c.val[0, 0, :2].tolist() == [[448, 16], [448, 1]] and c.exp[0, 0].tolist() == [1, -127]
+    c.append(0, torch.tensor([[[2.0 ** -140, 0.0]]]), 64)
+    assert c.exp[0, 0, 1] == -127
+
+
+def test_mxfp4_buffer_sizes():
+    lib = _lib.load()
+    assert lib.mx_mxfp4_code_bytes(1, 1) == 1024 and lib.mx_mxfp4_scale_bytes(1, 1) == 256
+    assert lib.mx_mxfp4_code_bytes(17, 129) == 4096 and lib.mx_mxfp4_scale_bytes(17, 513) == 1024
+    assert lib.mx_mxfp4_code_bytes(0, 5) == 0 and lib.mx_mxfp4_scale_bytes(5, -1) == 0
+    assert lib.mx_mxfp4_code_bytes(2 ** 31 - 16, 2 ** 20) == (2 ** 31 - 16) * 2 ** 19
+
+
+def test_mxfp4_refusals():
+    lib = _lib.load()
+    qz = lambda **kw: lib.mx_quant_mxfp4(*{**dict(st=None, x=A16, ldx=64, c=A16, s=A16, M=4, K=64), **kw}.values())
+    assert qz(x=None) == -6 and qz(c=None) == -6 and qz(s=None) == -6
+    assert qz(M=0) == -2 and qz(K=0) == -2 and qz(ldx=-1) == -2 and qz(M=2 ** 31 - 1, K=10 ** 6) == -2
+    assert qz(x=A16 + 1) == -4 and qz(c=A16 + 8) == -4 and qz(s=A16 + 2) == -4
+    vl = lambda **kw: lib.mx_mxfp4_values(*{**dict(st=None, c=A16, s=A16, y=A16, ldy=64, M=4, K=64), **kw}.values())
+    assert vl(y=None) == -6 and vl(ldy=63) == -2 and vl(y=A16 + 1) == -4
+    tail = dict(wc=A16, ws=A16, b=A16, R=None, ldr=0, rr=0, C=A16, ldc=64, M=4, N=64, K=64, act=0, af=0)
+    gv = lambda **kw: lib.mx_gemv_mxfp4(*{**dict(st=None, x=A16, ldx=64), **tail, **kw}.values())
+    gm = lambda **kw: lib.mx_gemm_mxfp4(*{**dict(st=None, xc=A16, xs=A16), **tail, **kw}.values())
+    rows = lib.mx_gemv_mxfp4_rows()
+    assert gv(M=rows + 1) == -2 and gv(x=None) == -6 and gv(x=A16 + 1) == -4 and gv(ldx=-8) == -2
+    assert gm(xc=None) == -6 and gm(xs=None) == -6 and gm(xc=A16 + 4) == -4 and gm(xs=A16 + 1) == -4
+    for f in (gv, gm):
+        assert f(wc=None) == -6 and f(ws=None) == -6 and f(C=None) == -6
+        assert f(act=3) == -1 and f(act=-1) == -1
+        assert f(M=0) == -2 and f(N=0) == -2 and f(K=0) == -2 and f(af=-1) == -2 and f(rr=-1) == -2 and f(ldc=63) == -2
+        assert f(R=A16, ldr=-1) == -2
+        assert f(wc=A16 + 8) == -4 and f(ws=A16 + 2) == -4 and f(b=A16 + 2) == -4 and f(C=A16 + 1) == -4
+
+
+def test_kv8_refusals():
+    lib = _lib.load()
+    ap = lambda **kw: lib.mx_kv8_append(*{**dict(
+        st=None, k=A16, kb=64, kh=64, kt=64, v=A16, vb=64, vh=64, vt=64, kc=A16, vc=A16, ks=A16, vs=A16, B=2, H=4, n=5, D=64,
+        ctx=100, slots=2, bcast=0, pos=None, pos_s=0, base=3, count=None, count_s=0, cs=None, ncs=0, q=None, qb=0, qh=0,
+        qt=0, Hq=0, qo=None), **kw}.values())
+    for name in ("k", "v", "kc", "vc", "ks", "vs"):
+        assert ap(**{name: None}) == -6
+    assert ap(D=72) == -1 and ap(D=128, cs=A16, ncs=100) == -1 and ap(cs=A16, ncs=0) == -1
+    assert ap(B=3) == -2 and ap(bcast=1) == -2 and ap(n=0) == -2 and ap(H=0) == -2 and ap(H=70000) == -2
+    assert ap(base=96) == -2 and ap(base=-1) == -2 and ap(ctx=0) == -2 and ap(ctx=2 ** 31 - 1) == -2
+    assert ap(q=A16) == -6 and ap(q=A16, cs=A16, ncs=100, qo=None, Hq=4) == -6 and ap(q=A16, cs=A16, ncs=100, qo=A16) == -6
+    assert ap(k=A16 + 1) == -4 and ap(kc=A16 + 8) == -4 and ap(pos=A16 + 2) == -4 and ap(count=A16 + 1) == -4
+    rd = lambda **kw: lib.mx_kv8_read(*{**dict(st=None, kc=A16, vc=A16, ks=A16, vs=A16, k=A16, v=A16, slots=1, H=1, n=10,
+                                               D=64, ctx=10), **kw}.values())
+    assert rd(k=None) == -6 and rd(D=96) == -1 and rd(n=11) == -2 and rd(n=0) == -2 and rd(v=A16 + 8) == -4
+    sd = lambda **kw: lib.mx_kv8_sdpa(*{**dict(
+        st=None, q=A16, qb=64, qh=64, qt=64, kc=A16, vc=A16, ks=A16, vs=A16, o=A16, ob=64, ot=64, B=1, H=1, G=1, Tq=1, D=64,
+        ctx=100, len=None, len_s=0, base=50, qpos=0, qend=1, cf=0, scale=0.125, part=None, pe=0), **kw}.values())
+    for name in ("q", "kc", "vc", "ks", "vs", "o"):
+        assert sd(**{name: None}) == -6
+    assert sd(D=72) == -1
+    assert sd(B=0) == -2 and sd(G=0) == -2 and sd(Tq=0) == -2 and sd(ctx=0) == -2 and sd(cf=-1) == -2
+    assert sd(Tq=2 ** 30, G=4) == -2 and sd(scale=0.0) == -2 and sd(scale=float("nan")) == -2 and sd(scale=math.inf) == -2
+    assert sd(qt=4) == -2 and sd(ot=2) == -2 and sd(q=A16 + 8) == -4 and sd(o=A16 + 4) == -4 and sd(len=A16 + 2) == -4
+    need = lib.mx_kv8_sdpa_ws(1, 1, 1, 1, 10 ** 6, 64)
+    assert need > 0 and lib.mx_kv8_sdpa_ws(1, 1, 1, 1, 64, 64) == 0 and lib.mx_kv8_sdpa_ws(0, 1, 1, 1, 64, 64) == 0
+    assert sd(ctx=10 ** 6) == -3 and sd(ctx=10 ** 6, part=A16, pe=need - 1) == -3 and sd(ctx=10 ** 6, part=A16 + 4, pe=need) == -3
+
+
+def raises(match, f, *a, **kw):
+    with pytest.raises(ValueError, match=match):
+        f(*a, **kw)
+
+
+def test_python_refusals():
+    x = torch.zeros(3, 64, dtype=BF)
+    raises("bfloat16", ops.quant_mxfp4, x.float())
+    raises("GPU", ops.quant_mxfp4, x)
+    raises("column", ops.quant_mxfp4, torch.zeros(3, 0, dtype=BF))
+    raises("bf16", ops.MxFp4Lin, x, None, torch.float16)
+    w = ops.MxFp4(torch.zeros(1024, dtype=torch.uint8), torch.zeros(256, dtype=torch.uint8), 10, 64)
+    lin = ops.MxFp4Lin.from_quantized(w, None)
+    raises("bias", ops.MxFp4Lin.from_quantized, w, torch.zeros(11))
+    raises("width 32", lin, x[:, :32])
+    raises("gated", lin, x, act="glu")
+    raises("act_from", lin, x, act_from=-1)
+    raises("float32", lin, x.float())
+    raises("out must", lin, x, out=torch.zeros(3, 9, dtype=BF))
+    raises("residual width", lin, x, res=torch.zeros(3, 9, dtype=BF))
+    raises("residual rows", lin, x, res=torch.zeros(2, 10, dtype=BF))
+    raises("different rows", lin, x, pre=ops.MxFp4(w.codes, w.scales, 4, 64))
+    raises("width 32", lin, None, pre=ops.MxFp4(w.codes, w.scales, 4, 32))
+    raises("GPU", lin, x)
+    raises("out must", w.values, out=torch.zeros(10, 65, dtype=BF))
+    for a in ((0, 1, 8, 64), (1, 1, 0, 64), (1, 1, 8, 72)):
+        raises("must be positive", ops.KV8Cache, *a, device="cpu")
+    c = ops.KV8Cache(2, 2, 100, 64, device="cpu")
+    k = torch.zeros(2, 2, 5, 64, dtype=BF)
+    i = lambda *v: torch.tensor(v, dtype=torch.int32)
+    raises("k, v must", c.append, k, k[:, :, :4])
+    raises("k, v must", c.append, k[:, :1], k[:, :1])
+    raises("sequences", c.append, k, k, bcast=True)
+    raises("sequences", c.append, k.repeat(2, 1, 1, 1), k.repeat(2, 1, 1, 1))
+    raises("outside", c.append, k, k, 96)
+    raises("outside", c.append, k, k, -1)
+    raises("2 values", c.append, k, k, i(1))
+    raises("int32", c.append, k, k, i(1, 2).long())
+    raises("count", c.append, k, k, count=3)
+    raises("q goes", c.append, k, k, q=k)
+    raises("rotary table", c.append, k, k, 3, cs=torch.zeros(7, 16, 2))
+    raises("cs must", c.append, k, k, 3, cs=torch.zeros(70, 32, 2))
+    raises("q must", c.append, k, k, cs=torch.zeros(100, 16, 2), q=k[:, :, :3])
+    raises("float32", c.append, k.float(), k.float())
+    raises("GPU", c.append, k, k)
+    raises("outside", c.read, 101)
+    q = torch.zeros(2, 4, 3, 64, dtype=BF)
+    raises("does not fit", ops.sdpa_kv8, q[:, :3], c, 5)
+    raises("does not fit", ops.sdpa_kv8, q.repeat(2, 1, 1, 1), c, 5)
+    raises("does not fit", ops.sdpa_kv8, q[..., :32], c, 5)
+    raises("bfloat16", ops.sdpa_kv8, q.half(), c, 5)
+    raises("outside", ops.sdpa_kv8, q, c, 101)
+    raises("2 values", ops.sdpa_kv8, q, c, i(1, 2, 3))
+    raises("positive and finite", ops.sdpa_kv8, q, c, 5, scale=0.0)
+    raises("causal_from", ops.sdpa_kv8, q, c, 5, causal_from=-1)
+    raises("out must", ops.sdpa_kv8, q, c, 5, out=torch.zeros(2, 3, 255, dtype=BF))
+    raises("GPU", ops.sdpa_kv8, q, c, 5)
+    assert c.append(k[:, :, :0], k[:, :, :0], 100) is None and ops.sdpa_kv8(q[:, :, :0], c, 5).shape == (2, 0, 256)
