@@ -65,11 +65,14 @@ __device__ __forceinline__ u32x4 roped8(const uint16_t* row, int c, const float*
 }
 
 // One workgroup per (block, head, slot); with a rotary table, heads H .. H + Hq - 1 of the grid rotate the queries.
-// K: thread = (token, 8 columns). V: thread = (4 tokens, 8 columns), whose codes go out as 8 dwords. The block is put
-// together in LDS and leaves in 16-byte stores; a block that keeps earlier rows is read first.
+// K: thread = (token, 8 columns). V: thread = 4 tokens x D / 16 columns, whose codes are transposed in registers to a dword
+// per column. The block is put together in LDS and leaves in 16-byte stores; a block that keeps earlier rows is read
+// first, together with the new rows (every load is issued before the first is used). The bound is HBM for long prompts
+// (4 sequences x 8001 rows x 8 heads x 128), and for single rows the chain position -> rows -> maximum -> stores.
 template <int D, bool ROPE>
 __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs p) {
-  constexpr int CPR = D / 8, NC = 64 * CPR / 256;  // chunks of 8 columns per row, per thread
+  constexpr int CPR = D / 8, NC = 64 * CPR / 256;   // K: chunks of 8 columns per row, per thread
+  constexpr int VC = D / 16, NO = 64 * D / 16 / 256;  // V: columns per thread; 16-byte pieces of the block per thread
   __shared__ __attribute__((aligned(16))) uint8_t kb[64 * D], vb[64 * D];
   __shared__ uint32_t red[2][4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -100,8 +103,20 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs p) {
   const uint16_t* kr = p.k + b * p.sk_b + h * p.sk_h + (blk * 64 - pos) * p.sk_t;  // token 0 of the block
   const uint16_t* vr = p.v + b * p.sv_b + h * p.sv_h + (blk * 64 - pos) * p.sv_t;
 
-  u32x4 xk[NC], xv[NC];
+  uint8_t* kg = p.kc + cell * (64 * D);
+  uint8_t* vg = p.vc + cell * (64 * D);
+  const bool part = t_lo > 0 || t_hi < 64;  // the block keeps some of its bytes
+  u32x4 xk[NC], ok[NO], ov[NO];
+  uint32_t xv[4][VC / 2];
   uint32_t mk = 0, mv = 0;
+  const int vq = 4 * (tid / 16), vcol = VC * (tid % 16);
+  const int bk0 = p.ks[cell], bv0 = p.vs[cell];
+  if (part)
+#pragma unroll
+    for (int i = 0; i < NO; i++) {
+      ok[i] = *reinterpret_cast<const u32x4*>(kg + 16 * (tid + 256 * i));
+      ov[i] = *reinterpret_cast<const u32x4*>(vg + 16 * (tid + 256 * i));
+    }
 #pragma unroll
   for (int i = 0; i < NC; i++) {
     const int c = tid + 256 * i, t = c / CPR, cc = c % CPR;
@@ -112,23 +127,40 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs p) {
       else
         xk[i] = ld8(kr + (long)t * p.sk_t + 8 * cc, p.vec);
     }
-    // V: chunk column cc of tokens 4 tq + i4; NC chunks per thread = NC tokens of a quad (D = 128) or half of one (D = 64)
-    const int tv = D == 128 ? 4 * (tid / CPR) + i : 4 * (tid / 16) + 2 * ((tid >> 3) & 1) + i, cv = tid % CPR;
-    xv[i] = u32x4{0u, 0u, 0u, 0u};
-    if (tv >= t_lo && tv < t_hi) xv[i] = ld8(vr + (long)tv * p.sv_t + 8 * cv, p.vec);
+  }
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      mk = max(mk, amax_fin(xk[i][e]));
-      mv = max(mv, amax_fin(xv[i][e]));
+  for (int i = 0; i < 4; i++) {
+    const int t = vq + i;
+    const uint16_t* row = vr + (long)t * p.sv_t + vcol;
+#pragma unroll
+    for (int e = 0; e < VC / 2; e++) xv[i][e] = 0;
+    if (t >= t_lo && t < t_hi) {
+      if constexpr (VC == 8) {
+        const u32x4 v = ld8(row, p.vec);
+#pragma unroll
+        for (int e = 0; e < 4; e++) xv[i][e] = v[e];
+      } else if (p.vec) {
+        const u32x2 v = *reinterpret_cast<const u32x2*>(row);
+        xv[i][0] = v.x, xv[i][1] = v.y;
+      } else {
+        xv[i][0] = (uint32_t)row[0] | (uint32_t)row[1] << 16, xv[i][1] = (uint32_t)row[2] | (uint32_t)row[3] << 16;
+      }
     }
   }
+#pragma unroll
+  for (int i = 0; i < NC; i++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) mk = max(mk, amax_fin(xk[i][e]));
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+#pragma unroll
+    for (int e = 0; e < VC / 2; e++) mv = max(mv, amax_fin(xv[i][e]));
   mk = (uint32_t)wave_max((float)mk);  // exact: below 2^15
   mv = (uint32_t)wave_max((float)mv);
   if (lane == 0) {
     red[0][wave] = mk;
     red[1][wave] = mv;
   }
-  const int bk0 = p.ks[cell], bv0 = p.vs[cell];
   __syncthreads();
   int bk = kv8_scale_byte(max(max(red[0][0], red[0][1]), max(red[0][2], red[0][3])));
   int bv = kv8_scale_byte(max(max(red[1][0], red[1][1]), max(red[1][2], red[1][3])));
@@ -136,14 +168,12 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs p) {
     bk = max(bk, bk0);
     bv = max(bv, bv0);
   }
-  uint8_t* kg = p.kc + cell * (64 * D);
-  uint8_t* vg = p.vc + cell * (64 * D);
-  if (t_lo > 0 || t_hi < 64) {  // keep what is there, rounded to the block's new exponent before the new rows
+  if (part) {  // keep what is there, rounded to the block's new exponent before the new rows
     const float fk = bk > bk0 ? inv_pow2(min(127 + bk - bk0, 254)) : 1.f, fv = bv > bv0 ? inv_pow2(min(127 + bv - bv0, 254)) : 1.f;
 #pragma unroll
-    for (int i = 0; i < 64 * D / 16 / 256; i++) {
+    for (int i = 0; i < NO; i++) {
       const int c = tid + 256 * i, l = c & 31, hh = (c >> 5) & 1, grp = c >> 6;
-      u32x4 a = *reinterpret_cast<const u32x4*>(kg + 16 * c), w = *reinterpret_cast<const u32x4*>(vg + 16 * c);
+      u32x4 a = ok[i], w = ov[i];
       if (bk > bk0 && (grp / (D / 32)) * 32 + l < t_lo)
 #pragma unroll
         for (int e = 0; e < 4; e++) a[e] = requant4(a[e], fk);
@@ -167,16 +197,31 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs p) {
     if (t >= t_lo && t < t_hi)
       *reinterpret_cast<u32x2*>(kb + kv8_koff<D>(t, 8 * cc)) =
           u32x2{code4(xk[i][0], xk[i][1], fk), code4(xk[i][2], xk[i][3], fk)};
-    const int tv = D == 128 ? 4 * (tid / CPR) + i : 4 * (tid / 16) + 2 * ((tid >> 3) & 1) + i, cv = tid % CPR;
-    if (tv >= t_lo && tv < t_hi) {
-      const uint32_t c0 = code4(xv[i][0], xv[i][1], fv), c1 = code4(xv[i][2], xv[i][3], fv);
+  }
 #pragma unroll
-      for (int e = 0; e < 8; e++) vb[kv8_voff(tv, 8 * cv + e)] = (uint8_t)((e < 4 ? c0 : c1) >> (8 * (e & 3)));
+  for (int e = 0; e < VC; e += 4) {  // 4 tokens x 4 columns
+    uint32_t c[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) c[i] = code4(xv[i][e / 2], xv[i][e / 2 + 1], fv);
+    const uint32_t a0 = __builtin_amdgcn_perm(c[1], c[0], 0x05010400u), a1 = __builtin_amdgcn_perm(c[3], c[2], 0x05010400u);
+    const uint32_t b0 = __builtin_amdgcn_perm(c[1], c[0], 0x07030602u), b1 = __builtin_amdgcn_perm(c[3], c[2], 0x07030602u);
+    const uint32_t t[4] = {__builtin_amdgcn_perm(a1, a0, 0x05040100u), __builtin_amdgcn_perm(a1, a0, 0x07060302u),
+                           __builtin_amdgcn_perm(b1, b0, 0x05040100u), __builtin_amdgcn_perm(b1, b0, 0x07060302u)};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      uint8_t* o = vb + kv8_voff(vq, vcol + e + j);
+      if (vq >= t_lo && vq + 4 <= t_hi) {
+        *reinterpret_cast<uint32_t*>(o) = t[j];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (vq + i >= t_lo && vq + i < t_hi) o[i] = (uint8_t)(t[j] >> (8 * i));
+      }
     }
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 64 * D / 16 / 256; i++) {
+  for (int i = 0; i < NO; i++) {
     const int c = 16 * (tid + 256 * i);
     *reinterpret_cast<u32x4*>(kg + c) = *reinterpret_cast<const u32x4*>(kb + c);
     *reinterpret_cast<u32x4*>(vg + c) = *reinterpret_cast<const u32x4*>(vb + c);

@@ -260,13 +260,17 @@ __global__ __launch_bounds__(64 * NK) void kv8_rows_kernel(Attn8Args p) {
       const bool masked = (blk + 1) * 64 > kall;
       const int key0 = blk * 64 + 32 * (g >> 1) + 4 * (g & 1);
       float mx = -INFINITY;
+      if (masked) {
+        asm volatile("");  // keeps the branch: as selects the mask would be computed for every block
+#pragma unroll
+        for (int tt = 0; tt < 4; tt++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) st[tt][r] = key0 + 8 * tt + r < lim ? st[tt][r] : -INFINITY;
+      }
 #pragma unroll
       for (int tt = 0; tt < 4; tt++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-          if (masked) st[tt][r] = key0 + 8 * tt + r < lim ? st[tt][r] : -INFINITY;
-          mx = fmaxf(mx, st[tt][r]);
-        }
+        for (int r = 0; r < 4; r++) mx = fmaxf(mx, st[tt][r]);
       const int el = block_exponent(quarters_max(mx) * p.sl2), mn = max(m, el);
       if (__any(mn != m)) {
         const float al = __builtin_amdgcn_ldexpf(1.f, m - mn);
@@ -477,6 +481,7 @@ __global__ __launch_bounds__(64 * NQW * NKW, 2) void kv8_tile_kernel(Attn8Args p
     const int key0 = blk * 64 + 4 * hk;
     float mx = -INFINITY;
     if (masked) {
+      asm volatile("");  // keeps the branch: as selects the mask would cost every block 100 instructions
 #pragma unroll
       for (int t = 0; t < 2; t++)
 #pragma unroll

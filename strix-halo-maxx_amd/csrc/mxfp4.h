@@ -1,27 +1,35 @@
 // MXFP4 operands of this library: 4-bit e2m1 codes with one power-of-two scale (E8M0 byte: exponent + 127, 255 = NaN)
-// for each block of 32 along a row, stored in the order the 16x16x128 scaled MFMA reads them.
-//  * codes: tiles of 16 rows x 128 columns, 1 KB each, tile (rt, kt) at (rt * nkt + kt) * 1024. Within a tile the 16 bytes
-//    of lane l are row (l & 15), columns 32 (l >> 4) .. + 31, the even column in the low nibble: one tile is one operand,
-//    read by one 16-byte load per lane from 1 KB in a row, also after a linear copy to LDS (no bank conflicts, no swizzle).
-//  * scales: one dword per lane and four tiles along the row, tile kt in byte kt & 3, at ((rt * nks + kt / 4) * 64 + l) * 4:
-//    one register serves four MFMAs, which pick their byte.
-// Rows past the last one and columns past K have code 0 and scale byte 0.
+// for each block of 32 along a row, stored in the order the 32x32x64 scaled MFMA reads them.
+//  * codes: tiles of 32 rows x 64 columns, 1 KB each, tile (rt, kt) at (rt * nkt + kt) * 1024, nkt even. Within a tile the
+//    16 bytes of lane l are row (l & 31), columns 32 (l >> 5) .. + 31, the even column in the low nibble: one tile is one
+//    operand, read by one 16-byte load per lane from 1 KB in a row, also after a linear copy to LDS (no bank conflicts, no
+//    swizzle).
+//  * scales: one dword per lane for two tiles along the row (128 columns) of two row tiles (64 rows), tile (rt, kt) in
+//    byte 2 (rt & 1) + (kt & 1), at ((rt / 2 * (nkt / 2) + kt / 2) * 64 + l) * 4.
+// Columns past K of a row have code 0 and scale byte 0; rows past the last one are not written (they meet no result that
+// is stored).
 #pragma once
 #include "common.h"
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-__host__ __device__ __forceinline__ int mx4_nkt(int K) { return (K + 127) / 128; }
-__host__ __device__ __forceinline__ int mx4_nks(int K) { return (mx4_nkt(K) + 3) / 4; }
-__host__ __device__ __forceinline__ long mx4_rt(long M) { return (M + 15) / 16; }
+__host__ __device__ __forceinline__ int mx4_nk(int K) { return (K + 127) / 128; }       // steps of 128 columns
+__host__ __device__ __forceinline__ int mx4_nkt(int K) { return 2 * mx4_nk(K); }        // tiles along a row
+__host__ __device__ __forceinline__ long mx4_groups(long M) { return (M + 63) / 64; }   // groups of 64 rows
 
-// D += A B^T over 128 columns of one 16-row tile each; byte B of the scale registers. Lane l: D column (l & 15) (the row
-// of b), D rows 4 (l >> 4) + r (the rows of a).
-template <int BYTE>
+__device__ __forceinline__ i32x8 mx4_operand(u32x4 v) {
+  return i32x8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
+}
+// D += A B^T on 4-bit operands, byte SA / SB of the scale registers.
+// 32x32x64: one tile each. Lane l: D column (l & 31) (the row of b), D rows 8 (r / 4) + 4 (l >> 5) + r % 4 (rows of a).
+template <int SA, int SB>
+__device__ __forceinline__ f32x16 mfma_mx4(u32x4 a, u32x4 b, f32x16 c, int sa, int sb) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx4_operand(a), mx4_operand(b), c, 4, 4, SA, sa, SB, sb);
+}
+// 16x16x128: lane l gives row (l & 15), columns 32 (l >> 4) .. + 31 and their scale. D column (l & 15), rows
+// 4 (l >> 4) + r.
 __device__ __forceinline__ f32x4 mfma_mx4(u32x4 a, u32x4 b, f32x4 c, int sa, int sb) {
-  const i32x8 A = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
-  const i32x8 B = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, c, 4, 4, BYTE, sa, BYTE, sb);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx4_operand(a), mx4_operand(b), c, 4, 4, 0, sa, 0, sb);
 }
 
 // The scale byte of a block whose largest |bf16| has these bits (sign cleared): floor(log2 amax) - 2, at least 2^-127

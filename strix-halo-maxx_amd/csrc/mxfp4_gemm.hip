@@ -1,11 +1,15 @@
 // MXFP4 Linear: C[m, n] = act(sum_k Xq[m, k] Wq[n, k] + b[n]) + R[m, n], both operands in MXFP4 (mxfp4.h), on the
-// 16x16x128 scaled MFMA, which multiplies every block's product by both scales itself. The sum, the bias, the activation
+// scaled MFMA, which multiplies every block's product by both scales itself. The sum, the bias, the activation
 // and the residual stay in fp32; the one rounding is the store to bf16.
 #include "mxfp4.h"
 
+#include <algorithm>
 #include <type_traits>
+#include <utility>
 
 namespace {
+
+constexpr int GEMV_ROWS = 8;  // rows that the bf16 form takes
 
 struct Mx4Epi {
   const float* bias;
@@ -52,7 +56,7 @@ __device__ __forceinline__ void mx4_store(const Mx4Epi& p, int m, int n, f32x4 v
 }
 
 // ---------------------------------------------------------------------------------------------- few rows
-// At most 16 MT rows. A workgroup owns 16 columns of C (16 rows of W); its waves take the groups of 512 columns of K in
+// 16 MT rows per workgroup (grid y). It owns 16 columns of C (16 rows of W); its waves take the groups of 512 columns of K in
 // turn (4 KB of W each, read in one piece) and their sums meet in LDS. PRE = false: x arrives in bf16 and each wave
 // quantises the 512 columns it multiplies (its own slice: no wave waits for another before the end).
 template <int NW, int MT, bool PRE, int ACT>
@@ -62,68 +66,87 @@ __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(const uint16_t* __res
                                                            const uint8_t* __restrict__ wc,
                                                            const uint32_t* __restrict__ ws, int K, Mx4Epi p) {
   static_assert(PRE || MT == 1, "bf16 rows come in one tile");
-  __shared__ __attribute__((aligned(16))) uint32_t xq[PRE ? 1 : NW][16][64];  // a row's codes of the wave's 512 columns
-  __shared__ __attribute__((aligned(16))) uint8_t xsc[PRE ? 1 : NW][16][16];  // its scale bytes, [32-block % 4][tile]
+  __shared__ __attribute__((aligned(16))) uint32_t xq[PRE ? 1 : NW][GEMV_ROWS][64];  // a row's codes of the wave's columns
+  __shared__ __attribute__((aligned(16))) uint8_t xsc[PRE ? 1 : NW][GEMV_ROWS][16];  // its scale bytes, [block % 4][step]
   __shared__ f32x4 red[NW][MT][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int nkt = mx4_nkt(K), nks = mx4_nks(K);
+  const int nk = mx4_nk(K), nks = (nk + 3) / 4;
   const long nt = blockIdx.x;
+  const int mt = blockIdx.y * MT;  // first row tile
   const int r16 = lane & 15, g = lane >> 4;
+  // The 16 rows of tile u in the operand order of the 16x16x128 MFMA: half u & 1 of row tile u / 2, lane (r16, g) the 16
+  // bytes of block g & 1 of column tile g / 2; its scale byte 2 ((u / 2) & 1) + g / 2 of dword lane 32 (g & 1) + row.
+  auto codes = [&](const uint8_t* c, long u) {
+    return c + ((u >> 1) * 2 * nk + (g >> 1)) * 1024 + (32 * (g & 1) + 16 * (u & 1) + r16) * 16;
+  };
+  auto scale = [&](const uint32_t* s, long u, int k) {
+    return (int)(s[((u >> 2) * nk + k) * 64 + 32 * (g & 1) + 16 * (u & 1) + r16] >> (16 * ((u >> 1) & 1) + 8 * (g >> 1)));
+  };
   f32x4 acc[MT];
 #pragma unroll
   for (int i = 0; i < MT; i++) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int ks = wave; ks < nks; ks += NW) {
     u32x4 w[4], b[MT][4];
-    const int left = nkt - 4 * ks;
-    const uint8_t* wt = wc + (nt * nkt + 4 * ks) * 1024 + lane * 16;
+    int sw[4], sx[MT][4];
+    const int left = nk - 4 * ks;
+    const uint8_t* wt = codes(wc, nt) + (long)ks * 8192;
 #pragma unroll
     for (int t = 0; t < 4; t++) {
       w[t] = u32x4{0u, 0u, 0u, 0u};
-      if (t < left) w[t] = *reinterpret_cast<const u32x4*>(wt + t * 1024);
+      sw[t] = 0;
+      if (t < left) {
+        w[t] = *reinterpret_cast<const u32x4*>(wt + t * 2048);
+        sw[t] = scale(ws, nt, 4 * ks + t);
+      }
     }
-    const int sw = (int)ws[(nt * nks + ks) * 64 + lane];
-    int sx[MT];
     if constexpr (PRE) {
 #pragma unroll
       for (int i = 0; i < MT; i++) {
-        const uint8_t* xt = xc + ((long)i * nkt + 4 * ks) * 1024 + lane * 16;
-        const bool on = 16 * i < p.M;
+        const uint8_t* xt = codes(xc, mt + i) + (long)ks * 8192;
+        const bool on = 16 * (mt + i) < p.M;
 #pragma unroll
         for (int t = 0; t < 4; t++) {
           b[i][t] = u32x4{0u, 0u, 0u, 0u};
-          if (on && t < left) b[i][t] = *reinterpret_cast<const u32x4*>(xt + t * 1024);
+          sx[i][t] = 0;
+          if (on && t < left) {
+            b[i][t] = *reinterpret_cast<const u32x4*>(xt + t * 2048);
+            sx[i][t] = scale(xs, mt + i, 4 * ks + t);
+          }
         }
-        sx[i] = on ? (int)xs[((long)i * nks + ks) * 64 + lane] : 0;
       }
     } else {
       const int blk = lane >> 2, k = ks * 512 + lane * 8;
-      for (int m = 0; m < p.M; m++) {
-        u32x4 v = {0u, 0u, 0u, 0u};
-        if (k < K) v = load8(x + m * ldx, k, K, vecx);
-        const uint32_t byte = mx4_scale_byte(quad_max(amax8(v)));
-        xq[wave][m][lane] = byte == 255u ? 0u : mx4_pack8(v, e8m0_float(byte));
+      u32x4 v[GEMV_ROWS];
+#pragma unroll
+      for (int m = 0; m < GEMV_ROWS; m++) {
+        v[m] = u32x4{0u, 0u, 0u, 0u};
+        if (m < p.M && k < K) v[m] = load8(x + m * ldx, k, K, vecx);
+      }
+#pragma unroll
+      for (int m = 0; m < GEMV_ROWS; m++) {
+        if (m >= p.M) break;
+        const uint32_t byte = mx4_scale_byte(quad_max(amax8(v[m])));
+        xq[wave][m][lane] = byte == 255u ? 0u : mx4_pack8(v[m], e8m0_float(byte));
         if ((lane & 3) == 0) xsc[wave][m][(blk & 3) * 4 + (blk >> 2)] = (uint8_t)byte;
       }
       // the wave reads only what it wrote: in order, once its LDS writes are done
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_wave_barrier();
       const bool on = r16 < p.M;
+      const uint32_t s4 = on ? *reinterpret_cast<const uint32_t*>(&xsc[wave][r16][g * 4]) : 0u;
 #pragma unroll
       for (int t = 0; t < 4; t++) {
         b[0][t] = u32x4{0u, 0u, 0u, 0u};
         if (on) b[0][t] = *reinterpret_cast<const u32x4*>(&xq[wave][r16][(4 * t + g) * 4]);
+        sx[0][t] = (int)(s4 >> (8 * t));
       }
-      sx[0] = on ? *reinterpret_cast<const int*>(&xsc[wave][r16][g * 4]) : 0;
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_wave_barrier();
     }
 #pragma unroll
-    for (int i = 0; i < MT; i++) {
-      acc[i] = mfma_mx4<0>(w[0], b[i][0], acc[i], sw, sx[i]);
-      acc[i] = mfma_mx4<1>(w[1], b[i][1], acc[i], sw, sx[i]);
-      acc[i] = mfma_mx4<2>(w[2], b[i][2], acc[i], sw, sx[i]);
-      acc[i] = mfma_mx4<3>(w[3], b[i][3], acc[i], sw, sx[i]);
-    }
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+      for (int i = 0; i < MT; i++) acc[i] = mfma_mx4(w[t], b[i][t], acc[i], sw[t], sx[i][t]);
   }
 #pragma unroll
   for (int i = 0; i < MT; i++) red[wave][i][lane] = acc[i];
@@ -132,62 +155,339 @@ __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(const uint16_t* __res
     f32x4 s = red[0][i][lane];
 #pragma unroll
     for (int u = 1; u < NW; u++) s += red[u][i][lane];
-    mx4_store<ACT>(p, 16 * i + r16, (int)nt * 16 + 4 * g, s);
+    mx4_store<ACT>(p, 16 * (mt + i) + r16, (int)nt * 16 + 4 * g, s);
   }
 }
 
 // ---------------------------------------------------------------------------------------------- tiles
-// 128 x 128 tiles, 4 waves of 64 x 64, operands straight from memory.
-template <int ACT>
-__global__ __launch_bounds__(256) void mx4_tile_kernel(const uint8_t* __restrict__ xc, const uint32_t* __restrict__ xs,
-                                                       const uint8_t* __restrict__ wc, const uint32_t* __restrict__ ws,
-                                                       int K, Mx4Epi p, int tiles_n) {
+// 64 lanes x 16 bytes through a buffer resource (byte offset per lane; lanes outside the resource read zeros) into LDS at
+// lds + LO + 16 * lane.
+template <int LO>
+__device__ __forceinline__ void dma16r(u32x4 rsrc, uint32_t voff, uint32_t lds) {
+  asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "s"(lds),
+               "n"(LO)
+               : "memory", "m0", "scc");
+}
+__device__ __forceinline__ u32x4 resource(const void* base, long bytes) {
+  const uint64_t u = (uint64_t)(uintptr_t)base;
+  return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)u),
+               (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(u >> 32) & 0xffffu),
+               (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(bytes < 0x7ffffff0L ? bytes : 0x7ffffff0L)), 0x00020000u};
+}
+
+// 64 FB rows of x against 64 FA rows of W per tile, 4 waves (2 x 2), each 32 FB x 32 FA of it in registers; persistent
+// workgroups. A step is 128 columns: two column tiles of every row tile and one dword of scales per 64 rows. The LDS ring
+// holds S steps, copied by the asynchronous LDS-DMA load, across the end of a tile into the next one. Two sets of operand
+// registers take turns, one multiplied while the other is read. Between the two halves of a step lies its only barrier:
+// the next step has landed, and this one's slot, all read, is refilled. The loop has no branch around its products (the
+// compiler would move them over it, to the end): the loads' tile changes by selection.
+template <int FA, int FB, int S, int GM, int ACT, bool VEC>
+__global__ __launch_bounds__(256, FA * FB > 8 ? 1 : 2) void mx4_ring_kernel(const uint8_t* __restrict__ xc,
+                                                                          const uint8_t* __restrict__ xs,
+                                                                          const uint8_t* __restrict__ wc,
+                                                                          const uint8_t* __restrict__ ws, int K, Mx4Epi p,
+                                                                          int tiles_m, int tiles_n) {
+  constexpr int XB = FB * 4096, WB = FA * 4096;  // a step's codes
+  constexpr int SI = (FA + FB + 3) / 4;          // load instructions of scales: 4 groups each, one by each of SI waves
+  constexpr int STG = XB + WB + SI * 1024;
+  constexpr int LPS = FA + FB;                   // load instructions of codes per wave and step
+  constexpr int NST = VEC ? 2 * FA * FB : 0;
+  constexpr int GA = (FA + 1) / 2, GB = (FB + 1) / 2;  // scale registers
+  static_assert((S - 2) * (LPS + 1) + NST <= 63 && S * STG + 2048 <= 160 * 1024 && FA <= 4, "schedule");
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[S * STG + 2048];  // the ring, two bias rows
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int nkt = mx4_nkt(K), nks = mx4_nks(K);
-  const int m0 = (blockIdx.x / tiles_n) * 128 + (wave & 1) * 64, n0 = (blockIdx.x % tiles_n) * 128 + (wave >> 1) * 64;
-  const int mrt = (p.M + 15) / 16 - 1, nrt = (p.N + 15) / 16 - 1;  // last row tiles
-  long xr[4], wr[4];
+  const int wm = wave & 1, wn = wave >> 1;
+  const uint32_t sbase = lds_off(smem);
+  const int nk = mx4_nk(K);  // > S (the caller)
+  const int mrt = (p.M + 31) / 32, nrt = (p.N + 31) / 32;
+
+  // this workgroup's tiles: XCD x (= block % 8) owns a contiguous run of the tile sequence, its workgroups take the
+  // run's tiles in turn
+  const int nt = tiles_m * tiles_n, nx = min(8, (int)gridDim.x);
+  const int xcd = blockIdx.x % nx, stride = ((int)gridDim.x - xcd + nx - 1) / nx;
+  const int per = nt / nx, rem = nt % nx;
+  const int run0 = xcd * per + min(xcd, rem), run1 = run0 + per + (xcd < rem ? 1 : 0);
+  const int t0 = run0 + (int)blockIdx.x / nx;
+  if (t0 >= run1) return;
+  auto origin = [&](int t, int& mt, int& ntl) {  // row groups of GM tiles, column-major inside a group
+    const int grp = t / (GM * tiles_n), first = grp * GM, gs = min(tiles_m - first, GM);
+    const int r = t - grp * GM * tiles_n;
+    mt = first + r % gs;
+    ntl = r / gs;
+  };
+
+  // ---- what is loaded next: step pk of the tile that rx, rw, psc describe; n*: the tile after it (past the last tile it
+  // repeats that tile: the loads keep the counts of the waits true)
+  struct Src {
+    u32x4 x, w;
+    const uint8_t* sc;  // this lane's 16 bytes of scales of the tile's first step
+  };
+  const int piece = min(min(wave, SI - 1) * 4 + (lane >> 4), FA + FB - 1);
+  auto aim = [&](int t) {
+    int mt, ntl;
+    origin(t, mt, ntl);
+    Src s;
+    s.x = resource(xc + (long)mt * (2 * FB) * nk * 2048, (long)(mrt - mt * 2 * FB) * nk * 2048);
+    s.w = resource(wc + (long)ntl * (2 * FA) * nk * 2048, (long)(nrt - ntl * 2 * FA) * nk * 2048);
+    const bool isx = piece < FB;
+    const long grp = isx ? min((long)mt * FB + piece, (mrt - 1L) / 2) : min((long)ntl * FA + piece - FB, (nrt - 1L) / 2);
+    s.sc = (isx ? xs : ws) + grp * nk * 256 + (lane & 15) * 16;
+    return s;
+  };
+  Src src = aim(t0), nxt = aim(min(t0 + stride, run1 - 1));
+  int pk = 0;
+  uint32_t pdst = sbase;
+  const uint32_t rs = (uint32_t)nk * 2048;  // a row tile's codes
+  // instruction q = wave F + e of an operand: 1 KB, column tile q & 1 of row tile q / 2
+  const uint32_t vx = lane * 16 + (wave * FB / 2) * rs + (wave * FB % 2) * 1024;
+  const uint32_t vw = lane * 16 + (wave * FA / 2) * rs + (wave * FA % 2) * 1024;
+  auto load = [&](auto ec) {
+    constexpr int e = decltype(ec)::value, f = e < FB ? FB : FA, i = e < FB ? e : e - FB;
+    // the wave's first instruction may be the second half of a row tile (odd f)
+    const uint32_t step = f % 2 == 0 ? (i / 2) * rs + (i % 2) * 1024
+                                     : (uint32_t)((wave * f + i) / 2 - wave * f / 2) * rs + (uint32_t)((wave * f + i) % 2 - wave * f % 2) * 1024;
+    dma16r<e < FB ? 0 : XB>(e < FB ? src.x : src.w, (e < FB ? vx : vw) + (uint32_t)pk * 2048 + step, pdst + (wave * f + i) * 1024);
+  };
+  auto load_scales = [&]() {  // every wave (one count for the waits): those past SI repeat the last
+    dma16(src.sc + (long)pk * 256, pdst + XB + WB + min(wave, SI - 1) * 1024);
+  };
+  auto next = [&]() {
+    pdst = pdst == sbase + (S - 1) * STG ? sbase : pdst + STG;
+    const bool wrap = ++pk == nk;
+    pk = wrap ? 0 : pk;
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    xr[i] = min(m0 / 16 + i, mrt);
-    wr[i] = min(n0 / 16 + i, nrt);
-  }
-  f32x4 acc[4][4];
-#pragma unroll
-  for (int i = 0; i < 4; i++)
-#pragma unroll
-    for (int j = 0; j < 4; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int ks = 0; ks < nks; ks++) {
-    int sx[4], sw[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      sx[i] = (int)xs[(xr[i] * nks + ks) * 64 + lane];
-      sw[i] = (int)ws[(wr[i] * nks + ks) * 64 + lane];
+    for (int e = 0; e < 4; e++) {
+      src.x[e] = wrap ? nxt.x[e] : src.x[e];
+      src.w[e] = wrap ? nxt.w[e] : src.w[e];
     }
-    auto step = [&](auto tc) {
-      constexpr int t = decltype(tc)::value;
-      if (4 * ks + t >= nkt) return;
-      u32x4 a[4], b[4];
+    src.sc = wrap ? nxt.sc : src.sc;
+  };
+
+  f32x16 acc[FA][FB];
+  u32x4 a[2][FA], b[2][FB];
+  int sa[GA], sb[GB], na[GA], nb[GB];
+  const uint8_t* xb = smem + wm * FB * 2048 + lane * 16;
+  const uint8_t* wb = smem + XB + wn * FA * 2048 + lane * 16;
+  const uint8_t* scb = smem + XB + WB + lane * 4;
+  auto ld = [](const uint8_t* q) { return *reinterpret_cast<const u32x4*>(q); };
+  // scale dwords in the slot at so; a wave with one row tile takes the half of its group that is its own
+  auto scale_a = [&](uint32_t so, int i) {
+    const int v = *reinterpret_cast<const int*>(scb + so + (FB + (FA == 1 ? 0 : wn * GA + i)) * 256);
+    return FA == 1 ? v >> (16 * wn) : v;
+  };
+  auto scale_b = [&](uint32_t so, int j) {
+    const int v = *reinterpret_cast<const int*>(scb + so + (FB == 1 ? 0 : wm * GB + j) * 256);
+    return FB == 1 ? v >> (16 * wm) : v;
+  };
+  static_assert(FA == 1 || FA % 2 == 0, "a wave's rows of W start with a scale group");
+  static_assert(FB == 1 || FB % 2 == 0, "a wave's rows of x start with a scale group");
+
+  int after = 0;     // waits left whose counts include the write-out's stores
+  uint32_t cur = 0;  // slot of the step being multiplied
+  auto step = [&](auto firstc) {  // FIRST: the sums start at 0
+    constexpr bool FIRST = decltype(firstc)::value;
+    constexpr int NM = FA * FB;
+    // ---- first half: set 0, while set 1 is read
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        b[i] = *reinterpret_cast<const u32x4*>(xc + (xr[i] * nkt + 4 * ks + t) * 1024 + lane * 16);
-        a[i] = *reinterpret_cast<const u32x4*>(wc + (wr[i] * nkt + 4 * ks + t) * 1024 + lane * 16);
+    for (int i = 0; i < FA; i++)
+#pragma unroll
+      for (int j = 0; j < FB; j++) {
+        f32x16 z = acc[i][j];
+        if (FIRST)
+#pragma unroll
+          for (int e = 0; e < 16; e++) z[e] = 0.f;
+        acc[i][j] = (i & 1) ? ((j & 1) ? mfma_mx4<2, 2>(a[0][i], b[0][j], z, sa[i / 2], sb[j / 2])
+                                       : mfma_mx4<2, 0>(a[0][i], b[0][j], z, sa[i / 2], sb[j / 2]))
+                            : ((j & 1) ? mfma_mx4<0, 2>(a[0][i], b[0][j], z, sa[i / 2], sb[j / 2])
+                                       : mfma_mx4<0, 0>(a[0][i], b[0][j], z, sa[i / 2], sb[j / 2]));
+        __builtin_amdgcn_sched_barrier(0);
+        if (j == 0) a[1][i] = ld(wb + cur + (2 * i + 1) * 1024);
+        if (i == 0) b[1][j] = ld(xb + cur + (2 * j + 1) * 1024);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    // ---- second half: set 1, while set 0 of the next step is read and the slot refilled
+    if (after > 0) {
+      after--;
+      wait_vm<(S - 2) * (LPS + 1) + NST>();
+    } else {
+      wait_vm<(S - 2) * (LPS + 1)>();
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    cur = cur == (S - 1) * STG ? 0 : cur + STG;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < FA; i++)
+#pragma unroll
+      for (int j = 0; j < FB; j++) {
+        acc[i][j] = (i & 1) ? ((j & 1) ? mfma_mx4<3, 3>(a[1][i], b[1][j], acc[i][j], sa[i / 2], sb[j / 2])
+                                       : mfma_mx4<3, 1>(a[1][i], b[1][j], acc[i][j], sa[i / 2], sb[j / 2]))
+                            : ((j & 1) ? mfma_mx4<1, 3>(a[1][i], b[1][j], acc[i][j], sa[i / 2], sb[j / 2])
+                                       : mfma_mx4<1, 1>(a[1][i], b[1][j], acc[i][j], sa[i / 2], sb[j / 2]));
+        __builtin_amdgcn_sched_barrier(0);
+        if (j == 0) {
+          a[0][i] = ld(wb + cur + 2 * i * 1024);
+          if (i % 2 == 0) na[i / 2] = scale_a(cur, i / 2);
+        }
+        if (i == 0) {
+          b[0][j] = ld(xb + cur + 2 * j * 1024);
+          if (j % 2 == 0) nb[j / 2] = scale_b(cur, j / 2);
+        }
+        if (i + j == 0) load_scales();
+        [&]<int... e>(std::integer_sequence<int, e...>) {
+          ((e * NM / LPS == i * FB + j ? load(std::integral_constant<int, e>{}) : void()), ...);
+        }(std::make_integer_sequence<int, LPS>{});
+        __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
-      for (int j = 0; j < 4; j++)
+    for (int i = 0; i < GA; i++) sa[i] = na[i];
 #pragma unroll
-        for (int i = 0; i < 4; i++) acc[i][j] = mfma_mx4<t>(a[j], b[i], acc[i][j], sw[j], sx[i]);
-    };
-    step(std::integral_constant<int, 0>{});
-    step(std::integral_constant<int, 1>{});
-    step(std::integral_constant<int, 2>{});
-    step(std::integral_constant<int, 3>{});
+    for (int j = 0; j < GB; j++) sb[j] = nb[j];
+    next();
+  };
+
+  // ---- prologue
+#pragma unroll
+  for (int i = 0; i < S; i++) {
+    load_scales();
+    [&]<int... e>(std::integer_sequence<int, e...>) { (load(std::integral_constant<int, e>{}), ...); }
+    (std::make_integer_sequence<int, LPS>{});
+    next();
   }
-  const int r16 = lane & 15, g = lane >> 4;
+  wait_vm<(S - 1) * (LPS + 1)>();
+  __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 4; i++)
+  for (int i = 0; i < FA; i++) a[0][i] = ld(wb + 2 * i * 1024);
 #pragma unroll
-    for (int j = 0; j < 4; j++) mx4_store<ACT>(p, m0 + 16 * i + r16, n0 + 16 * j + 4 * g, acc[i][j]);
+  for (int j = 0; j < FB; j++) b[0][j] = ld(xb + 2 * j * 1024);
+#pragma unroll
+  for (int i = 0; i < GA; i++) sa[i] = scale_a(0, i);
+#pragma unroll
+  for (int j = 0; j < GB; j++) sb[j] = scale_b(0, j);
+
+  int brow = 0;
+  for (int t = t0; t < run1; t += stride) {
+    int mt0, nt0;
+    origin(t, mt0, nt0);
+    const int m0 = mt0 * 64 * FB, n0 = nt0 * 64 * FA, mw = wm * FB * 32, nw = wn * FA * 32;
+    if (VEC && p.bias && wave == 0)  // read after nk > S steps, whose waits and barriers cover it
+      dma16s(p.bias, (uint32_t)min(n0 + 4 * lane, p.N - 4) * 4, sbase + S * STG + brow * 1024);
+    step(std::true_type{});
+    for (int k = 1; k < nk; k++) step(std::false_type{});
+    // the loads have gone on to the next tile (nk > S steps ago they were at most S ahead): the one after it
+    nxt = aim(min(t + 2 * stride, run1 - 1));
+
+    int ln = lane;
+    asm volatile("" : "+v"(ln));  // the lane's addresses are computed here, per tile: hoisted they would take registers
+    const int lr = ln & 31, hk = ln >> 5;
+    if constexpr (VEC) {
+      // A lane holds 4 columns in a row at 8 u + 4 hk, the lane 32 further the other 4 of the 8: a swap of halves between u
+      // and u + 1 leaves 8 in a row in every lane. Stores go through a buffer resource, always the same number of them.
+      const long cb = ((long)(p.M - m0 - 1) * p.ldc + p.N - n0) * 2, rb = p.R ? ((long)(p.M - m0 - 1) * p.ldr + p.N - n0) * 2 : 0;
+      const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc(p.C + (long)m0 * p.ldc + n0, (short)0,
+                                                                          (int)(cb < 0x7ffffff0L ? cb : 0x7ffffff0L), 0x00020000);
+      const __amdgpu_buffer_rsrc_t rr = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<uint16_t*>(p.R ? p.R + (long)m0 * p.ldr + n0 : nullptr), (short)0,
+          (int)(rb < 0x7ffffff0L ? rb : 0x7ffffff0L), 0x00020000);
+      // Unit q: row tile q / 2, columns 16 (q & 1) .. + 15. The residuals are loaded units ahead: memory operations finish in
+      // order, so a load behind a unit's stores would wait for them.
+      constexpr int NU = 2 * FA, RD = NU < 4 ? NU : 4;
+      u32x4 res[RD][FB];
+      auto column = [&](int q) { return nw + 32 * (q >> 1) + 16 * (q & 1) + 8 * hk; };  // of the lane's stores
+      auto row = [&](int j) { return mw + 32 * j + lr; };
+      auto fetch = [&](int q) {
+#pragma unroll
+        for (int j = 0; j < FB; j++)
+          res[q % RD][j] = __builtin_bit_cast(
+              u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                         rr, n0 + column(q) < p.N ? (uint32_t)(row(j) * (int)p.ldr + column(q)) * 2 : 0x80000000u, 0, 0));
+      };
+      const uint8_t* brp = smem + S * STG + brow * 1024 + (nw + 4 * hk) * 4;
+      brow ^= 1;
+      if (p.R)
+#pragma unroll
+        for (int q = 0; q < RD - 1; q++) fetch(q);
+#pragma unroll
+      for (int q = 0; q < NU; q++) {
+        if (p.R && q + RD - 1 < NU) fetch(q + RD - 1);
+        f32x4 bias[2];
+#pragma unroll
+        for (int v = 0; v < 2; v++)
+          bias[v] = p.bias ? *reinterpret_cast<const f32x4*>(brp + (32 * (q >> 1) + 16 * (q & 1) + 8 * v) * 4)
+                           : f32x4{0.f, 0.f, 0.f, 0.f};
+        const int i = q >> 1, u = 2 * (q & 1);
+        const bool on = n0 + column(q) < p.N;
+#pragma unroll
+        for (int j = 0; j < FB; j++) {
+          u32x4 r = {0u, 0u, 0u, 0u};
+          if (p.R) {
+            r = res[q % RD][j];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              const auto w = __builtin_amdgcn_permlane32_swap(r[e], r[2 + e], false, false);
+              r[e] = w[0], r[2 + e] = w[1];
+            }
+          }
+          uint32_t o[2][2];
+#pragma unroll
+          for (int v = 0; v < 2; v++) {
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              y[e] = acc[i][j][4 * (u + v) + e] + bias[v][e];
+              if (ACT && n0 + nw + 32 * i + 8 * (u + v) + 4 * hk + e >= p.act_from)
+                y[e] = ACT == 1 ? gelu_tanh(y[e]) : gelu_erf(y[e]);
+              if (p.R) y[e] += (e & 1) ? hi_bf(r[2 * v + (e >> 1)]) : lo_bf(r[2 * v + (e >> 1)]);
+            }
+            o[v][0] = pack2(y[0], y[1]), o[v][1] = pack2(y[2], y[3]);
+          }
+          const auto x = __builtin_amdgcn_permlane32_swap(o[0][0], o[1][0], false, false);
+          const auto z = __builtin_amdgcn_permlane32_swap(o[0][1], o[1][1], false, false);
+          __builtin_amdgcn_raw_buffer_store_b128(u32x4{x[0], z[0], x[1], z[1]}, rc,
+                                                 on ? (uint32_t)(row(j) * (int)p.ldc + column(q)) * 2 : 0x80000000u, 0, 0);
+        }
+      }
+      after = S - 1;
+    } else {
+#pragma unroll
+      for (int i = 0; i < FA; i++)
+#pragma unroll
+        for (int j = 0; j < FB; j++)
+#pragma unroll
+          for (int u = 0; u < 4; u++)
+            mx4_store<ACT>(p, m0 + mw + 32 * j + lr, n0 + nw + 32 * i + 8 * u + 4 * hk,
+                           f32x4{acc[i][j][4 * u], acc[i][j][4 * u + 1], acc[i][j][4 * u + 2], acc[i][j][4 * u + 3]});
+    }
+  }
+  wait_vm<0>();  // the loads past the last tile land before the workgroup's LDS is given away
+}
+
+template <int FA, int FB, int S, int GM>
+hipError_t launch_ring(hipStream_t st, const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, int K,
+                       int act, const Mx4Epi& p) {
+  const long tm = ((long)p.M + 64 * FB - 1) / (64 * FB), tn = ((long)p.N + 64 * FA - 1) / (64 * FA), nt = tm * tn;
+  int dev = 0, cus = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e == hipSuccess) e = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
+  if (e != hipSuccess) return e;
+  constexpr int lds = S * ((FA + FB) * 4096 + (FA + FB + 3) / 4 * 1024) + 2048;
+  const long most = (long)cus * std::min(FA * FB > 8 ? 1 : FA * FB > 4 ? 2 : 3, 160 * 1024 / lds);
+  if (nt > 0x3fffffffL) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)(nt < most ? nt : most));
+  auto go = [&](auto kern) {
+    hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, xc, xs, wc, ws, K, p, (int)tm, (int)tn);
+    return hipGetLastError();
+  };
+  // 16-byte accesses to whole chunks of 8 columns at 32-bit offsets
+  const bool vec = p.N % 8 == 0 && p.ldc % 8 == 0 && !((uintptr_t)p.C & 15) && p.ldc < (1L << 21) && p.r_rows == 0 &&
+                   (!p.R || (p.ldr % 8 == 0 && !((uintptr_t)p.R & 15) && p.ldr < (1L << 21))) && !((uintptr_t)p.bias & 15);
+  if (vec)
+    return act == 0   ? go(mx4_ring_kernel<FA, FB, S, GM, 0, true>)
+           : act == 1 ? go(mx4_ring_kernel<FA, FB, S, GM, 1, true>)
+                      : go(mx4_ring_kernel<FA, FB, S, GM, 2, true>);
+  return act == 0   ? go(mx4_ring_kernel<FA, FB, S, GM, 0, false>)
+         : act == 1 ? go(mx4_ring_kernel<FA, FB, S, GM, 1, false>)
+                    : go(mx4_ring_kernel<FA, FB, S, GM, 2, false>);
 }
 
 int check(const void* wc, const void* ws, const float* bias, const uint16_t* R, long ldr, int r_rows, const uint16_t* C,
@@ -209,13 +509,13 @@ Mx4Epi epi(const float* bias, const uint16_t* R, long ldr, int r_rows, uint16_t*
 template <int MT, bool PRE>
 hipError_t launch_rows(hipStream_t st, const uint16_t* x, long ldx, int vecx, const uint8_t* xc, const uint8_t* xs,
                        const uint8_t* wc, const uint8_t* ws, int K, int act, const Mx4Epi& p) {
-  const dim3 grid((unsigned)((p.N + 15) / 16));
+  const dim3 grid((unsigned)((p.N + 15L) / 16), (unsigned)((p.M + 16L * MT - 1) / (16 * MT)));
   auto go = [&](auto kern, int nw) {
     hipLaunchKernelGGL(kern, grid, dim3(64 * nw), 0, st, x, ldx, vecx, xc, (const uint32_t*)xs, wc, (const uint32_t*)ws, K,
                        p);
     return hipGetLastError();
   };
-  if (mx4_nks(K) <= 4) {
+  if (mx4_nk(K) <= 16) {
     if (act == 0) return go(mx4_rows_kernel<4, MT, PRE, 0>, 4);
     if (act == 1) return go(mx4_rows_kernel<4, MT, PRE, 1>, 4);
     return go(mx4_rows_kernel<4, MT, PRE, 2>, 4);
@@ -228,7 +528,7 @@ hipError_t launch_rows(hipStream_t st, const uint16_t* x, long ldx, int vecx, co
 }  // namespace
 
 // Rows that mx_gemv_mxfp4 takes.
-extern "C" int mx_gemv_mxfp4_rows(void) { return 16; }
+extern "C" int mx_gemv_mxfp4_rows(void) { return GEMV_ROWS; }
 
 extern "C" int mx_gemv_mxfp4(hipStream_t st, const uint16_t* x, long ldx, const uint8_t* wc, const uint8_t* ws,
                              const float* bias, const uint16_t* R, long ldr, int r_rows, uint16_t* C, long ldc, int M,
@@ -236,7 +536,7 @@ extern "C" int mx_gemv_mxfp4(hipStream_t st, const uint16_t* x, long ldx, const 
   if (!x) return MX_ENULL;
   const int rc = check(wc, ws, bias, R, ldr, r_rows, C, ldc, M, N, K, act, act_from);
   if (rc) return rc;
-  if (M > 16 || ldx < 0) return MX_ESHAPE;
+  if (M > GEMV_ROWS || ldx < 0) return MX_ESHAPE;
   if ((uintptr_t)x & 1) return MX_ELAYOUT;
   const int vecx = !((uintptr_t)x & 15) && ldx % 8 == 0;
   const hipError_t e = launch_rows<1, false>(st, x, ldx, vecx, nullptr, nullptr, wc, ws, K, act,
@@ -253,21 +553,36 @@ extern "C" int mx_gemm_mxfp4(hipStream_t st, const uint8_t* xc, const uint8_t* x
   if (((uintptr_t)xc & 15) || ((uintptr_t)xs & 3)) return MX_ELAYOUT;
   const Mx4Epi p = epi(bias, R, ldr, r_rows, C, ldc, M, N, act_from);
   hipError_t e;
+  // Which kernel, by the grid it makes (us on one MI355X; N x K after the rows):
+  //  * the few-row kernel up to 64 rows, and beyond while its grid (16 columns x 64 rows each) is one workgroup per CU, two
+  //    with the 4 waves of K <= 2048: a CU fetches about 20 bytes a clock, so the product of few rows goes as fast as its
+  //    weights are spread. Against 64 x 64 tiles: 64 rows, 2048 x 8192 8.4 / 15.2, 192 rows 15.0 / 15.7; 256 rows, 2048 x
+  //    2048 6.7 / 7.5, 512 rows 10.9 / 7.7;
+  //  * the smallest tile whose grid is at most one workgroup per CU, for the same reason (64 x 64, 64 x 128, 128 x 128,
+  //    128 x 256): 512 rows, 2048 x 2048 7.9 / 9.4 / 10.4 / 14.6; 256 rows, 8192 x 2048 10.5 / 10.0 / 10.8 / 14.7;
+  //  * 128 x 128 below two full rounds of 128 x 256: 4096 rows, 4304 x 1152 30.2 / 26.6 / 22.6 / 25.7;
+  //  * 128 x 256 beyond, for its fewer LDS reads per product: 9477 rows, 8192 x 2048 182 / 142 / 110 / 105; 8192^3 492 /
+  //    380 / 306 / 265.
+  const auto tiles = [&](int bm, int bn) { return ((long)M + bm - 1) / bm * (((long)N + bn - 1) / bn); };
+  const int nk = mx4_nk(K);
+  if (tiles(64, 64) > 0x3fffffffL || nk > (1 << 15)) return MX_ESHAPE;
   if (M <= 16) {
     e = launch_rows<1, true>(st, nullptr, 0, 0, xc, xs, wc, ws, K, act, p);
   } else if (M <= 32) {
     e = launch_rows<2, true>(st, nullptr, 0, 0, xc, xs, wc, ws, K, act, p);
-  } else if (M <= 64) {
+  } else if (M <= 64 || tiles(64, 16) <= (nk <= 16 ? 512 : 256) || nk <= 2) {
+    if (M > 64 * 65535) return MX_ESHAPE;  // (nk <= 2: the tiles' loads run at most one tile ahead, so they need more steps)
     e = launch_rows<4, true>(st, nullptr, 0, 0, xc, xs, wc, ws, K, act, p);
+  } else if (nk <= 4) {
+    e = launch_ring<2, 2, 2, 8>(st, xc, xs, wc, ws, K, act, p);
+  } else if (tiles(64, 64) <= 256) {
+    e = launch_ring<1, 1, 4, 8>(st, xc, xs, wc, ws, K, act, p);
+  } else if (tiles(64, 128) <= 256) {
+    e = launch_ring<2, 1, 4, 8>(st, xc, xs, wc, ws, K, act, p);
+  } else if (tiles(128, 256) < 1024) {
+    e = launch_ring<2, 2, 4, 8>(st, xc, xs, wc, ws, K, act, p);
   } else {
-    const long tm = (M + 127) / 128, tn = (N + 127) / 128;
-    if (tm * tn > 0xffffffL) return MX_ESHAPE;  // 2^32 threads in a grid
-    auto go = [&](auto kern) {
-      hipLaunchKernelGGL(kern, dim3((unsigned)(tm * tn)), dim3(256), 0, st, xc, (const uint32_t*)xs, wc,
-                         (const uint32_t*)ws, K, p, (int)tn);
-      return hipGetLastError();
-    };
-    e = act == 0 ? go(mx4_tile_kernel<0>) : act == 1 ? go(mx4_tile_kernel<1>) : go(mx4_tile_kernel<2>);
+    e = launch_ring<4, 2, 3, 8>(st, xc, xs, wc, ws, K, act, p);
   }
   return e == hipSuccess ? MX_OK : MX_ELAUNCH;
 }

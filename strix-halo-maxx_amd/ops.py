@@ -690,23 +690,42 @@ def _need(t, name, dev, dtype=BF):
         raise ValueError(f"{name} is on {t.device}, not on {dev}")
 
 
-class MxFp4:
-    """A matrix (rows, K) in MXFP4: 4-bit e2m1 codes and a power-of-two scale for each 32 columns of a row, held in the
-    order of the matrix instruction's operands (codes, scales: uint8 buffers of their own layout)."""
+def _rows2(x):
+    """2-D view (M, K) of x with unit column stride (copied if it has another)."""
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
 
-    def __init__(self, codes, scales, rows, K):
-        self.codes, self.scales, self.rows, self.K = codes, scales, rows, K
+
+class MxFp4:
+    """A matrix (rows, K) in MXFP4: 4-bit e2m1 codes and a power-of-two scale for each 32 columns of a row, in one buffer
+    (uint8; the codes, then the scales, each in the order of the matrix instruction's operands)."""
+
+    def __init__(self, data, rows, K):
+        self.data, self.rows, self.K = data, rows, K
+        self.dev = data.device
+
+    @staticmethod
+    def cells(rows, K):
+        """Pieces of 64 rows x 128 columns: 4 KB of codes and 256 bytes of scales each."""
+        return (rows + 63) // 64 * ((K + 127) // 128)
+
+    def ptrs(self):
+        p = self.data.data_ptr()
+        return p, p + MxFp4.cells(self.rows, self.K) * 4096
 
     def values(self, out=None):
         """(rows, K) bf16: the values the codes stand for, exact."""
-        dev = self.codes.device
-        y = out if out is not None else torch.empty(self.rows, self.K, device=dev, dtype=BF)
-        _need(y, "out", dev)
-        if y.shape != (self.rows, self.K) or y.stride(1) != 1:
-            raise ValueError(f"out must be ({self.rows}, {self.K}) with unit column stride")
-        if y.numel():
-            _call_on(dev, "mx_mxfp4_values", self.codes.data_ptr(), self.scales.data_ptr(), y.data_ptr(), y.stride(0),
-                     self.rows, self.K)
+        dev, M, K = self.dev, self.rows, self.K
+        if out is None:
+            y = torch.empty(M, K, device=dev, dtype=BF)
+        else:
+            y = out
+            _need(y, "out", dev)
+            if y.shape != (M, K) or y.stride(1) != 1:
+                raise ValueError(f"out must be ({M}, {K}) with unit column stride")
+        if M:
+            _call_on(dev, "mx_mxfp4_values", *self.ptrs(), y.data_ptr(), y.stride(0), M, K)
         return y
 
 
@@ -716,18 +735,12 @@ def quant_mxfp4(x):
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("x needs at least one column")
     _need(x, "x", x.device)
-    K = x.shape[-1]
-    x2 = x.reshape(-1, K)
-    if x2.stride(1) != 1 and K > 1:
-        x2 = x2.contiguous()
-    M = x2.shape[0]
-    nkt = (K + 127) // 128
-    rt = (M + 15) // 16
-    codes = torch.empty(rt * nkt * 1024, device=x.device, dtype=torch.uint8)
-    scales = torch.empty(rt * ((nkt + 3) // 4) * 256, device=x.device, dtype=torch.uint8)
+    x2 = _rows2(x)
+    M, K = x2.shape
+    q = MxFp4(torch.empty(MxFp4.cells(M, K) * 4352, device=x.device, dtype=torch.uint8), M, K)
     if M:
-        _call_on(x.device, "mx_quant_mxfp4", x2.data_ptr(), x2.stride(0), codes.data_ptr(), scales.data_ptr(), M, K)
-    return MxFp4(codes, scales, M, K)
+        _call_on(x.device, "mx_quant_mxfp4", x2.data_ptr(), x2.stride(0), *q.ptrs(), M, K)
+    return q
 
 
 class MxFp4Lin:
@@ -752,7 +765,7 @@ class MxFp4Lin:
 
     def _set(self, w, bias):
         self.wq, self.N, self.K = w, w.rows, w.K
-        self.dev = w.codes.device
+        self.dev = w.dev
         if self.N < 1:
             raise ValueError("the weight needs at least one row")
         if bias is not None and bias.shape != (self.N,):
@@ -774,46 +787,43 @@ class MxFp4Lin:
             if x.shape[-1] != K:
                 raise ValueError(f"input width {x.shape[-1]} != {K}")
             _need(x, "x", self.dev)
-            x2 = x.reshape(-1, K)
-            if x2.stride(1) != 1 and K > 1:
-                x2 = x2.contiguous()
+            x2 = _rows2(x)
             M = x2.shape[0]
         else:
-            if pre.K != K or pre.codes.device != self.dev:
-                raise ValueError(f"pre: width {pre.K} on {pre.codes.device}, need {K} on {self.dev}")
+            if pre.K != K or pre.dev != self.dev:
+                raise ValueError(f"pre: width {pre.K} on {pre.dev}, need {K} on {self.dev}")
             M = pre.rows
             if x is not None and x.numel() != M * x.shape[-1]:
                 raise ValueError("x and pre have different rows")
-        y = out if out is not None else torch.empty(M, N, device=self.dev, dtype=BF)
-        y2 = y if y.dim() == 2 else y.view(-1, N)
-        if y2.shape != (M, N) or (y2.stride(1) != 1 and N > 1):
-            raise ValueError(f"out must be ({M}, {N}) with unit column stride")
-        _need(y2, "out", self.dev)
+        if out is None:
+            y = y2 = torch.empty(M, N, device=self.dev, dtype=BF)
+        else:
+            y = out
+            _need(y, "out", self.dev)
+            y2 = y if y.dim() == 2 else y.view(-1, N)
+            if y2.shape != (M, N) or (y2.stride(1) != 1 and N > 1):
+                raise ValueError(f"out must be ({M}, {N}) with unit column stride")
         r2, r_rows, ldr = None, 0, 0
         if res is not None:
             _need(res, "res", self.dev)
             if res.shape[-1] != N:
                 raise ValueError(f"residual width {res.shape[-1]} != {N}")
-            r2 = res.reshape(-1, N)
-            if r2.stride(1) != 1 and N > 1:
-                r2 = r2.contiguous()
+            r2 = _rows2(res)
             ldr = r2.stride(0)
             if r2.shape[0] != M:
                 if not r2.shape[0] or M % r2.shape[0]:
                     raise ValueError("residual rows must equal or divide the output rows")
                 r_rows = r2.shape[0]
         if M:
-            w = self.wq
-            tail = (w.codes.data_ptr(), w.scales.data_ptr(), ptr(self.b), ptr(r2), ldr, r_rows, y2.data_ptr(),
-                    y2.stride(0), M, N, K, a, act_from)
+            tail = (*self.wq.ptrs(), ptr(self.b), ptr(r2), ldr, r_rows, y2.data_ptr(), y2.stride(0), M, N, K, a, act_from)
             if pre is None and M <= self.rows:
                 _call_on(self.dev, "mx_gemv_mxfp4", x2.data_ptr(), x2.stride(0), *tail)
             else:
                 q = quant_mxfp4(x2) if pre is None else pre
-                _call_on(self.dev, "mx_gemm_mxfp4", q.codes.data_ptr(), q.scales.data_ptr(), *tail)
-        if out is not None:
+                _call_on(self.dev, "mx_gemm_mxfp4", *q.ptrs(), *tail)
+        if out is not None or x is None or x.dim() == 2:
             return y
-        return y2 if x is None else y2.view(*x.shape[:-1], N)
+        return y.view(*x.shape[:-1], N)
 
 
 def _where(v, B, dev, name):

@@ -77,6 +77,8 @@ def close(y, ref, mag, act=None):
 SHAPES = [(1, 1, 1), (1, 8192, 2048), (1, 2048, 8192), (2, 100, 4304), (7, 37, 100), (16, 64, 129), (17, 768, 768),
           (33, 130, 1000), (64, 260, 512), (65, 129, 640), (128, 128, 128), (130, 259, 1152), (300, 1000, 385),
           (520, 516, 2304)]
+# more tiles than workgroups, in every remainder of the four steps that share a scale register, ragged and whole edges
+LARGE = [(2100, 4304, 128), (1800, 5000, 257), (2600, 3333, 384), (1500, 6144, 513), (2049, 4100, 1152)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -95,6 +97,20 @@ def test_linear(dev, M, N, K):
     close(lin(xd, gelu=True, res=rd, act_from=f).cpu(), *ol.mxfp4_linear(x, w, b, "tanh", r, f), act="tanh")
     # quantised beforehand: the same codes, another order of the sum at most
     close(lin(None, pre=lin.quant(xd)).cpu(), *ol.mxfp4_linear(x, w, b))
+
+
+@pytest.mark.parametrize("M,N,K", LARGE)
+def test_linear_many_tiles(dev, M, N, K):
+    """Against the fp32 product of the quantised values (exact products; its sum's error is covered like the kernel's)."""
+    g = torch.Generator(device=dev).manual_seed(M)
+    x, w = torch.randn(M, K, generator=g, device=dev).to(BF), torch.randn(N, K, generator=g, device=dev).to(BF)
+    b, r = torch.randn(N, generator=g, device=dev).to(BF), torch.randn(M, N, generator=g, device=dev).to(BF)
+    lin = ops.MxFp4Lin(w, b, device=dev)
+    xq, wq = lin.quant(x).values().float(), lin.wq.values().float()
+    y = torch.matmul(xq, wq.t().contiguous()) + b.float()
+    mag = torch.matmul(xq.abs(), wq.t().abs().contiguous()) + b.float().abs()
+    close(lin(x), y.double(), mag.double())
+    close(lin(x, res=r, act="tanh"), ol.gelu(y.double(), "tanh") + r.double(), mag.double(), act="tanh")
 
 
 def test_linear_views_and_leading_dims(dev):
