@@ -8,6 +8,9 @@ yes/no logits off one prefill, md2fast.py:10-11); the greedy loop here is the de
 rebuilt for batch-1 HBM streaming:
   * per layer 3 kernels: LN fused into the [qkv | fc1] GEMV, rope + KV append fused into split-KV attention, and
     the fc2 / proj GEMVs fused with the two residual adds;
+  * in fewer bits: `mxfp4` runs the layers' Linears in MXFP4, `kv8` keeps the K/V cache in 8 bits; each works with every
+    form of the other, in prefill, query and decode (a decode step then goes operator by operator, 4 to 7 launches a
+    layer, still one HIP graph);
   * the LM head GEMV carries the argmax, and the next step's embedding lookup reduces it on the device, so one HIP
     graph replays a whole step with the token and position kept in device memory (no host round trip per token).
 The yes/no query is the reference's own fast path (FastMD2._encode / _query / decide, md2fast.py:201-212, 266-279):
@@ -29,13 +32,21 @@ BOS = 50256  # moondream2's tokenizer bos_id (the Phi / GPT-2 <|endoftext|> id)
 
 class TextDecoder:
     def __init__(self, weights, lin_cls=ops.MxLin, device="cuda", ctx=1024, attn_splits=1, w8a8=False, nq=1, L=32,
-                 yes_ids=(), no_ids=()):
+                 yes_ids=(), no_ids=(), mxfp4=False, kv8=False):
         """w8a8: the four text Linears of every layer run the reference's W8A8 path (its default text linear class,
         HI8Lin, moondream/gpu/bench.py:20) in prefill and decode; the LM head stays bf16 (md2fast.py:115).
         nq, L: questions per query and tokens per question (the reference's NQ, L, md2fast.py:71-86); the KV cache
         holds nq slots (decode uses slot 0). yes_ids / no_ids: the token ids the yes/no head keeps (the reference
-        derives them from its tokenizer, md2fast.py:138-142; there is no tokenizer here, the caller passes them)."""
+        derives them from its tokenizer, md2fast.py:138-142; there is no tokenizer here, the caller passes them).
+        mxfp4 (or lin_cls=ops.MxFp4Lin): the four text Linears in MXFP4, weights and activations; the LM head stays bf16.
+        kv8: the cache as ops.KV8Cache, one per layer (self.kv), in place of the bf16 kc / vc."""
         c = TXT
+        mxfp4 = mxfp4 or lin_cls is ops.MxFp4Lin
+        if mxfp4 and w8a8:
+            raise ValueError("the Linears are either W8A8 or MXFP4")
+        if mxfp4 and lin_cls not in (ops.MxLin, ops.MxFp4Lin):
+            raise ValueError("mxfp4 chooses the Linear class itself")
+        self.mxfp4, self.kv8 = mxfp4, kv8
         self.dev = torch.device(device)
         self.D, self.H, self.hd, self.eps = c["dim"], c["heads"], c["hd"], c["ln_eps"]
         self.ctx = ctx
@@ -68,6 +79,11 @@ class TextDecoder:
                            fc2=ops.MxI8Lin(weights[p + "mlp.fc2.weight"], weights[p + "mlp.fc2.bias"], BF, dev))
                 blk["wp"], blk["swp"] = blk["proj"].wq, blk["proj"].sw
                 blk["w2"], blk["sw2"] = blk["fc2"].wq, blk["fc2"].sw
+            elif mxfp4:
+                blk.update(qf=ops.MxFp4Lin(wqf, bqf, BF, dev),
+                           proj=ops.MxFp4Lin(weights[p + "attn.proj.weight"], weights[p + "attn.proj.bias"], BF, dev),
+                           fc2=ops.MxFp4Lin(weights[p + "mlp.fc2.weight"], weights[p + "mlp.fc2.bias"], BF, dev))
+                del wqf
             else:
                 blk.update(wqf=wqf,
                            proj=lin_cls(weights[p + "attn.proj.weight"], weights[p + "attn.proj.bias"], BF),
@@ -82,8 +98,17 @@ class TextDecoder:
         self.post_ln = (g("post_ln.weight"), g("post_ln.bias"))
         self.w_lm, self.b_lm = g("lm_head.weight"), f32("lm_head.bias")
         self.cs = freqs_cis(c["rot"], max(ctx, 2048), c["theta"]).to(dev).contiguous()
-        self.kc = [torch.zeros(self.nq, self.H, ctx, self.hd, device=dev, dtype=BF) for _ in self.blocks]
-        self.vc = [torch.zeros(self.nq, self.H, ctx, self.hd, device=dev, dtype=BF) for _ in self.blocks]
+        if kv8:
+            # every layer's cache in one set of buffers, so that one copy saves the blocks that the prefix ends in
+            nb = -(-ctx // ops.KV8Cache.BLOCK)
+            z = lambda *s: torch.zeros(n, self.nq, self.H, *s, device=dev, dtype=torch.uint8)
+            self.kv_all = (z(nb, 64 * self.hd), z(nb, 64 * self.hd), z(nb), z(nb))
+            self.kv_end = (z(64 * self.hd), z(64 * self.hd), z(), z())  # the prefix's last block, as the prefill left it
+            self.kv = [ops.KV8Cache.over(*(t[i] for t in self.kv_all), ctx) for i in range(n)]
+            self.kc = self.vc = None
+        else:
+            self.kc = [torch.zeros(self.nq, self.H, ctx, self.hd, device=dev, dtype=BF) for _ in self.blocks]
+            self.vc = [torch.zeros(self.nq, self.H, ctx, self.hd, device=dev, dtype=BF) for _ in self.blocks]
         # ---- yes/no query state (md2fast.py:128-143)
         self.yes_ids, self.no_ids = list(yes_ids), list(no_ids)
         self.yn_ids = self.yes_ids + self.no_ids
@@ -116,8 +141,9 @@ class TextDecoder:
         self.state = torch.zeros(2, device=dev, dtype=torch.int32)
         self.tokens = torch.zeros(ctx, device=dev, dtype=torch.int32)
         self.xd = [torch.zeros(self.D, device=dev, dtype=BF) for _ in range(2)]
-        self.qkv_d = torch.zeros(3 * self.D, device=dev, dtype=BF)
-        self.g_d = torch.zeros(c["ff"], device=dev, dtype=BF)
+        qf_d = torch.zeros(3 * self.D + c["ff"], device=dev, dtype=BF)  # one row of the fused [qkv | fc1] product
+        self.qf_d, self.qkv_d, self.g_d = qf_d[None], qf_d[:3 * self.D], qf_d[3 * self.D:]
+        self.h_d = torch.zeros(1, self.D, device=dev, dtype=BF)
         self.a_d = torch.zeros(self.D, device=dev, dtype=BF)
         self.y2_d = torch.zeros(self.D, device=dev, dtype=BF)  # bf16(fc2(g) + b2) of the decode step
         # decode: fc2 shares the attention's launch (mx_decode_attn_fc2) and proj + residual follow (mx_gemv_res2);
@@ -139,7 +165,7 @@ class TextDecoder:
         # wait for nobody, unless the program sets use_mk = True for a decoder that has the device to itself (before
         # capture_step; 4 W8A8 layers at 1500 keys: 140 us a step per layer, 122 in one launch).
         self.mk_layers = self.mk_ll = self.mk_ep = None
-        if (dev.type == "cuda" and attn_splits == 1 and (self.D, self.H, self.hd, c["ff"]) == (2048, 32, 64, 8192)
+        if (dev.type == "cuda" and attn_splits == 1 and not mxfp4 and not kv8 and (self.D, self.H, self.hd, c["ff"]) == (2048, 32, 64, 8192)
                 and ctx <= 2048 and self.V <= 65536
                 and torch.cuda.get_device_properties(dev).multi_processor_count >= lib.mx_decode_mk_grid()):
             self._init_mk()
@@ -198,10 +224,13 @@ class TextDecoder:
                 qkv, f = y[:, :b["nq"]], y[:, b["nq"]:]
             else:
                 qkv, f = b["qkv"](h, pre=pre), None
-            q = torch.empty(B, H, n, hd, device=self.dev, dtype=BF)
-            call("mx_rope_kv", stream(), qkv.data_ptr(), qkv.stride(0), self.cs.data_ptr(), q.data_ptr(),
-                 self.kc[i].data_ptr(), self.vc[i].data_ptr(), B, n, H, self.ctx, pos0, self.nq, int(bcast))
-            a = ops.sdpa(q, self.kc[i][:B, :, :Tk], self.vc[i][:B, :, :Tk], qpos0=pos0, causal_from=causal_from)
+            if self.kv8:
+                a = self._attend_kv8(i, qkv, pos0, Tk, causal_from, B, bcast)
+            else:
+                q = torch.empty(B, H, n, hd, device=self.dev, dtype=BF)
+                call("mx_rope_kv", stream(), qkv.data_ptr(), qkv.stride(0), self.cs.data_ptr(), q.data_ptr(),
+                     self.kc[i].data_ptr(), self.vc[i].data_ptr(), B, n, H, self.ctx, pos0, self.nq, int(bcast))
+                a = ops.sdpa(q, self.kc[i][:B, :, :Tk], self.vc[i][:B, :, :Tk], qpos0=pos0, causal_from=causal_from)
             r = b["proj"](a.view(B * n, self.D), res=x)
             if f is None:
                 f = b["fc1"](h, gelu=True, pre=pre)
@@ -213,6 +242,29 @@ class TextDecoder:
             else:
                 x, h = b["fc2"](f, res=r), None
         return x
+
+    def _attend_kv8(self, i, qkv, pos0, kv_len, causal_from, B, bcast):
+        """Layer i's rotary embedding, append to the 8-bit cache and attention for B sequences of fused rows qkv
+        (B * n, >= 3 D) at pos0 ..; the attention reads the quantised rows, the new ones too."""
+        n = qkv.shape[0] // B
+        q, k, v = qkv[:, :3 * self.D].view(B, n, 3, self.H, self.hd).permute(2, 0, 3, 1, 4)
+        q = self.kv[i].append(k, v, pos0, bcast=bcast, cs=self.cs, q=q)
+        return ops.sdpa_kv8(q, self.kv[i], kv_len, qpos0=pos0, causal_from=causal_from)
+
+    def _save_prefix_end(self):
+        """The block that the prefix ends in also takes the rows behind it, and their size may round the prefix's rows once
+        more: kept here as the prefill left it, so that every query finds the same prefix."""
+        if self.kv8:
+            for t, e in zip(self.kv_all, self.kv_end):
+                e.copy_(t[:, :, :, self._end_block()])
+
+    def _restore_prefix_end(self):
+        if self.kv8:
+            for t, e in zip(self.kv_all, self.kv_end):
+                t[:, :, :, self._end_block()].copy_(e)
+
+    def _end_block(self):
+        return (self.prefix - 1) // ops.KV8Cache.BLOCK
 
     def _fuse_next_ln(self, lin, M):
         """fc2 + residual + the next layer's LayerNorm as partials + one row kernel: bf16 Linears whose row count has a
@@ -249,6 +301,7 @@ class TextDecoder:
             raise ValueError(f"prefill of {x.shape[0]} tokens exceeds the cache ({self.ctx})")
         xp = self._text_layers(x, 0, P, bcast=True)[P:]
         self.prefix = P
+        self._save_prefix_end()
         self.pos_base = x.shape[0]
         self.lm_argmax(xp[-1], logits=True)
         return xp
@@ -285,6 +338,7 @@ class TextDecoder:
         x = torch.cat([self.wte[BOS:BOS + 1], img_emb.to(self.dev, BF)], dim=0)
         self._text_layers(x, 0, None, bcast=True)
         self.prefix = x.shape[0]
+        self._save_prefix_end()
         return self.prefix
 
     # ------------------------------------------------------------------ yes/no query (md2fast.py:208-212, 266-279)
@@ -310,6 +364,7 @@ class TextDecoder:
         if self.prefix is None:
             raise RuntimeError("encode() the image prefix before querying")
         P = self.prefix
+        self._restore_prefix_end()
         x = self.wte[self.tok_buf.view(-1)]                                   # (nq * L, D)
         x = self._text_layers(x, P, P, B=self.nq)
         h = ops.layernorm(x.index_select(0, self.last_idx), *self.post_ln, eps=self.eps)  # (nq, D)
@@ -421,7 +476,10 @@ class TextDecoder:
         xi = 0
         for i, b in enumerate(self.blocks):
             x, xn = self.xd[xi], self.xd[xi ^ 1]
-            if self.w8a8:
+            if self.mxfp4:
+                ops.layernorm(x[None], *b["ln"], eps=self.eps, out=self.h_d)
+                b["qf"](self.h_d, act="tanh", act_from=b["nq"], out=self.qf_d)
+            elif self.w8a8:
                 _lib.check(lib.mx_ln_gemv2_i8(st, x.data_ptr(), b["ln"][0].data_ptr(), b["ln"][1].data_ptr(),
                                               float(self.eps), b["wqf"].data_ptr(), b["wqf"].stride(0),
                                               b["sqf"].data_ptr(), b["bqf"].data_ptr(), b["wqf"].shape[0], self.D,
@@ -431,15 +489,23 @@ class TextDecoder:
                                            float(self.eps), b["wqf"].data_ptr(), b["wqf"].stride(0), b["bqf"].data_ptr(),
                                            b["wqf"].shape[0], self.D, b["nq"], self.qkv_d.data_ptr(),
                                            self.g_d.data_ptr(), 1), "mx_ln_gemv2")
-            if self.fc2_with_attn:
+            if self.fc2_with_attn and not (self.mxfp4 or self.kv8):
                 self._attn_fc2_res(b, i, x, xn)
                 xi ^= 1
                 continue
-            _lib.check(lib.mx_decode_attn(st, self.qkv_d.data_ptr(), self.cs.data_ptr(), self.kc[i].data_ptr(),
-                                          self.vc[i].data_ptr(), self.H, self.ctx, self.state.data_ptr(), self.S,
-                                          float(self.hd ** -0.5), self.attn_ws.data_ptr(), self.attn_cnt.data_ptr(),
-                                          self.a_d.data_ptr()), "mx_decode_attn")
-            if self.w8a8:
+            if self.kv8:  # the position is on the device: state[1]
+                q, k, v = self.qkv_d.view(3, 1, self.H, 1, self.hd)
+                q = self.kv[i].append(k, v, self.state[1:], cs=self.cs, q=q)
+                ops.sdpa_kv8(q, self.kv[i], self.state[1:], base=1, out=self.a_d.view(1, 1, -1))
+            else:
+                _lib.check(lib.mx_decode_attn(st, self.qkv_d.data_ptr(), self.cs.data_ptr(), self.kc[i].data_ptr(),
+                                              self.vc[i].data_ptr(), self.H, self.ctx, self.state.data_ptr(), self.S,
+                                              float(self.hd ** -0.5), self.attn_ws.data_ptr(), self.attn_cnt.data_ptr(),
+                                              self.a_d.data_ptr()), "mx_decode_attn")
+            if self.mxfp4:
+                r = b["proj"](self.a_d[None], res=x[None])
+                b["fc2"](self.g_d[None], res=r, out=xn[None])
+            elif self.w8a8:
                 _lib.check(lib.mx_gemv_dual_res_i8(st, self.g_d.data_ptr(), b["w2"].data_ptr(), b["sw2"].data_ptr(),
                                                    b["b2"].data_ptr(), b["w2"].shape[1], self.a_d.data_ptr(),
                                                    b["wp"].data_ptr(), b["swp"].data_ptr(), b["bp"].data_ptr(),

@@ -858,6 +858,23 @@ class KV8Cache:
         self.ks, self.vs = z(slots, heads, nb), z(slots, heads, nb)
         self.dev = self.kc.device
 
+    @classmethod
+    def over(cls, kc, vc, ks, vs, ctx):
+        """A cache of ctx tokens over given storage (uint8, contiguous, zero at first): codes (slots, heads, blocks, 64 *
+        hd) and scales (slots, heads, blocks) of ceil(ctx / 64) blocks."""
+        slots, heads, nb, w = kc.shape
+        self = cls.__new__(cls)
+        self.slots, self.heads, self.ctx, self.hd = slots, heads, ctx, w // 64
+        if nb < 1 or nb != -(-ctx // cls.BLOCK) or w not in (64 * 64, 64 * 128):
+            raise ValueError(f"codes {tuple(kc.shape)} do not hold {ctx} tokens of head dim 64 or 128")
+        for t, shape in ((kc, kc.shape), (vc, kc.shape), (ks, kc.shape[:3]), (vs, kc.shape[:3])):
+            if t.shape != shape or t.dtype != torch.uint8 or not t.is_contiguous() or t.device != kc.device:
+                raise ValueError("storage must be contiguous uint8 tensors of matching shapes on one device")
+        if kc.data_ptr() % 16 or vc.data_ptr() % 16:
+            raise ValueError("codes must be 16-byte aligned")
+        self.kc, self.vc, self.ks, self.vs, self.dev = kc, vc, ks, vs, kc.device
+        return self
+
     def _ptrs(self):
         return self.kc.data_ptr(), self.vc.data_ptr(), self.ks.data_ptr(), self.vs.data_ptr()
 

@@ -1,0 +1,139 @@
+"""The text decoder with MXFP4 Linears and / or the 8-bit cache: it is the public operators, composed (bit for bit: the same
+kernels on the same values, whether positions come from the host or the device); it stays near the bf16 decoder by as much
+as the formats allow; captured graphs equal the eager calls; a query finds the same prefix whatever was asked before."""
+import pytest
+import torch
+
+import strix_halo_maxx_amd.md2text as mt
+import strix_halo_maxx_amd.ops as ops
+import strix_halo_maxx_amd.synth as S
+from strix_halo_maxx_amd import _lib
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+D, H, HD, FF = 2048, 32, 64, 8192
+FORMS = [dict(mxfp4=True), dict(kv8=True), dict(mxfp4=True, kv8=True), dict(w8a8=True, kv8=True)]
+
+
+def name(f):
+    return "+".join(f)
+
+
+def inputs(dev, n_img=70, n_ids=25):
+    return S.activations(7, (n_img, D), "img").to(dev), S.prompt_ids(8, n_ids).to(dev)
+
+
+class Composed:
+    """Two MXFP4 layers over 8-bit caches from the public operators alone."""
+
+    def __init__(self, w, dev, ctx):
+        self.dev, self.layers = dev, []
+        g = lambda n: w[n].to(dev, BF).contiguous()
+        for i in range(2):
+            p = f"blocks.{i}."
+            lin = lambda *names: ops.MxFp4Lin(torch.cat([w[p + n + ".weight"] for n in names]),
+                                              torch.cat([w[p + n + ".bias"] for n in names]), device=dev)
+            self.layers.append(dict(ln=(g(p + "ln.weight"), g(p + "ln.bias")), qf=lin("attn.qkv", "mlp.fc1"),
+                                    proj=lin("attn.proj"), fc2=lin("mlp.fc2"),
+                                    kv=ops.KV8Cache(1, H, ctx, HD, device=dev)))
+        self.post = (g("post_ln.weight"), g("post_ln.bias"))
+        self.cs = S.freqs_cis(32, 2048).to(dev)
+
+    def run(self, x, pos, causal_from):
+        n = x.shape[0]
+        for L in self.layers:
+            h = ops.layernorm(x, *L["ln"])
+            y = L["qf"](h, act="tanh", act_from=3 * D)
+            q, k, v = y[:, :3 * D].reshape(n, 3, H, HD).permute(1, 2, 0, 3)[:, None]
+            q = L["kv"].append(k, v, pos, cs=self.cs, q=q)
+            a = ops.sdpa_kv8(q, L["kv"], pos + n, causal_from=causal_from)
+            x = L["fc2"](y[:, 3 * D:], res=L["proj"](a[0], res=x))
+        return x
+
+
+def test_prefill_and_decode_are_the_operators_composed(dev):
+    w = S.text_weights(3, layers=2)
+    dec = mt.TextDecoder(w, ctx=256, mxfp4=True, kv8=True)
+    assert not dec.use_mk and dec.kc is None and "wqf" not in dec.blocks[0]
+    img, ids = inputs(dev)
+    ref = Composed(w, dev, 256)
+    x = torch.cat([dec.wte[mt.BOS:mt.BOS + 1], img.to(BF), dec.wte[ids]])
+    want = ref.run(x, 0, 71)[71:]
+    got = dec.prefill(img, ids)
+    assert torch.equal(got, want)
+    for L, kv in zip(ref.layers, dec.kv):
+        assert all(torch.equal(a, b) for a, b in zip(L["kv"].read(96), kv.read(96)))
+    dec.start_decode()
+    for t in range(40):  # across a block border at 128
+        row = dec.xd[0].clone()[None]
+        dec.decode_step(logits=True)
+        want = ref.run(row, 96 + t, None)
+        lm = torch.empty(dec.V, device=dev, dtype=BF)
+        part = torch.zeros_like(dec.part)
+        _lib.call("mx_ln_gemv_argmax", _lib.stream(), want.data_ptr(), dec.post_ln[0].data_ptr(), dec.post_ln[1].data_ptr(),
+                  1e-5, dec.w_lm.data_ptr(), dec.w_lm.stride(0), dec.b_lm.data_ptr(), dec.V, D, lm.data_ptr(),
+                  part.data_ptr(), dec.nparts)
+        assert torch.equal(dec.logits, lm), t
+
+
+@pytest.mark.parametrize("form", FORMS, ids=name)
+def test_near_the_bf16_decoder(dev, form):
+    """The last layer's output against the bf16 decoder's. MXFP4: a code is off by at most a quarter of a value above half a
+    unit, about an eighth in the root mean square of a normal block, for weights and activations, so a Linear's output by
+    about 0.18 and the residual sum of two layers by less than 0.35. The cache: e4m3 is off by at most 2^-4 of a value.
+    W8A8: by 2^-7 of the largest, below that."""
+    w = S.text_weights(4, layers=2)
+    img, ids = inputs(dev, 200, 30)
+    ref = mt.TextDecoder(w, ctx=512).prefill(img, ids).float()
+    got = mt.TextDecoder(w, ctx=512, **form).prefill(img, ids).float()
+    r = float((got - ref).norm() / ref.norm())
+    print(name(form), "rel-L2 vs bf16", r, flush=True)
+    assert r < (0.35 if form.get("mxfp4") else 2.0 ** -4)
+
+
+@pytest.mark.parametrize("form", FORMS, ids=name)
+def test_generate_graph_equals_eager(dev, form):
+    """Prefill and 60 greedy tokens, eager and as captured graphs (prefill and step), twice in a row on one decoder."""
+    w = S.text_weights(5, layers=2)
+    img, ids = inputs(dev)
+    dec = mt.TextDecoder(w, ctx=192, **form)
+    eager = dec.generate(img, ids, 60, use_graph=False).tolist()
+    dec.capture_prefill(img.shape[0], ids.shape[0])
+    for _ in range(2):
+        assert dec.generate(img, ids, 60).tolist() == eager
+    with pytest.raises(ValueError):
+        dec.generate(img, ids, 98)
+
+
+@pytest.mark.parametrize("form", FORMS, ids=name)
+def test_query_finds_the_same_prefix_again(dev, form):
+    """Question A, then B, then A again: A's logits are the same bits, eager and as a graph, and after a prefill with
+    decoded tokens over the same slots the prefix is again what encode() left."""
+    w = S.text_weights(6, layers=2)
+    dec = mt.TextDecoder(w, ctx=256, nq=2, L=16, yes_ids=[11, 222, 3333, 44444], no_ids=[55, 666, 7777, 50000], **form)
+    img, _ = inputs(dev, 70)
+    ask = lambda s: dec.set_questions([S.prompt_ids(s, 9).tolist(), S.prompt_ids(s + 1, 16).tolist()])
+    dec.encode(img)
+    ask(1)
+    a = dec.query().clone()
+    ask(30)
+    b = dec.query().clone()
+    ask(1)
+    assert torch.equal(dec.query(), a) and not torch.equal(a, b)
+    dec.capture_query()
+    for s, want in ((30, b), (1, a), (1, a), (30, b)):
+        ask(s)
+        assert torch.equal(dec.query(), want)
+    dec.generate(img, S.prompt_ids(9, 16), 10, use_graph=False)
+    dec.encode(img)
+    ask(1)
+    assert torch.equal(dec.query(), a)
+
+
+def test_formats_that_exclude_each_other(dev):
+    w = S.text_weights(2, layers=1)
+    with pytest.raises(ValueError, match="either"):
+        mt.TextDecoder(w, mxfp4=True, w8a8=True)
+    with pytest.raises(ValueError, match="Linear class"):
+        mt.TextDecoder(w, lin_cls=ops.MxI8Lin, mxfp4=True)
+    assert mt.TextDecoder(w, lin_cls=ops.MxFp4Lin, ctx=64).mxfp4

@@ -118,6 +118,11 @@ def test_python_refusals():
     raises("out must", w.values, out=torch.zeros(10, 65, dtype=BF))
     for a in ((0, 1, 8, 64), (1, 1, 0, 64), (1, 1, 8, 72)):
         raises("must be positive", ops.KV8Cache, *a, device="cpu")
+    z = lambda *s: torch.zeros(*s, dtype=torch.uint8)
+    assert ops.KV8Cache.over(z(2, 2, 2, 4096), z(2, 2, 2, 4096), z(2, 2, 2), z(2, 2, 2), 100).hd == 64
+    raises("do not hold", ops.KV8Cache.over, z(2, 2, 2, 4096), z(2, 2, 2, 4096), z(2, 2, 2), z(2, 2, 2), 129)
+    raises("do not hold", ops.KV8Cache.over, z(2, 2, 2, 4608), z(2, 2, 2, 4608), z(2, 2, 2), z(2, 2, 2), 100)
+    raises("storage", ops.KV8Cache.over, z(2, 2, 2, 4096), z(2, 2, 2, 4096), z(2, 2, 3), z(2, 2, 2), 100)
     c = ops.KV8Cache(2, 2, 100, 64, device="cpu")
     k = torch.zeros(2, 2, 5, 64, dtype=BF)
     i = lambda *v: torch.tensor(v, dtype=torch.int32)
