@@ -360,8 +360,7 @@ __global__ __launch_bounds__(64 * NK) void kv8_rows_kernel(Attn8Args p) {
 // ---------------------------------------------------------------------------------------------- many rows
 // 32 NQW rows per workgroup, on the 32x32x64 MFMA: NQW query waves x NKW key waves. A stage of the LDS ring holds NKW
 // blocks of K and V as they lie in the cache, copied by the asynchronous LDS-DMA load a stage or more ahead; key wave u
-// takes block u of every stage, and the shares of the key waves are added at the end. The weights' sums come from the
-// MFMA too: one more tile of V's rows, all ones.
+// takes block u of every stage, and the shares of the key waves are added at the end.
 template <int D, int NQW, int NKW, int S>
 struct Tile8 {
   static constexpr int NW = NQW * NKW;
@@ -385,6 +384,7 @@ __global__ __launch_bounds__(64 * NQW * NKW, 2) void kv8_tile_kernel(Attn8Args p
   const long cell = blockIdx.x / p.splits;
   // the row groups of a causal prompt's end see the most keys: they start first
   const int rt = p.nrt - 1 - (int)(cell % p.nrt), bh = (int)(cell / p.nrt), b = bh / p.H, h = bh % p.H;
+  const long rec = ((long)bh * p.nrt + rt) * p.splits + s;  // the share's record (rows in order, not as they start)
   const int R = p.Tq * p.G, r0 = rt * 32 * NQW, row = r0 + 32 * qg + c, rc = min(row, R - 1);
   const Seq sq = sequence(p, b);
   const int lim = limit(p, sq, rc / p.G);
@@ -406,14 +406,13 @@ __global__ __launch_bounds__(64 * NQW * NKW, 2) void kv8_tile_kernel(Attn8Args p
       dma16s(src, (uint32_t)lane * 16, dst + q * 1024);
     }
   };
-  f32x16 o[NT], ls;
+  f32x16 o[NT];
 #pragma unroll
-  for (int e = 0; e < 16; e++) {
-    ls[e] = 0.f;
+  for (int t = 0; t < NT; t++)
 #pragma unroll
-    for (int t = 0; t < NT; t++) o[t][e] = 0.f;
-  }
+    for (int e = 0; e < 16; e++) o[t][e] = 0.f;
   int m = M_NONE;
+  float l = 0.f;
   i32x8 qh[NS], ql[NS];
   int sqh;
   // the scale bytes of the next 64 blocks, one per lane (a load per block would wait for the copies in flight behind it)
@@ -449,8 +448,6 @@ __global__ __launch_bounds__(64 * NQW * NKW, 2) void kv8_tile_kernel(Attn8Args p
 #pragma unroll
   for (int i = 1; i < S - 1; i++)
     if (i < ns) issue(i);
-  constexpr uint32_t ONE4 = 0x38383838u;
-  const i32x8 ones = join(u32x4{ONE4, ONE4, ONE4, ONE4}, u32x4{ONE4, ONE4, ONE4, ONE4});
 
   for (int i = 0; i < ns; i++) {
     wait_stages<C::LPS, S - 2>(ns - 1 - i);
@@ -464,6 +461,9 @@ __global__ __launch_bounds__(64 * NQW * NKW, 2) void kv8_tile_kernel(Attn8Args p
     auto ld = [](const uint8_t* q) { return *reinterpret_cast<const u32x4*>(q); };
     const int sk = __builtin_amdgcn_readlane(skl, rel % 64), sv = __builtin_amdgcn_readlane(svl, rel % 64);
     f32x16 st[2];
+    // a wave in its products goes first: the two waves of a SIMD fall out of step, and one's softmax runs under the other's
+    // products (512 us for 527 without, 2048 rows x 16001 keys, 32 heads x 128)
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int t = 0; t < 2; t++) {
       i32x8 kk[NS];
@@ -477,6 +477,7 @@ __global__ __launch_bounds__(64 * NQW * NKW, 2) void kv8_tile_kernel(Attn8Args p
 #pragma unroll
       for (int u = 0; u < NS; u++) st[t] = mfma8(kk[u], ql[u], st[t], sk, sqh - 4);
     }
+    __builtin_amdgcn_s_setprio(0);
     const bool masked = (blk + 1) * 64 > kall;
     const int key0 = blk * 64 + 4 * hk;
     float mx = -INFINITY;
@@ -495,28 +496,30 @@ __global__ __launch_bounds__(64 * NQW * NKW, 2) void kv8_tile_kernel(Attn8Args p
     const int el = block_exponent(halves_max(mx) * p.sl2), mn = max(m, el);
     if (__any(mn != m)) {
       const float al = __builtin_amdgcn_ldexpf(1.f, m - mn);
+      l *= al;
 #pragma unroll
       for (int e = 0; e < 16; e++) {
-        ls[e] *= al;
 #pragma unroll
         for (int t = 0; t < NT; t++) o[t][e] *= al;
       }
       m = mn;
     }
     const float sh = (float)(8 - el);
+    float sum = 0.f;
     i32x8 ph, pl;
 #pragma unroll
     for (int w = 0; w < 8; w++) {
       float y[4];
 #pragma unroll
       for (int e = 0; e < 4; e++) y[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[w >> 2][4 * (w & 3) + e], p.sl2, sh));
+      sum += (y[0] + y[1]) + (y[2] + y[3]);
       uint32_t a, d;
       split4(y[0], y[1], y[2], y[3], a, d);
       ph[w] = (int)a, pl[w] = (int)d;
     }
     const int sp = weight_byte(el, mn);
-    ls = mfma8(ones, ph, ls, 127, sp);
-    ls = mfma8(ones, pl, ls, 127, sp - 4);
+    l += __builtin_amdgcn_ldexpf(halves_sum(sum), el - 8 - mn);
+    __builtin_amdgcn_s_setprio(1);
     bool nan = false;
     if (masked) {
       uint32_t nb = 0;
@@ -540,9 +543,10 @@ __global__ __launch_bounds__(64 * NQW * NKW, 2) void kv8_tile_kernel(Attn8Args p
       o[t] = mfma8(join(v0, v1), ph, o[t], sv, sp);
       o[t] = mfma8(join(v0, v1), pl, o[t], sv, sp - 4);
     }
+    __builtin_amdgcn_s_setprio(0);
   }
 
-  float L = ls[0];
+  float L = l;
   if constexpr (NKW > 1) {
     // ---- the key waves' shares, added in wave order; wave kw finishes the register groups u with u % NKW = kw
     float* cm = reinterpret_cast<float*>(smem);
@@ -567,7 +571,7 @@ __global__ __launch_bounds__(64 * NQW * NKW, 2) void kv8_tile_kernel(Attn8Args p
       L += cm[(w * NQW + qg) * 128 + 64 + lane] * f[w];
     }
     if (row >= R) return;
-    const Out t = target<D>(p, b, h, row, blockIdx.x, gridDim.x, L);
+    const Out t = target<D>(p, b, h, row, rec, gridDim.x, L);
     if (!t.whole && kw == 0 && hk == 0) {
       t.pm[0] = __int_as_float(m);
       t.pm[p.rw] = L;
@@ -584,7 +588,7 @@ __global__ __launch_bounds__(64 * NQW * NKW, 2) void kv8_tile_kernel(Attn8Args p
     }
   } else {
     if (row >= R) return;
-    const Out t = target<D>(p, b, h, row, blockIdx.x, gridDim.x, L);
+    const Out t = target<D>(p, b, h, row, rec, gridDim.x, L);
     if (!t.whole && hk == 0) {
       t.pm[0] = __int_as_float(m);
       t.pm[p.rw] = L;
@@ -649,7 +653,15 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Attn8Args p, long nrec) {
 }
 
 // How a problem is cut: rw rows per workgroup (16: the few-row kernel), nkw key waves, nrt row groups, `splits` runs of
-// `chunk` blocks.
+// `chunk` blocks. us on one MI355X (query waves x key waves; sequences x key heads x group, head dim, queries, keys):
+//  * up to 32 rows: the few-row kernel; runs of keys until there are 3 workgroups per CU (a CU holds 2 or 3);
+//  * 4 x 1 where 128-row groups give two workgroups per CU: 4 x 8 x 4, 128, 512, 512 30.2 (4 x 2 37.7, 2 x 2 37.4);
+//  * 4 x 2 down to three quarters of one per CU: 1 x 8 x 4, 128, 1024, 8000 152 (4 x 1 209, 2 x 4 183, 1 x 4 314);
+//  * 2 x 4, 64-row groups, down to the same: 1 x 8 x 4, 128, 512, 4000 54 (4 x 2 70, 1 x 4 92);
+//  * 1 x 8 (head dim 128: 1 x 4, its LDS) below: 1 x 32 x 1, 64, 64, 794 9.9 (2 x 4 13.1, 4 x 2 17.6); 1 x 8 x 4, 128, 256,
+//    2000 27 (2 x 4 35, 4 x 2 42);
+//  * few rows over 16384 keys or more (bound by the keys' bytes): all rows of a head in a workgroup, if 64 or 128 hold
+//    them, and runs of keys: 1 x 8 x 4, 128, 16, 100000 2 x 4 56, 1 x 4 80, 4 x 2 73.
 struct Plan {
   int rw, nkw, nrt, splits, chunk;
 };
@@ -657,12 +669,23 @@ Plan plan(int B, int H, int G, int Tq, int ctx, int D) {
   Plan q;
   const long R = (long)Tq * G;
   const int nb = kv8_blocks(ctx);
-  q.rw = R <= 32 ? 16 : 128;
+  const auto cells = [&](int rw) { return (long)B * H * ((R + rw - 1) / rw); };
+  if (R <= 32) {
+    q.rw = 16, q.nkw = 4;
+  } else if (cells(128) >= 512) {
+    q.rw = 128, q.nkw = 1;
+  } else if (cells(128) >= 192) {
+    q.rw = 128, q.nkw = 2;
+  } else if (cells(64) >= 192) {
+    q.rw = 64, q.nkw = 4;
+  } else if (nb >= 256) {
+    q.rw = R <= 64 ? 64 : 128, q.nkw = R <= 64 ? 4 : 2;
+  } else {
+    q.rw = 32, q.nkw = D == 64 ? 8 : 4;
+  }
+  const long n = cells(q.rw);
   q.nrt = (int)((R + q.rw - 1) / q.rw);
-  const long cells = (long)B * H * q.nrt;
-  q.nkw = q.rw == 16 ? 4 : cells >= 512 ? 1 : 2;
-  const long want = q.rw == 16 ? 768 : 256;
-  long sp = (want + cells - 1) / cells;
+  long sp = q.rw == 16 ? (768 + n - 1) / n : n <= 128 ? 256 / n : 1;
   const long most = (nb + 15) / 16;
   if (sp > most) sp = most;
   if (sp > 1024) sp = 1024;
@@ -677,12 +700,19 @@ hipError_t launch(hipStream_t st, Attn8Args a, const Plan& q) {
   const long nrec = (long)a.B * a.H * q.nrt * q.splits;
   a.rw = q.rw, a.nrt = q.nrt, a.splits = q.splits, a.chunk = q.chunk;
   const dim3 grid((unsigned)nrec);
-  if (q.rw == 16)
-    hipLaunchKernelGGL((kv8_rows_kernel<D, 4>), grid, dim3(256), 0, st, a);
-  else if (q.nkw == 1)
-    hipLaunchKernelGGL((kv8_tile_kernel<D, 4, 1, 4>), grid, dim3(256), 0, st, a);
-  else
-    hipLaunchKernelGGL((kv8_tile_kernel<D, 4, 2, 3>), grid, dim3(512), 0, st, a);
+  auto go = [&](auto kern, int waves) { hipLaunchKernelGGL(kern, grid, dim3(64 * waves), 0, st, a); };
+  if (q.rw == 16) {
+    go(kv8_rows_kernel<D, 4>, 4);
+  } else if (q.rw == 128) {
+    if (q.nkw == 1) go(kv8_tile_kernel<D, 4, 1, 3>, 4);
+    else go(kv8_tile_kernel<D, 4, 2, 2>, 8);
+  } else if (q.rw == 64) {
+    go(kv8_tile_kernel<D, 2, 4, 2>, 8);
+  } else if constexpr (D == 64) {
+    go(kv8_tile_kernel<D, 1, 8, 2>, 8);
+  } else {
+    go(kv8_tile_kernel<D, 1, 4, 2>, 4);
+  }
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && q.splits > 1) {
     hipLaunchKernelGGL(kv8_join_kernel<D>, dim3((unsigned)((long)a.B * a.H * a.Tq * a.G)), dim3(256), 0, st, a, nrec);

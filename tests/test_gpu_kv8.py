@@ -178,6 +178,11 @@ SDPA = [((1,), 1, 1, 64, 1, None), ((0, 1, 63, 64, 65), 2, 1, 64, 1, None), ((13
         ((1000,), 32, 1, 64, 1, 0), ((2100, 17), 2, 8, 128, 1, None), ((70, 3), 1, 32, 64, 1, None),
         ((40, 200), 3, 3, 64, 5, 0), ((33, 90, 0), 2, 1, 64, 40, 0), ((300, 64), 2, 4, 128, 37, 50),
         ((150,), 2, 2, 64, 150, 100), ((128, 129), 1, 7, 128, 129, 0), ((4500,), 1, 2, 64, 3, 0)]
+# one for each way a prompt is cut: heads x rows of two workgroups per CU, of one, 64-row groups, 32-row groups, runs of keys
+# with 64 and 128 rows, each head dim
+CUTS = [((200,), 64, 8, 64, 130, 0), ((200,), 32, 8, 128, 130, 60), ((130,), 32, 7, 64, 120, 0), ((150,), 24, 8, 128, 128, None),
+        ((200, 190), 48, 1, 64, 130, 0), ((300,), 32, 4, 128, 100, 0), ((500, 13), 8, 1, 64, 70, 0), ((700,), 4, 4, 128, 30, 0),
+        ((17000,), 1, 1, 64, 50, 0), ((16700,), 1, 4, 128, 16, None), ((16500,), 1, 4, 64, 40, 100), ((16900,), 1, 8, 128, 12, 0)]
 
 
 @pytest.mark.parametrize("lens,H,G,D,Tq,cf", SDPA)
@@ -196,6 +201,34 @@ def test_sdpa(dev, lens, H, G, D, Tq, cf):
         assert torch.equal(ops.sdpa_kv8(q.to(dev), c.c, lens[0], causal_from=cf), y)
         assert torch.equal(ops.sdpa_kv8(q.to(dev), c.c, lens[0], causal_from=cf, qpos0=lens[0] - Tq), y)
     assert torch.equal(ops.sdpa_kv8(q.to(dev), c.c, i32(dev, *[n - 7 for n in lens]), base=7, causal_from=cf), y)
+
+
+@pytest.mark.parametrize("lens,H,G,D,Tq,cf", CUTS)
+def test_sdpa_cuts(dev, lens, H, G, D, Tq, cf):
+    """The bound of check_sdpa, the oracle as matrix products in 64 bits on the GPU."""
+    g = torch.Generator(device=dev).manual_seed(sum(lens) + H + Tq)
+    B, n = len(lens), max(lens)
+    r = lambda *s: torch.randn(*s, generator=g, device=dev).to(BF)
+    c = ops.KV8Cache(B, H, n, D, device=dev)
+    c.append(r(B, H, n, D), r(B, H, n, D) * 3, 0, count=i32(dev, *lens))
+    q = r(B, H * G, Tq, D)
+    print("cut", lens, H, G, D, Tq, cf, flush=True)
+    y = ops.sdpa_kv8(q, c, i32(dev, *lens), causal_from=cf).double().view(B, Tq, H, G, D)
+    k, v = (x.double() for x in c.read())
+    for b, t in enumerate(lens):
+        j, i = torch.arange(t, device=dev)[None], torch.arange(Tq, device=dev)[:, None]
+        seen = (j < t) if cf is None else (j < cf) | (j <= t - Tq + i)
+        for h in range(H):
+            kk, vv = k[b, h, :t], v[b, h, :t]
+            qq = q[b, h * G:(h + 1) * G].double()
+            s = (torch.matmul(qq, kk.t().contiguous()) * D ** -0.5).masked_fill(~seen, -float("inf"))
+            size = torch.matmul(qq.abs(), kk.t().abs().contiguous()).amax(-1, keepdim=True) * D ** -0.5
+            p = torch.nan_to_num(torch.softmax(s, -1))
+            ref, avg = torch.matmul(p, vv), torch.matmul(p, vv.abs())
+            out = y[b, :, h].transpose(0, 1)
+            tol = 2.0 ** -8 * ref.abs() + (2.0 ** -8 + 2.0 ** -12 + 2 * 2.0 ** -12 * (1 + size)) * avg
+            ok = bool(((out - ref).abs() <= tol).all())
+            assert ok, (b, h, ((out - ref).abs() - tol).max().item())
 
 
 def test_sdpa_rows_that_see_nothing_are_zero(dev):
