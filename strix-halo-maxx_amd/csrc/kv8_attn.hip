@@ -671,7 +671,7 @@ Plan plan(int B, int H, int G, int Tq, int ctx, int D) {
   const int nb = kv8_blocks(ctx);
   const auto cells = [&](int rw) { return (long)B * H * ((R + rw - 1) / rw); };
   if (R <= 32) {
-    q.rw = 16, q.nkw = 4;
+    q.rw = 16, q.nkw = 4;  // 8 below, where the runs leave CUs idle
   } else if (cells(128) >= 512) {
     q.rw = 128, q.nkw = 1;
   } else if (cells(128) >= 192) {
@@ -692,6 +692,7 @@ Plan plan(int B, int H, int G, int Tq, int ctx, int D) {
   if (sp < 1) sp = 1;
   q.chunk = (int)((nb + sp - 1) / sp);
   q.splits = (nb + q.chunk - 1) / q.chunk;
+  if (q.rw == 16 && n * q.splits <= 256) q.nkw = 8;
   return q;
 }
 
@@ -702,7 +703,8 @@ hipError_t launch(hipStream_t st, Attn8Args a, const Plan& q) {
   const dim3 grid((unsigned)nrec);
   auto go = [&](auto kern, int waves) { hipLaunchKernelGGL(kern, grid, dim3(64 * waves), 0, st, a); };
   if (q.rw == 16) {
-    go(kv8_rows_kernel<D, 4>, 4);
+    if (q.nkw == 8) go(kv8_rows_kernel<D, 8>, 8);
+    else go(kv8_rows_kernel<D, 4>, 4);
   } else if (q.rw == 128) {
     if (q.nkw == 1) go(kv8_tile_kernel<D, 4, 1, 3>, 4);
     else go(kv8_tile_kernel<D, 4, 2, 2>, 8);

@@ -9,8 +9,8 @@ rebuilt for batch-1 HBM streaming:
   * per layer 3 kernels: LN fused into the [qkv | fc1] GEMV, rope + KV append fused into split-KV attention, and
     the fc2 / proj GEMVs fused with the two residual adds;
   * in fewer bits: `mxfp4` runs the layers' Linears in MXFP4, `kv8` keeps the K/V cache in 8 bits; each works with every
-    form of the other, in prefill, query and decode (a decode step then goes operator by operator, 4 to 7 launches a
-    layer, still one HIP graph);
+    form of the other, in prefill, query and decode (a decode step then goes operator by operator, 4 or 5 launches
+    a layer, still one HIP graph);
   * the LM head GEMV carries the argmax, and the next step's embedding lookup reduces it on the device, so one HIP
     graph replays a whole step with the token and position kept in device memory (no host round trip per token).
 The yes/no query is the reference's own fast path (FastMD2._encode / _query / decide, md2fast.py:201-212, 266-279):
@@ -80,10 +80,11 @@ class TextDecoder:
                 blk["wp"], blk["swp"] = blk["proj"].wq, blk["proj"].sw
                 blk["w2"], blk["sw2"] = blk["fc2"].wq, blk["fc2"].sw
             elif mxfp4:
-                blk.update(qf=ops.MxFp4Lin(wqf, bqf, BF, dev),
-                           proj=ops.MxFp4Lin(weights[p + "attn.proj.weight"], weights[p + "attn.proj.bias"], BF, dev),
-                           fc2=ops.MxFp4Lin(weights[p + "mlp.fc2.weight"], weights[p + "mlp.fc2.bias"], BF, dev))
-                del wqf
+                # fc2 and proj add up in the parallel block: one product over [fc1's output | attention] and [Wfc2 | Wproj]
+                wo = torch.cat([weights[p + "mlp.fc2.weight"], weights[p + "attn.proj.weight"]], dim=1).to(dev, BF)
+                bo = f32(p + "mlp.fc2.bias") + f32(p + "attn.proj.bias")
+                blk.update(qf=ops.MxFp4Lin(wqf, bqf, BF, dev), out=ops.MxFp4Lin(wo, bo, BF, dev))
+                del wqf, wo
             else:
                 blk.update(wqf=wqf,
                            proj=lin_cls(weights[p + "attn.proj.weight"], weights[p + "attn.proj.bias"], BF),
@@ -141,10 +142,12 @@ class TextDecoder:
         self.state = torch.zeros(2, device=dev, dtype=torch.int32)
         self.tokens = torch.zeros(ctx, device=dev, dtype=torch.int32)
         self.xd = [torch.zeros(self.D, device=dev, dtype=BF) for _ in range(2)]
-        qf_d = torch.zeros(3 * self.D + c["ff"], device=dev, dtype=BF)  # one row of the fused [qkv | fc1] product
-        self.qf_d, self.qkv_d, self.g_d = qf_d[None], qf_d[:3 * self.D], qf_d[3 * self.D:]
+        # one row of [qkv | fc1 | attention]: what the MXFP4 layers' products write and read in one piece
+        nqf = 3 * self.D + c["ff"]
+        row = torch.zeros(nqf + self.D, device=dev, dtype=BF)
+        self.qf_d, self.ga_d = row[None, :nqf], row[None, 3 * self.D:]
+        self.qkv_d, self.g_d, self.a_d = row[:3 * self.D], row[3 * self.D:nqf], row[nqf:]
         self.h_d = torch.zeros(1, self.D, device=dev, dtype=BF)
-        self.a_d = torch.zeros(self.D, device=dev, dtype=BF)
         self.y2_d = torch.zeros(self.D, device=dev, dtype=BF)  # bf16(fc2(g) + b2) of the decode step
         # decode: fc2 shares the attention's launch (mx_decode_attn_fc2) and proj + residual follow (mx_gemv_res2);
         # False: attention, then both GEMVs in one pass (mx_gemv_dual_res). Same roundings either way.
@@ -214,7 +217,13 @@ class TextDecoder:
                 h = ops.layernorm(x, *b["ln"], eps=self.eps)
             # W8A8: the LN output is quantised once for qkv and fc1 (SHARE_QUANT, md2fast.py:52, 174)
             pre = b["qkv"].quant(h) if self.w8a8 else None
-            if "qf" in b:
+            a = None  # where the attention goes
+            if self.mxfp4:
+                nqf = b["qf"].N  # rows of [qkv | fc1 | attention]
+                y = torch.empty(B * n, nqf + self.D, device=self.dev, dtype=BF)
+                b["qf"](h, act="tanh", act_from=b["nq"], out=y[:, :nqf])
+                qkv, a = y[:, :b["nq"]], y[:, nqf:].view(B, n, self.D)
+            elif "qf" in b:
                 # qkv and fc1 (its GELU on its own columns) as one product over the fused rows: a launch less, and a
                 # grid of 14336 columns fills the device (us, two products -> one, cold weights: 32 rows 23.5 -> 16.4,
                 # 256 36.1 -> 27.3, 730 58.4 -> 43.6, 794 56.3 -> 55.7, 1100 74.7 -> 72.0, 1409 89.6 -> 86.5). Where two
@@ -225,12 +234,15 @@ class TextDecoder:
             else:
                 qkv, f = b["qkv"](h, pre=pre), None
             if self.kv8:
-                a = self._attend_kv8(i, qkv, pos0, Tk, causal_from, B, bcast)
+                a = self._attend_kv8(i, qkv, pos0, Tk, causal_from, B, bcast, a)
             else:
                 q = torch.empty(B, H, n, hd, device=self.dev, dtype=BF)
                 call("mx_rope_kv", stream(), qkv.data_ptr(), qkv.stride(0), self.cs.data_ptr(), q.data_ptr(),
                      self.kc[i].data_ptr(), self.vc[i].data_ptr(), B, n, H, self.ctx, pos0, self.nq, int(bcast))
-                a = ops.sdpa(q, self.kc[i][:B, :, :Tk], self.vc[i][:B, :, :Tk], qpos0=pos0, causal_from=causal_from)
+                a = ops.sdpa(q, self.kc[i][:B, :, :Tk], self.vc[i][:B, :, :Tk], out=a, qpos0=pos0, causal_from=causal_from)
+            if self.mxfp4:
+                x, h = b["out"](y[:, b["nq"]:], res=x), None
+                continue
             r = b["proj"](a.view(B * n, self.D), res=x)
             if f is None:
                 f = b["fc1"](h, gelu=True, pre=pre)
@@ -243,13 +255,13 @@ class TextDecoder:
                 x, h = b["fc2"](f, res=r), None
         return x
 
-    def _attend_kv8(self, i, qkv, pos0, kv_len, causal_from, B, bcast):
+    def _attend_kv8(self, i, qkv, pos0, kv_len, causal_from, B, bcast, out=None):
         """Layer i's rotary embedding, append to the 8-bit cache and attention for B sequences of fused rows qkv
         (B * n, >= 3 D) at pos0 ..; the attention reads the quantised rows, the new ones too."""
         n = qkv.shape[0] // B
         q, k, v = qkv[:, :3 * self.D].view(B, n, 3, self.H, self.hd).permute(2, 0, 3, 1, 4)
         q = self.kv[i].append(k, v, pos0, bcast=bcast, cs=self.cs, q=q)
-        return ops.sdpa_kv8(q, self.kv[i], kv_len, qpos0=pos0, causal_from=causal_from)
+        return ops.sdpa_kv8(q, self.kv[i], kv_len, qpos0=pos0, causal_from=causal_from, out=out)
 
     def _save_prefix_end(self):
         """The block that the prefix ends in also takes the rows behind it, and their size may round the prefix's rows once
@@ -503,8 +515,7 @@ class TextDecoder:
                                               float(self.hd ** -0.5), self.attn_ws.data_ptr(), self.attn_cnt.data_ptr(),
                                               self.a_d.data_ptr()), "mx_decode_attn")
             if self.mxfp4:
-                r = b["proj"](self.a_d[None], res=x[None])
-                b["fc2"](self.g_d[None], res=r, out=xn[None])
+                b["out"](self.ga_d, res=x[None], out=xn[None])
             elif self.w8a8:
                 _lib.check(lib.mx_gemv_dual_res_i8(st, self.g_d.data_ptr(), b["w2"].data_ptr(), b["sw2"].data_ptr(),
                                                    b["b2"].data_ptr(), b["w2"].shape[1], self.a_d.data_ptr(),

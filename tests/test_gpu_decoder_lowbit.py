@@ -31,10 +31,11 @@ class Composed:
         g = lambda n: w[n].to(dev, BF).contiguous()
         for i in range(2):
             p = f"blocks.{i}."
-            lin = lambda *names: ops.MxFp4Lin(torch.cat([w[p + n + ".weight"] for n in names]),
-                                              torch.cat([w[p + n + ".bias"] for n in names]), device=dev)
-            self.layers.append(dict(ln=(g(p + "ln.weight"), g(p + "ln.bias")), qf=lin("attn.qkv", "mlp.fc1"),
-                                    proj=lin("attn.proj"), fc2=lin("mlp.fc2"),
+            qf = ops.MxFp4Lin(torch.cat([w[p + "attn.qkv.weight"], w[p + "mlp.fc1.weight"]]),
+                              torch.cat([w[p + "attn.qkv.bias"], w[p + "mlp.fc1.bias"]]), device=dev)
+            out = ops.MxFp4Lin(torch.cat([w[p + "mlp.fc2.weight"], w[p + "attn.proj.weight"]], 1),
+                               w[p + "mlp.fc2.bias"].float() + w[p + "attn.proj.bias"].float(), device=dev)
+            self.layers.append(dict(ln=(g(p + "ln.weight"), g(p + "ln.bias")), qf=qf, out=out,
                                     kv=ops.KV8Cache(1, H, ctx, HD, device=dev)))
         self.post = (g("post_ln.weight"), g("post_ln.bias"))
         self.cs = S.freqs_cis(32, 2048).to(dev)
@@ -47,7 +48,7 @@ class Composed:
             q, k, v = y[:, :3 * D].reshape(n, 3, H, HD).permute(1, 2, 0, 3)[:, None]
             q = L["kv"].append(k, v, pos, cs=self.cs, q=q)
             a = ops.sdpa_kv8(q, L["kv"], pos + n, causal_from=causal_from)
-            x = L["fc2"](y[:, 3 * D:], res=L["proj"](a[0], res=x))
+            x = L["out"](torch.cat([y[:, 3 * D:], a[0]], 1), res=x)
         return x
 
 
