@@ -677,10 +677,14 @@ def _call_on(dev, name, *args):
     """call() on the current stream of the tensors' own device."""
     if dev.type != "cuda":
         raise ValueError(f"{name} needs tensors on the GPU, got {dev}")
-    if dev.index == torch.cuda.current_device():
-        return call(name, stream(), *args)
+    cur = torch.cuda.current_device()
+    if dev.index == cur:
+        rc = getattr(_lib._lib or _lib.load(), name)(torch._C._cuda_getCurrentRawStream(cur), *args)
+        if rc:
+            _lib.check(rc, name)
+        return
     with torch.cuda.device(dev):
-        return call(name, stream(), *args)
+        call(name, stream(), *args)
 
 
 def _need(t, name, dev, dtype=BF):
@@ -704,15 +708,13 @@ class MxFp4:
     def __init__(self, data, rows, K):
         self.data, self.rows, self.K = data, rows, K
         self.dev = data.device
+        p = data.data_ptr()
+        self.ptrs = p, p + MxFp4.cells(rows, K) * 4096  # codes, scales
 
     @staticmethod
     def cells(rows, K):
         """Pieces of 64 rows x 128 columns: 4 KB of codes and 256 bytes of scales each."""
         return (rows + 63) // 64 * ((K + 127) // 128)
-
-    def ptrs(self):
-        p = self.data.data_ptr()
-        return p, p + MxFp4.cells(self.rows, self.K) * 4096
 
     def values(self, out=None):
         """(rows, K) bf16: the values the codes stand for, exact."""
@@ -725,7 +727,7 @@ class MxFp4:
             if y.shape != (M, K) or y.stride(1) != 1:
                 raise ValueError(f"out must be ({M}, {K}) with unit column stride")
         if M:
-            _call_on(dev, "mx_mxfp4_values", *self.ptrs(), y.data_ptr(), y.stride(0), M, K)
+            _call_on(dev, "mx_mxfp4_values", *self.ptrs, y.data_ptr(), y.stride(0), M, K)
         return y
 
 
@@ -739,7 +741,7 @@ def quant_mxfp4(x):
     M, K = x2.shape
     q = MxFp4(torch.empty(MxFp4.cells(M, K) * 4352, device=x.device, dtype=torch.uint8), M, K)
     if M:
-        _call_on(x.device, "mx_quant_mxfp4", x2.data_ptr(), x2.stride(0), *q.ptrs(), M, K)
+        _call_on(x.device, "mx_quant_mxfp4", x2.data_ptr(), x2.stride(0), *q.ptrs, M, K)
     return q
 
 
@@ -771,6 +773,7 @@ class MxFp4Lin:
         if bias is not None and bias.shape != (self.N,):
             raise ValueError(f"bias must be ({self.N},)")
         self.b = None if bias is None else bias.detach().to(device=self.dev, dtype=torch.float32).contiguous()
+        self.bp = ptr(self.b)
         self.rows = _lib.load().mx_gemv_mxfp4_rows()
 
     def quant(self, x):
@@ -815,12 +818,12 @@ class MxFp4Lin:
                     raise ValueError("residual rows must equal or divide the output rows")
                 r_rows = r2.shape[0]
         if M:
-            tail = (*self.wq.ptrs(), ptr(self.b), ptr(r2), ldr, r_rows, y2.data_ptr(), y2.stride(0), M, N, K, a, act_from)
+            tail = (*self.wq.ptrs, self.bp, None if r2 is None else r2.data_ptr(), ldr, r_rows, y2.data_ptr(), y2.stride(0), M, N, K, a, act_from)
             if pre is None and M <= self.rows:
                 _call_on(self.dev, "mx_gemv_mxfp4", x2.data_ptr(), x2.stride(0), *tail)
             else:
                 q = quant_mxfp4(x2) if pre is None else pre
-                _call_on(self.dev, "mx_gemm_mxfp4", *q.ptrs(), *tail)
+                _call_on(self.dev, "mx_gemm_mxfp4", *q.ptrs, *tail)
         if out is not None or x is None or x.dim() == 2:
             return y
         return y.view(*x.shape[:-1], N)
@@ -854,9 +857,7 @@ class KV8Cache:
         self.slots, self.heads, self.ctx, self.hd = slots, heads, ctx, hd
         nb = -(-ctx // self.BLOCK)
         z = lambda *s: torch.zeros(*s, device=device, dtype=torch.uint8)
-        self.kc, self.vc = z(slots, heads, nb, 64 * hd), z(slots, heads, nb, 64 * hd)
-        self.ks, self.vs = z(slots, heads, nb), z(slots, heads, nb)
-        self.dev = self.kc.device
+        self._hold(z(slots, heads, nb, 64 * hd), z(slots, heads, nb, 64 * hd), z(slots, heads, nb), z(slots, heads, nb))
 
     @classmethod
     def over(cls, kc, vc, ks, vs, ctx):
@@ -872,11 +873,13 @@ class KV8Cache:
                 raise ValueError("storage must be contiguous uint8 tensors of matching shapes on one device")
         if kc.data_ptr() % 16 or vc.data_ptr() % 16:
             raise ValueError("codes must be 16-byte aligned")
-        self.kc, self.vc, self.ks, self.vs, self.dev = kc, vc, ks, vs, kc.device
+        self._hold(kc, vc, ks, vs)
         return self
 
-    def _ptrs(self):
-        return self.kc.data_ptr(), self.vc.data_ptr(), self.ks.data_ptr(), self.vs.data_ptr()
+    def _hold(self, kc, vc, ks, vs):
+        self.kc, self.vc, self.ks, self.vs, self.dev = kc, vc, ks, vs, kc.device
+        self.ptrs = kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr()
+        self._ws = {}  # workspace floats of an attention call by (sequences, group, queries)
 
     def append(self, k, v, pos=0, base=0, count=None, bcast=False, cs=None, q=None):
         """Writes k, v (B, heads, n, hd) at positions base + pos_b + t of slot b (bcast: B = 1, into every slot). pos: an
@@ -920,7 +923,7 @@ class KV8Cache:
         if k.numel():
             k, v = _rows4(k), _rows4(v)
             _call_on(self.dev, "mx_kv8_append", k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3],
-                     *self._ptrs(), B, H, n, D, self.ctx, self.slots, int(bcast), pp, ps, base, cp, cstr, ptr(cs),
+                     *self.ptrs, B, H, n, D, self.ctx, self.slots, int(bcast), pp, ps, base, cp, cstr, ptr(cs),
                      0 if cs is None else cs.shape[0], *qa)
         return q_out
 
@@ -932,7 +935,7 @@ class KV8Cache:
         k = torch.empty(self.slots, self.heads, n, self.hd, device=self.dev, dtype=BF)
         v = torch.empty_like(k)
         if n:
-            _call_on(self.dev, "mx_kv8_read", *self._ptrs(), k.data_ptr(), v.data_ptr(), self.slots, self.heads, n, self.hd,
+            _call_on(self.dev, "mx_kv8_read", *self.ptrs, k.data_ptr(), v.data_ptr(), self.slots, self.heads, n, self.hd,
                      self.ctx)
         return k, v
 
@@ -974,9 +977,11 @@ def sdpa_kv8(q, cache, kv_len, base=0, out=None, scale=None, qpos0=None, causal_
             q = q.clone()
         s = q.stride()
     G = Hq // cache.heads
-    need = _lib.load().mx_kv8_sdpa_ws(B, cache.heads, G, Tq, cache.ctx, D)
+    need = cache._ws.get((B, G, Tq))
+    if need is None:
+        need = cache._ws[(B, G, Tq)] = _lib.load().mx_kv8_sdpa_ws(B, cache.heads, G, Tq, cache.ctx, D)
     part = torch.empty(need, device=dev, dtype=torch.float32) if need else None
-    _call_on(dev, "mx_kv8_sdpa", q.data_ptr(), s[0], s[1], s[2], *cache._ptrs(), out.data_ptr(), out.stride(0),
+    _call_on(dev, "mx_kv8_sdpa", q.data_ptr(), s[0], s[1], s[2], *cache.ptrs, out.data_ptr(), out.stride(0),
              out.stride(1), B, cache.heads, G, Tq, D, cache.ctx, lp, ls, base, 0 if qpos0 is None else int(qpos0),
              int(qpos0 is None), cf, sc, ptr(part), need)
     return out
