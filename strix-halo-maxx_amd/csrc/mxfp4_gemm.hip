@@ -495,6 +495,7 @@ int check(const void* wc, const void* ws, const float* bias, const uint16_t* R, 
   if (!wc || !ws || !C) return MX_ENULL;
   if (act < 0 || act > 2) return MX_EBADCFG;
   if (M < 1 || N < 1 || K < 1 || act_from < 0 || r_rows < 0 || (M > 1 && ldc < N)) return MX_ESHAPE;
+  if (N > 1 << 27) return MX_ESHAPE;  // few rows: 16 columns a workgroup of up to 512 threads, 2^32 threads in a grid
   if (R && ldr < 0) return MX_ESHAPE;
   if ((((uintptr_t)wc) & 15) || ((uintptr_t)ws & 3) || ((uintptr_t)bias & 3) || ((uintptr_t)R & 1) || ((uintptr_t)C & 1))
     return MX_ELAYOUT;

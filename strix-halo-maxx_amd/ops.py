@@ -701,11 +701,23 @@ def _rows2(x):
     return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
 
 
+def _apart(a, b):
+    """Whether the memory of the 2-D a, from its first element to its last, and that of b do not meet."""
+    p, q = a.data_ptr(), b.data_ptr()
+    return (p + ((a.shape[0] - 1) * a.stride(0) + a.shape[1]) * a.element_size() <= q
+            or q + ((b.shape[0] - 1) * b.stride(0) + b.shape[1]) * b.element_size() <= p)
+
+
 class MxFp4:
     """A matrix (rows, K) in MXFP4: 4-bit e2m1 codes and a power-of-two scale for each 32 columns of a row, in one buffer
     (uint8; the codes, then the scales, each in the order of the matrix instruction's operands)."""
 
     def __init__(self, data, rows, K):
+        need = MxFp4.cells(rows, K) * 4352
+        if rows < 0 or K < 1 or data.dtype != torch.uint8 or not data.is_contiguous() or data.numel() < need:
+            raise ValueError(f"({rows}, {K}) in MXFP4 takes {need} contiguous uint8, got {tuple(data.shape)} {data.dtype}")
+        if data.data_ptr() % 16:
+            raise ValueError("data must be 16-byte aligned")
         self.data, self.rows, self.K = data, rows, K
         self.dev = data.device
         p = data.data_ptr()
@@ -748,14 +760,17 @@ def quant_mxfp4(x):
 class MxFp4Lin:
     """MXFP4 Linear: y = act(x W^T + b) [+ res] with W quantised once and x per call (quant_mxfp4's rule for both), on the
     scaled MFMA; fp32 throughout, rounded to bf16 once. `pre` takes an already quantised input (MxFp4), so layers that
-    read the same activation share one quantisation. Any (N, K). act: None / "tanh" / "erf", on columns >= act_from.
-    Few rows are quantised inside the product's launch; the results are the same."""
+    read the same activation share one quantisation. Any (N, K); inputs have K columns, or K rounded up to 8 (Kp), of
+    which the first K are read. act: None / "tanh" / "erf", on columns >= act_from. `out` may be x or res itself. Few rows
+    are quantised inside the product's launch; the results are the same."""
     fused_gelu = True
     fused_res = True
 
     def __init__(self, weight, bias, dtype=BF, device="cuda"):
         if dtype != BF:
             raise ValueError("bf16 activations only")
+        if weight.dim() != 2:
+            raise ValueError(f"weight must be (N, K), got {tuple(weight.shape)}")
         self._set(quant_mxfp4(weight.detach().to(device=device, dtype=BF)), bias)
 
     @classmethod
@@ -767,6 +782,7 @@ class MxFp4Lin:
 
     def _set(self, w, bias):
         self.wq, self.N, self.K = w, w.rows, w.K
+        self.Kp = (w.K + 7) // 8 * 8  # the input width MxLin asks for
         self.dev = w.dev
         if self.N < 1:
             raise ValueError("the weight needs at least one row")
@@ -788,7 +804,9 @@ class MxFp4Lin:
         N, K = self.N, self.K
         if pre is None:
             if x.shape[-1] != K:
-                raise ValueError(f"input width {x.shape[-1]} != {K}")
+                if x.shape[-1] != self.Kp:
+                    raise ValueError(f"input width {x.shape[-1]} != {K}")
+                x = x[..., :K]
             _need(x, "x", self.dev)
             x2 = _rows2(x)
             M = x2.shape[0]
@@ -819,7 +837,7 @@ class MxFp4Lin:
                 r_rows = r2.shape[0]
         if M:
             tail = (*self.wq.ptrs, self.bp, None if r2 is None else r2.data_ptr(), ldr, r_rows, y2.data_ptr(), y2.stride(0), M, N, K, a, act_from)
-            if pre is None and M <= self.rows:
+            if pre is None and M <= self.rows and (out is None or _apart(x2, y2)):
                 _call_on(self.dev, "mx_gemv_mxfp4", x2.data_ptr(), x2.stride(0), *tail)
             else:
                 q = quant_mxfp4(x2) if pre is None else pre
@@ -830,13 +848,19 @@ class MxFp4Lin:
 
 
 def _where(v, B, dev, name):
-    """(pointer, stride, base) of a position or length: an int, or an int32 tensor of B values."""
+    """(pointer, stride, value) of a position or length: an int, or an int32 tensor of B values."""
     if isinstance(v, torch.Tensor):
         if v.dim() != 1 or v.shape[0] != B:
             raise ValueError(f"{name} must be an int or a tensor of {B} values")
         _need(v, name, dev, torch.int32)
         return v.data_ptr(), v.stride(0), 0
     return None, 0, int(v)
+
+
+def _int32(v, name):
+    if not -0x80000000 <= v <= 0x7fffffff:
+        raise ValueError(f"{name} {v} does not fit 32 bits")
+    return v
 
 
 def _rows4(t):
@@ -898,7 +922,7 @@ class KV8Cache:
         _need(k, "k", self.dev)
         _need(v, "v", self.dev)
         pp, ps, p0 = _where(pos, B, self.dev, "pos")
-        base = int(base) + p0
+        base = _int32(int(base) + p0, "base")
         if pp is None and not 0 <= base <= self.ctx - n:
             raise ValueError(f"positions {base} .. {base + n - 1} outside the {self.ctx}-entry cache")
         cp, cstr, _ = (None, 0, 0) if count is None else _where(count, B, self.dev, "count")
@@ -946,22 +970,24 @@ def sdpa_kv8(q, cache, kv_len, base=0, out=None, scale=None, qpos0=None, causal_
 
     kv_len: an int, or an int32 tensor (B,) read on the device (values outside 0 .. ctx are clamped). Mask, as in sdpa:
     key j is visible to query i iff j < len_b and (j < causal_from or j <= qpos0 + i); causal_from=None: no mask;
-    qpos0=None: the queries are the last Tq tokens of their sequence, qpos0 = len_b - Tq. Rows that see no key are 0."""
+    qpos0=None: the queries are the last Tq tokens of their sequence, qpos0 = len_b - Tq. Rows that see no key are 0.
+    Scores (times scale) have to stay below 2^29 in size: larger ones come out as 0 or NaN."""
     if q.dim() != 4 or q.shape[3] != cache.hd or q.shape[1] < 1 or q.shape[1] % cache.heads or q.shape[0] > cache.slots:
         raise ValueError(f"q {tuple(q.shape)} does not fit a cache of {cache.slots} x {cache.heads} heads x {cache.hd}")
     B, Hq, Tq, D = q.shape
     dev = cache.dev
     _need(q, "q", dev)
     lp, ls, l0 = _where(kv_len, B, dev, "kv_len")
-    base = int(base) + l0
+    base = _int32(int(base) + l0, "base")
     if lp is None and not 0 <= base <= cache.ctx:
         raise ValueError(f"length {base} outside the {cache.ctx}-entry cache")
     sc = D ** -0.5 if scale is None else float(scale)
     if not 0.0 < sc < float("inf"):
         raise ValueError(f"scale {sc} must be positive and finite")
-    cf = 0x7fffffff if causal_from is None else int(causal_from)
+    cf = 0x7fffffff if causal_from is None else min(int(causal_from), 0x7fffffff)
     if cf < 0:
         raise ValueError("causal_from must not be negative")
+    q0 = 0 if qpos0 is None else max(-0x80000000, min(int(qpos0), 0x7fffffff))  # positions all lie inside 31 bits
     if out is None:
         out = torch.empty(B, Tq, Hq * D, device=dev, dtype=BF)
     else:
@@ -982,8 +1008,7 @@ def sdpa_kv8(q, cache, kv_len, base=0, out=None, scale=None, qpos0=None, causal_
         need = cache._ws[(B, G, Tq)] = _lib.load().mx_kv8_sdpa_ws(B, cache.heads, G, Tq, cache.ctx, D)
     part = torch.empty(need, device=dev, dtype=torch.float32) if need else None
     _call_on(dev, "mx_kv8_sdpa", q.data_ptr(), s[0], s[1], s[2], *cache.ptrs, out.data_ptr(), out.stride(0),
-             out.stride(1), B, cache.heads, G, Tq, D, cache.ctx, lp, ls, base, 0 if qpos0 is None else int(qpos0),
-             int(qpos0 is None), cf, sc, ptr(part), need)
+             out.stride(1), B, cache.heads, G, Tq, D, cache.ctx, lp, ls, base, q0, int(qpos0 is None), cf, sc, ptr(part), need)
     return out
 
 

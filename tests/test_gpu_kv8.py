@@ -348,3 +348,70 @@ def test_step_in_a_graph(dev, n, D, G):
             torch.cuda.synchronize()
         for x, z in zip(a.read(), b.read()):
             assert torch.equal(x, z)
+
+
+def test_offsets_past_32_bits(dev):
+    """Codes beyond 4 GB: the last slot's last tokens are written, read by attention, and the rest stays as it was. Every
+    other key is zero, so it weighs exp(0) and adds nothing; the reference counts them."""
+    g = gen(41)
+    H, D, n = 17, 128, 300
+    ctx = (1 << 20) - 5
+    c = ops.KV8Cache(2, H, ctx, D, device=dev)
+    k, v, q = rows(g, 2, H, n, D), rows(g, 2, H, n, D), rows(g, 2, 2 * H, 20, D)
+    c.append(k.to(dev), v.to(dev), i32(dev, 0, ctx - n))
+    assert c.kc.numel() > 1 << 32
+    ko, vo = ol.KV8(1, H, 320, D), ol.KV8(1, H, 320, D)
+    off = (ctx - n) % 64
+    ko.append(0, k[1], off), vo.append(0, v[1], off)
+    kk, vv = ko.val[0, :, off:off + n].to(F64), vo.val[0, :, off:off + n].to(F64)
+    for Tq in (1, 20):
+        y = ops.sdpa_kv8(q[:, :, :Tq].to(dev).contiguous(), c, ctx).to(F64).view(2, Tq, 2 * H, D).cpu()
+        for h in (0, 2 * H - 1):
+            qq = q[1, h, :Tq].to(F64)
+            s = torch.matmul(qq, kk[h // 2].t().contiguous()) * D ** -0.5
+            size = (torch.matmul(qq.abs(), kk[h // 2].t().abs().contiguous()) * D ** -0.5).amax(-1, keepdim=True)
+            m = s.amax(-1, keepdim=True).clamp_min(0)
+            p = torch.exp(s - m)
+            l = p.sum(-1, keepdim=True) + (ctx - n) * torch.exp(-m)
+            ref, avg = torch.matmul(p, vv[h // 2]) / l, torch.matmul(p, vv[h // 2].abs()) / l
+            tol = 2.0 ** -8 * ref.abs() + (2.0 ** -8 + 2.0 ** -12 + 2 * 2.0 ** -12 * (1 + size)) * avg
+            # the fp32 running sums of a million weights: at most 2^14 terms each before they are joined
+            tol = tol + 2.0 ** -10 * avg
+            err = ((y[1, :, h] - ref).abs() - tol).max().item()
+            assert err <= 0, (Tq, h, err)
+    blk = (ctx - n) // 64
+    assert not bool(c.kc[1, :, :blk].any()) and not bool(c.kc[0, :, 5:].any()) and not bool(c.ks[1, :, :blk].any())
+
+
+def test_two_calls_at_once(dev):
+    """Attention over one cache from two streams at the same time, each cut into runs of keys: every call has its own
+    workspace."""
+    g = gen(43)
+    H, D, n = 4, 64, 9000
+    c = ops.KV8Cache(1, H, n, D, device=dev)
+    c.append(rows(g, 1, H, n, D).to(dev), rows(g, 1, H, n, D).to(dev), 0)
+    qs = [rows(g, 1, H, 1, D).to(dev) for _ in range(2)]
+    want = [ops.sdpa_kv8(q, c, n) for q in qs]
+    torch.cuda.synchronize()
+    st = [torch.cuda.Stream() for _ in qs]
+    got = [[], []]
+    for _ in range(20):
+        for i in (0, 1):
+            with torch.cuda.stream(st[i]):
+                got[i].append(ops.sdpa_kv8(qs[i], c, n))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        assert all(torch.equal(y, want[i]) for y in got[i])
+
+
+def test_far_positions_and_masks(dev):
+    """Mask positions beyond 32 bits mean what they say: every key, or none."""
+    g = gen(44)
+    c = Both(dev, 1, 2, 100, 64)
+    c.append(rows(g, 1, 2, 100, 64), rows(g, 1, 2, 100, 64), 0)
+    q = rows(g, 1, 2, 40, 64)
+    full = ops.sdpa_kv8(q.to(dev), c.c, 100)
+    for kw in (dict(causal_from=2 ** 33), dict(causal_from=0, qpos0=2 ** 32 + 5), dict(causal_from=0, qpos0=2 ** 31 - 1)):
+        assert torch.equal(ops.sdpa_kv8(q.to(dev), c.c, 100, **kw), full), kw
+    for q0 in (-2 ** 31, -2 ** 32 + 50):
+        assert not bool(ops.sdpa_kv8(q.to(dev), c.c, 100, causal_from=0, qpos0=q0).any()), q0

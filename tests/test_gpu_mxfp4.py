@@ -173,3 +173,58 @@ def test_linear_in_a_graph_and_on_a_side_stream(dev, M):
         gr.replay()
         assert torch.equal(y, want[s - 1])
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("M", [3, 200])
+def test_linear_onto_its_own_input_and_residual(dev, M):
+    """out may be x (few rows: every workgroup reads all of x, so the product must not write it) or res."""
+    g = gen(M + 1)
+    w = (torch.randn(512, 512, generator=g) * 0.1).to(BF)
+    lin = ops.MxFp4Lin(w, None, device=dev)
+    x = torch.randn(M, 512, generator=g).to(BF).to(dev)
+    want, add = lin(x), lin(x, res=x)
+    buf = x.clone()
+    assert lin(buf, out=buf) is buf and torch.equal(buf, want)
+    buf = x.clone()
+    lin(x, res=buf, out=buf)
+    assert torch.equal(buf, add)
+    row = torch.zeros(M, 1024, device=dev, dtype=BF)  # x and out side by side in the rows of one buffer
+    row[:, :512] = x
+    lin(row[:, :512], out=row[:, 512:])
+    assert torch.equal(row[:, 512:], want) and torch.equal(row[:, :512], x)
+
+
+def test_vision_tower_takes_it(dev):
+    """The Linear as the tower's lin_cls: the patch embedding (588 columns, read from rows padded to 592, its residual the
+    positions) against the formula, and a block."""
+    import strix_halo_maxx_amd.md2 as md2
+    import strix_halo_maxx_amd.synth as S
+    w = S.vision_weights(0, layers=1)
+    vt = md2.VisionTower(w, lin_cls=ops.MxFp4Lin)
+    img = S.images_u8(3, 2).to(dev)
+    a = ops.patchify(img, vt.P, mode=0, ldo=592)
+    emb = vt.embed(img)
+    ref, mag = ol.mxfp4_linear(a[:, :588].cpu(), w["patch_emb.weight"].to(BF), w["patch_emb.bias"].to(BF))
+    close(emb.cpu(), ref + w["pos_emb"].to(BF).view(-1, ref.shape[1]).to(F64).repeat(2, 1), mag)
+    y = vt(img)
+    assert y.shape == (2, 729, 1152) and bool(y.isfinite().all())
+
+
+def test_offsets_past_32_bits(dev):
+    """Inputs, codes and outputs beyond 4 GB: the last rows are those of a short call."""
+    M, K = 300_017, 8192
+    x = torch.zeros(M, K, device=dev, dtype=BF)
+    x[-70:] = torch.randn(70, K, generator=gen(5)).to(BF).to(dev)
+    q = ops.quant_mxfp4(x)
+    y = q.values(out=x)  # 4.9 GB
+    tail = ops.quant_mxfp4(y[-70:].contiguous()).values()
+    assert torch.equal(y[-70:], tail) and not bool(y[:1000].any())
+    del q, y, x
+    w = (torch.randn(8192, 640, generator=gen(6)) * 0.1).to(BF)
+    lin = ops.MxFp4Lin(w, None, device=dev)
+    x = torch.zeros(M, 640, device=dev, dtype=BF)
+    x[-70:] = torch.randn(70, 640, generator=gen(7)).to(BF).to(dev)
+    ref, mag = ol.mxfp4_linear(x[-70:].cpu(), w)
+    y = lin(x)
+    close(y[-70:].cpu(), ref, mag)
+    assert not bool(y[:1000].any()) and not bool(y[150_000:151_000].any())

@@ -154,3 +154,40 @@ def test_python_refusals():
     raises("out must", ops.sdpa_kv8, q, c, 5, out=torch.zeros(2, 3, 255, dtype=BF))
     raises("GPU", ops.sdpa_kv8, q, c, 5)
     assert c.append(k[:, :, :0], k[:, :, :0], 100) is None and ops.sdpa_kv8(q[:, :, :0], c, 5).shape == (2, 0, 256)
+
+
+def test_buffers_that_do_not_hold_the_matrix():
+    z = lambda n, dt=torch.uint8: torch.zeros(n, dtype=dt)
+    assert ops.MxFp4(z(4352), 64, 128).K == 128
+    raises("takes 4352", ops.MxFp4, z(4351), 10, 64)
+    raises("takes 8704", ops.MxFp4, z(4352), 65, 64)
+    raises("takes 8704", ops.MxFp4, z(4352), 3, 129)
+    raises("takes 4352", ops.MxFp4, z(4352, torch.int8), 10, 64)
+    raises("takes 4352", ops.MxFp4, z(8704)[::2], 10, 64)
+    raises("in MXFP4", ops.MxFp4, z(4352), 10, 0)
+    raises("in MXFP4", ops.MxFp4, z(4352), -1, 64)
+    raises("aligned", ops.MxFp4, z(4400)[3:], 10, 64)
+    raises("weight must", ops.MxFp4Lin, torch.zeros(64, dtype=BF), None)
+    raises("weight must", ops.MxFp4Lin, torch.zeros(2, 3, 64, dtype=BF), None)
+
+
+def test_values_past_32_bits():
+    c = ops.KV8Cache(1, 1, 100, 64, device="cpu")
+    k, p = torch.zeros(1, 1, 5, 64, dtype=BF), torch.zeros(1, dtype=torch.int32)
+    raises("32 bits", c.append, k, k, p, base=2 ** 32)
+    raises("32 bits", c.append, k, k, 2 ** 31)
+    raises("32 bits", ops.sdpa_kv8, k, c, p, base=-2 ** 31 - 1)
+    lib = _lib.load()
+    tail = dict(wc=A16, ws=A16, b=None, R=None, ldr=0, rr=0, C=A16, ldc=2 ** 28, M=4, N=2 ** 27 + 1, K=64, act=0, af=0)
+    assert lib.mx_gemv_mxfp4(*{**dict(st=None, x=A16, ldx=64), **tail}.values()) == -2  # 2^32 threads in a grid
+    assert lib.mx_gemm_mxfp4(*{**dict(st=None, xc=A16, xs=A16), **tail}.values()) == -2
+
+
+def test_widths_that_the_linear_takes():
+    lin = ops.MxFp4Lin.from_quantized(ops.MxFp4(torch.zeros(5 * 4352, dtype=torch.uint8), 10, 588), None)
+    assert lin.Kp == 592
+    x = torch.zeros(3, 600, dtype=BF)
+    raises("GPU", lin, x[:, :588])
+    raises("GPU", lin, x[:, :592])
+    raises("width 600", lin, x)
+    raises("width 590", lin, x[:, :590])
