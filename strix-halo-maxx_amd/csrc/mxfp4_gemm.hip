@@ -57,17 +57,21 @@ __device__ __forceinline__ void mx4_store(const Mx4Epi& p, int m, int n, f32x4 v
 
 // ---------------------------------------------------------------------------------------------- few rows
 // 16 MT rows per workgroup (grid y). It owns 16 columns of C (16 rows of W); its waves take the groups of 512 columns of K in
-// turn (4 KB of W each, read in one piece) and their sums meet in LDS. PRE = false: x arrives in bf16 and each wave
-// quantises the 512 columns it multiplies (its own slice: no wave waits for another before the end).
-template <int NW, int MT, bool PRE, int ACT>
-__global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(const uint16_t* __restrict__ x, long ldx, int vecx,
+// turn (4 KB of W each, read in one piece) and their sums meet in LDS. PRE = false: x arrives in bf16, XR rows at most (XV:
+// rows that 16-byte loads may read), and each wave quantises the 512 columns it multiplies (its own slice: no wave waits
+// for another before the end). The bound is the fetch of W from HBM behind one latency: us for 1 / 8 / 16 / 64 rows, weights
+// not in any cache, 2048 x 10240 5.7 / 9.4 / 6.6 / 10.0 (11 MB; 9.9 / 13.3 / 9.9 / 14.7 with branches around the loads, which
+// then wait for each other), 8192 x 2048 4.8 / 6.3 / 4.9 / 6.5, 768 x 768 2.8 / 4.1 / 2.9 / 3.8 (a launch alone takes about
+// 2). With 8 rows the quantisation, which every workgroup repeats, takes the time.
+template <int NW, int MT, bool PRE, int XR, bool XV, int ACT>
+__global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(const uint16_t* __restrict__ x, long ldx,
                                                            const uint8_t* __restrict__ xc,
                                                            const uint32_t* __restrict__ xs,
                                                            const uint8_t* __restrict__ wc,
                                                            const uint32_t* __restrict__ ws, int K, Mx4Epi p) {
   static_assert(PRE || MT == 1, "bf16 rows come in one tile");
-  __shared__ __attribute__((aligned(16))) uint32_t xq[PRE ? 1 : NW][GEMV_ROWS][64];  // a row's codes of the wave's columns
-  __shared__ __attribute__((aligned(16))) uint8_t xsc[PRE ? 1 : NW][GEMV_ROWS][16];  // its scale bytes, [block % 4][step]
+  __shared__ __attribute__((aligned(16))) uint32_t xq[PRE ? 1 : NW][XR][64];  // a row's codes of the wave's columns
+  __shared__ __attribute__((aligned(16))) uint8_t xsc[PRE ? 1 : NW][XR][16];  // its scale bytes, [block % 4][step]
   __shared__ f32x4 red[NW][MT][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nk = mx4_nk(K), nks = (nk + 3) / 4;
@@ -85,68 +89,93 @@ __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(const uint16_t* __res
   f32x4 acc[MT];
 #pragma unroll
   for (int i = 0; i < MT; i++) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int ks = wave; ks < nks; ks += NW) {
-    u32x4 w[4], b[MT][4];
-    int sw[4], sx[MT][4];
+  // What a step reads. The loads have no branches (past the end they repeat the last place and x counts as zero), so the
+  // compiler can count them: the next step's are in flight while this one's are multiplied.
+  struct Step {
+    u32x4 w[4], x[PRE ? MT : 1][PRE ? 4 : XR];  // W; x: its codes, or its rows in bf16
+    int sw[4], sx[PRE ? MT : 1][4];
+  };
+  auto fetch = [&](Step& q, int ks) {
     const int left = nk - 4 * ks;
     const uint8_t* wt = codes(wc, nt) + (long)ks * 8192;
 #pragma unroll
     for (int t = 0; t < 4; t++) {
-      w[t] = u32x4{0u, 0u, 0u, 0u};
-      sw[t] = 0;
-      if (t < left) {
-        w[t] = *reinterpret_cast<const u32x4*>(wt + t * 2048);
-        sw[t] = scale(ws, nt, 4 * ks + t);
-      }
+      const int u = min(t, left - 1);
+      q.w[t] = *reinterpret_cast<const u32x4*>(wt + u * 2048);
+      q.sw[t] = scale(ws, nt, 4 * ks + u);
     }
     if constexpr (PRE) {
 #pragma unroll
       for (int i = 0; i < MT; i++) {
-        const uint8_t* xt = codes(xc, mt + i) + (long)ks * 8192;
-        const bool on = 16 * (mt + i) < p.M;
+        const int ut = min(mt + i, (p.M - 1) / 16);
+        const uint8_t* xt = codes(xc, ut) + (long)ks * 8192;
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-          b[i][t] = u32x4{0u, 0u, 0u, 0u};
-          sx[i][t] = 0;
-          if (on && t < left) {
-            b[i][t] = *reinterpret_cast<const u32x4*>(xt + t * 2048);
-            sx[i][t] = scale(xs, mt + i, 4 * ks + t);
-          }
+          const int u = min(t, left - 1);
+          q.x[i][t] = *reinterpret_cast<const u32x4*>(xt + u * 2048);
+          q.sx[i][t] = scale(xs, ut, 4 * ks + u);
         }
       }
     } else {
-      const int blk = lane >> 2, k = ks * 512 + lane * 8;
-      u32x4 v[GEMV_ROWS];
+      const int k = ks * 512 + lane * 8;
 #pragma unroll
-      for (int m = 0; m < GEMV_ROWS; m++) {
-        v[m] = u32x4{0u, 0u, 0u, 0u};
-        if (m < p.M && k < K) v[m] = load8(x + m * ldx, k, K, vecx);
+      for (int m = 0; m < XR; m++) {
+        const uint16_t* row = x + min(m, p.M - 1) * ldx;
+        if constexpr (XV)
+          q.x[0][m] = *reinterpret_cast<const u32x4*>(row + min(k, K - 8));
+        else
+          q.x[0][m] = load8(row, k, K, false);
       }
+    }
+  };
+  auto multiply = [&](Step& q, int ks) {
+    const int left = nk - 4 * ks;
+    const u32x4 none = {0u, 0u, 0u, 0u};
+    if constexpr (PRE) {
 #pragma unroll
-      for (int m = 0; m < GEMV_ROWS; m++) {
-        if (m >= p.M) break;
-        const uint32_t byte = mx4_scale_byte(quad_max(amax8(v[m])));
-        xq[wave][m][lane] = byte == 255u ? 0u : mx4_pack8(v[m], e8m0_float(byte));
+      for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+          acc[i] = mfma_mx4(q.w[t], t < left ? q.x[i][t] : none, acc[i], q.sw[t], t < left ? q.sx[i][t] : 0);
+    } else {
+      const int blk = lane >> 2, k = ks * 512 + lane * 8;
+#pragma unroll
+      for (int m = 0; m < XR; m++) {
+        const u32x4 v = k < K ? q.x[0][m] : none;
+        const uint32_t byte = mx4_scale_byte(quad_max(amax8(v)));
+        xq[wave][m][lane] = byte == 255u ? 0u : mx4_pack8(v, e8m0_float(byte));
         if ((lane & 3) == 0) xsc[wave][m][(blk & 3) * 4 + (blk >> 2)] = (uint8_t)byte;
       }
       // the wave reads only what it wrote: in order, once its LDS writes are done
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_wave_barrier();
-      const bool on = r16 < p.M;
-      const uint32_t s4 = on ? *reinterpret_cast<const uint32_t*>(&xsc[wave][r16][g * 4]) : 0u;
+      const int r = min(r16, XR - 1);  // rows of the operand past XR meet no result that is stored
+      const uint32_t s4 = *reinterpret_cast<const uint32_t*>(&xsc[wave][r][g * 4]);
+      u32x4 b[4];
 #pragma unroll
-      for (int t = 0; t < 4; t++) {
-        b[0][t] = u32x4{0u, 0u, 0u, 0u};
-        if (on) b[0][t] = *reinterpret_cast<const u32x4*>(&xq[wave][r16][(4 * t + g) * 4]);
-        sx[0][t] = (int)(s4 >> (8 * t));
-      }
+      for (int t = 0; t < 4; t++) b[t] = *reinterpret_cast<const u32x4*>(&xq[wave][r][(4 * t + g) * 4]);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int t = 0; t < 4; t++) acc[0] = mfma_mx4(q.w[t], b[t], acc[0], q.sw[t], (int)(s4 >> (8 * t)));
     }
-#pragma unroll
-    for (int t = 0; t < 4; t++)
-#pragma unroll
-      for (int i = 0; i < MT; i++) acc[i] = mfma_mx4(w[t], b[i][t], acc[i], sw[t], sx[i][t]);
+  };
+  if (wave < nks) {
+    Step cur;
+    fetch(cur, wave);
+    int ks = wave;
+    for (; ks + NW < nks; ks += NW) {
+      if constexpr (MT == 1) {
+        Step nxt;
+        fetch(nxt, ks + NW);
+        multiply(cur, ks);
+        cur = nxt;
+      } else {  // (the registers of two steps would not fit)
+        multiply(cur, ks);
+        fetch(cur, ks + NW);
+      }
+    }
+    multiply(cur, ks);
   }
 #pragma unroll
   for (int i = 0; i < MT; i++) red[wave][i][lane] = acc[i];
@@ -507,23 +536,22 @@ Mx4Epi epi(const float* bias, const uint16_t* R, long ldr, int r_rows, uint16_t*
   return Mx4Epi{bias, R, ldr, r_rows, C, ldc, M, N, act_from, vec};
 }
 
-template <int MT, bool PRE>
-hipError_t launch_rows(hipStream_t st, const uint16_t* x, long ldx, int vecx, const uint8_t* xc, const uint8_t* xs,
-                       const uint8_t* wc, const uint8_t* ws, int K, int act, const Mx4Epi& p) {
+template <int MT, bool PRE, int XR, bool XV>
+hipError_t launch_rows(hipStream_t st, const uint16_t* x, long ldx, const uint8_t* xc, const uint8_t* xs, const uint8_t* wc,
+                       const uint8_t* ws, int K, int act, const Mx4Epi& p) {
   const dim3 grid((unsigned)((p.N + 15L) / 16), (unsigned)((p.M + 16L * MT - 1) / (16 * MT)));
   auto go = [&](auto kern, int nw) {
-    hipLaunchKernelGGL(kern, grid, dim3(64 * nw), 0, st, x, ldx, vecx, xc, (const uint32_t*)xs, wc, (const uint32_t*)ws, K,
-                       p);
+    hipLaunchKernelGGL(kern, grid, dim3(64 * nw), 0, st, x, ldx, xc, (const uint32_t*)xs, wc, (const uint32_t*)ws, K, p);
     return hipGetLastError();
   };
   if (mx4_nk(K) <= 16) {
-    if (act == 0) return go(mx4_rows_kernel<4, MT, PRE, 0>, 4);
-    if (act == 1) return go(mx4_rows_kernel<4, MT, PRE, 1>, 4);
-    return go(mx4_rows_kernel<4, MT, PRE, 2>, 4);
+    if (act == 0) return go(mx4_rows_kernel<4, MT, PRE, XR, XV, 0>, 4);
+    if (act == 1) return go(mx4_rows_kernel<4, MT, PRE, XR, XV, 1>, 4);
+    return go(mx4_rows_kernel<4, MT, PRE, XR, XV, 2>, 4);
   }
-  if (act == 0) return go(mx4_rows_kernel<8, MT, PRE, 0>, 8);
-  if (act == 1) return go(mx4_rows_kernel<8, MT, PRE, 1>, 8);
-  return go(mx4_rows_kernel<8, MT, PRE, 2>, 8);
+  if (act == 0) return go(mx4_rows_kernel<8, MT, PRE, XR, XV, 0>, 8);
+  if (act == 1) return go(mx4_rows_kernel<8, MT, PRE, XR, XV, 1>, 8);
+  return go(mx4_rows_kernel<8, MT, PRE, XR, XV, 2>, 8);
 }
 
 }  // namespace
@@ -539,9 +567,13 @@ extern "C" int mx_gemv_mxfp4(hipStream_t st, const uint16_t* x, long ldx, const 
   if (rc) return rc;
   if (M > GEMV_ROWS || ldx < 0) return MX_ESHAPE;
   if ((uintptr_t)x & 1) return MX_ELAYOUT;
-  const int vecx = !((uintptr_t)x & 15) && ldx % 8 == 0;
-  const hipError_t e = launch_rows<1, false>(st, x, ldx, vecx, nullptr, nullptr, wc, ws, K, act,
-                                             epi(bias, R, ldr, r_rows, C, ldc, M, N, act_from));
+  const bool vec = !((uintptr_t)x & 15) && ldx % 8 == 0 && K % 8 == 0;
+  const Mx4Epi p = epi(bias, R, ldr, r_rows, C, ldc, M, N, act_from);
+  auto go = [&](auto launch) { return launch(st, x, ldx, nullptr, nullptr, wc, ws, K, act, p); };
+  const hipError_t e = !vec     ? go(launch_rows<1, false, GEMV_ROWS, false>)
+                       : M == 1 ? go(launch_rows<1, false, 1, true>)
+                       : M <= 4 ? go(launch_rows<1, false, 4, true>)
+                                : go(launch_rows<1, false, GEMV_ROWS, true>);
   return e == hipSuccess ? MX_OK : MX_ELAUNCH;
 }
 
@@ -555,10 +587,10 @@ extern "C" int mx_gemm_mxfp4(hipStream_t st, const uint8_t* xc, const uint8_t* x
   const Mx4Epi p = epi(bias, R, ldr, r_rows, C, ldc, M, N, act_from);
   hipError_t e;
   // Which kernel, by the grid it makes (us on one MI355X; N x K after the rows):
-  //  * the few-row kernel up to 64 rows, and beyond while its grid (16 columns x 64 rows each) is one workgroup per CU, two
-  //    with the 4 waves of K <= 2048: a CU fetches about 20 bytes a clock, so the product of few rows goes as fast as its
-  //    weights are spread. Against 64 x 64 tiles: 64 rows, 2048 x 8192 8.4 / 15.2, 192 rows 15.0 / 15.7; 256 rows, 2048 x
-  //    2048 6.7 / 7.5, 512 rows 10.9 / 7.7;
+  //  * the few-row kernel up to 32 rows, and beyond while its grid (16 columns x 64 rows each) is at most two workgroups per
+  //    CU: a CU fetches about 20 bytes a clock, so the product of few rows goes as fast as its weights are spread. Against
+  //    tiles, weights from HBM: 2048 x 8192, 64 rows 8.8 / 17.4, 256 rows 14.3 / 17.2, 384 rows 19.8 / 17.5; 2048 x 2048, 256
+  //    rows 5.3 / 6.7, 384 rows 7.6 / 6.9; 64 rows, 8192 x 2048 6.5 / 7.6, 14336 x 2048 10.6 / 8.2;
   //  * the smallest tile whose grid is at most one workgroup per CU, for the same reason (64 x 64, 64 x 128, 128 x 128,
   //    128 x 256): 512 rows, 2048 x 2048 7.9 / 9.4 / 10.4 / 14.6; 256 rows, 8192 x 2048 10.5 / 10.0 / 10.8 / 14.7;
   //  * 128 x 128 below two full rounds of 128 x 256: 4096 rows, 4304 x 1152 30.2 / 26.6 / 22.6 / 25.7;
@@ -568,12 +600,12 @@ extern "C" int mx_gemm_mxfp4(hipStream_t st, const uint8_t* xc, const uint8_t* x
   const int nk = mx4_nk(K);
   if (tiles(64, 64) > 0x3fffffffL || nk > (1 << 15)) return MX_ESHAPE;
   if (M <= 16) {
-    e = launch_rows<1, true>(st, nullptr, 0, 0, xc, xs, wc, ws, K, act, p);
+    e = launch_rows<1, true, 1, true>(st, nullptr, 0, xc, xs, wc, ws, K, act, p);
   } else if (M <= 32) {
-    e = launch_rows<2, true>(st, nullptr, 0, 0, xc, xs, wc, ws, K, act, p);
-  } else if (M <= 64 || tiles(64, 16) <= (nk <= 16 ? 512 : 256) || nk <= 2) {
+    e = launch_rows<2, true, 1, true>(st, nullptr, 0, xc, xs, wc, ws, K, act, p);
+  } else if (tiles(64, 16) <= 512 || nk <= 2) {
     if (M > 64 * 65535) return MX_ESHAPE;  // (nk <= 2: the tiles' loads run at most one tile ahead, so they need more steps)
-    e = launch_rows<4, true>(st, nullptr, 0, 0, xc, xs, wc, ws, K, act, p);
+    e = launch_rows<4, true, 1, true>(st, nullptr, 0, xc, xs, wc, ws, K, act, p);
   } else if (nk <= 4) {
     e = launch_ring<2, 2, 2, 8>(st, xc, xs, wc, ws, K, act, p);
   } else if (tiles(64, 64) <= 256) {
