@@ -654,7 +654,12 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Attn8Args p, long nrec) {
 
 // How a problem is cut: rw rows per workgroup (16: the few-row kernel), nkw key waves, nrt row groups, `splits` runs of
 // `chunk` blocks. us on one MI355X (query waves x key waves; sequences x key heads x group, head dim, queries, keys):
-//  * up to 32 rows: the few-row kernel; runs of keys until there are 3 workgroups per CU (a CU holds 2 or 3);
+//  * up to 32 rows: the few-row kernel; runs of keys until there are 3 workgroups per CU (a CU holds 2 or 3), of 16 blocks
+//    at least. Where those leave half of the CUs idle, runs of 8 (the join costs 3 us; caches that no other call has just
+//    read: 1 x 8 x 4, 128, 1, 4000 11.0, runs of 16 13.0; 4 x 8 x 4, 128, 1, 2000 11.6 / 13.6), or one run up to 24 blocks (1
+//    x 32 x 1, 64, 1, 1100 7.5, two runs 9.2; 4 x 8 x 4, 128, 1, 1536 12.3, runs of 8 11.2). 8 waves instead of 4 where
+//    there is at most one workgroup per CU (8 x 32 x 1, 64, 1, 794 7.4 / 8.1; with 512 workgroups, 64 x 8 x 4, 128, 1, 1000,
+//    24.8 / 23.8);
 //  * 4 x 1 where 128-row groups give two workgroups per CU: 4 x 8 x 4, 128, 512, 512 30.2 (4 x 2 37.7, 2 x 2 37.4);
 //  * 4 x 2 down to three quarters of one per CU: 1 x 8 x 4, 128, 1024, 8000 152 (4 x 1 209, 2 x 4 183, 1 x 4 314);
 //  * 2 x 4, 64-row groups, down to the same: 1 x 8 x 4, 128, 512, 4000 54 (4 x 2 70, 1 x 4 92);
@@ -671,7 +676,7 @@ Plan plan(int B, int H, int G, int Tq, int ctx, int D) {
   const int nb = kv8_blocks(ctx);
   const auto cells = [&](int rw) { return (long)B * H * ((R + rw - 1) / rw); };
   if (R <= 32) {
-    q.rw = 16, q.nkw = 4;  // 8 below, where the runs leave CUs idle
+    q.rw = 16, q.nkw = 4;
   } else if (cells(128) >= 512) {
     q.rw = 128, q.nkw = 1;
   } else if (cells(128) >= 192) {
@@ -686,7 +691,8 @@ Plan plan(int B, int H, int G, int Tq, int ctx, int D) {
   const long n = cells(q.rw);
   q.nrt = (int)((R + q.rw - 1) / q.rw);
   long sp = q.rw == 16 ? (768 + n - 1) / n : n <= 128 ? 256 / n : 1;
-  const long most = (nb + 15) / 16;
+  long most = (nb + 15) / 16;
+  if (q.rw == 16 && n * most <= 128) most = nb <= 24 ? 1 : (nb + 7) / 8;
   if (sp > most) sp = most;
   if (sp > 1024) sp = 1024;
   if (sp < 1) sp = 1;
