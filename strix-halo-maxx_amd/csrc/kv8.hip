@@ -20,7 +20,7 @@ struct AppendArgs {
   const int *pos, *count;
   const float* cs;
   long pos_s, count_s;
-  int H, Hq, n, ctx, base, ncs, bcast, nslots, vec;
+  int H, Hq, n, ctx, base, ncs, bcast, nslots;
 };
 
 // Four codes times 2^-d (d > 0), rounded again.
@@ -43,17 +43,15 @@ __device__ __forceinline__ uint32_t amax_fin(uint32_t w) {
 // 1 / 2^(byte - 127); byte 0: 2^127, byte 254 does not occur (bf16 needs at most 247)
 __device__ __forceinline__ float inv_pow2(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }
 
-__device__ __forceinline__ u32x4 ld8(const uint16_t* p, bool vec) {
-  if (vec) return *reinterpret_cast<const u32x4*>(p);
-  u32x4 v;
-#pragma unroll
-  for (int e = 0; e < 4; e++) v[e] = (uint32_t)p[2 * e] | (uint32_t)p[2 * e + 1] << 16;
-  return v;
-}
+// Rows may start at any column: global memory takes wide accesses at any address, which the compiler uses for types that
+// are aligned to 2 bytes.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+__device__ __forceinline__ u32x4 ld8(const uint16_t* p) { return *reinterpret_cast<const u32x4_any*>(p); }
 // Columns 8 c .. 8 c + 7 of a 64-wide row after the rotary embedding of rope.hip (rotary width 32: out[2j] =
 // a_j cos - b_j sin, out[2j + 1] = a_j sin + b_j cos with a = x[0:16], b = x[16:32]), in its arithmetic and rounding.
-__device__ __forceinline__ u32x4 roped8(const uint16_t* row, int c, const float* cp, bool vec) {
-  if (c >= 4) return ld8(row + 8 * c, vec);
+__device__ __forceinline__ u32x4 roped8(const uint16_t* row, int c, const float* cp) {
+  if (c >= 4) return ld8(row + 8 * c);
   u32x4 o;
 #pragma unroll
   for (int e = 0; e < 4; e++) {
@@ -67,8 +65,9 @@ __device__ __forceinline__ u32x4 roped8(const uint16_t* row, int c, const float*
 // One workgroup per (block, head, slot); with a rotary table, heads H .. H + Hq - 1 of the grid rotate the queries.
 // K: thread = (token, 8 columns). V: thread = 4 tokens x D / 16 columns, whose codes are transposed in registers to a dword
 // per column. The block is put together in LDS and leaves in 16-byte stores; a block that keeps earlier rows is read
-// first, together with the new rows (every load is issued before the first is used). The bound is HBM for long prompts
-// (4 sequences x 8001 rows x 8 heads x 128), and for single rows the chain position -> rows -> maximum -> stores.
+// first, together with the new rows (every load is issued before the first is used). The bound is HBM for long prompts (4
+// sequences x 8001 rows x 8 heads x 128: 36 us, 4.5 TB/s), and for single rows the chain position -> rows -> maximum ->
+// stores behind a launch (1 x 32 heads x 64 3.8 us, 32 x 8 x 128 10).
 template <int D, bool ROPE>
 __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs p) {
   constexpr int CPR = D / 8, NC = 64 * CPR / 256;   // K: chunks of 8 columns per row, per thread
@@ -88,7 +87,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs p) {
       if (t >= p.n) break;
       const long cp = min(max(pos + t, 0L), (long)p.ncs - 1) * 32;
       *reinterpret_cast<u32x4*>(p.q_out + (((long)b * p.Hq + hq) * p.n + t) * D + 8 * (c % CPR)) =
-          roped8(p.q + b * p.sq_b + hq * p.sq_h + t * p.sq_t, c % CPR, p.cs + cp, p.vec);
+          roped8(p.q + b * p.sq_b + hq * p.sq_h + t * p.sq_t, c % CPR, p.cs + cp);
     }
     return;
   }
@@ -123,9 +122,9 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs p) {
     xk[i] = u32x4{0u, 0u, 0u, 0u};
     if (t >= t_lo && t < t_hi) {
       if constexpr (ROPE)
-        xk[i] = roped8(kr + (long)t * p.sk_t, cc, p.cs + min(blk * 64 + t, (long)p.ncs - 1) * 32, p.vec);
+        xk[i] = roped8(kr + (long)t * p.sk_t, cc, p.cs + min(blk * 64 + t, (long)p.ncs - 1) * 32);
       else
-        xk[i] = ld8(kr + (long)t * p.sk_t + 8 * cc, p.vec);
+        xk[i] = ld8(kr + (long)t * p.sk_t + 8 * cc);
     }
   }
 #pragma unroll
@@ -136,14 +135,12 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs p) {
     for (int e = 0; e < VC / 2; e++) xv[i][e] = 0;
     if (t >= t_lo && t < t_hi) {
       if constexpr (VC == 8) {
-        const u32x4 v = ld8(row, p.vec);
+        const u32x4 v = ld8(row);
 #pragma unroll
         for (int e = 0; e < 4; e++) xv[i][e] = v[e];
-      } else if (p.vec) {
-        const u32x2 v = *reinterpret_cast<const u32x2*>(row);
-        xv[i][0] = v.x, xv[i][1] = v.y;
       } else {
-        xv[i][0] = (uint32_t)row[0] | (uint32_t)row[1] << 16, xv[i][1] = (uint32_t)row[2] | (uint32_t)row[3] << 16;
+        const u32x2 v = *reinterpret_cast<const u32x2_any*>(row);
+        xv[i][0] = v.x, xv[i][1] = v.y;
       }
     }
   }
@@ -232,7 +229,8 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs p) {
   }
 }
 
-// Rows 0 .. n - 1 of every slot and head back as bf16: one workgroup per (block, head x slot), the block by way of LDS.
+// Rows 0 .. n - 1 of every slot and head back as bf16: one workgroup per (block, head x slot), the block by way of LDS. HBM
+// bound: 4 slots x 8 heads x 16002 x 128 74 us (5.3 TB/s); the stores are not kept in the caches (79 us if they are).
 template <int D>
 __global__ __launch_bounds__(256) void kv8_read_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
                                                        const uint8_t* __restrict__ ks, const uint8_t* __restrict__ vs,
@@ -264,8 +262,8 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(const uint8_t* __restrict
       const auto z = __builtin_amdgcn_cvt_pk_f32_fp8(w, false);
       yv[e] = pack2(z[0] * fv, z[1] * fv);
     }
-    *reinterpret_cast<u32x4*>(k + o) = yk;
-    *reinterpret_cast<u32x4*>(v + o) = yv;
+    __builtin_nontemporal_store(yk, reinterpret_cast<u32x4*>(k + o));
+    __builtin_nontemporal_store(yv, reinterpret_cast<u32x4*>(v + o));
   }
 }
 
@@ -287,10 +285,8 @@ extern "C" int mx_kv8_append(hipStream_t st, const uint16_t* k, long sk_b, long 
   if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)q) & 1) return MX_ELAYOUT;
   if (((uintptr_t)kc | (uintptr_t)vc | (uintptr_t)q_out) & 15) return MX_ELAYOUT;
   if (((uintptr_t)pos | (uintptr_t)count | (uintptr_t)cs) & 3) return MX_ELAYOUT;
-  AppendArgs a{k, v, q, sk_b, sk_h, sk_t, sv_b, sv_h, sv_t, sq_b, sq_h, sq_t, kc, vc, ks, vs, q_out, pos, count, cs, pos_s,
-               count_s, H, Hq, n, ctx, base, ncs, bcast, nslots, 0};
-  a.vec = !(((uintptr_t)k | (uintptr_t)v | (uintptr_t)q) & 15) &&
-          !((sk_b | sk_h | sk_t | sv_b | sv_h | sv_t | (q ? sq_b | sq_h | sq_t : 0)) % 8);
+  const AppendArgs a{k, v, q, sk_b, sk_h, sk_t, sv_b, sv_h, sv_t, sq_b, sq_h, sq_t, kc, vc, ks, vs, q_out, pos, count, cs, pos_s,
+               count_s, H, Hq, n, ctx, base, ncs, bcast, nslots};
   // blocks that n rows can touch wherever they start; the queries need ceil(n / 64), which is no more
   const int nx = pos ? (int)(((long)n + 62) / 64 + 1) : (base + n - 1) / 64 - base / 64 + 1;
   const int gx = cs && q ? (nx > (n + 63) / 64 ? nx : (n + 63) / 64) : nx;

@@ -68,9 +68,11 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
   v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xb1, 0xf, 0xf, false));  // quad_perm [1, 0, 3, 2]
   return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4e, 0xf, 0xf, false));  // quad_perm [2, 3, 0, 1]
 }
-// Columns k .. k + 7 of a row, zeros past K; vec: the row is 16-byte aligned and so is every multiple of 8 columns.
-__device__ __forceinline__ u32x4 load8(const uint16_t* __restrict__ row, int k, int K, bool vec) {
-  if (vec && k + 8 <= K) return *reinterpret_cast<const u32x4*>(row + k);
+// Columns k .. k + 7 of a row, zeros past K. Rows may start at any column: global memory takes 16-byte accesses at any
+// address, which the compiler uses for a type that is aligned to 2 bytes.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ u32x4 load8(const uint16_t* __restrict__ row, int k, int K) {
+  if (k + 8 <= K) return *reinterpret_cast<const u32x4_any*>(row + k);
   u32x4 v = {0u, 0u, 0u, 0u};
 #pragma unroll
   for (int e = 0; e < 8; e++)

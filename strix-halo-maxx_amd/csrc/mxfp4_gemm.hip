@@ -57,8 +57,8 @@ __device__ __forceinline__ void mx4_store(const Mx4Epi& p, int m, int n, f32x4 v
 
 // ---------------------------------------------------------------------------------------------- few rows
 // 16 MT rows per workgroup (grid y). It owns 16 columns of C (16 rows of W); its waves take the groups of 512 columns of K in
-// turn (4 KB of W each, read in one piece) and their sums meet in LDS. PRE = false: x arrives in bf16, XR rows at most (XV:
-// rows that 16-byte loads may read), and each wave quantises the 512 columns it multiplies (its own slice: no wave waits
+// turn (4 KB of W each, read in one piece) and their sums meet in LDS. PRE = false: x arrives in bf16, XR rows at most (XV: K
+// is a multiple of 8, whole 16-byte loads), and each wave quantises the 512 columns it multiplies (its own slice: no wave waits
 // for another before the end). The bound is the fetch of W from HBM behind one latency: us for 1 / 8 / 16 / 64 rows, weights
 // not in any cache, 2048 x 10240 5.7 / 9.4 / 6.6 / 10.0 (11 MB; 9.9 / 13.3 / 9.9 / 14.7 with branches around the loads, which
 // then wait for each other), 8192 x 2048 4.8 / 6.3 / 4.9 / 6.5, 768 x 768 2.8 / 4.1 / 2.9 / 3.8 (a launch alone takes about
@@ -122,9 +122,9 @@ __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(const uint16_t* __res
       for (int m = 0; m < XR; m++) {
         const uint16_t* row = x + min(m, p.M - 1) * ldx;
         if constexpr (XV)
-          q.x[0][m] = *reinterpret_cast<const u32x4*>(row + min(k, K - 8));
+          q.x[0][m] = *reinterpret_cast<const u32x4_any*>(row + min(k, K - 8));
         else
-          q.x[0][m] = load8(row, k, K, false);
+          q.x[0][m] = load8(row, k, K);
       }
     }
   };
@@ -567,7 +567,7 @@ extern "C" int mx_gemv_mxfp4(hipStream_t st, const uint16_t* x, long ldx, const 
   if (rc) return rc;
   if (M > GEMV_ROWS || ldx < 0) return MX_ESHAPE;
   if ((uintptr_t)x & 1) return MX_ELAYOUT;
-  const bool vec = !((uintptr_t)x & 15) && ldx % 8 == 0 && K % 8 == 0;
+  const bool vec = K % 8 == 0;
   const Mx4Epi p = epi(bias, R, ldr, r_rows, C, ldc, M, N, act_from);
   auto go = [&](auto launch) { return launch(st, x, ldx, nullptr, nullptr, wc, ws, K, act, p); };
   const hipError_t e = !vec     ? go(launch_rows<1, false, GEMV_ROWS, false>)
