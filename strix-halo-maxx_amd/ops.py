@@ -677,7 +677,7 @@ def _call_on(dev, name, *args):
     """call() on the current stream of the tensors' own device."""
     if dev.type != "cuda":
         raise ValueError(f"{name} needs tensors on the GPU, got {dev}")
-    cur = torch.cuda.current_device()
+    cur = torch._C._cuda_getDevice()  # a tensor is there, so the GPU is set up
     if dev.index == cur:
         rc = getattr(_lib._lib or _lib.load(), name)(torch._C._cuda_getCurrentRawStream(cur), *args)
         if rc:
@@ -718,10 +718,14 @@ class MxFp4:
             raise ValueError(f"({rows}, {K}) in MXFP4 takes {need} contiguous uint8, got {tuple(data.shape)} {data.dtype}")
         if data.data_ptr() % 16:
             raise ValueError("data must be 16-byte aligned")
+        self._hold(data, rows, K)
+
+    def _hold(self, data, rows, K):
         self.data, self.rows, self.K = data, rows, K
         self.dev = data.device
         p = data.data_ptr()
         self.ptrs = p, p + MxFp4.cells(rows, K) * 4096  # codes, scales
+        return self
 
     @staticmethod
     def cells(rows, K):
@@ -751,7 +755,8 @@ def quant_mxfp4(x):
     _need(x, "x", x.device)
     x2 = _rows2(x)
     M, K = x2.shape
-    q = MxFp4(torch.empty(MxFp4.cells(M, K) * 4352, device=x.device, dtype=torch.uint8), M, K)
+    buf = torch.empty(MxFp4.cells(M, K) * 4352, device=x.device, dtype=torch.uint8)
+    q = MxFp4.__new__(MxFp4)._hold(buf, M, K)
     if M:
         _call_on(x.device, "mx_quant_mxfp4", x2.data_ptr(), x2.stride(0), *q.ptrs, M, K)
     return q
