@@ -156,7 +156,7 @@ long mx_gemm_ws_counters(int cfg, int splits, int M, int N);
  * mx_mxfp4_code_bytes / mx_mxfp4_scale_bytes (rows M, columns K), codes 16-byte and scales 4-byte aligned. Any M, K. */
 long mx_mxfp4_code_bytes(int M, int K);
 long mx_mxfp4_scale_bytes(int M, int K);
-/* bf16 rows (row stride ldx, any alignment; 16-byte aligned rows are read fastest) to MXFP4, and the values that the
+/* bf16 rows (row stride ldx, any alignment) to MXFP4, and the values that the
  * codes stand for as bf16 (exact). */
 int mx_quant_mxfp4(hipStream_t st, const uint16_t* x, long ldx, uint8_t* codes, uint8_t* scales, int M, int K);
 int mx_mxfp4_values(hipStream_t st, const uint8_t* codes, const uint8_t* scales, uint16_t* y, long ldy, int M, int K);
@@ -165,6 +165,12 @@ int mx_mxfp4_values(hipStream_t st, const uint8_t* codes, const uint8_t* scales,
  * mx_gemm_mxfp4 takes quantised rows; mx_gemv_mxfp4 takes at most mx_gemv_mxfp4_rows() rows in bf16 and quantises them
  * on the way (the same result). */
 int mx_gemv_mxfp4_rows(void);
+/* The same for the LayerNorm of one row, C = act(LayerNorm(x) W^T + bias): what mx_layernorm and mx_gemv_mxfp4 give, in one
+ * launch. K a multiple of 8, at most mx_ln_gemv_mxfp4_cols(). */
+int mx_ln_gemv_mxfp4_cols(void);
+int mx_ln_gemv_mxfp4(hipStream_t st, const uint16_t* x, const uint16_t* gamma, const uint16_t* beta, float eps,
+                     const uint8_t* wc, const uint8_t* ws, const float* bias, uint16_t* C, int N, int K, int act,
+                     int act_from);
 int mx_gemv_mxfp4(hipStream_t st, const uint16_t* x, long ldx, const uint8_t* wc, const uint8_t* ws, const float* bias,
                   const uint16_t* R, long ldr, int r_rows, uint16_t* C, long ldc, int M, int N, int K, int act,
                   int act_from);

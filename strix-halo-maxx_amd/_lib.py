@@ -43,6 +43,8 @@ SIGNATURES = {
     "mx_quant_mxfp4": [P, P, L, P, P, I, I],
     "mx_mxfp4_values": [P, P, P, P, L, I, I],
     "mx_gemv_mxfp4_rows": [],
+    "mx_ln_gemv_mxfp4_cols": [],
+    "mx_ln_gemv_mxfp4": [P, P, P, P, F, P, P, P, P, I, I, I, I],
     "mx_gemv_mxfp4": [P, P, L, P, P, P, P, L, I, P, L, I, I, I, I, I],
     "mx_gemm_mxfp4": [P, P, P, P, P, P, P, L, I, P, L, I, I, I, I, I],
     "mx_kv8_append": [P, P, L, L, L, P, L, L, L, P, P, P, P, I, I, I, I, I, I, I, P, L, I, P, L, P, I, P, L, L, L, I, P],

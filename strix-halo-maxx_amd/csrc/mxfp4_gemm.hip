@@ -55,6 +55,22 @@ __device__ __forceinline__ void mx4_store(const Mx4Epi& p, int m, int n, f32x4 v
   }
 }
 
+// LayerNorm of the one row of x before its quantisation.
+struct Mx4Ln {
+  const uint16_t *gamma, *beta;
+  float eps;
+};
+// The sum over a wave in the order of wave_sum (xor 32, 16, 8, 4, 2, 1), without its round trips through LDS.
+__device__ __forceinline__ float wave_sum_reg(float v) {
+  v = halves_sum(v);
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  v += dpp_mov<0x128>(0.f, v);                     // row_ror 8: lane ^ 8
+  v += dpp_mov<0x1b>(0.f, dpp_mov<0x141>(0.f, v));  // quad_perm [3, 2, 1, 0] of row_half_mirror: lane ^ 3 ^ 7
+  v += dpp_mov<0x4e>(0.f, v);                      // lane ^ 2
+  return v + dpp_mov<0xb1>(0.f, v);                // lane ^ 1
+}
+
 // ---------------------------------------------------------------------------------------------- few rows
 // 16 MT rows per workgroup (grid y). It owns 16 columns of C (16 rows of W); its waves take the groups of 512 columns of K in
 // turn (4 KB of W each, read in one piece) and their sums meet in LDS. PRE = false: x arrives in bf16, XR rows at most (XV: K
@@ -63,13 +79,18 @@ __device__ __forceinline__ void mx4_store(const Mx4Epi& p, int m, int n, f32x4 v
 // not in any cache, 2048 x 10240 5.7 / 9.4 / 6.6 / 10.0 (11 MB; 9.9 / 13.3 / 9.9 / 14.7 with branches around the loads, which
 // then wait for each other), 8192 x 2048 4.8 / 6.3 / 4.9 / 6.5, 768 x 768 2.8 / 4.1 / 2.9 / 3.8 (a launch alone takes about
 // 2). With 8 rows the quantisation, which every workgroup repeats, takes the time.
-template <int NW, int MT, bool PRE, int XR, bool XV, int ACT>
+// LN (one row of at most 512 NW columns): the row is normalised first, in layernorm_kernel's arithmetic and order. Every wave
+// takes the row's sums, whose lanes hold the columns that they hold there, and normalises the 512 that it multiplies, while
+// its part of W is on the way: us in one launch / two, weights from HBM, 14336 x 2048 8.6 / 9.2, 8192 x 2048 6.3 / 7.8, 4304
+// x 1152 4.7 / 6.1 (every workgroup repeats the norm, so a wider W gains less).
+template <int NW, int MT, bool PRE, int XR, bool XV, bool LN, int ACT>
 __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(const uint16_t* __restrict__ x, long ldx,
                                                            const uint8_t* __restrict__ xc,
                                                            const uint32_t* __restrict__ xs,
                                                            const uint8_t* __restrict__ wc,
-                                                           const uint32_t* __restrict__ ws, int K, Mx4Epi p) {
+                                                           const uint32_t* __restrict__ ws, int K, Mx4Epi p, Mx4Ln ln) {
   static_assert(PRE || MT == 1, "bf16 rows come in one tile");
+  static_assert(!LN || (!PRE && XR == 1 && XV), "one row is normalised");
   __shared__ __attribute__((aligned(16))) uint32_t xq[PRE ? 1 : NW][XR][64];  // a row's codes of the wave's columns
   __shared__ __attribute__((aligned(16))) uint8_t xsc[PRE ? 1 : NW][XR][16];  // its scale bytes, [block % 4][step]
   __shared__ f32x4 red[NW][MT][64];
@@ -94,9 +115,18 @@ __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(const uint16_t* __res
   struct Step {
     u32x4 w[4], x[PRE ? MT : 1][PRE ? 4 : XR];  // W; x: its codes, or its rows in bf16
     int sw[4], sx[PRE ? MT : 1][4];
+    u32x4 row[LN ? NW : 1], gamma, beta;
   };
   auto fetch = [&](Step& q, int ks) {
     const int left = nk - 4 * ks;
+    if constexpr (LN) {
+#pragma unroll
+      for (int i = 0; i < NW; i++)
+        q.row[i] = *reinterpret_cast<const u32x4_any*>(x + min(i * 512 + lane * 8, K - 8));
+      const int k = min(ks * 512 + lane * 8, K - 8);
+      q.gamma = *reinterpret_cast<const u32x4_any*>(ln.gamma + k);
+      q.beta = *reinterpret_cast<const u32x4_any*>(ln.beta + k);
+    }
     const uint8_t* wt = codes(wc, nt) + (long)ks * 8192;
 #pragma unroll
     for (int t = 0; t < 4; t++) {
@@ -116,7 +146,7 @@ __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(const uint16_t* __res
           q.sx[i][t] = scale(xs, ut, 4 * ks + u);
         }
       }
-    } else {
+    } else if constexpr (!LN) {
       const int k = ks * 512 + lane * 8;
 #pragma unroll
       for (int m = 0; m < XR; m++) {
@@ -128,7 +158,39 @@ __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(const uint16_t* __res
       }
     }
   };
+  auto normalise = [&](Step& q, int ks) {
+    float s = 0.f, ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < NW; i++) {
+      const bool on = i * 512 + lane * 8 < K;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        s += on ? lo_bf(q.row[i][e]) : 0.f;
+        s += on ? hi_bf(q.row[i][e]) : 0.f;
+      }
+    }
+    const float mean = wave_sum_reg(s) / (float)K;
+#pragma unroll
+    for (int i = 0; i < NW; i++) {
+      const bool on = i * 512 + lane * 8 < K;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float a = lo_bf(q.row[i][e]) - mean, b = hi_bf(q.row[i][e]) - mean;
+        ss += on ? a * a : 0.f;
+        ss += on ? b * b : 0.f;
+      }
+    }
+    const float rstd = 1.0f / sqrtf(wave_sum_reg(ss) / (float)K + ln.eps);
+    u32x4 own = q.row[0];
+#pragma unroll
+    for (int i = 1; i < NW; i++) own = ks == i ? q.row[i] : own;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      q.x[0][0][e] = pack2((lo_bf(own[e]) - mean) * rstd * lo_bf(q.gamma[e]) + lo_bf(q.beta[e]),
+                           (hi_bf(own[e]) - mean) * rstd * hi_bf(q.gamma[e]) + hi_bf(q.beta[e]));
+  };
   auto multiply = [&](Step& q, int ks) {
+    if constexpr (LN) normalise(q, ks);
     const int left = nk - 4 * ks;
     const u32x4 none = {0u, 0u, 0u, 0u};
     if constexpr (PRE) {
@@ -541,17 +603,18 @@ hipError_t launch_rows(hipStream_t st, const uint16_t* x, long ldx, const uint8_
                        const uint8_t* ws, int K, int act, const Mx4Epi& p) {
   const dim3 grid((unsigned)((p.N + 15L) / 16), (unsigned)((p.M + 16L * MT - 1) / (16 * MT)));
   auto go = [&](auto kern, int nw) {
-    hipLaunchKernelGGL(kern, grid, dim3(64 * nw), 0, st, x, ldx, xc, (const uint32_t*)xs, wc, (const uint32_t*)ws, K, p);
+    hipLaunchKernelGGL(kern, grid, dim3(64 * nw), 0, st, x, ldx, xc, (const uint32_t*)xs, wc, (const uint32_t*)ws, K, p,
+                       Mx4Ln{});
     return hipGetLastError();
   };
   if (mx4_nk(K) <= 16) {
-    if (act == 0) return go(mx4_rows_kernel<4, MT, PRE, XR, XV, 0>, 4);
-    if (act == 1) return go(mx4_rows_kernel<4, MT, PRE, XR, XV, 1>, 4);
-    return go(mx4_rows_kernel<4, MT, PRE, XR, XV, 2>, 4);
+    if (act == 0) return go(mx4_rows_kernel<4, MT, PRE, XR, XV, false, 0>, 4);
+    if (act == 1) return go(mx4_rows_kernel<4, MT, PRE, XR, XV, false, 1>, 4);
+    return go(mx4_rows_kernel<4, MT, PRE, XR, XV, false, 2>, 4);
   }
-  if (act == 0) return go(mx4_rows_kernel<8, MT, PRE, XR, XV, 0>, 8);
-  if (act == 1) return go(mx4_rows_kernel<8, MT, PRE, XR, XV, 1>, 8);
-  return go(mx4_rows_kernel<8, MT, PRE, XR, XV, 2>, 8);
+  if (act == 0) return go(mx4_rows_kernel<8, MT, PRE, XR, XV, false, 0>, 8);
+  if (act == 1) return go(mx4_rows_kernel<8, MT, PRE, XR, XV, false, 1>, 8);
+  return go(mx4_rows_kernel<8, MT, PRE, XR, XV, false, 2>, 8);
 }
 
 }  // namespace
@@ -574,6 +637,30 @@ extern "C" int mx_gemv_mxfp4(hipStream_t st, const uint16_t* x, long ldx, const 
                        : M == 1 ? go(launch_rows<1, false, 1, true>)
                        : M <= 4 ? go(launch_rows<1, false, 4, true>)
                                 : go(launch_rows<1, false, GEMV_ROWS, true>);
+  return e == hipSuccess ? MX_OK : MX_ELAUNCH;
+}
+
+// Widest row that mx_ln_gemv_mxfp4 takes: four waves' 512 columns.
+extern "C" int mx_ln_gemv_mxfp4_cols(void) { return 2048; }
+
+extern "C" int mx_ln_gemv_mxfp4(hipStream_t st, const uint16_t* x, const uint16_t* gamma, const uint16_t* beta, float eps,
+                                const uint8_t* wc, const uint8_t* ws, const float* bias, uint16_t* C, int N, int K, int act,
+                                int act_from) {
+  if (!x || !gamma || !beta) return MX_ENULL;
+  const int rc = check(wc, ws, bias, nullptr, 0, 0, C, N, 1, N, K, act, act_from);
+  if (rc) return rc;
+  if (K % 8 || K > 2048) return MX_ESHAPE;
+  if (((uintptr_t)x | (uintptr_t)gamma | (uintptr_t)beta) & 1) return MX_ELAYOUT;
+  const dim3 grid((unsigned)((N + 15L) / 16));
+  const Mx4Epi p = epi(bias, nullptr, 0, 0, C, N, 1, N, act_from);
+  auto go = [&](auto kern) {
+    hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, x, 0L, nullptr, nullptr, wc, (const uint32_t*)ws, K, p,
+                       Mx4Ln{gamma, beta, eps});
+    return hipGetLastError();
+  };
+  const hipError_t e = act == 0   ? go(mx4_rows_kernel<4, 1, false, 1, true, true, 0>)
+                       : act == 1 ? go(mx4_rows_kernel<4, 1, false, 1, true, true, 1>)
+                                  : go(mx4_rows_kernel<4, 1, false, 1, true, true, 2>);
   return e == hipSuccess ? MX_OK : MX_ELAUNCH;
 }
 

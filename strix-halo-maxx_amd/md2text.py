@@ -9,7 +9,7 @@ rebuilt for batch-1 HBM streaming:
   * per layer 3 kernels: LN fused into the [qkv | fc1] GEMV, rope + KV append fused into split-KV attention, and
     the fc2 / proj GEMVs fused with the two residual adds;
   * in fewer bits: `mxfp4` runs the layers' Linears in MXFP4, `kv8` keeps the K/V cache in 8 bits; each works with every
-    form of the other, in prefill, query and decode (a decode step then goes operator by operator, 4 or 5 launches
+    form of the other, in prefill, query and decode (a decode step then goes operator by operator, 3 to 5 launches
     a layer, still one HIP graph);
   * the LM head GEMV carries the argmax, and the next step's embedding lookup reduces it on the device, so one HIP
     graph replays a whole step with the token and position kept in device memory (no host round trip per token).
@@ -147,7 +147,6 @@ class TextDecoder:
         row = torch.zeros(nqf + self.D, device=dev, dtype=BF)
         self.qf_d, self.ga_d = row[None, :nqf], row[None, 3 * self.D:]
         self.qkv_d, self.g_d, self.a_d = row[:3 * self.D], row[3 * self.D:nqf], row[nqf:]
-        self.h_d = torch.zeros(1, self.D, device=dev, dtype=BF)
         self.y2_d = torch.zeros(self.D, device=dev, dtype=BF)  # bf16(fc2(g) + b2) of the decode step
         # decode: fc2 shares the attention's launch (mx_decode_attn_fc2) and proj + residual follow (mx_gemv_res2);
         # False: attention, then both GEMVs in one pass (mx_gemv_dual_res). Same roundings either way.
@@ -489,8 +488,7 @@ class TextDecoder:
         for i, b in enumerate(self.blocks):
             x, xn = self.xd[xi], self.xd[xi ^ 1]
             if self.mxfp4:
-                ops.layernorm(x[None], *b["ln"], eps=self.eps, out=self.h_d)
-                b["qf"](self.h_d, act="tanh", act_from=b["nq"], out=self.qf_d)
+                b["qf"].ln(x[None], b["ln"], eps=self.eps, act="tanh", act_from=b["nq"], out=self.qf_d)
             elif self.w8a8:
                 _lib.check(lib.mx_ln_gemv2_i8(st, x.data_ptr(), b["ln"][0].data_ptr(), b["ln"][1].data_ptr(),
                                               float(self.eps), b["wqf"].data_ptr(), b["wqf"].stride(0),

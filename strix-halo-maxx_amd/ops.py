@@ -795,7 +795,7 @@ class MxFp4Lin:
             raise ValueError(f"bias must be ({self.N},)")
         self.b = None if bias is None else bias.detach().to(device=self.dev, dtype=torch.float32).contiguous()
         self.bp = ptr(self.b)
-        self.rows = _lib.load().mx_gemv_mxfp4_rows()
+        self.rows, self.ln_cols = _lib.load().mx_gemv_mxfp4_rows(), _lib.load().mx_ln_gemv_mxfp4_cols()
 
     def quant(self, x):
         return quant_mxfp4(x)
@@ -850,6 +850,35 @@ class MxFp4Lin:
         if out is not None or x is None or x.dim() == 2:
             return y
         return y.view(*x.shape[:-1], N)
+
+
+    def ln(self, x, ln, eps=1e-5, act=None, out=None, act_from=0):
+        """layernorm(x, *ln, eps) through the Linear: the same result; one row of at most 2048 columns (a multiple of 8) is
+        normalised inside the product's launch."""
+        N, K = self.N, self.K
+        if x.shape[-1] != K or any(t.shape != (K,) or not t.is_contiguous() for t in ln):
+            raise ValueError(f"x (..., {K}) and two contiguous ({K},) vectors, got {tuple(x.shape)}, {[tuple(t.shape) for t in ln]}")
+        for t, name in ((x, "x"), (ln[0], "gamma"), (ln[1], "beta")):
+            _need(t, name, self.dev)
+        if x.numel() != K or K % 8 or K > self.ln_cols:
+            if self.dev.type != "cuda":
+                raise ValueError(f"ln needs tensors on the GPU, got {self.dev}")
+            with torch.cuda.device(self.dev):
+                return self(layernorm(x, *ln, eps=eps), act=act, out=out, act_from=act_from)
+        a = ACT[act]
+        if a == 3 or act_from < 0:
+            raise ValueError("no gated GELU in the MXFP4 path, and act_from must not be negative")
+        x2 = _rows2(x)
+        y = torch.empty(1, N, device=self.dev, dtype=BF) if out is None else out
+        _need(y, "out", self.dev)
+        y2 = y if y.dim() == 2 else y.view(-1, N)
+        if y2.shape != (1, N) or (y2.stride(1) != 1 and N > 1):
+            raise ValueError(f"out must be (1, {N}) with unit column stride")
+        if not _apart(x2, y2):
+            x2 = x2.clone()
+        _call_on(self.dev, "mx_ln_gemv_mxfp4", x2.data_ptr(), ln[0].data_ptr(), ln[1].data_ptr(), float(eps), *self.wq.ptrs,
+                 self.bp, y2.data_ptr(), N, K, a, act_from)
+        return y if out is not None or x.dim() == 2 else y.view(*x.shape[:-1], N)
 
 
 def _where(v, B, dev, name):

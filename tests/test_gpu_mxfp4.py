@@ -228,3 +228,48 @@ def test_offsets_past_32_bits(dev):
     y = lin(x)
     close(y[-70:].cpu(), ref, mag)
     assert not bool(y[:1000].any()) and not bool(y[150_000:151_000].any())
+
+
+@pytest.mark.parametrize("K", [8, 520, 1152, 2040, 2048, 2056])
+def test_linear_of_a_layernorm(dev, K):
+    """LayerNorm and Linear in one launch (one row, K up to 2048; beyond, two calls) give the bits of the two operators: rows
+    with a large mean, a constant row, a NaN, an infinity, a row of zeros; outputs in place and inside a buffer."""
+    g = gen(K)
+    N = 300
+    lin = ops.MxFp4Lin((torch.randn(N, K, generator=g) * 0.1).to(BF), torch.randn(N, generator=g), device=dev)
+    ln = [(torch.randn(K, generator=g) * s + m).to(BF).to(dev) for s, m in ((0.2, 1.0), (0.1, 0.0))]
+    x = torch.randn(7, K, generator=g)
+    x[1] += 100.0
+    x[2], x[3] = 3.25, 0.0
+    x[4, K // 2], x[5, K - 1] = float("nan"), float("inf")
+    x = x.to(BF).to(dev)
+    for r in range(7):
+        for eps, kw in ((1e-5, {}), (1e-3, dict(act="tanh", act_from=133)), (1e-5, dict(act="erf"))):
+            got, want = lin.ln(x[r:r + 1], ln, eps=eps, **kw), lin(ops.layernorm(x[r:r + 1], *ln, eps=eps), **kw)
+            assert same(got.cpu(), want.cpu()), (r, kw)
+    want = lin(ops.layernorm(x, *ln))
+    assert same(lin.ln(x, ln).cpu(), want.cpu())
+    assert lin.ln(x[0], ln).shape == (N,) and torch.equal(lin.ln(x[0], ln), want[0])
+    buf = torch.full((3, N + 9), 5.0, device=dev, dtype=BF)
+    lin.ln(x[:1], ln, out=buf[1:2, 3:N + 3])
+    assert torch.equal(buf[1, 3:N + 3], want[0])
+    buf[1, 3:N + 3] = 5.0
+    assert bool((buf == 5.0).all())
+    row, gr = x[:1].clone(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        y = lin.ln(row, ln)
+    for r in (0, 1, 6, 0):
+        row.copy_(x[r:r + 1])
+        gr.replay()
+        assert torch.equal(y[0], want[r])
+        torch.cuda.synchronize()
+
+
+def test_linear_of_a_layernorm_onto_its_input(dev):
+    g = gen(77)
+    lin = ops.MxFp4Lin((torch.randn(512, 512, generator=g) * 0.1).to(BF), None, device=dev)
+    ln = [torch.randn(512, generator=g).to(BF).to(dev) for _ in range(2)]
+    x = torch.randn(1, 512, generator=g).to(BF).to(dev)
+    want = lin.ln(x, ln)
+    lin.ln(x, ln, out=x)
+    assert torch.equal(x, want)

@@ -191,3 +191,23 @@ def test_widths_that_the_linear_takes():
     raises("GPU", lin, x[:, :592])
     raises("width 600", lin, x)
     raises("width 590", lin, x[:, :590])
+
+
+def test_layernorm_linear_refusals():
+    lib = _lib.load()
+    f = lambda **kw: lib.mx_ln_gemv_mxfp4(*{**dict(st=None, x=A16, g=A16, be=A16, eps=1e-5, wc=A16, ws=A16, b=None, C=A16, N=64,
+                                                   K=64, act=0, af=0), **kw}.values())
+    for name in ("x", "g", "be", "wc", "ws", "C"):
+        assert f(**{name: None}) == -6
+    assert f(K=60) == -2 and f(K=lib.mx_ln_gemv_mxfp4_cols() + 8) == -2 and f(K=0) == -2 and f(N=0) == -2 and f(act=3) == -1
+    assert f(x=A16 + 1) == -4 and f(g=A16 + 1) == -4 and f(af=-1) == -2 and f(N=2 ** 27 + 1) == -2
+    lin = ops.MxFp4Lin.from_quantized(ops.MxFp4(torch.zeros(4352, dtype=torch.uint8), 10, 64), None)
+    x, v = torch.zeros(1, 64, dtype=BF), torch.ones(64, dtype=BF)
+    raises("GPU", lin.ln, x, (v, v))
+    raises("GPU", lin.ln, x.expand(3, -1), (v, v))
+    raises("contiguous", lin.ln, x[:, :32], (v, v))
+    raises("contiguous", lin.ln, x, (v[:32], v))
+    raises("contiguous", lin.ln, x, (v, torch.ones(128, dtype=BF)[::2]))
+    raises("float32", lin.ln, x, (v.float(), v))
+    raises("gated", lin.ln, x, (v, v), act="glu")
+    raises("out must", lin.ln, x, (v, v), out=torch.zeros(1, 9, dtype=BF))
