@@ -156,27 +156,26 @@ long mx_gemm_ws_counters(int cfg, int splits, int M, int N);
  * mx_mxfp4_code_bytes / mx_mxfp4_scale_bytes (rows M, columns K), codes 16-byte and scales 4-byte aligned. Any M, K. */
 long mx_mxfp4_code_bytes(int M, int K);
 long mx_mxfp4_scale_bytes(int M, int K);
-/* bf16 rows (row stride ldx, any alignment) to MXFP4, and the values that the
- * codes stand for as bf16 (exact). */
+/* bf16 rows (row stride ldx, any alignment) to MXFP4, and the values that the codes stand for as bf16 (exact). */
 int mx_quant_mxfp4(hipStream_t st, const uint16_t* x, long ldx, uint8_t* codes, uint8_t* scales, int M, int K);
 int mx_mxfp4_values(hipStream_t st, const uint8_t* codes, const uint8_t* scales, uint16_t* y, long ldy, int M, int K);
 /* C[m, n] = act(sum_k x[m, k] W[n, k] + bias[n]) + R[m % r_rows or m, n], both operands in MXFP4, fp32 throughout and
- * rounded to bf16 once. act: 0 none, 1 GELU-tanh, 2 GELU-erf, on columns >= act_from. bias, R nullable; any M, N, K.
- * mx_gemm_mxfp4 takes quantised rows; mx_gemv_mxfp4 takes at most mx_gemv_mxfp4_rows() rows in bf16 and quantises them
+ * rounded to bf16 once. act: 0 none, 1 GELU-tanh, 2 GELU-erf, on columns >= act_from. bias, R nullable; any M, N up to
+ * 2^27, K up to 2^22. R may be C itself; C must not meet x. mx_gemm_mxfp4 takes quantised rows; mx_gemv_mxfp4 takes at most mx_gemv_mxfp4_rows() rows in bf16 and quantises them
  * on the way (the same result). */
 int mx_gemv_mxfp4_rows(void);
-/* The same for the LayerNorm of one row, C = act(LayerNorm(x) W^T + bias): what mx_layernorm and mx_gemv_mxfp4 give, in one
- * launch. K a multiple of 8, at most mx_ln_gemv_mxfp4_cols(). */
-int mx_ln_gemv_mxfp4_cols(void);
-int mx_ln_gemv_mxfp4(hipStream_t st, const uint16_t* x, const uint16_t* gamma, const uint16_t* beta, float eps,
-                     const uint8_t* wc, const uint8_t* ws, const float* bias, uint16_t* C, int N, int K, int act,
-                     int act_from);
 int mx_gemv_mxfp4(hipStream_t st, const uint16_t* x, long ldx, const uint8_t* wc, const uint8_t* ws, const float* bias,
                   const uint16_t* R, long ldr, int r_rows, uint16_t* C, long ldc, int M, int N, int K, int act,
                   int act_from);
 int mx_gemm_mxfp4(hipStream_t st, const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws,
                   const float* bias, const uint16_t* R, long ldr, int r_rows, uint16_t* C, long ldc, int M, int N, int K,
                   int act, int act_from);
+/* The same for the LayerNorm of one row, C = act(LayerNorm(x) W^T + bias): what mx_layernorm and mx_gemv_mxfp4 give, in one
+ * launch. K a multiple of 8, at most mx_ln_gemv_mxfp4_cols(). */
+int mx_ln_gemv_mxfp4_cols(void);
+int mx_ln_gemv_mxfp4(hipStream_t st, const uint16_t* x, const uint16_t* gamma, const uint16_t* beta, float eps,
+                     const uint8_t* wc, const uint8_t* ws, const float* bias, uint16_t* C, int N, int K, int act,
+                     int act_from);
 
 /* ============================================================================================ attention
  * O[b, i, h*D + d] = softmax(scale * Q K^T) V over visible keys; key j visible to query i iff j < Tk and
@@ -203,8 +202,9 @@ void mx_sdpa_tiling(int B, int H, int Tq, int D, int* t);
 /* Rows t < n of B sequences (k, v: strides per sequence, head, row; unit column stride) to positions pos_b + t of slot b
  * (bcast: B = 1, to every slot). count (nullable): only the first count[b] rows of sequence b. A block's exponent is the
  * smallest e with max |x| <= 448 2^e (at least -127) over the new rows, and not less than before if it holds earlier
- * rows, whose codes are rounded to it; what the last block holds behind the new rows is undefined. Infinities and NaN are stored as NaN. cs (nullable, D = 64): the (ncs, 16, 2)
- * rotary table of mx_rope_kv, applied to k and to the Hq query heads q -> q_out [B][Hq][n][D] (q nullable). */
+ * rows, whose codes are rounded to it; what the last block holds behind the new rows is undefined. Infinities and NaN are
+ * stored as NaN. cs (nullable, D = 64): the (ncs, 16, 2) rotary table of mx_rope_kv, applied to k and to the Hq query heads
+ * q -> q_out [B][Hq][n][D] (q nullable). */
 int mx_kv8_append(hipStream_t st, const uint16_t* k, long sk_b, long sk_h, long sk_t, const uint16_t* v, long sv_b,
                   long sv_h, long sv_t, uint8_t* kc, uint8_t* vc, uint8_t* ks, uint8_t* vs, int B, int H, int n, int D,
                   int ctx, int nslots, int bcast, const int* pos, long pos_s, int base, const int* count, long count_s,
