@@ -4,13 +4,15 @@
 //   no key gets zeros.
 //
 // The codes go from the cache into the 32x32x64 MFMA as they are; nothing is converted to bf16.
-//  * S^T = K Q^T: Q is two e4m3 terms, q = 2^e (hi + lo / 16) with one exponent per row, which hold a bf16's 8 bits (what
-//    falls below 2^-23 of the row's largest value is lost), so both products together are the bf16 product. The scales
-//    of the K block and of Q are the MFMA's own scale operands.
+//  * S^T = K Q^T: Q is two e4m3 terms, q = 2^e (hi + lo / 16) with one exponent per row, which hold a bf16's 8 bits, so both
+//    products together are the bf16 product. The row's largest value lies in [128, 256) and lo's last step is 2^-13, so
+//    values below 2^-14, which is 2^-22 to 2^-21 of the largest, become 0. The scales of the K block and of Q are the
+//    MFMA's own scale operands.
 //  * O^T += V^T P^T: the weights of 64 keys are two e4m3 terms too, with a power of two of their own for every query and
 //    block: p = 2^(el - 8 - m) (hi + lo / 16), el the next integer above the block's largest score (base 2), m the
-//    running one. Relative to the block's largest weight that keeps 2^-9 of each weight and everything above 2^-22. The
+//    running one. That keeps each weight to 2^-9 of itself, and every weight above 2^-21 of the block's largest. The
 //    running maximum is an integer, so rescaling is exact. Sums of weights are taken in fp32 before that rounding.
+//    Scores up to 2^29 in size (2^30 in base 2, where the integers end) give what the formula gives; beyond, 0 or NaN.
 //  * The token order inside a V block is the order in which S^T leaves its keys in a lane's registers (kv8.h).
 // The fp8 MFMA adds its 64 products to the fp32 accumulator with an error of about 2^-16 of the result's size (measured:
 // 1.3e-5 of the root mean square on normal data, without bias), a hundredth of the bf16 rounding of the output.
@@ -51,7 +53,7 @@ __device__ __forceinline__ i32x8 join(u32x4 a, u32x4 b) {
   return i32x8{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
 }
 typedef short s16x2 __attribute__((ext_vector_type(2)));
-// a, b, c, d (|.| <= 448) as hi + lo / 16
+// a, b, c, d (|.| <= 448) as hi + lo / 16; with a power of two `unit` a / unit .. are
 __device__ __forceinline__ void split4(float a, float b, float c, float d, uint32_t& hi, uint32_t& lo) {
   uint32_t h = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
   h = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, h, true);
@@ -60,6 +62,19 @@ __device__ __forceinline__ void split4(float a, float b, float c, float d, uint3
   l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, a - x[0], b - x[1], 0.0625f, false);
   l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, c - y[0], d - y[1], 0.0625f, true);
   hi = h, lo = __builtin_bit_cast(uint32_t, l);
+}
+
+__device__ __forceinline__ void split4(float a, float b, float c, float d, float unit, uint32_t& hi, uint32_t& lo) {
+  s16x2 h = {0, 0}, l = {0, 0};
+  h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, a, b, unit, false);
+  h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, c, d, unit, true);
+  hi = __builtin_bit_cast(uint32_t, h);
+  const auto x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, unit, false);
+  const auto y = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, unit, true);
+  const float part = unit * 0.0625f;
+  l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, a - x[0], b - x[1], part, false);
+  l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, c - y[0], d - y[1], part, true);
+  lo = __builtin_bit_cast(uint32_t, l);
 }
 
 // What a sequence's length and position give.
@@ -109,10 +124,21 @@ __device__ __forceinline__ uint32_t bits_max(u32x4 v) {
   for (int e = 0; e < 4; e++) m = max(m, max(v[e] & 0x7fffu, (v[e] >> 16) & 0x7fffu));
   return m;
 }
-// The running maximum (an integer, base 2) takes in a block whose largest score is mx: the block's own integer, the new
-// maximum.
-__device__ __forceinline__ int block_exponent(float mx) {
-  return (int)fminf(fmaxf(ceilf(mx), (float)M_NONE), (float)-M_NONE);
+// What a block whose largest score is mx makes of its scores s: weights exp2(fma(s, sl2, neg)), at most 256 unit, whose codes
+// count 2^(el - 8), for a power of two unit near 2^-8. neg is a float exactly and the fma rounds once, next to 0, so this also
+// holds where mx sl2 is rounded to far more than 1 (from 2^24 on): what that rounding is off by goes into unit.
+struct Block8 {
+  float neg, unit;
+  int el, e0;  // e0 = -neg
+};
+__device__ __forceinline__ Block8 block_scale(float mx, float sl2) {
+  Block8 s;
+  const float top = fminf(fmaxf(ceilf(mx * sl2), (float)M_NONE), -(float)M_NONE - 128.f);
+  const int over = (int)fminf(fmaxf(ceilf(__builtin_fmaf(mx, sl2, -top)), -64.f), 64.f);  // 0, but for that rounding
+  s.neg = -top, s.e0 = (int)top;
+  s.el = max(s.e0 + over, M_NONE);
+  s.unit = __uint_as_float((uint32_t)(127 - 8 + over) << 23);
+  return s;
 }
 // scale byte of a block's weights (hi; lo: 4 less)
 __device__ __forceinline__ int weight_byte(int el, int m) { return max(127 - 8 + max(el - m, -240), 4); }
@@ -274,7 +300,8 @@ __global__ __launch_bounds__(64 * NK) void kv8_rows_kernel(Attn8Args p) {
       for (int tt = 0; tt < 4; tt++)
 #pragma unroll
         for (int r = 0; r < 4; r++) mx = fmaxf(mx, st[tt][r]);
-      const int el = block_exponent(quarters_max(mx) * p.sl2), mn = max(m, el);
+      const Block8 bs = block_scale(quarters_max(mx), p.sl2);
+      const int el = bs.el, mn = max(m, el);
       if (__any(mn != m)) {
         const float al = __builtin_amdgcn_ldexpf(1.f, m - mn);
         l *= al;
@@ -284,7 +311,6 @@ __global__ __launch_bounds__(64 * NK) void kv8_rows_kernel(Attn8Args p) {
           for (int r = 0; r < 4; r++) o[t][r] *= al;
         m = mn;
       }
-      const float sh = (float)(8 - el);
       float sum = 0.f;
       u32x4 hi, lo;
 #pragma unroll
@@ -292,14 +318,14 @@ __global__ __launch_bounds__(64 * NK) void kv8_rows_kernel(Attn8Args p) {
         float y[4];
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-          y[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[tt][r], p.sl2, sh));
+          y[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[tt][r], p.sl2, bs.neg));
           sum += y[r];
         }
         uint32_t a, d;
-        split4(y[0], y[1], y[2], y[3], a, d);
+        split4(y[0], y[1], y[2], y[3], bs.unit, a, d);
         hi[tt] = a, lo[tt] = d;
       }
-      l += __builtin_amdgcn_ldexpf(quarters_sum(sum), el - 8 - mn);
+      l += __builtin_amdgcn_ldexpf(quarters_sum(sum), bs.e0 - mn);
       if (masked) {
         uint32_t nb = 0;
 #pragma unroll
@@ -498,7 +524,8 @@ __global__ __launch_bounds__(64 * NQW * NKW, 2) void kv8_tile_kernel(Attn8Args p
     for (int t = 0; t < 2; t++)
 #pragma unroll
       for (int r = 0; r < 16; r++) mx = fmaxf(mx, st[t][r]);
-    const int el = block_exponent(halves_max(mx) * p.sl2), mn = max(m, el);
+    const Block8 bs = block_scale(halves_max(mx), p.sl2);
+    const int el = bs.el, mn = max(m, el);
     if (__any(mn != m)) {
       const float al = __builtin_amdgcn_ldexpf(1.f, m - mn);
       l *= al;
@@ -509,21 +536,20 @@ __global__ __launch_bounds__(64 * NQW * NKW, 2) void kv8_tile_kernel(Attn8Args p
       }
       m = mn;
     }
-    const float sh = (float)(8 - el);
     float sum = 0.f;
     i32x8 ph, pl;
 #pragma unroll
     for (int w = 0; w < 8; w++) {
       float y[4];
 #pragma unroll
-      for (int e = 0; e < 4; e++) y[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[w >> 2][4 * (w & 3) + e], p.sl2, sh));
+      for (int e = 0; e < 4; e++) y[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[w >> 2][4 * (w & 3) + e], p.sl2, bs.neg));
       sum += (y[0] + y[1]) + (y[2] + y[3]);
       uint32_t a, d;
-      split4(y[0], y[1], y[2], y[3], a, d);
+      split4(y[0], y[1], y[2], y[3], bs.unit, a, d);
       ph[w] = (int)a, pl[w] = (int)d;
     }
     const int sp = weight_byte(el, mn);
-    l += __builtin_amdgcn_ldexpf(halves_sum(sum), el - 8 - mn);
+    l += __builtin_amdgcn_ldexpf(halves_sum(sum), bs.e0 - mn);
     __builtin_amdgcn_s_setprio(1);
     bool nan = false;
     if (masked) {

@@ -415,3 +415,39 @@ def test_far_positions_and_masks(dev):
         assert torch.equal(ops.sdpa_kv8(q.to(dev), c.c, 100, **kw), full), kw
     for q0 in (-2 ** 31, -2 ** 32 + 50):
         assert not bool(ops.sdpa_kv8(q.to(dev), c.c, 100, causal_from=0, qpos0=q0).any()), q0
+
+
+# H, G, D, Tq, keys: the few-row kernel, 32-, 64- and 128-row tiles, runs of keys that are joined
+BIG = [(2, 1, 64, 30, 130), (1, 4, 128, 8, 130), (2, 1, 64, 90, 130), (1, 4, 128, 40, 130), (128, 1, 64, 60, 130), (32, 8, 128, 90, 70),
+       (1, 1, 64, 30, 5000), (1, 1, 128, 50, 17000)]
+
+
+@pytest.mark.parametrize("H,G,D,Tq,n", BIG)
+def test_sdpa_scores_up_to_the_stated_limit(dev, H, G, D, Tq, n):
+    """Scores of either sign from 2^-2 to 2^29 in size, mantissas of all kinds. One column of q and k is not zero, so a score is
+    one exact product and the softmax in 64 bits is known: beyond small scores it is the mean of the values at the largest.
+    A weight may be off by 2^-8 and by the exponential's 2^-12 with the score's rounding (2^-23 of scores below 32, where two
+    different ones both count): numerator and denominator, twice."""
+    g = torch.Generator(device=dev).manual_seed(H + D + Tq + n)
+    r = lambda *s: torch.rand(*s, generator=g, device=dev)
+    sign = lambda *s: torch.where(r(*s) < 0.5, -1.0, 1.0)
+    k = torch.zeros(1, H, n, D, device=dev)
+    k[..., 5] = 13 * 2.0 ** 12 * sign(1, H, n)
+    k[:, :, :64, 5] = -13 * 2.0 ** 12  # the running maximum moves
+    v = torch.randn(1, H, n, D, generator=g, device=dev).to(BF)
+    q = torch.zeros(1, H * G, Tq, D, device=dev)
+    top = 2.0 ** 29 / (13 * 2.0 ** 12 * D ** -0.5)
+    q[..., 5] = sign(1, H * G, Tq) * top * 0.99 * torch.exp2(-31 * r(1, H * G, Tq) * (r(1, H * G, Tq) < 0.7))
+    q = q.to(BF)
+    c = ops.KV8Cache(1, H, n, D, device=dev)
+    c.append(k.to(BF), v, 0)
+    print("large scores", H, G, D, Tq, n, flush=True)
+    for m in (n, 1, 67):  # 1: one visible key is its value
+        y = ops.sdpa_kv8(q, c, m).double().view(Tq, H, G, D)
+        kk, vv = (x[0, :, :m].double() for x in c.read())
+        s = (q.double().view(H, G * Tq, D)[..., 5:6] * kk[:, None, :, 5]) * D ** -0.5
+        p = torch.softmax(s, -1)
+        back = lambda x: x.view(H, G, Tq, D).permute(2, 0, 1, 3)
+        ref, avg = back(torch.matmul(p, vv)), back(torch.matmul(p, vv.abs()))
+        err = ((y - ref).abs() - 2.0 ** -8 * ref.abs() - 2 * (2.0 ** -8 + 2.0 ** -12) * avg).max().item()
+        assert err <= 0, (m, err)
