@@ -214,7 +214,7 @@ int mx_kv8_read(hipStream_t st, const uint8_t* kc, const uint8_t* vc, const uint
                 uint16_t* v, int nslots, int H, int n, int D, int ctx);
 /* o[b, i, h D ..] = softmax(scale q[b, h, i] K^T) V over the visible keys of slot b, key head h / G, for H G query heads:
  * j < len_b and (j < causal_from or j <= qpos + i) (qend: qpos = len_b - Tq; causal_from = INT_MAX: no mask); a row that
- * sees none is zero. scale > 0. Scores (times scale) have to stay below 2^29 in size: rows with
+ * sees none is zero. scale > 0, and scale log2(e) finite. Scores (times scale) have to stay below 2^29 in size: rows with
  * larger ones come out as 0 or NaN. q rows and strides 16-byte aligned, o 8-byte. part: mx_kv8_sdpa_ws() floats, 16-byte
  * aligned, free again once the call's kernels have run (null where that is 0). */
 long mx_kv8_sdpa_ws(int B, int H, int G, int Tq, int ctx, int D);

@@ -775,7 +775,7 @@ extern "C" int mx_kv8_sdpa(hipStream_t st, const uint16_t* q, long sq_b, long sq
   if (!q || !kc || !vc || !ks || !vs || !o) return MX_ENULL;
   if (D != 64 && D != 128) return MX_EBADCFG;
   if (B < 1 || H < 1 || G < 1 || Tq < 1 || ctx < 1 || ctx > 0x7fffff00 || (long)Tq * G > 0x7fffff00L) return MX_ESHAPE;
-  if (!(scale > 0.f) || !(scale < INFINITY) || causal_from < 0) return MX_ESHAPE;
+  if (!(scale > 0.f) || !(scale * 1.4426950408889634f < INFINITY) || causal_from < 0) return MX_ESHAPE;
   if ((sq_b | sq_h | sq_t) % 8 || (so_b | so_t) % 4) return MX_ESHAPE;
   if (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc) & 15 || ((uintptr_t)o & 7) || ((uintptr_t)len & 3)) return MX_ELAYOUT;
   const Plan pl = plan(B, H, G, Tq, ctx, D);

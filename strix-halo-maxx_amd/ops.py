@@ -1016,8 +1016,8 @@ def sdpa_kv8(q, cache, kv_len, base=0, out=None, scale=None, qpos0=None, causal_
     if lp is None and not 0 <= base <= cache.ctx:
         raise ValueError(f"length {base} outside the {cache.ctx}-entry cache")
     sc = D ** -0.5 if scale is None else float(scale)
-    if not 0.0 < sc < float("inf"):
-        raise ValueError(f"scale {sc} must be positive and finite")
+    if not 0.0 < sc <= 2.0 ** 127:  # the kernel multiplies by scale log2(e), a float
+        raise ValueError(f"scale {sc} must be positive and finite, at most 2^127")
     cf = 0x7fffffff if causal_from is None else min(int(causal_from), 0x7fffffff)
     if cf < 0:
         raise ValueError("causal_from must not be negative")

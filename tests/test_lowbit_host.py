@@ -211,3 +211,12 @@ def test_layernorm_linear_refusals():
     raises("float32", lin.ln, x, (v.float(), v))
     raises("gated", lin.ln, x, (v, v), act="glu")
     raises("out must", lin.ln, x, (v, v), out=torch.zeros(1, 9, dtype=BF))
+
+
+def test_scale_whose_product_overflows():
+    """scale log2(e) is what the kernel multiplies by: infinite, it would make 0 times it NaN."""
+    lib = _lib.load()
+    sd = lambda scale: lib.mx_kv8_sdpa(None, A16, 64, 64, 64, A16, A16, A16, A16, A16, 64, 64, 1, 1, 1, 1, 64, 100, None, 0, 50, 0,
+                                       1, 0, scale, None, 0)
+    assert sd(3e38) == -2 and sd(math.inf) == -2
+    raises("at most 2", ops.sdpa_kv8, torch.zeros(1, 1, 1, 64, dtype=BF), ops.KV8Cache(1, 1, 9, 64, device="cpu"), 5, scale=3e38)
