@@ -740,7 +740,7 @@ class MxFp4:
         else:
             y = out
             _need(y, "out", dev)
-            if y.shape != (M, K) or y.stride(1) != 1:
+            if y.shape != (M, K) or (y.stride(1) != 1 and K > 1):
                 raise ValueError(f"out must be ({M}, {K}) with unit column stride")
         if M:
             _call_on(dev, "mx_mxfp4_values", *self.ptrs, y.data_ptr(), y.stride(0), M, K)
@@ -897,6 +897,11 @@ def _int32(v, name):
     return v
 
 
+def _steps(t):
+    """The strides of t, 0 for dimensions of size 1: what those carry is never walked."""
+    return [s if n > 1 else 0 for n, s in zip(t.shape, t.stride())]
+
+
 def _rows4(t):
     """t with unit column stride (copied if it has another)."""
     return t if t.stride(-1) == 1 else t.contiguous()
@@ -1024,25 +1029,27 @@ def sdpa_kv8(q, cache, kv_len, base=0, out=None, scale=None, qpos0=None, causal_
     q0 = 0 if qpos0 is None else max(-0x80000000, min(int(qpos0), 0x7fffffff))  # positions all lie inside 31 bits
     if out is None:
         out = torch.empty(B, Tq, Hq * D, device=dev, dtype=BF)
+        so = out.stride()
     else:
         _need(out, "out", dev)
-        if out.shape != (B, Tq, Hq * D) or out.stride(2) != 1 or (out.stride(0) | out.stride(1)) % 4 or out.data_ptr() % 8:
+        so = _steps(out)
+        if out.shape != (B, Tq, Hq * D) or so[2] != 1 or (so[0] | so[1]) % 4 or out.data_ptr() % 8:
             raise ValueError(f"out must be ({B}, {Tq}, {Hq * D}) with 8-byte aligned rows of unit stride")
     if not out.numel():
         return out
-    s = q.stride()
+    s = _steps(q)
     if s[3] != 1 or (s[0] | s[1] | s[2]) % 8 or q.data_ptr() % 16:
         q = q.contiguous()
         if q.data_ptr() % 16:
             q = q.clone()
-        s = q.stride()
+        s = _steps(q)
     G = Hq // cache.heads
     need = cache._ws.get((B, G, Tq))
     if need is None:
         need = cache._ws[(B, G, Tq)] = _lib.load().mx_kv8_sdpa_ws(B, cache.heads, G, Tq, cache.ctx, D)
     part = torch.empty(need, device=dev, dtype=torch.float32) if need else None
-    _call_on(dev, "mx_kv8_sdpa", q.data_ptr(), s[0], s[1], s[2], *cache.ptrs, out.data_ptr(), out.stride(0),
-             out.stride(1), B, cache.heads, G, Tq, D, cache.ctx, lp, ls, base, q0, int(qpos0 is None), cf, sc, ptr(part), need)
+    _call_on(dev, "mx_kv8_sdpa", q.data_ptr(), s[0], s[1], s[2], *cache.ptrs, out.data_ptr(), so[0], so[1],
+             B, cache.heads, G, Tq, D, cache.ctx, lp, ls, base, q0, int(qpos0 is None), cf, sc, ptr(part), need)
     return out
 
 

@@ -451,3 +451,27 @@ def test_sdpa_scores_up_to_the_stated_limit(dev, H, G, D, Tq, n):
         ref, avg = back(torch.matmul(p, vv)), back(torch.matmul(p, vv.abs()))
         err = ((y - ref).abs() - 2.0 ** -8 * ref.abs() - 2 * (2.0 ** -8 + 2.0 ** -12) * avg).max().item()
         assert err <= 0, (m, err)
+
+
+@pytest.mark.parametrize("D,Hq,Tq", [(64, 4, 1), (64, 4, 9), (128, 2, 1), (64, 1, 3)])
+def test_sdpa_dimensions_of_size_one_carry_any_stride(dev, D, Hq, Tq):
+    """One sequence, one token or one head, cut from buffers of odd pitch: strides that are never walked refuse nothing, for q and
+    for out."""
+    g = gen(D + Hq + Tq)
+    c = Both(dev, 1, 1, 100, D)
+    c.append(rows(g, 1, 1, 90, D), rows(g, 1, 1, 90, D), 0)
+    q = rows(g, 1, Hq, Tq, D)
+    want = ops.sdpa_kv8(q.to(dev), c.c, 90)
+    check_sdpa(want.cpu(), q, c, (90,))
+    W = Hq * D
+    # (B, Tq, W) rows inside odd pitches: the batch's, and with one token the row's
+    pitch = W + (3 if Tq == 1 else 8)
+    fused = torch.empty(Tq * pitch + 8, device=dev, dtype=BF)
+    view = fused.as_strided((1, Hq, Tq, D), (Tq * pitch + 3, D if Hq > 1 else 5, pitch, 1))
+    view.copy_(q)
+    big = torch.full((2 * (Tq * pitch + 8),), 5.0, device=dev, dtype=BF)
+    out = big.as_strided((1, Tq, W), (Tq * pitch + 3, pitch, 1), 8)
+    assert ops.sdpa_kv8(view, c.c, 90, out=out) is out and torch.equal(out, want)
+    out.fill_(5.0)
+    assert bool((big == 5.0).all())
+    assert torch.equal(ops.sdpa_kv8(view, c.c, 90), want)

@@ -220,3 +220,13 @@ def test_scale_whose_product_overflows():
                                        1, 0, scale, None, 0)
     assert sd(3e38) == -2 and sd(math.inf) == -2
     raises("at most 2", ops.sdpa_kv8, torch.zeros(1, 1, 1, 64, dtype=BF), ops.KV8Cache(1, 1, 9, 64, device="cpu"), 5, scale=3e38)
+
+
+def test_strides_of_size_one_are_not_looked_at():
+    c = ops.KV8Cache(1, 1, 100, 64, device="cpu")
+    q = torch.zeros(1, 2, 1, 64, dtype=BF)
+    raises("GPU", ops.sdpa_kv8, q, c, 5, out=torch.zeros(400, dtype=BF).as_strided((1, 1, 128), (131, 129, 1)))
+    raises("out must", ops.sdpa_kv8, torch.zeros(1, 2, 2, 64, dtype=BF), c, 5,
+           out=torch.zeros(400, dtype=BF).as_strided((1, 2, 128), (1, 129, 1)))
+    w = ops.MxFp4(torch.zeros(4352, dtype=torch.uint8), 10, 1)
+    raises("GPU", w.values, out=torch.zeros(1, 10, dtype=BF).t())
