@@ -701,11 +701,14 @@ def _rows2(x):
     return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
 
 
+def _end(t):
+    """The address behind the last element of a tensor that is not empty."""
+    return t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+
+
 def _apart(a, b):
-    """Whether the memory of the 2-D a, from its first element to its last, and that of b do not meet."""
-    p, q = a.data_ptr(), b.data_ptr()
-    return (p + ((a.shape[0] - 1) * a.stride(0) + a.shape[1]) * a.element_size() <= q
-            or q + ((b.shape[0] - 1) * b.stride(0) + b.shape[1]) * b.element_size() <= p)
+    """Whether the memory of a, from its first element to its last, and that of b do not meet."""
+    return _end(a) <= b.data_ptr() or _end(b) <= a.data_ptr()
 
 
 class MxFp4:
@@ -766,8 +769,9 @@ class MxFp4Lin:
     """MXFP4 Linear: y = act(x W^T + b) [+ res] with W quantised once and x per call (quant_mxfp4's rule for both), on the
     scaled MFMA; fp32 throughout, rounded to bf16 once. `pre` takes an already quantised input (MxFp4), so layers that
     read the same activation share one quantisation. Any (N, K); inputs have K columns, or K rounded up to 8 (Kp), of
-    which the first K are read. act: None / "tanh" / "erf", on columns >= act_from. `out` may be x or res itself. Few rows
-    are quantised inside the product's launch; the results are the same."""
+    which the first K are read. act: None / "tanh" / "erf", on columns >= act_from. `out` may lie in the memory of x or res (res
+    is copied first unless each of its elements is where its result goes). Few rows are quantised inside the product's
+    launch; the results are the same."""
     fused_gelu = True
     fused_res = True
 
@@ -840,6 +844,11 @@ class MxFp4Lin:
                 if not r2.shape[0] or M % r2.shape[0]:
                     raise ValueError("residual rows must equal or divide the output rows")
                 r_rows = r2.shape[0]
+            if M and out is not None and not _apart(r2, y2) and (
+                    r_rows or r2.data_ptr() != y2.data_ptr() or (r2.stride(0) != y2.stride(0) and M > 1)):
+                # only where every element of res lies in the place of its own result may the product write over it
+                r2 = r2.clone(memory_format=torch.contiguous_format)
+                ldr = r2.stride(0)
         if M:
             tail = (*self.wq.ptrs, self.bp, None if r2 is None else r2.data_ptr(), ldr, r_rows, y2.data_ptr(), y2.stride(0), M, N, K, a, act_from)
             if pre is None and M <= self.rows and (out is None or _apart(x2, y2)):

@@ -273,3 +273,29 @@ def test_linear_of_a_layernorm_onto_its_input(dev):
     want = lin.ln(x, ln)
     lin.ln(x, ln, out=x)
     assert torch.equal(x, want)
+
+
+@pytest.mark.parametrize("M,N,K", [(4, 96, 256), (12, 512, 512), (60, 1000, 320), (768, 2048, 640)])
+def test_residual_that_overlaps_the_output(dev, M, N, K):
+    """A residual in the output's memory, other than as the output itself: rows that repeat, rows or columns further on, one row
+    for all, another pitch. Each result takes the residual as it was before the call."""
+    g = gen(M + N + K)
+    lin = ops.MxFp4Lin((torch.randn(N, K, generator=g) * 0.1).to(BF), torch.randn(N, generator=g), device=dev)
+    x = torch.randn(M, K, generator=g).to(BF).to(dev)
+    buf0 = torch.randn((M + 3) * (N + 16), generator=g).to(BF).to(dev)
+    at = lambda b, rows, ld, off=0, step=1: b.as_strided((rows, N), (ld, step), off)
+    ld = N + 16
+    views = [(at(buf0, M // 2, ld), 0), (at(buf0, 1, ld), 0), (at(buf0, M, ld, ld), 0), (at(buf0, M, ld, 8), 0), (at(buf0, M, ld), 8),
+             (at(buf0, M, 0, 2 * ld), 0), (at(buf0, M, N), 0), (at(buf0, M // 4, ld, ld), 0)]
+    for r0, off in views:
+        want = lin(x, res=r0.clone())
+        for _ in range(3):
+            buf = buf0.clone()
+            res = buf.as_strided(r0.shape, r0.stride(), r0.storage_offset())
+            y = at(buf, M, ld, off)
+            assert lin(x, res=res, out=y) is y and torch.equal(y, want), (r0.shape, r0.stride(), r0.storage_offset(), off)
+    # as the output itself nothing is copied, and a single row's pitch does not matter
+    buf = buf0.clone()
+    want = lin(x, res=at(buf0, M, ld).clone())
+    lin(x, res=at(buf, M, ld), out=at(buf, M, ld))
+    assert torch.equal(at(buf, M, ld), want)
