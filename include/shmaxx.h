@@ -215,8 +215,8 @@ int mx_kv8_read(hipStream_t st, const uint8_t* kc, const uint8_t* vc, const uint
 /* o[b, i, h D ..] = softmax(scale q[b, h, i] K^T) V over the visible keys of slot b, key head h / G, for H G query heads:
  * j < len_b and (j < causal_from or j <= qpos + i) (qend: qpos = len_b - Tq; causal_from = INT_MAX: no mask); a row that
  * sees none is zero. scale > 0, and scale log2(e) finite. Scores (times scale) have to stay below 2^29 in size: rows with
- * larger ones come out as 0 or NaN. q rows and strides 16-byte aligned, o 8-byte. part: mx_kv8_sdpa_ws() floats, 16-byte
- * aligned, free again once the call's kernels have run (null where that is 0). */
+ * larger ones come out as 0 or NaN. q rows and strides 16-byte aligned, o 8-byte; o must not meet q. part:
+ * mx_kv8_sdpa_ws() floats, 16-byte aligned, free again once the call's kernels have run (null where that is 0). */
 long mx_kv8_sdpa_ws(int B, int H, int G, int Tq, int ctx, int D);
 int mx_kv8_sdpa(hipStream_t st, const uint16_t* q, long sq_b, long sq_h, long sq_t, const uint8_t* kc, const uint8_t* vc,
                 const uint8_t* ks, const uint8_t* vs, uint16_t* o, long so_b, long so_t, int B, int H, int G, int Tq,

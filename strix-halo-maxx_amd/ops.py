@@ -1019,6 +1019,7 @@ def sdpa_kv8(q, cache, kv_len, base=0, out=None, scale=None, qpos0=None, causal_
     kv_len: an int, or an int32 tensor (B,) read on the device (values outside 0 .. ctx are clamped). Mask, as in sdpa:
     key j is visible to query i iff j < len_b and (j < causal_from or j <= qpos0 + i); causal_from=None: no mask;
     qpos0=None: the queries are the last Tq tokens of their sequence, qpos0 = len_b - Tq. Rows that see no key are 0.
+    out may lie in q's memory.
     Scores (times scale) have to stay below 2^29 in size: larger ones come out as 0 or NaN."""
     if q.dim() != 4 or q.shape[3] != cache.hd or q.shape[1] < 1 or q.shape[1] % cache.heads or q.shape[0] > cache.slots:
         raise ValueError(f"q {tuple(q.shape)} does not fit a cache of {cache.slots} x {cache.heads} heads x {cache.hd}")
@@ -1036,7 +1037,8 @@ def sdpa_kv8(q, cache, kv_len, base=0, out=None, scale=None, qpos0=None, causal_
     if cf < 0:
         raise ValueError("causal_from must not be negative")
     q0 = 0 if qpos0 is None else max(-0x80000000, min(int(qpos0), 0x7fffffff))  # positions all lie inside 31 bits
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(B, Tq, Hq * D, device=dev, dtype=BF)
         so = out.stride()
     else:
@@ -1046,6 +1048,8 @@ def sdpa_kv8(q, cache, kv_len, base=0, out=None, scale=None, qpos0=None, causal_
             raise ValueError(f"out must be ({B}, {Tq}, {Hq * D}) with 8-byte aligned rows of unit stride")
     if not out.numel():
         return out
+    if given and not _apart(q, out):
+        q = q.clone()  # a row's output may lie over another's query
     s = _steps(q)
     if s[3] != 1 or (s[0] | s[1] | s[2]) % 8 or q.data_ptr() % 16:
         q = q.contiguous()

@@ -475,3 +475,22 @@ def test_sdpa_dimensions_of_size_one_carry_any_stride(dev, D, Hq, Tq):
     out.fill_(5.0)
     assert bool((big == 5.0).all())
     assert torch.equal(ops.sdpa_kv8(view, c.c, 90), want)
+
+
+# more workgroups than the device holds at once: the last ones would read what the first ones have written
+@pytest.mark.parametrize("B,H,G,D,Tq", [(2, 4, 2, 64, 1), (1, 4096, 1, 64, 32), (1, 32, 1, 128, 4096), (1, 64, 1, 64, 4096)])
+def test_sdpa_onto_its_own_queries(dev, B, H, G, D, Tq):
+    """out in q's memory: (B, Hq, Tq, D) read, (B, Tq, Hq D) written over it, and a shifted view."""
+    g = torch.Generator(device=dev).manual_seed(B + H + Tq)
+    r = lambda *s: torch.randn(*s, generator=g, device=dev).to(BF)
+    c = ops.KV8Cache(B, H, 300, D, device=dev)
+    c.append(r(B, H, 300, D), r(B, H, 300, D), 0)
+    n = B * H * G * Tq * D
+    mem = r(n + 8)
+    q = mem[:n].view(B, H * G, Tq, D)
+    want = ops.sdpa_kv8(q, c, 300, causal_from=0)
+    for off in (0, 8):
+        for _ in range(3):
+            buf = mem.clone()
+            out = buf[off:n + off].view(B, Tq, H * G * D)
+            assert ops.sdpa_kv8(buf[:n].view(q.shape), c, 300, causal_from=0, out=out) is out and torch.equal(out, want), off
