@@ -161,8 +161,9 @@ int mx_quant_mxfp4(hipStream_t st, const uint16_t* x, long ldx, uint8_t* codes, 
 int mx_mxfp4_values(hipStream_t st, const uint8_t* codes, const uint8_t* scales, uint16_t* y, long ldy, int M, int K);
 /* C[m, n] = act(sum_k x[m, k] W[n, k] + bias[n]) + R[m % r_rows or m, n], both operands in MXFP4, fp32 throughout and
  * rounded to bf16 once. act: 0 none, 1 GELU-tanh, 2 GELU-erf, on columns >= act_from. bias, R nullable; any M, N up to
- * 2^27, K up to 2^22. R may be C itself; C must not meet x. mx_gemm_mxfp4 takes quantised rows; mx_gemv_mxfp4 takes at most
- * mx_gemv_mxfp4_rows() rows in bf16 and quantises them on the way (the same result). */
+ * 2^27, K up to 2^22. R may be C itself (the same address and row stride, r_rows 0); C must not meet R otherwise, nor x.
+ * mx_gemm_mxfp4 takes quantised rows; mx_gemv_mxfp4 takes at most mx_gemv_mxfp4_rows() rows in bf16 and quantises them on
+ * the way (the same result). */
 int mx_gemv_mxfp4_rows(void);
 int mx_gemv_mxfp4(hipStream_t st, const uint16_t* x, long ldx, const uint8_t* wc, const uint8_t* ws, const float* bias,
                   const uint16_t* R, long ldr, int r_rows, uint16_t* C, long ldc, int M, int N, int K, int act,
