@@ -126,6 +126,7 @@ class TextDecoder:
         self.full_logits = False  # True: all V logits (the reference's diagnostics switch, md2fast.py:116)
         self.tok_buf = torch.zeros(self.nq, self.L, device=dev, dtype=torch.int64)
         self.last_idx = torch.zeros(self.nq, device=dev, dtype=torch.int64)
+        self.q_len = torch.full((self.nq,), self.L, device=dev, dtype=torch.int32)  # ids of each question, without padding
         self.prefix = None
         self.query_graph = None
         self.prefill_graph = None  # (graph, hidden-state output, image rows, prompt length) of capture_prefill
@@ -202,11 +203,12 @@ class TextDecoder:
             self.mk_ep.zero_()
 
     # ------------------------------------------------------------------ prefill (md2fast.py:169-212)
-    def _text_layers(self, x, pos0, causal_from, B=1, bcast=False):
+    def _text_layers(self, x, pos0, causal_from, B=1, bcast=False, count=None):
         """x (B * n, D) bf16: B sequences (cache slots 0 .. B - 1) of n tokens at positions pos0 .. pos0 + n - 1;
         attends to keys 0 .. pos0 + n - 1 of its own slot (key j visible to query i iff j < causal_from or
         j <= pos0 + i; causal_from=None: all). bcast (B = 1): the K/V rows go to every cache slot (the shared image
-        prefix, md2fast.py:177 rope_cache(..., bcast=(pos0 == 0)))."""
+        prefix, md2fast.py:177 rope_cache(..., bcast=(pos0 == 0))). count (int32 (B,), 8-bit cache only): rows of each
+        sequence that go into the cache; the rest is padding, whose size would raise the exponents of the blocks."""
         n = x.shape[0] // B
         H, hd = self.H, self.hd
         Tk = pos0 + n
@@ -233,7 +235,7 @@ class TextDecoder:
             else:
                 qkv, f = b["qkv"](h, pre=pre), None
             if self.kv8:
-                a = self._attend_kv8(i, qkv, pos0, Tk, causal_from, B, bcast, a)
+                a = self._attend_kv8(i, qkv, pos0, Tk, causal_from, B, bcast, a, count)
             else:
                 q = torch.empty(B, H, n, hd, device=self.dev, dtype=BF)
                 call("mx_rope_kv", stream(), qkv.data_ptr(), qkv.stride(0), self.cs.data_ptr(), q.data_ptr(),
@@ -254,12 +256,12 @@ class TextDecoder:
                 x, h = b["fc2"](f, res=r), None
         return x
 
-    def _attend_kv8(self, i, qkv, pos0, kv_len, causal_from, B, bcast, out=None):
+    def _attend_kv8(self, i, qkv, pos0, kv_len, causal_from, B, bcast, out=None, count=None):
         """Layer i's rotary embedding, append to the 8-bit cache and attention for B sequences of fused rows qkv
         (B * n, >= 3 D) at pos0 ..; the attention reads the quantised rows, the new ones too."""
         n = qkv.shape[0] // B
         q, k, v = qkv[:, :3 * self.D].view(B, n, 3, self.H, self.hd).permute(2, 0, 3, 1, 4)
-        q = self.kv[i].append(k, v, pos0, bcast=bcast, cs=self.cs, q=q)
+        q = self.kv[i].append(k, v, pos0, count=count, bcast=bcast, cs=self.cs, q=q)
         return ops.sdpa_kv8(q, self.kv[i], kv_len, qpos0=pos0, causal_from=causal_from, out=out)
 
     def _save_prefix_end(self):
@@ -370,6 +372,7 @@ class TextDecoder:
             last[b] = b * self.L + ids.numel() - 1
         self.tok_buf.copy_(buf)
         self.last_idx.copy_(last)
+        self.q_len.copy_(last - torch.arange(self.nq) * self.L + 1)
 
     def _query(self):
         if self.prefix is None:
@@ -377,7 +380,7 @@ class TextDecoder:
         P = self.prefix
         self._restore_prefix_end()
         x = self.wte[self.tok_buf.view(-1)]                                   # (nq * L, D)
-        x = self._text_layers(x, P, P, B=self.nq)
+        x = self._text_layers(x, P, P, B=self.nq, count=self.q_len)
         h = ops.layernorm(x.index_select(0, self.last_idx), *self.post_ln, eps=self.eps)  # (nq, D)
         if self.full_logits:
             if self.lm_full is None:

@@ -138,3 +138,63 @@ def test_formats_that_exclude_each_other(dev):
     with pytest.raises(ValueError, match="Linear class"):
         mt.TextDecoder(w, lin_cls=ops.MxI8Lin, mxfp4=True)
     assert mt.TextDecoder(w, lin_cls=ops.MxFp4Lin, ctx=64).mxfp4
+
+
+def questions(dev, **kw):
+    w = S.text_weights(6, layers=kw.pop("layers", 2))
+    return mt.TextDecoder(w, ctx=256, nq=2, yes_ids=[11, 222, 3333, 44444], no_ids=[55, 666, 7777, 50000], **kw)
+
+
+def cached(dec, n):
+    """What the caches hold of positions 0 .. n - 1 of each slot (n: a length for each)."""
+    return [x[s, :, :m].clone() for kv in dec.kv for x in kv.read() for s, m in enumerate(n)]
+
+
+def scales(dec, n):
+    return [x[s, :, :-(-m // 64)].clone() for kv in dec.kv for x in (kv.ks, kv.vs) for s, m in enumerate(n)]
+
+
+def equal(a, b):
+    return len(a) == len(b) and all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("form", [f for f in FORMS if f.get("kv8")], ids=name)
+def test_question_does_not_depend_on_its_padding(dev, form):
+    """Rows behind a question's end leave its logits, its cached rows and the exponents of their blocks alone: other embeddings of
+    the padding id change nothing, eager and captured; and the ids of one question nothing in the other."""
+    dec = questions(dev, L=24, **form)
+    img, _ = inputs(dev, 70)
+    dec.encode(img)
+    q = [S.prompt_ids(1, 9).tolist(), S.prompt_ids(2, 14).tolist()]
+    dec.set_questions(q)
+    n = [71 + len(x) for x in q]
+    want = dec.query().clone(), cached(dec, n), scales(dec, n)
+    pads = S.activations(3, (4, D), "pad").to(dev)
+    pads[2, 7], pads[3] = 300.0, 0
+    for pad in pads:
+        dec.wte[0] = pad
+        assert torch.equal(dec.query(), want[0]) and equal(cached(dec, n), want[1]) and equal(scales(dec, n), want[2])
+    dec.capture_query()
+    for pad in pads:
+        dec.wte[0] = pad
+        assert torch.equal(dec.query(), want[0]) and equal(cached(dec, n), want[1]) and equal(scales(dec, n), want[2])
+    dec.set_questions([q[0], S.prompt_ids(5, 24).tolist()])  # longer: the replayed graph follows the lengths
+    got = dec.query().clone()
+    assert torch.equal(got[0], want[0][0]) and not torch.equal(got[1], want[0][1])
+    dec.query_graph = None
+    assert torch.equal(dec.query(), got)
+
+
+def test_question_does_not_depend_on_the_rows_it_is_padded_to(dev):
+    """MXFP4 products give a row the same bits whatever the number of rows up to 32: L = 10 and L = 16 agree."""
+    img, _ = inputs(dev, 70)
+    q = [S.prompt_ids(1, 9).tolist(), S.prompt_ids(2, 10).tolist()]
+    n, out = [71 + len(x) for x in q], []
+    for L in (10, 16):
+        dec = questions(dev, L=L, mxfp4=True, kv8=True)
+        dec.wte[0] = 0
+        dec.wte[0, 7] = 300.0
+        dec.encode(img)
+        dec.set_questions(q)
+        out.append((dec.query().clone(), cached(dec, n), scales(dec, n)))
+    assert torch.equal(out[0][0], out[1][0]) and equal(out[0][1], out[1][1]) and equal(out[0][2], out[1][2])
