@@ -104,8 +104,10 @@ class TextDecoder:
             nb = -(-ctx // ops.KV8Cache.BLOCK)
             z = lambda *s: torch.zeros(n, self.nq, self.H, *s, device=dev, dtype=torch.uint8)
             self.kv_all = (z(nb, 64 * self.hd), z(nb, 64 * self.hd), z(nb), z(nb))
-            self.kv_end = (z(64 * self.hd), z(64 * self.hd), z(), z())  # the prefix's last block, as the prefill left it
             self.kv = [ops.KV8Cache.over(*(t[i] for t in self.kv_all), ctx) for i in range(n)]
+            # the block that the prefix ends in with the prefix's rows alone: a cache of one block per layer
+            self.kv_end_all = (z(1, 64 * self.hd), z(1, 64 * self.hd), z(1), z(1))
+            self.kv_end = [ops.KV8Cache.over(*(t[i] for t in self.kv_end_all), ops.KV8Cache.BLOCK) for i in range(n)]
             self.kc = self.vc = None
         else:
             self.kc = [torch.zeros(self.nq, self.H, ctx, self.hd, device=dev, dtype=BF) for _ in self.blocks]
@@ -203,12 +205,13 @@ class TextDecoder:
             self.mk_ep.zero_()
 
     # ------------------------------------------------------------------ prefill (md2fast.py:169-212)
-    def _text_layers(self, x, pos0, causal_from, B=1, bcast=False, count=None):
+    def _text_layers(self, x, pos0, causal_from, B=1, bcast=False, count=None, prefix=None):
         """x (B * n, D) bf16: B sequences (cache slots 0 .. B - 1) of n tokens at positions pos0 .. pos0 + n - 1;
         attends to keys 0 .. pos0 + n - 1 of its own slot (key j visible to query i iff j < causal_from or
         j <= pos0 + i; causal_from=None: all). bcast (B = 1): the K/V rows go to every cache slot (the shared image
         prefix, md2fast.py:177 rope_cache(..., bcast=(pos0 == 0))). count (int32 (B,), 8-bit cache only): rows of each
-        sequence that go into the cache; the rest is padding, whose size would raise the exponents of the blocks."""
+        sequence that go into the cache; the rest is padding, whose size would raise the exponents of the blocks. prefix
+        (8-bit cache only): keep the block that the first `prefix` rows end in as those rows alone give it."""
         n = x.shape[0] // B
         H, hd = self.H, self.hd
         Tk = pos0 + n
@@ -235,7 +238,7 @@ class TextDecoder:
             else:
                 qkv, f = b["qkv"](h, pre=pre), None
             if self.kv8:
-                a = self._attend_kv8(i, qkv, pos0, Tk, causal_from, B, bcast, a, count)
+                a = self._attend_kv8(i, qkv, pos0, Tk, causal_from, B, bcast, a, count, prefix)
             else:
                 q = torch.empty(B, H, n, hd, device=self.dev, dtype=BF)
                 call("mx_rope_kv", stream(), qkv.data_ptr(), qkv.stride(0), self.cs.data_ptr(), q.data_ptr(),
@@ -256,28 +259,34 @@ class TextDecoder:
                 x, h = b["fc2"](f, res=r), None
         return x
 
-    def _attend_kv8(self, i, qkv, pos0, kv_len, causal_from, B, bcast, out=None, count=None):
+    def _attend_kv8(self, i, qkv, pos0, kv_len, causal_from, B, bcast, out=None, count=None,
+                    prefix=None):
         """Layer i's rotary embedding, append to the 8-bit cache and attention for B sequences of fused rows qkv
         (B * n, >= 3 D) at pos0 ..; the attention reads the quantised rows, the new ones too."""
         n = qkv.shape[0] // B
         q, k, v = qkv[:, :3 * self.D].view(B, n, 3, self.H, self.hd).permute(2, 0, 3, 1, 4)
         q = self.kv[i].append(k, v, pos0, count=count, bcast=bcast, cs=self.cs, q=q)
+        if prefix is not None:
+            lo = self._end_block(prefix) * ops.KV8Cache.BLOCK
+            self.kv_end[i].append(k[:, :, lo:prefix], v[:, :, lo:prefix], 0, bcast=True, cs=self.cs[lo:])
         return ops.sdpa_kv8(q, self.kv[i], kv_len, qpos0=pos0, causal_from=causal_from, out=out)
 
+    # The block that the prefix ends in also takes the rows behind it, and their size may round the prefix's rows once more:
+    # it is kept as the prefix's rows alone give it, so that every query finds the same prefix.
     def _save_prefix_end(self):
-        """The block that the prefix ends in also takes the rows behind it, and their size may round the prefix's rows once
-        more: kept here as the prefill left it, so that every query finds the same prefix."""
+        """After a pass over the prefix alone (one over the prompt too keeps the block itself)."""
         if self.kv8:
-            for t, e in zip(self.kv_all, self.kv_end):
-                e.copy_(t[:, :, :, self._end_block()])
+            for t, e in zip(self.kv_all, self.kv_end_all):
+                e[:, :, :, 0].copy_(t[:, :, :, self._end_block(self.prefix)])
 
     def _restore_prefix_end(self):
         if self.kv8:
-            for t, e in zip(self.kv_all, self.kv_end):
-                t[:, :, :, self._end_block()].copy_(e)
+            for t, e in zip(self.kv_all, self.kv_end_all):
+                t[:, :, :, self._end_block(self.prefix)].copy_(e[:, :, :, 0])
 
-    def _end_block(self):
-        return (self.prefix - 1) // ops.KV8Cache.BLOCK
+    @staticmethod
+    def _end_block(prefix):
+        return (prefix - 1) // ops.KV8Cache.BLOCK
 
     def _fuse_next_ln(self, lin, M):
         """fc2 + residual + the next layer's LayerNorm as partials + one row kernel: bf16 Linears whose row count has a
@@ -292,7 +301,8 @@ class TextDecoder:
         j <= i: prefix queries see the prefix only, mask-free; prompt queries the prefix and the prompt up to
         themselves). All rows' K/V go into every cache slot (the prefix's must; the prompt rows in slots other than 0
         are rewritten by query() before it reads them). Leaves the first generated token's argmax in `part` and returns
-        the prompt's hidden states.
+        the prompt's hidden states. With the 8-bit cache, a block that holds the prefix's end and prompt rows has one exponent
+        for both while this pass attends to it; query() finds that block as the layer's prefix rows alone give it.
         With a graph from capture_prefill() for these shapes, the inputs are copied into its buffers and it is replayed
         (the returned tensor is then the graph's output buffer, overwritten by the next replay)."""
         pg = self.prefill_graph
@@ -312,9 +322,8 @@ class TextDecoder:
         x = torch.cat([self.wte[BOS:BOS + 1], img_emb.to(self.dev, BF), self.wte[prompt_ids.to(self.dev)]], dim=0)
         if x.shape[0] > self.ctx:
             raise ValueError(f"prefill of {x.shape[0]} tokens exceeds the cache ({self.ctx})")
-        xp = self._text_layers(x, 0, P, bcast=True)[P:]
+        xp = self._text_layers(x, 0, P, bcast=True, prefix=P if self.kv8 else None)[P:]
         self.prefix = P
-        self._save_prefix_end()
         self.pos_base = x.shape[0]
         self.lm_argmax(xp[-1], logits=True)
         return xp

@@ -198,3 +198,28 @@ def test_question_does_not_depend_on_the_rows_it_is_padded_to(dev):
         dec.set_questions(q)
         out.append((dec.query().clone(), cached(dec, n), scales(dec, n)))
     assert torch.equal(out[0][0], out[1][0]) and equal(out[0][1], out[1][1]) and equal(out[0][2], out[1][2])
+
+
+@pytest.mark.parametrize("form", [dict(mxfp4=True, kv8=True), dict(w8a8=True, kv8=True)], ids=name)
+@pytest.mark.parametrize("n_img", [70, 63, 126])  # the prefix ends inside a block, with it, and on a block's last row but one
+def test_query_after_prefill_and_after_encode(dev, form, n_img):
+    """One layer, Linears that give a row the same bits in both passes: the prompt behind the prefix leaves the prefix that query()
+    reads as encode() leaves it, whatever the prompt, eager and captured, and so the logits."""
+    dec = questions(dev, L=16, layers=1, **form)
+    img, _ = inputs(dev, n_img)
+    q = [S.prompt_ids(1, 9).tolist(), S.prompt_ids(2, 16).tolist()]
+    dec.set_questions(q)
+    dec.encode(img)
+    n = [n_img + 1 + len(x) for x in q]
+    want = dec.query().clone(), cached(dec, n), scales(dec, n)
+    for graph in (False, True):
+        if graph:
+            dec.capture_prefill(n_img, 40)
+        for seed in (21, 22, 23):
+            hidden = dec.prefill(img, S.prompt_ids(seed, 40).to(dev)).clone()
+            assert torch.equal(dec.query(), want[0]) and equal(cached(dec, n), want[1]) and equal(scales(dec, n), want[2]), seed
+            assert torch.equal(dec.prefill(img, S.prompt_ids(seed, 40).to(dev)), hidden)
+            dec.start_decode()
+            for _ in range(3):
+                dec.decode_step()
+            assert torch.equal(dec.query(), want[0]) and equal(cached(dec, n), want[1]) and equal(scales(dec, n), want[2]), seed
