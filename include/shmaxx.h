@@ -160,10 +160,10 @@ long mx_mxfp4_scale_bytes(int M, int K);
 int mx_quant_mxfp4(hipStream_t st, const uint16_t* x, long ldx, uint8_t* codes, uint8_t* scales, int M, int K);
 int mx_mxfp4_values(hipStream_t st, const uint8_t* codes, const uint8_t* scales, uint16_t* y, long ldy, int M, int K);
 /* C[m, n] = act(sum_k x[m, k] W[n, k] + bias[n]) + R[m % r_rows or m, n], both operands in MXFP4, fp32 throughout and
- * rounded to bf16 once. act: 0 none, 1 GELU-tanh, 2 GELU-erf, on columns >= act_from. bias, R nullable; any M, N up to
- * 2^27, K up to 2^22. R may be C itself (the same address and row stride, r_rows 0); C must not meet R otherwise, nor x.
- * mx_gemm_mxfp4 takes quantised rows; mx_gemv_mxfp4 takes at most mx_gemv_mxfp4_rows() rows in bf16 and quantises them on
- * the way (the same result). */
+ * rounded to bf16 once. act: 0 none, 1 GELU-tanh, 2 GELU-erf, on columns >= act_from. bias, R nullable; any M (up to
+ * 64 * 65535 where K <= 256), N up to 2^27, K up to 2^22. R may be C itself (the same address and row stride, r_rows 0); C
+ * must not meet R otherwise, nor x. mx_gemm_mxfp4 takes quantised rows; mx_gemv_mxfp4 takes at most mx_gemv_mxfp4_rows()
+ * rows in bf16 and quantises them on the way (the same result). */
 int mx_gemv_mxfp4_rows(void);
 int mx_gemv_mxfp4(hipStream_t st, const uint16_t* x, long ldx, const uint8_t* wc, const uint8_t* ws, const float* bias,
                   const uint16_t* R, long ldr, int r_rows, uint16_t* C, long ldc, int M, int N, int K, int act,
@@ -171,6 +171,9 @@ int mx_gemv_mxfp4(hipStream_t st, const uint16_t* x, long ldx, const uint8_t* wc
 int mx_gemm_mxfp4(hipStream_t st, const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws,
                   const float* bias, const uint16_t* R, long ldr, int r_rows, uint16_t* C, long ldc, int M, int N, int K,
                   int act, int act_from);
+/* The kernel that mx_gemm_mxfp4 takes for a shape, for reading profiles: t[4] = rows and columns of C per workgroup, steps of
+ * 128 columns in the LDS ring (0: the few-row kernel), waves per workgroup (all 0 for sizes below 1). */
+void mx_gemm_mxfp4_tiling(int M, int N, int K, int* t);
 /* The same for the LayerNorm of one row, C = act(LayerNorm(x) W^T + bias): what mx_layernorm and mx_gemv_mxfp4 give, in one
  * launch. K a multiple of 8, at most mx_ln_gemv_mxfp4_cols(). */
 int mx_ln_gemv_mxfp4_cols(void);
@@ -219,6 +222,9 @@ int mx_kv8_read(hipStream_t st, const uint8_t* kc, const uint8_t* vc, const uint
  * larger ones come out as 0 or NaN. q rows and strides 16-byte aligned, o 8-byte; o must not meet q. part:
  * mx_kv8_sdpa_ws() floats, 16-byte aligned, free again once the call's kernels have run (null where that is 0). */
 long mx_kv8_sdpa_ws(int B, int H, int G, int Tq, int ctx, int D);
+/* How mx_kv8_sdpa cuts a call, for reading profiles: t[4] = rows per workgroup (16: the few-row kernel), waves that share the
+ * keys, runs of keys, blocks of 64 keys per run. */
+void mx_kv8_sdpa_tiling(int B, int H, int G, int Tq, int ctx, int D, int* t);
 int mx_kv8_sdpa(hipStream_t st, const uint16_t* q, long sq_b, long sq_h, long sq_t, const uint8_t* kc, const uint8_t* vc,
                 const uint8_t* ks, const uint8_t* vs, uint16_t* o, long so_b, long so_t, int B, int H, int G, int Tq,
                 int D, int ctx, const int* len, long len_s, int base, int qpos, int qend, int causal_from, float scale,

@@ -47,9 +47,11 @@ SIGNATURES = {
     "mx_ln_gemv_mxfp4": [P, P, P, P, F, P, P, P, P, I, I, I, I],
     "mx_gemv_mxfp4": [P, P, L, P, P, P, P, L, I, P, L, I, I, I, I, I],
     "mx_gemm_mxfp4": [P, P, P, P, P, P, P, L, I, P, L, I, I, I, I, I],
+    "mx_gemm_mxfp4_tiling": [I, I, I, P],
     "mx_kv8_append": [P, P, L, L, L, P, L, L, L, P, P, P, P, I, I, I, I, I, I, I, P, L, I, P, L, P, I, P, L, L, L, I, P],
     "mx_kv8_read": [P, P, P, P, P, P, P, I, I, I, I, I],
     "mx_kv8_sdpa_ws": [I, I, I, I, I, I],
+    "mx_kv8_sdpa_tiling": [I, I, I, I, I, I, P],
     "mx_kv8_sdpa": [P, P, L, L, L, P, P, P, P, P, L, L, I, I, I, I, I, I, P, L, I, I, I, I, F, P, L],
     "mx_sdpa": [P, P, L, L, L, P, L, L, L, P, L, L, L, P, L, L, L, I, I, I, I, I, F, I, I],
     "mx_sdpa_check": [P, L, P, L, P, L, P, L, I, I, I, I, I],
@@ -96,8 +98,9 @@ STATUS = {0: "ok", -1: "bad config", -2: "unsupported shape/stride", -3: "split-
           -4: "operand layout/alignment", -5: "HIP launch failed", -6: "null pointer"}
 
 RESTYPE = {"mx_gemm_ws_elems": L, "mx_gemm_ws_counters": L, "mx_track_head_blob_elems": L,
-           "mx_gemm_noalloc_max_ws": L, "mx_sdpa_tiling": None, "mx_gemm_res_ln_stats_words": L,
-           "mx_gemm_res_ln_sync_words": L, "mx_mxfp4_code_bytes": L, "mx_mxfp4_scale_bytes": L, "mx_kv8_sdpa_ws": L}
+           "mx_gemm_noalloc_max_ws": L, "mx_sdpa_tiling": None, "mx_gemm_mxfp4_tiling": None,
+           "mx_kv8_sdpa_tiling": None, "mx_gemm_res_ln_stats_words": L, "mx_gemm_res_ln_sync_words": L,
+           "mx_mxfp4_code_bytes": L, "mx_mxfp4_scale_bytes": L, "mx_kv8_sdpa_ws": L}
 
 _lib = None
 

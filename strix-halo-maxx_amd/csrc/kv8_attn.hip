@@ -768,6 +768,15 @@ extern "C" long mx_kv8_sdpa_ws(int B, int H, int G, int Tq, int ctx, int D) {
   return q.splits == 1 ? 0 : (long)B * H * q.nrt * q.splits * q.rw * (D + 2);
 }
 
+// How mx_kv8_sdpa cuts a call: t = rows per workgroup (16: the few-row kernel), waves that share the keys, runs of keys, blocks
+// of 64 keys per run.
+extern "C" void mx_kv8_sdpa_tiling(int B, int H, int G, int Tq, int ctx, int D, int* t) {
+  t[0] = t[1] = t[2] = t[3] = 0;
+  if (B < 1 || H < 1 || G < 1 || Tq < 1 || ctx < 1 || (D != 64 && D != 128)) return;
+  const Plan q = plan(B, H, G, Tq, ctx, D);
+  t[0] = q.rw, t[1] = q.nkw, t[2] = q.splits, t[3] = q.chunk;
+}
+
 extern "C" int mx_kv8_sdpa(hipStream_t st, const uint16_t* q, long sq_b, long sq_h, long sq_t, const uint8_t* kc,
                            const uint8_t* vc, const uint8_t* ks, const uint8_t* vs, uint16_t* o, long so_b, long so_t,
                            int B, int H, int G, int Tq, int D, int ctx, const int* len, long len_s, int base, int qpos,

@@ -617,6 +617,31 @@ hipError_t launch_rows(hipStream_t st, const uint16_t* x, long ldx, const uint8_
   return go(mx4_rows_kernel<8, MT, PRE, XR, XV, false, 2>, 8);
 }
 
+// Which kernel, by the grid it makes (us on one MI355X; N x K after the rows):
+//  * the few-row kernel up to 32 rows, and beyond while its grid (16 columns x 64 rows each) is at most two workgroups per
+//    CU: a CU fetches about 20 bytes a clock, so the product of few rows goes as fast as its weights are spread. Against
+//    tiles, weights from HBM: 2048 x 8192, 64 rows 8.8 / 17.4, 256 rows 14.3 / 17.2, 384 rows 19.8 / 17.5; 2048 x 2048, 256
+//    rows 5.3 / 6.7, 384 rows 7.6 / 6.9; 64 rows, 8192 x 2048 6.5 / 7.6, 14336 x 2048 10.6 / 8.2;
+//  * the smallest tile whose grid is at most one workgroup per CU, for the same reason (64 x 64, 64 x 128, 128 x 128,
+//    128 x 256): 512 rows, 2048 x 2048 7.9 / 9.4 / 10.4 / 14.6; 256 rows, 8192 x 2048 10.5 / 10.0 / 10.8 / 14.7;
+//  * 128 x 128 below two full rounds of 128 x 256: 4096 rows, 4304 x 1152 30.2 / 26.6 / 22.6 / 25.7;
+//  * 128 x 256 beyond, for its fewer LDS reads per product: 9477 rows, 8192 x 2048 182 / 142 / 110 / 105; 8192^3 492 /
+//    380 / 306 / 265;
+//  * K up to 256: the few-row kernel (the tiles' loads run at most one tile ahead, so they need more steps than the ring has),
+//    up to 512 a ring of two steps.
+enum Mx4Kernel { ROWS16, ROWS32, ROWS64, SHORT128X128, RING64X64, RING64X128, RING128X128, RING128X256 };
+Mx4Kernel mx4_kernel(int M, int N, int K) {
+  const auto tiles = [&](int bm, int bn) { return ((long)M + bm - 1) / bm * (((long)N + bn - 1) / bn); };
+  const int nk = mx4_nk(K);
+  if (M <= 16) return ROWS16;
+  if (M <= 32) return ROWS32;
+  if (tiles(64, 16) <= 512 || nk <= 2) return ROWS64;
+  if (nk <= 4) return SHORT128X128;
+  if (tiles(64, 64) <= 256) return RING64X64;
+  if (tiles(64, 128) <= 256) return RING64X128;
+  return tiles(128, 256) < 1024 ? RING128X128 : RING128X256;
+}
+
 }  // namespace
 
 // Rows that mx_gemv_mxfp4 takes.
@@ -673,36 +698,31 @@ extern "C" int mx_gemm_mxfp4(hipStream_t st, const uint8_t* xc, const uint8_t* x
   if (((uintptr_t)xc & 15) || ((uintptr_t)xs & 3)) return MX_ELAYOUT;
   const Mx4Epi p = epi(bias, R, ldr, r_rows, C, ldc, M, N, act_from);
   hipError_t e;
-  // Which kernel, by the grid it makes (us on one MI355X; N x K after the rows):
-  //  * the few-row kernel up to 32 rows, and beyond while its grid (16 columns x 64 rows each) is at most two workgroups per
-  //    CU: a CU fetches about 20 bytes a clock, so the product of few rows goes as fast as its weights are spread. Against
-  //    tiles, weights from HBM: 2048 x 8192, 64 rows 8.8 / 17.4, 256 rows 14.3 / 17.2, 384 rows 19.8 / 17.5; 2048 x 2048, 256
-  //    rows 5.3 / 6.7, 384 rows 7.6 / 6.9; 64 rows, 8192 x 2048 6.5 / 7.6, 14336 x 2048 10.6 / 8.2;
-  //  * the smallest tile whose grid is at most one workgroup per CU, for the same reason (64 x 64, 64 x 128, 128 x 128,
-  //    128 x 256): 512 rows, 2048 x 2048 7.9 / 9.4 / 10.4 / 14.6; 256 rows, 8192 x 2048 10.5 / 10.0 / 10.8 / 14.7;
-  //  * 128 x 128 below two full rounds of 128 x 256: 4096 rows, 4304 x 1152 30.2 / 26.6 / 22.6 / 25.7;
-  //  * 128 x 256 beyond, for its fewer LDS reads per product: 9477 rows, 8192 x 2048 182 / 142 / 110 / 105; 8192^3 492 /
-  //    380 / 306 / 265.
-  const auto tiles = [&](int bm, int bn) { return ((long)M + bm - 1) / bm * (((long)N + bn - 1) / bn); };
-  const int nk = mx4_nk(K);
-  if (tiles(64, 64) > 0x3fffffffL || nk > (1 << 15)) return MX_ESHAPE;
-  if (M <= 16) {
-    e = launch_rows<1, true, 1, true>(st, nullptr, 0, xc, xs, wc, ws, K, act, p);
-  } else if (M <= 32) {
-    e = launch_rows<2, true, 1, true>(st, nullptr, 0, xc, xs, wc, ws, K, act, p);
-  } else if (tiles(64, 16) <= 512 || nk <= 2) {
-    if (M > 64 * 65535) return MX_ESHAPE;  // (nk <= 2: the tiles' loads run at most one tile ahead, so they need more steps)
-    e = launch_rows<4, true, 1, true>(st, nullptr, 0, xc, xs, wc, ws, K, act, p);
-  } else if (nk <= 4) {
-    e = launch_ring<2, 2, 2, 8>(st, xc, xs, wc, ws, K, act, p);
-  } else if (tiles(64, 64) <= 256) {
-    e = launch_ring<1, 1, 4, 8>(st, xc, xs, wc, ws, K, act, p);
-  } else if (tiles(64, 128) <= 256) {
-    e = launch_ring<2, 1, 4, 8>(st, xc, xs, wc, ws, K, act, p);
-  } else if (tiles(128, 256) < 1024) {
-    e = launch_ring<2, 2, 4, 8>(st, xc, xs, wc, ws, K, act, p);
-  } else {
-    e = launch_ring<4, 2, 3, 8>(st, xc, xs, wc, ws, K, act, p);
+  if (((long)M + 63) / 64 * (((long)N + 63) / 64) > 0x3fffffffL || mx4_nk(K) > (1 << 15)) return MX_ESHAPE;
+  switch (mx4_kernel(M, N, K)) {
+    case ROWS16: e = launch_rows<1, true, 1, true>(st, nullptr, 0, xc, xs, wc, ws, K, act, p); break;
+    case ROWS32: e = launch_rows<2, true, 1, true>(st, nullptr, 0, xc, xs, wc, ws, K, act, p); break;
+    case ROWS64:
+      if (M > 64 * 65535) return MX_ESHAPE;
+      e = launch_rows<4, true, 1, true>(st, nullptr, 0, xc, xs, wc, ws, K, act, p);
+      break;
+    case SHORT128X128: e = launch_ring<2, 2, 2, 8>(st, xc, xs, wc, ws, K, act, p); break;
+    case RING64X64: e = launch_ring<1, 1, 4, 8>(st, xc, xs, wc, ws, K, act, p); break;
+    case RING64X128: e = launch_ring<2, 1, 4, 8>(st, xc, xs, wc, ws, K, act, p); break;
+    case RING128X128: e = launch_ring<2, 2, 4, 8>(st, xc, xs, wc, ws, K, act, p); break;
+    default: e = launch_ring<4, 2, 3, 8>(st, xc, xs, wc, ws, K, act, p);
   }
   return e == hipSuccess ? MX_OK : MX_ELAUNCH;
+}
+
+// The kernel that mx_gemm_mxfp4 takes: t = rows and columns of C per workgroup, steps in the LDS ring (0: the few-row kernel),
+// waves per workgroup.
+extern "C" void mx_gemm_mxfp4_tiling(int M, int N, int K, int* t) {
+  static constexpr int shape[8][3] = {{16, 16, 0}, {32, 16, 0}, {64, 16, 0}, {128, 128, 2}, {64, 64, 4}, {64, 128, 4},
+                                      {128, 128, 4}, {128, 256, 3}};
+  std::fill(t, t + 4, 0);
+  if (M < 1 || N < 1 || K < 1) return;
+  const int k = mx4_kernel(M, N, K);
+  std::copy(shape[k], shape[k] + 3, t);
+  t[3] = k <= ROWS64 && mx4_nk(K) > 16 ? 8 : 4;
 }

@@ -890,6 +890,14 @@ class MxFp4Lin:
         return y if out is not None or x.dim() == 2 else y.view(*x.shape[:-1], N)
 
 
+def mxfp4_tiling(M, N, K):
+    """(rows, columns per workgroup, ring steps (0: the few-row kernel), waves) of the product of M quantised rows."""
+    import ctypes
+    t = (ctypes.c_int * 4)()
+    _lib.load().mx_gemm_mxfp4_tiling(M, N, K, ctypes.cast(t, ctypes.c_void_p))
+    return tuple(t)
+
+
 def _where(v, B, dev, name):
     """(pointer, stride, value) of a position or length: an int, or an int32 tensor of B values."""
     if isinstance(v, torch.Tensor):
@@ -1064,6 +1072,15 @@ def sdpa_kv8(q, cache, kv_len, base=0, out=None, scale=None, qpos0=None, causal_
     _call_on(dev, "mx_kv8_sdpa", q.data_ptr(), s[0], s[1], s[2], *cache.ptrs, out.data_ptr(), so[0], so[1],
              B, cache.heads, G, Tq, D, cache.ctx, lp, ls, base, q0, int(qpos0 is None), cf, sc, ptr(part), need)
     return out
+
+
+def sdpa_kv8_tiling(B, heads, G, Tq, ctx, hd):
+    """(rows per workgroup (16: the few-row kernel), waves that share the keys, runs of keys, blocks per run) of sdpa_kv8 for B
+    sequences, G query heads per key head, in a cache of ctx positions."""
+    import ctypes
+    t = (ctypes.c_int * 4)()
+    _lib.load().mx_kv8_sdpa_tiling(B, heads, G, Tq, ctx, hd, ctypes.cast(t, ctypes.c_void_p))
+    return tuple(t)
 
 
 def gemm_tile(cfg):

@@ -3,6 +3,7 @@ attention within a bound derived from its roundings."""
 import pytest
 import torch
 
+import lowbit_cases as lc
 import oracle.lowbit as ol
 import strix_halo_maxx_amd.ops as ops
 from strix_halo_maxx_amd import _lib
@@ -178,8 +179,8 @@ SDPA = [((1,), 1, 1, 64, 1, None), ((0, 1, 63, 64, 65), 2, 1, 64, 1, None), ((13
         ((1000,), 32, 1, 64, 1, 0), ((2100, 17), 2, 8, 128, 1, None), ((70, 3), 1, 32, 64, 1, None),
         ((40, 200), 3, 3, 64, 5, 0), ((33, 90, 0), 2, 1, 64, 40, 0), ((300, 64), 2, 4, 128, 37, 50),
         ((150,), 2, 2, 64, 150, 100), ((128, 129), 1, 7, 128, 129, 0), ((4500,), 1, 2, 64, 3, 0)]
-# one for each way a prompt is cut: heads x rows of two workgroups per CU, of one, 64-row groups, 32-row groups, runs of keys
-# with 64 and 128 rows, each head dim
+# ways a prompt is cut: heads x rows of two workgroups per CU, of one, 64-row groups, 32-row groups, runs of keys with 64 and 128
+# rows; a case for each kernel: lowbit_cases.py
 CUTS = [((200,), 64, 8, 64, 130, 0), ((200,), 32, 8, 128, 130, 60), ((130,), 32, 7, 64, 120, 0), ((150,), 24, 8, 128, 128, None),
         ((200, 190), 48, 1, 64, 130, 0), ((300,), 32, 4, 128, 100, 0), ((500, 13), 8, 1, 64, 70, 0), ((700,), 4, 4, 128, 30, 0),
         ((17000,), 1, 1, 64, 50, 0), ((16700,), 1, 4, 128, 16, None), ((16500,), 1, 4, 64, 40, 100), ((16900,), 1, 8, 128, 12, 0)]
@@ -494,3 +495,82 @@ def test_sdpa_onto_its_own_queries(dev, B, H, G, D, Tq):
             buf = mem.clone()
             out = buf[off:n + off].view(B, Tq, H * G * D)
             assert ops.sdpa_kv8(buf[:n].view(q.shape), c, 300, causal_from=0, out=out) is out and torch.equal(out, want), off
+
+
+def exact_heads(q, k, v, n, cf, D):
+    """Each (sequence, head) of q (B, H, G, Tq, D) over k, v (B, H, ctx, D) in 64 bits on the GPU: the output (G, Tq, D), the mean
+    |v| under the weights, the root of the sum of squared weights times values, the largest sum |q k| scale of a row."""
+    B, H, G, Tq, _ = q.shape
+    for b in range(B):
+        j, i = torch.arange(n[b], device=q.device)[None], torch.arange(Tq, device=q.device)[:, None]
+        seen = (j < n[b]).expand(Tq, -1) if cf is None else (j < cf) | (j <= n[b] - Tq + i)
+        for h in range(H):
+            kk, vv, qq = k[b, h, :n[b]].double(), v[b, h, :n[b]].double(), q[b, h].double().reshape(G * Tq, D)
+            s = torch.matmul(qq, kk.t().contiguous()).view(G, Tq, -1) * D ** -0.5
+            size = torch.matmul(qq.abs(), kk.t().abs().contiguous()).view(G, Tq, -1) * D ** -0.5
+            p = torch.nan_to_num(torch.softmax(s.masked_fill(~seen, -float("inf")), -1)).view(G * Tq, -1)
+            back = lambda x: x.view(G, Tq, D)
+            yield (b, h, back(torch.matmul(p, vv)), back(torch.matmul(p, vv.abs())),
+                   back(torch.matmul(p * p, vv * vv)).sqrt(), size.amax(-1, keepdim=True) if n[b] else size.new_zeros(G, Tq, 1))
+
+
+@pytest.mark.parametrize("lens,H,G,D,Tq,cf,ctx", lc.ATTENTION)
+def test_sdpa_every_kernel(dev, lens, H, G, D, Tq, cf, ctx):
+    """check_sdpa's bound on each value, and one on the whole in norm that lost bits would not pass (test_lowbit_host.py plants
+    them): the output's rounding and the MFMA's sums, 2^-8 and 2^-14 of it; the weights' errors, 2^-9 each from their terms and
+    2^-15 of the largest |q k| sum from their scores (the MFMA's 2^-16, twice), independent of one another, so that they add
+    up in squares (spread), taken twice."""
+    g = torch.Generator(device=dev).manual_seed(sum(lens) + H + Tq + D)
+    r = lambda *s: torch.randn(*s, generator=g, device=dev).to(BF)
+    B, n = len(lens), max(lens)
+    c = ops.KV8Cache(B, H, ctx or n, D, device=dev)
+    c.append(r(B, H, n, D), r(B, H, n, D) * 3, 0, count=i32(dev, *lens))
+    q = r(B, H * G, Tq, D)
+    print("kernel", lens, H, G, D, Tq, cf, ctx, ops.sdpa_kv8_tiling(B, H, G, Tq, c.ctx, D), flush=True)
+    y = ops.sdpa_kv8(q, c, i32(dev, *lens), causal_from=cf).view(B, Tq, H, G, D)
+    k, v = c.read(n)
+    err2 = ref2 = spread2 = 0.0
+    for b, h, ref, avg, spread, size in exact_heads(q.view(B, H, G, Tq, D), k, v, lens, cf, D):
+        err = (y[b, :, h].double().transpose(0, 1) - ref).abs()
+        worst = (err - 2.0 ** -8 * ref.abs() - (2.0 ** -8 + 2.0 ** -12 + 2 * 2.0 ** -12 * (1 + size)) * avg).max().item()
+        assert worst <= 0, (b, h, worst)
+        err2 += err.square().sum()
+        ref2 += ref.square().sum()
+        spread2 += ((2.0 ** -9 + 2.0 ** -15 * (1 + size)) * spread).square().sum()
+    bound = (2.0 ** -8 + 2.0 ** -14) * float(ref2) ** 0.5 + 2 * float(spread2) ** 0.5
+    print("norm", float(err2) ** 0.5, "bound", bound, "output", float(ref2) ** 0.5, flush=True)
+    assert float(err2) ** 0.5 <= bound
+
+
+@pytest.mark.parametrize("H,G,D,Tq", lc.MASKED)
+def test_sdpa_masked_nan_changes_no_bit(dev, H, G, D, Tq):
+    """On every kernel: keys and values of NaN behind the sequence, and behind each query, leave its bits as zeros there do (they
+    do not count for a block's exponent either); queries that see one are NaN."""
+    g = torch.Generator(device=dev).manual_seed(H + D + Tq)
+    r = lambda *s: torch.randn(*s, generator=g, device=dev).to(BF)
+    n, ctx, at = 150, 200, 141
+    k, v, q = r(1, H, ctx, D), r(1, H, ctx, D), r(1, H * G, Tq, D)
+
+    def out(fill, *rows, which="kv"):
+        kk, vv = k.clone(), v.clone()
+        for t in rows:
+            if "k" in which:
+                kk[:, :, t] = fill
+            if "v" in which:
+                vv[:, :, t] = fill
+        c = ops.KV8Cache(1, H, ctx, D, device=dev)
+        c.append(kk, vv, 0)
+        return ops.sdpa_kv8(q, c, n, causal_from=0).view(Tq, -1)
+
+    print("masked", H, G, D, Tq, ops.sdpa_kv8_tiling(1, H, G, Tq, ctx, D), flush=True)
+    clean = out(0, *range(n, ctx))
+    assert bool(clean.isfinite().all())
+    for fill in (float("nan"), float("inf")):
+        assert torch.equal(out(fill, *range(n, ctx)), clean)
+    sees = torch.arange(Tq, device=dev) + n - Tq >= at
+    assert bool(sees.any()) and not bool(sees.all())
+    zero = out(0, at, *range(n, ctx))
+    for which in ("k", "v", "kv"):
+        y, z = out(float("nan"), at, *range(n, ctx), which=which), out(0, at, *range(n, ctx), which=which)
+        assert bool(y[sees].isnan().all()) and torch.equal(y[~sees], z[~sees]), which
+    assert torch.equal(zero[~sees], z[~sees])

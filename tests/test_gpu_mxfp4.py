@@ -3,6 +3,7 @@ the rounding of the code is exact), the Linear within its one bf16 rounding plus
 import pytest
 import torch
 
+import lowbit_cases as lc
 import oracle.lowbit as ol
 import strix_halo_maxx_amd.ops as ops
 
@@ -77,7 +78,8 @@ def close(y, ref, mag, act=None):
 SHAPES = [(1, 1, 1), (1, 8192, 2048), (1, 2048, 8192), (2, 100, 4304), (7, 37, 100), (16, 64, 129), (17, 768, 768),
           (33, 130, 1000), (64, 260, 512), (65, 129, 640), (128, 128, 128), (130, 259, 1152), (300, 1000, 385),
           (520, 516, 2304)]
-# more tiles than workgroups, in every remainder of the four steps that share a scale register, ragged and whole edges
+# more workgroups than fit at once, or more tiles than workgroups (128 x 128), K whole and just past a step, ragged edges; which
+# shape takes which kernel: lowbit_cases.py
 LARGE = [(2100, 4304, 128), (1800, 5000, 257), (2600, 3333, 384), (1500, 6144, 513), (2049, 4100, 1152)]
 
 
@@ -299,3 +301,39 @@ def test_residual_that_overlaps_the_output(dev, M, N, K):
     want = lin(x, res=at(buf0, M, ld).clone())
     lin(x, res=at(buf, M, ld), out=at(buf, M, ld))
     assert torch.equal(at(buf, M, ld), want)
+
+
+def product(x, w):
+    """The product of the quantised values in 64 bits, and that of their sizes (x, w on the GPU)."""
+    xq, wt = ops.quant_mxfp4(x).values().double(), ops.quant_mxfp4(w).values().double().t().contiguous()
+    return torch.matmul(xq, wt), torch.matmul(xq.abs(), wt.abs())
+
+
+@pytest.mark.parametrize("M,N,K", lc.ROWS + lc.TILES + lc.FEW)
+def test_every_kernel_against_64_bits(dev, M, N, K):
+    """Each kernel that the product takes, with what its write-out can do: bias, both activations from the first column or a later
+    one, a residual of as many rows, of fewer, and one row for all, an output inside a larger buffer (16-byte aligned, and not)."""
+    g = torch.Generator(device=dev).manual_seed(M + 3 * N + 7 * K)
+    r = lambda *s: torch.randn(*s, generator=g, device=dev)
+    x, w, b, res = r(M, K).to(BF), (r(N, K) * 0.05).to(BF), r(N).to(BF), r(M, N).to(BF)
+    x[M // 2] *= 50
+    w[N // 3] *= 7
+    lin, plain = ops.MxFp4Lin(w, b, device=dev), ops.MxFp4Lin(w, None, device=dev)
+    print(f"mxfp4 kernel {M} x {N} x {K}", flush=True)
+    y0, mag = product(x, w)
+    yb, magb = y0 + b.double(), mag + b.double().abs()
+    close(plain(x), y0, mag)
+    for act, f in (("tanh", 0), ("erf", N // 2 + 1), ("erf", 0), ("tanh", 8)):
+        ref = torch.cat([yb[:, :f], ol.gelu(yb[:, f:], act)], 1)
+        close(lin(x, act=act, act_from=f), ref, magb, act=act)
+        close(lin(x, act=act, act_from=f, res=res), ref + res.double(), magb, act=act)
+    close(lin(x, res=res[:1].expand(M, N)), yb + res[:1].double(), magb)
+    if M % 2 == 0:
+        close(lin(x, res=res[:M // 2]), yb + res[:M // 2].double().repeat(2, 1), magb)
+    buf = torch.full((M + 1, N + 24), 3.0, device=dev, dtype=BF)
+    for c0 in (8, 5):
+        out = buf[:-1, c0:c0 + N]
+        lin(x, res=res, out=out)
+        close(out, yb + res.double(), magb)
+        out.fill_(3.0)
+        assert bool((buf == 3.0).all())

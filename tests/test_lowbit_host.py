@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+import lowbit_cases as lc
 import oracle.lowbit as ol
 import strix_halo_maxx_amd.ops as ops
 from strix_halo_maxx_amd import _lib
@@ -230,3 +231,66 @@ def test_strides_of_size_one_are_not_looked_at():
            out=torch.zeros(400, dtype=BF).as_strided((1, 2, 128), (1, 129, 1)))
     w = ops.MxFp4(torch.zeros(4352, dtype=torch.uint8), 10, 1)
     raises("GPU", w.values, out=torch.zeros(1, 10, dtype=BF).t())
+
+
+def test_every_mxfp4_kernel_has_its_cases():
+    """The kernels that mx_gemm_mxfp4 takes over a sweep of shapes, tiles with and without 16-byte stores, against those that the
+    GPU tests check values of; and the forms of the launch that quantises its rows."""
+    sizes = sorted({s * m // 8 for s in (16, 64, 256, 1024, 4096, 16384) for m in range(4, 17)})
+    swept = {ops.mxfp4_tiling(m, n, k) for m in sizes for n in sizes for k in (64, 256, 257, 512, 513, 2048, 2049, 8192)}
+    assert len(swept) == 11
+    assert {ops.mxfp4_tiling(*s) for s in lc.ROWS} == {t for t in swept if not t[2]}
+    got = {(ops.mxfp4_tiling(*s), s[1] % 8 == 0) for s in lc.TILES}
+    assert got == {(t, v) for t in swept if t[2] for v in (True, False)}
+    form = lambda m, k: (8 if k % 8 or m > 4 else 1 if m == 1 else 4, k % 8 == 0, k > 2048)
+    assert {form(m, k) for m, n, k in lc.FEW} == {form(m, k) for m in range(1, 9) for k in (8, 9, 2048, 2049, 2056)}
+    assert all(m <= _lib.load().mx_gemv_mxfp4_rows() for m, n, k in lc.FEW)
+    assert ops.mxfp4_tiling(0, 5, 5) == ops.mxfp4_tiling(5, -1, 5) == (0, 0, 0, 0)
+
+
+def attention_kernel(B, H, G, Tq, ctx, D):
+    rows, waves, runs, chunk = ops.sdpa_kv8_tiling(B, H, G, Tq, ctx, D)
+    return D, rows, waves, runs > 1
+
+
+def test_every_attention_kernel_has_its_cases():
+    """The same for sdpa_kv8: each kernel with and without a join, each that reloads scales, each over masked NaN."""
+    swept = {attention_kernel(B, H, 1, Tq, ctx, D) for B in (1, 4, 32) for H in (1, 3, 8, 32, 64, 100, 200, 600)
+             for Tq in (1, 16, 17, 33, 60, 70, 129, 300, 1000, 4000) for ctx in (1, 500, 1600, 4000, 16000, 17000, 200000)
+             for D in (64, 128)}
+    assert len(swept) == 22
+    full = lambda c: (len(c[0]), c[1], c[2], c[4], c[6] or max(c[0]), c[3])
+    assert {attention_kernel(*full(c)) for c in lc.ATTENTION} == swept
+    long_runs = {attention_kernel(*full(c))[:3] for c in lc.ATTENTION if ops.sdpa_kv8_tiling(*full(c))[3] > 64}
+    assert long_runs >= {k[:3] for k in swept if k[1] > 16}
+    assert {attention_kernel(1, H, G, Tq, 200, D)[:3] for H, G, D, Tq in lc.MASKED} == {k[:3] for k in swept}
+    assert ops.sdpa_kv8_tiling(0, 1, 1, 1, 64, 64) == ops.sdpa_kv8_tiling(1, 1, 1, 1, 64, 72) == (0, 0, 0, 0)
+
+
+def test_norm_bound_tells_lost_bits():
+    """The bound in norm that the attention's GPU tests use, on the formula with its roundings planted: two e4m3 terms per weight
+    pass with room; a weight or a query without its low term does not."""
+    g = torch.Generator().manual_seed(0)
+    n, D, T = 1000, 64, 24
+    q, k, v = (torch.randn(s, D, generator=g).to(BF).double() for s in (T, n, n))
+    v = 3 * v
+    e4m3 = lambda x: ol.nearest(x, ol.E4M3)
+
+    def terms(x, low):  # relative to a power of two just above the row's largest, as e4m3 terms of up to 256
+        unit = torch.exp2(torch.ceil(torch.log2(x.abs().amax(-1, keepdim=True)))) / 256
+        hi = e4m3(x / unit)
+        return unit * (hi + (e4m3((x / unit - hi) * 16) / 16 if low else 0))
+
+    def attend(q, p_terms):
+        w = torch.exp(q @ k.t() * D ** -0.5 - 8)
+        return (p_terms(w) @ v) / w.sum(-1, keepdim=True), w / w.sum(-1, keepdim=True)
+
+    ref, p = attend(q, lambda w: w)
+    size = (q.abs() @ k.t().abs()).amax(-1, keepdim=True) * D ** -0.5
+    spread = ((p * p) @ (v * v)).sqrt()
+    bound = (2.0 ** -8 + 2.0 ** -14) * ref.norm() + 2 * ((2.0 ** -9 + 2.0 ** -15 * (1 + size)) * spread).norm()
+    off = lambda y: float((y.to(BF).double() - ref).norm() / bound)
+    assert torch.equal(terms(q, True), q)  # two terms hold a bf16
+    assert off(attend(q, lambda w: terms(w, True))[0]) < 0.5
+    assert off(attend(q, lambda w: terms(w, False))[0]) > 2
+    assert off(attend(terms(q, False), lambda w: terms(w, True))[0]) > 2
