@@ -594,11 +594,31 @@ def cpu_baseline_trecvit(frames=8):
                       f"tokens with 8 threads on its own CPU"}
 
 
-def decode_bench(steps_tokens=128, w8a8=False):
+# Forms of the text decoder in fewer bits, for --decode
+DECODE_FORMS = {"bf16": {}, "w8a8": dict(w8a8=True), "mxfp4": dict(mxfp4=True), "kv8": dict(kv8=True),
+                "mxfp4+kv8": dict(mxfp4=True, kv8=True), "w8a8+kv8": dict(w8a8=True, kv8=True)}
+
+
+def operator_case(name, passes=25):
+    """A listed case of perf/operators.py on the framework's kernels: set up, then `passes` passes one by one, for a kernel trace
+    or counters of its launches."""
+    import torch
+    import perf.operators as po
+    po.own = True
+    state = po.prepare(next(c for c in po.listed() if c["name"] == name), 1)
+    torch.cuda.synchronize()
+    for _ in range(passes):
+        po.run(state)
+        torch.cuda.synchronize()
+    print(f"{name}: {passes} passes", flush=True)
+
+
+def decode_bench(steps_tokens=128, w8a8=False, mxfp4=False, kv8=False):
     """Config 2: prefill (1 + 729 image tokens mask-free, then 64 prompt ids) + greedy decode on one HIP graph per
     step. Returns prefill ms, decode tok/s and the decode step's HBM roofline (algorithmic bytes = every weight once
     + the KV cache read per token). w8a8: the reference's default W8A8 text linears (int8 weights and activations;
-    the LM head stays bf16), reported beside the bf16 figures, never as them."""
+    the LM head stays bf16), reported beside the bf16 figures, never as them. mxfp4, kv8: the Linears in MXFP4 and the cache
+    in 8 bits, by --decode only."""
     import torch
     import strix_halo_maxx_amd.md2text as mt
     import strix_halo_maxx_amd.synth as S
@@ -606,7 +626,7 @@ def decode_bench(steps_tokens=128, w8a8=False):
     w = S.text_weights(0)
     # yes / no ids: 4 + 4 fixed ids (no tokenizer here); nq = 1 question of up to L = 32 ids (the reference's
     # FastMD2 defaults, md2fast.py:69)
-    dec = mt.TextDecoder(w, device=dev, ctx=1024, w8a8=w8a8, yes_ids=(11, 222, 3333, 44444),
+    dec = mt.TextDecoder(w, device=dev, ctx=1024, w8a8=w8a8, mxfp4=mxfp4, kv8=kv8, yes_ids=(11, 222, 3333, 44444),
                          no_ids=(55, 666, 7777, 50000))
     del w
     img = S.activations(3, (729, 2048), "img").to(dev)
@@ -664,9 +684,9 @@ def decode_bench(steps_tokens=128, w8a8=False):
     c = S.TXT
     D, F, L, V = c["dim"], c["ff"], c["layers"], c["vocab"]
     lin = L * (3 * D * D + D * D + 2 * D * F)  # text Linear weights: bf16, or int8 + fp32 per-row scales (W8A8)
-    wbytes = (lin + 4 * L * (3 * D + D + F + D) if w8a8 else 2 * lin) + 2 * V * D
+    wbytes = (lin + 4 * L * (3 * D + D + F + D) if w8a8 else lin * 17 // 32 if mxfp4 else 2 * lin) + 2 * V * D
     ctx_mid = dec.pos_base + steps_tokens // 2
-    kvbytes = 2 * 2 * L * ctx_mid * D
+    kvbytes = (1 if kv8 else 2) * 2 * L * ctx_mid * D
     bpt = wbytes + kvbytes
     traffic = {}
     mt_ = measured_decode_traffic() if dec.use_mk and not w8a8 else None
@@ -685,7 +705,9 @@ def decode_bench(steps_tokens=128, w8a8=False):
             "workload": "moondream2 text decoder, 24 layers, prefill 730 + 64 tokens (one HIP graph; eager beside it), "
                         f"greedy {steps_tokens} tokens, batch 1, one HIP graph per decode step; query_ms: one 32-id "
                         "yes/no query over the 730-token prefix (graph)"
-                        + (", W8A8 text Linears (int8 weights / activations, bf16 LM head)" if w8a8 else "")}
+                        + (", W8A8 text Linears (int8 weights / activations, bf16 LM head)" if w8a8 else "")
+                        + (", MXFP4 text Linears (weights / activations, bf16 LM head)" if mxfp4 else "")
+                        + (", 8-bit KV cache" if kv8 else "")}
 
 
 def frame_bench(reps=20):
@@ -1117,6 +1139,8 @@ def main():
     ap.add_argument("--warmup", type=int, default=5)
     ap.add_argument("--no-cpu", action="store_true")
     ap.add_argument("--no-extra", action="store_true", help="headline tower only (no batch 13 / 256, decoder, TRecViT)")
+    ap.add_argument("--decode", choices=DECODE_FORMS, help="only the text decoder (prefill, query, decode) in this form")
+    ap.add_argument("--case", help="only passes through one listed case of perf/operators.py, for a profiler")
     ap.add_argument("--traffic-probe", action="store_true",
                     help="only the eager launches that rocprofv3 --pmc FETCH_SIZE / WRITE_SIZE runs count (see traffic_probe)")
     ap.add_argument("--traffic-probe-decode", action="store_true",
@@ -1142,6 +1166,14 @@ def main():
         import torch
         with torch.inference_mode():
             probe(a.probe)
+        return
+    if a.decode or a.case:
+        import torch
+        with torch.inference_mode():
+            if a.case:
+                operator_case(a.case)
+            else:
+                print(json.dumps(decode_bench(**DECODE_FORMS[a.decode])))
         return
     if a.summarize_counters:
         print(summarize_counters(a.summarize_counters))
