@@ -307,8 +307,8 @@ extern "C" int mx_kv8_read(hipStream_t st, const uint8_t* kc, const uint8_t* vc,
   if (D != 64 && D != 128) return MX_EBADCFG;
   if (nslots < 1 || H < 1 || n < 1 || n > ctx || ctx > 0x7fffff00) return MX_ESHAPE;
   if (((uintptr_t)kc | (uintptr_t)vc | (uintptr_t)k | (uintptr_t)v) & 15) return MX_ELAYOUT;
-  const long wgs = (long)kv8_blocks(n) * nslots * H;
-  if (wgs > 0xffffffL) return MX_ESHAPE;
+  const long heads = (long)nslots * H, wgs = kv8_blocks(n) * heads;
+  if (heads > 0xffffffL || wgs > 0xffffffL) return MX_ESHAPE;
   if (D == 64)
     hipLaunchKernelGGL(kv8_read_kernel<64>, dim3((unsigned)wgs), dim3(256), 0, st, kc, vc, ks, vs, k, v, n, ctx);
   else

@@ -762,8 +762,14 @@ hipError_t launch(hipStream_t st, Attn8Args a, const Plan& q) {
 
 }  // namespace
 
+// Sizes that plan() can take: heads that a grid holds, and counts that stay in their types.
+static bool sizes_ok(int B, int H, int G, int Tq, int ctx) {
+  return B >= 1 && H >= 1 && G >= 1 && Tq >= 1 && ctx >= 1 && ctx <= 0x7fffff00 && (long)Tq * G <= 0x7fffff00L &&
+         (long)B * H <= 0x7fffffL;
+}
+
 extern "C" long mx_kv8_sdpa_ws(int B, int H, int G, int Tq, int ctx, int D) {
-  if (B < 1 || H < 1 || G < 1 || Tq < 1 || ctx < 1 || (D != 64 && D != 128)) return 0;
+  if (!sizes_ok(B, H, G, Tq, ctx) || (D != 64 && D != 128)) return 0;
   const Plan q = plan(B, H, G, Tq, ctx, D);
   return q.splits == 1 ? 0 : (long)B * H * q.nrt * q.splits * q.rw * (D + 2);
 }
@@ -772,7 +778,7 @@ extern "C" long mx_kv8_sdpa_ws(int B, int H, int G, int Tq, int ctx, int D) {
 // of 64 keys per run.
 extern "C" void mx_kv8_sdpa_tiling(int B, int H, int G, int Tq, int ctx, int D, int* t) {
   t[0] = t[1] = t[2] = t[3] = 0;
-  if (B < 1 || H < 1 || G < 1 || Tq < 1 || ctx < 1 || (D != 64 && D != 128)) return;
+  if (!sizes_ok(B, H, G, Tq, ctx) || (D != 64 && D != 128)) return;
   const Plan q = plan(B, H, G, Tq, ctx, D);
   t[0] = q.rw, t[1] = q.nkw, t[2] = q.splits, t[3] = q.chunk;
 }
@@ -783,7 +789,7 @@ extern "C" int mx_kv8_sdpa(hipStream_t st, const uint16_t* q, long sq_b, long sq
                            int qend, int causal_from, float scale, float* part, long part_elems) {
   if (!q || !kc || !vc || !ks || !vs || !o) return MX_ENULL;
   if (D != 64 && D != 128) return MX_EBADCFG;
-  if (B < 1 || H < 1 || G < 1 || Tq < 1 || ctx < 1 || ctx > 0x7fffff00 || (long)Tq * G > 0x7fffff00L) return MX_ESHAPE;
+  if (!sizes_ok(B, H, G, Tq, ctx)) return MX_ESHAPE;
   if (!(scale > 0.f) || !(scale * 1.4426950408889634f < INFINITY) || causal_from < 0) return MX_ESHAPE;
   if ((sq_b | sq_h | sq_t) % 8 || (so_b | so_t) % 4) return MX_ESHAPE;
   if (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc) & 15 || ((uintptr_t)o & 7) || ((uintptr_t)len & 3)) return MX_ELAYOUT;

@@ -294,3 +294,16 @@ def test_norm_bound_tells_lost_bits():
     assert off(attend(q, lambda w: terms(w, True))[0]) < 0.5
     assert off(attend(q, lambda w: terms(w, False))[0]) > 2
     assert off(attend(terms(q, False), lambda w: terms(w, True))[0]) > 2
+
+
+def test_counts_that_wrap():
+    """Sequences times heads past any grid: refused before the products of such counts wrap (to a division by zero, or to a few
+    workgroups over memory that nobody has)."""
+    lib, big = _lib.load(), 2 ** 30
+    assert lib.mx_kv8_sdpa_ws(big, big, 1, 2048, 64, 64) == 0 and ops.sdpa_kv8_tiling(big, big, 1, 2048, 64, 64) == (0, 0, 0, 0)
+    assert lib.mx_kv8_sdpa_ws(1, 1, 2 ** 16, 2 ** 16, 64, 64) == 0
+    sd = lambda B, H, Tq: lib.mx_kv8_sdpa(None, A16, 64, 64, 64, A16, A16, A16, A16, A16, 64, 64, B, H, 1, Tq, 64, 64, None, 0, 50, 0,
+                                          1, 0, 0.125, None, 0)
+    assert sd(big, big, 2048) == -2 and sd(2 ** 23, 1, 1) == -2
+    assert lib.mx_kv8_read(None, A16, A16, A16, A16, A16, A16, 2 ** 31 - 1, 2 ** 31 - 1, 256, 64, 256) == -2
+    assert lib.mx_kv8_read(None, A16, A16, A16, A16, A16, A16, big, big, 1024, 64, 1024) == -2
