@@ -219,7 +219,13 @@ int mx_kv8_read(hipStream_t st, const uint8_t* kc, const uint8_t* vc, const uint
 /* o[b, i, h D ..] = softmax(scale q[b, h, i] K^T) V over the visible keys of slot b, key head h / G, for H G query heads:
  * j < len_b and (j < causal_from or j <= qpos + i) (qend: qpos = len_b - Tq; causal_from = INT_MAX: no mask); a row that
  * sees none is zero. scale > 0, and scale log2(e) finite. Scores (times scale) have to stay below 2^29 in size: rows with
- * larger ones come out as 0 or NaN. q rows and strides 16-byte aligned, o 8-byte; o must not meet q. part:
+ * larger ones come out as 0 or NaN.
+ * Rounding: q and the softmax weights go into the products as two e4m3 terms each (8 bits; values of q below 2^-21 of their
+ * row's largest, and weights below 2^-21 of the largest of their 64 keys, are dropped), the fp8 MFMA adds up to about 2^-16
+ * of a sum, the sums of the weights are fp32. On normal data the output is as close to the formula as its rounding to
+ * bf16 allows, within a tenth.
+ * Grid and workspace are cut by ctx, not by the lengths: a cache much longer than its sequences costs one token up to 2.5
+ * times (16000 keys, 8 x 4 heads of 128: 11 us with ctx 16000, 28 with 262144). q rows and strides 16-byte aligned, o 8-byte; o must not meet q. part:
  * mx_kv8_sdpa_ws() floats, 16-byte aligned, free again once the call's kernels have run (null where that is 0). */
 long mx_kv8_sdpa_ws(int B, int H, int G, int Tq, int ctx, int D);
 /* How mx_kv8_sdpa cuts a call, for reading profiles: t[4] = rows per workgroup (16: the few-row kernel), waves that share the

@@ -391,7 +391,8 @@ __global__ __launch_bounds__(64 * NK) void kv8_rows_kernel(Attn8Args p) {
 // blocks of K and V as they lie in the cache, copied by the asynchronous LDS-DMA load a stage or more ahead; key wave u
 // takes block u of every stage, and the shares of the key waves are added at the end. The bound is the vector ALU beside
 // the MFMA: per key and row, four products of 8-bit terms, and an exponential and two roundings to e4m3. 2048 rows of a
-// 16001-key sequence, 32 heads x 128 over 8: 525 us, 0.95 PFLOP/s of the bf16 product (MFMA pipes 42 % busy, ALU 50 %).
+// 16001-key sequence, 32 heads x 128 over 8: 535 us, 0.93 PFLOP/s of the bf16 product (MFMA pipes busy in 41 % of the cycles,
+// ALU in 46 %; 600 us in a trace, at a lower clock).
 template <int D, int NQW, int NKW, int S>
 struct Tile8 {
   static constexpr int NW = NQW * NKW;
@@ -493,7 +494,7 @@ __global__ __launch_bounds__(64 * NQW * NKW, 2) void kv8_tile_kernel(Attn8Args p
     const int sk = __builtin_amdgcn_readlane(skl, rel % 64), sv = __builtin_amdgcn_readlane(svl, rel % 64);
     f32x16 st[2];
     // a wave in its products goes first: the two waves of a SIMD fall out of step, and one's softmax runs under the other's
-    // products (512 us for 527 without, 2048 rows x 16001 keys, 32 heads x 128)
+    // products (3 % of the time, 2048 rows x 16001 keys, 32 heads x 128)
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int t = 0; t < 2; t++) {
@@ -683,7 +684,8 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Attn8Args p, long nrec) {
       u32x2{pack2(a[0] * inv, a[1] * inv), pack2(a[2] * inv, a[3] * inv)};
 }
 
-// How a problem is cut: rw rows per workgroup (16: the few-row kernel), nkw key waves, nrt row groups, `splits` runs of
+// How a problem is cut, by the cache's capacity (grid and workspace have to be known on the host, the lengths may be on the
+// device; 1 x 8 x 4, 128, 1, 16000 keys take 11.2 with ctx 16000, 28.4 with 262144): rw rows per workgroup (16: the few-row kernel), nkw key waves, nrt row groups, `splits` runs of
 // `chunk` blocks. us on one MI355X (query waves x key waves; sequences x key heads x group, head dim, queries, keys):
 //  * up to 32 rows: the few-row kernel; runs of keys until there are 3 workgroups per CU (a CU holds 2 or 3), of 16 blocks
 //    at least. Where those leave half of the CUs idle, runs of 8 (the join costs 3 us; caches that no other call has just

@@ -1028,7 +1028,9 @@ def sdpa_kv8(q, cache, kv_len, base=0, out=None, scale=None, qpos0=None, causal_
     key j is visible to query i iff j < len_b and (j < causal_from or j <= qpos0 + i); causal_from=None: no mask;
     qpos0=None: the queries are the last Tq tokens of their sequence, qpos0 = len_b - Tq. Rows that see no key are 0.
     out may lie in q's memory.
-    Scores (times scale) have to stay below 2^29 in size: larger ones come out as 0 or NaN."""
+    Scores (times scale) have to stay below 2^29 in size: larger ones come out as 0 or NaN.
+    q and the softmax weights are taken in 8 bits (two e4m3 terms); sums of weights are fp32. The keys are cut into runs by the
+    cache's ctx, not by the lengths: one token over a cache much longer than its sequence takes up to 2.5 times as long."""
     if q.dim() != 4 or q.shape[3] != cache.hd or q.shape[1] < 1 or q.shape[1] % cache.heads or q.shape[0] > cache.slots:
         raise ValueError(f"q {tuple(q.shape)} does not fit a cache of {cache.slots} x {cache.heads} heads x {cache.hd}")
     B, Hq, Tq, D = q.shape
