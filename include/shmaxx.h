@@ -225,8 +225,9 @@ int mx_kv8_read(hipStream_t st, const uint8_t* kc, const uint8_t* vc, const uint
  * of a sum, the sums of the weights are fp32. On normal data the output is as close to the formula as its rounding to
  * bf16 allows, within a tenth.
  * Grid and workspace are cut by ctx, not by the lengths: a cache much longer than its sequences costs one token up to 2.5
- * times (16000 keys, 8 x 4 heads of 128: 11 us with ctx 16000, 28 with 262144). q rows and strides 16-byte aligned, o 8-byte; o must not meet q. part:
- * mx_kv8_sdpa_ws() floats, 16-byte aligned, free again once the call's kernels have run (null where that is 0). */
+ * times (16000 keys, 8 x 4 heads of 128: 11 us with ctx 16000, 28 with 262144).
+ * q rows and strides 16-byte aligned, o 8-byte; o must not meet q. part: mx_kv8_sdpa_ws() floats, 16-byte aligned, free again
+ * once the call's kernels have run (null where that is 0). */
 long mx_kv8_sdpa_ws(int B, int H, int G, int Tq, int ctx, int D);
 /* How mx_kv8_sdpa cuts a call, for reading profiles: t[4] = rows per workgroup (16: the few-row kernel), waves that share the
  * keys, runs of keys, blocks of 64 keys per run. */

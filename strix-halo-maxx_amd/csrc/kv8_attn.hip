@@ -685,8 +685,8 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Attn8Args p, long nrec) {
 }
 
 // How a problem is cut, by the cache's capacity (grid and workspace have to be known on the host, the lengths may be on the
-// device; 1 x 8 x 4, 128, 1, 16000 keys take 11.2 with ctx 16000, 28.4 with 262144): rw rows per workgroup (16: the few-row kernel), nkw key waves, nrt row groups, `splits` runs of
-// `chunk` blocks. us on one MI355X (query waves x key waves; sequences x key heads x group, head dim, queries, keys):
+// device; 1 x 8 x 4, 128, 1, 16000 keys take 11.2 with ctx 16000, 28.4 with 262144): rw rows per
+// workgroup (16: the few-row kernel), nkw key waves, nrt row groups, `splits` runs of `chunk` blocks. us on one MI355X (query waves x key waves; sequences x key heads x group, head dim, queries, keys):
 //  * up to 32 rows: the few-row kernel; runs of keys until there are 3 workgroups per CU (a CU holds 2 or 3), of 16 blocks
 //    at least. Where those leave half of the CUs idle, runs of 8 (the join costs 3 us; caches that no other call has just
 //    read: 1 x 8 x 4, 128, 1, 4000 11.0, runs of 16 13.0; 4 x 8 x 4, 128, 1, 2000 11.6 / 13.6), or one run up to 24 blocks (1

@@ -620,8 +620,9 @@ hipError_t launch_rows(hipStream_t st, const uint16_t* x, long ldx, const uint8_
 // Which kernel, by the grid it makes (us on one MI355X; N x K after the rows):
 //  * the few-row kernel up to 32 rows, and beyond while its grid (16 columns x 64 rows each) is at most two workgroups per
 //    CU: loads alone, on all CUs, reach 50 bytes a clock and CU from the XCD's own L2 and 11 from beyond it, so the product of
-//    few rows goes as fast as its weights are spread. Against tiles, weights from HBM: 2048 x 8192, 64 rows 8.8 / 17.4, 256 rows 14.3 / 17.2, 384 rows 19.8 / 17.5; 2048 x 2048, 256
-//    rows 5.3 / 6.7, 384 rows 7.6 / 6.9; 64 rows, 8192 x 2048 6.5 / 7.6, 14336 x 2048 10.6 / 8.2;
+//    few rows goes as fast as its weights are spread. Against tiles, weights from HBM: 2048 x 8192, 64 rows 8.8 / 17.4, 256
+//    rows 14.3 / 17.2, 384 rows 19.8 / 17.5; 2048 x 2048, 256 rows 5.3 / 6.7, 384 rows 7.6 / 6.9; 64 rows, 8192 x 2048 6.5
+//    / 7.6, 14336 x 2048 10.6 / 8.2;
 //  * the smallest tile whose grid is at most one workgroup per CU, for the same reason (64 x 64, 64 x 128, 128 x 128,
 //    128 x 256): 512 rows, 2048 x 2048 7.9 / 9.4 / 10.4 / 14.6; 256 rows, 8192 x 2048 10.5 / 10.0 / 10.8 / 14.7;
 //  * 128 x 128 below two full rounds of 128 x 256: 4096 rows, 4304 x 1152 30.2 / 26.6 / 22.6 / 25.7;
