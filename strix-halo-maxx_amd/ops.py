@@ -707,8 +707,16 @@ def _end(t):
 
 
 def _apart(a, b):
-    """Whether the memory of a, from its first element to its last, and that of b do not meet."""
-    return _end(a) <= b.data_ptr() or _end(b) <= a.data_ptr()
+    """Whether the elements of a and b (the same type, neither empty) are known not to meet: they lie one behind the other, or
+    side by side in the rows of one buffer."""
+    if _end(a) <= b.data_ptr() or _end(b) <= a.data_ptr():
+        return True
+    pitch = b.stride(-2) if b.dim() > 1 else 0
+    off, rest = divmod(b.data_ptr() - a.data_ptr(), b.element_size())
+    if pitch < 1 or rest:
+        return False
+    wide = lambda t: 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()) if s % pitch)  # columns; other steps are rows
+    return wide(a) <= off % pitch <= pitch - wide(b)
 
 
 class MxFp4:

@@ -307,3 +307,23 @@ def test_counts_that_wrap():
     assert sd(big, big, 2048) == -2 and sd(2 ** 23, 1, 1) == -2
     assert lib.mx_kv8_read(None, A16, A16, A16, A16, A16, A16, 2 ** 31 - 1, 2 ** 31 - 1, 256, 64, 256) == -2
     assert lib.mx_kv8_read(None, A16, A16, A16, A16, A16, A16, big, big, 1024, 64, 1024) == -2
+
+
+def test_what_lies_apart():
+    """_apart against the addresses themselves: blocks, columns of one buffer, heads of a fused projection, expanded rows."""
+    buf = torch.zeros(4000, dtype=BF)
+    views = [buf.as_strided(*v) for v in (
+        ((3, 20), (50, 1), 0), ((3, 20), (50, 1), 20), ((3, 20), (50, 1), 30), ((3, 20), (50, 1), 31), ((3, 20), (50, 1), 45),
+        ((3, 20), (60, 1), 20), ((1, 20), (50, 1), 70), ((1, 20), (50, 1), 60), ((3, 20), (0, 1), 20), ((3, 50), (50, 1), 150),
+        ((3, 50), (50, 1), 149), ((2, 2, 3, 10), (150, 10, 50, 1), 0), ((2, 3, 20), (150, 50, 1), 20), ((2, 3, 20), (150, 50, 1), 19),
+        ((2, 2, 3, 10), (150, 20, 50, 1), 5), ((2, 3, 20), (1000, 50, 1), 36), ((20,), (1,), 25))]
+    cells = [set((torch.arange(4000).as_strided(v.shape, v.stride(), v.storage_offset())).flatten().tolist()) for v in views]
+    sure = 0
+    for a, x in zip(views, cells):
+        for b, y in zip(views, cells):
+            if ops._apart(a, b):
+                assert not x & y, (a.shape, a.stride(), a.storage_offset(), b.shape, b.stride(), b.storage_offset())
+                sure += 1
+    assert ops._apart(views[0], views[1]) and ops._apart(views[0], views[2]) and not ops._apart(views[0], views[3])
+    assert ops._apart(views[11], views[12]) and not ops._apart(views[11], views[13]) and ops._apart(views[0], views[9])
+    assert sure >= 40
