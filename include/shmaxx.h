@@ -204,10 +204,10 @@ void mx_sdpa_tiling(int B, int H, int Tq, int D, int* t);
  * Positions: base + pos[b * pos_s] (pos null: base), lengths alike; device values outside the cache write nothing /
  * are clamped to it. */
 /* Rows t < n of B sequences (k, v: strides per sequence, head, row; unit column stride) to positions pos_b + t of slot b
- * (bcast: B = 1, to every slot); sequences written and H + Hq up to 65535. count (nullable): only the first count[b] rows of sequence b. A block's exponent is the
- * smallest e with max |x| <= 448 2^e (at least -127) over the new rows, and not less than before if it holds earlier
- * rows, whose codes are rounded to it; what the last block holds behind the new rows is undefined. Infinities and NaN are
- * stored as NaN. cs (nullable, D = 64): the (ncs, 16, 2) rotary table of mx_rope_kv, applied to k and to the Hq query heads
+ * (bcast: B = 1, to every slot); sequences written and H + Hq up to 65535. count (nullable): only the first count[b] rows
+ * of sequence b. A block's exponent is the smallest e with max |x| <= 448 2^e (at least -127) over the new rows, and not less
+ * than before if it holds earlier rows, whose codes are rounded to it; what the last block holds behind the new rows is
+ * undefined. Infinities and NaN are stored as NaN. cs (nullable, D = 64): the (ncs, 16, 2) rotary table of mx_rope_kv, applied to k and to the Hq query heads
  * q -> q_out [B][Hq][n][D] (q nullable). */
 int mx_kv8_append(hipStream_t st, const uint16_t* k, long sk_b, long sk_h, long sk_t, const uint16_t* v, long sv_b,
                   long sv_h, long sv_t, uint8_t* kc, uint8_t* vc, uint8_t* ks, uint8_t* vs, int B, int H, int n, int D,
