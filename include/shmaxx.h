@@ -380,6 +380,53 @@ int mx_decode_mk_words(void);
 int mx_decode_mk_grid(void);
 int mx_decode_mk_layer_bytes(void);
 
+/* ============================================================================================ shared prefixes, beam search
+ * No counterpart in the reference, which keeps a copy of the image prefix in every question's cache slot
+ * (moondream/gpu/md2fast.py:177) and never decodes.
+ *
+ * Attention of sequences that share a prefix: sequence b = n S + j has the first plen_n keys of prefix n (one copy for its S
+ * sequences) and, of its own T rows, the first len_b; own key t is visible to query i iff not causal or t <= len_b - Tq + i:
+ *   O[b, i, h] = sum softmax(scale <q, key>) value over the keys that the query sees, 0 where there are none.
+ * Head dims D 64 and 128; G query heads per key head (query head h G + g reads key head h). q [N S][H G][Tq][D], pk / pv
+ * [N][H][P][D], k / v [N S][H][T][D] by element strides (multiples of 8, unit stride along D, 16-byte aligned; row strides of
+ * keys and values 0 .. 2^23 - 1), o [N S][Tq][H G D] (strides multiples of 4, 8-byte aligned). plen / len: device int32 with
+ * strides plen_s / len_s, added to pbase / base, or null; what lies outside 0 .. P / 0 .. T is clamped. P = 0 or T = 0: pk, pv
+ * or k, v are not read. fp32 sums, weights rounded to bf16; scores (times scale) must stay below 2^29 in size. part: at least
+ * mx_sdpa_prefix_ws floats, 16-byte aligned, one for each call that may run at the same time; not read from call to call.
+ * N S H < 2^23, N S H G Tq < 2^26. mx_sdpa_prefix_tiling: t[6] = 0 rows, 1 both, 2 tiles; query and key waves and runs of the
+ * tile kernel; waves and runs of the 16-row kernel. */
+long mx_sdpa_prefix_ws(int N, int S, int H, int G, int Tq, int P, int T, int D);
+void mx_sdpa_prefix_tiling(int N, int S, int H, int G, int Tq, int P, int T, int D, int* t);
+int mx_sdpa_prefix(hipStream_t st, const uint16_t* q, long sq_b, long sq_h, long sq_t, const uint16_t* pk, long spk_n,
+                   long spk_h, long spk_t, const uint16_t* pv, long spv_n, long spv_h, long spv_t, const uint16_t* k, long sk_b,
+                   long sk_h, long sk_t, const uint16_t* v, long sv_b, long sv_h, long sv_t, uint16_t* o, long so_b, long so_t,
+                   int N, int S, int H, int G, int Tq, int D, int P, int T, const int* plen, long plen_s, int pbase,
+                   const int* len, long len_s, int base, int causal, float scale, float* part, long part_elems);
+/* Beam search's selection: of the values score[b, w] + x[b, w, v] - logsumexp(x[b, w, :]) of search b, the k largest in falling
+ * order (equal ones: lowest w, then lowest v). A finished beam (done[b, w] != 0; done may be null) offers eos alone, at its
+ * score. A beam whose score is not finite, or whose logits hold NaN or +infinity or nothing above -infinity, offers nothing;
+ * neither does a logit of -infinity. x: bf16 or (fp32 != 0) float [B][W][V] by element strides sx_b, sx_w, unit stride along V;
+ * score [B][W] float, done [B][W] bytes. Outputs [B][k]: o_score, o_parent (w), o_token (v), o_done (may be null: v == eos).
+ * Places without a candidate: score -infinity, parent 0, token max(eos, 0), done 1. eos < 0: none (done must be null).
+ * W <= 64, k <= 64, 24 (W ceil(V / 2048 or 8192) + k (k + 1) / 2) <= 64000. ws: mx_beam_select_ws bytes, 8-byte aligned, one
+ * for each call that may run at the same time. */
+long mx_beam_select_ws(int B, int W, int V, int k);
+int mx_beam_select(hipStream_t st, const void* x, int fp32, long sx_b, long sx_w, const float* score, const uint8_t* done,
+                   int eos, int B, int W, int V, int k, float* o_score, int* o_parent, int* o_token, uint8_t* o_done, void* ws,
+                   long ws_bytes);
+/* Slots of a cache, in place: x[n, g W + w, h, t] = x[n, g W + parent[g, w], h, t] for first <= t < ceil(rows / unit), with
+ * rows = base + len[parent's slot] (len may be null), at most T; other rows stay. parent [G][W] (strides sp_g, sp_w): a value
+ * outside 0 .. W - 1 leaves its slot. Strides and row_bytes in bytes; the rows of different (n, slot, h, t) must not overlap.
+ * W <= 64. */
+int mx_reorder_slots(hipStream_t st, void* x, long s_n, long s_s, long s_h, long s_t, int N, int G, int W, int H, int T,
+                     int row_bytes, const int* parent, long sp_g, long sp_w, const int* len, long len_s, int base, int unit,
+                     int first);
+/* mx_rope_kv for B sequences whose n rows start at cache row at[b * at_s] (device int32), at rotary position rot0 + the row. cs
+ * has ncs positions, kc / vc [B][H][ctx][64]. Rows outside the cache or the table are dropped; their q takes the nearest
+ * position of the table. */
+int mx_rope_kv_at(hipStream_t st, const uint16_t* qkv, long ldq, const float* cs, int ncs, uint16_t* q_out, uint16_t* kc,
+                  uint16_t* vc, int B, int n, int H, int ctx, const int* at, long at_s, int rot0);
+
 /* ============================================================================================ TRecViT recurrence
  * One streamed frame of conv_1d + block-diagonal gates + RG-LRU + y-gate (numerics of tapnext/npu/pack8.py:253-279
  * ssm_ref and tapnext/npu/r9/cpuemu.py:33-47 RGLRU.forward): taps x0 (current) .. x3 (t-3), h fp32 updated in place,

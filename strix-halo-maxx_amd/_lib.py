@@ -62,6 +62,14 @@ SIGNATURES = {
     "mx_rmsnorm": [P, P, L, P, P, L, I, I, F],
     "mx_patchify_u8": [P, P, P, L, I, I, I, I],
     "mx_rope_kv": [P, P, L, P, P, P, P, I, I, I, I, I, I, I],
+    "mx_rope_kv_at": [P, P, L, P, I, P, P, P, I, I, I, I, P, L, I],
+    "mx_sdpa_prefix_ws": [I, I, I, I, I, I, I, I],
+    "mx_sdpa_prefix_tiling": [I, I, I, I, I, I, I, I, P],
+    "mx_sdpa_prefix": [P, P, L, L, L, P, L, L, L, P, L, L, L, P, L, L, L, P, L, L, L, P, L, L, I, I, I, I, I, I, I, I, P, L, I, P, L,
+                       I, I, F, P, L],
+    "mx_beam_select_ws": [I, I, I, I],
+    "mx_beam_select": [P, P, I, L, L, P, P, I, I, I, I, I, P, P, P, P, P, L],
+    "mx_reorder_slots": [P, P, L, L, L, L, I, I, I, I, I, I, P, L, L, P, L, I, I, I],
     "mx_ln_gemv2": [P, P, P, P, F, P, L, P, I, I, I, P, P, I],
     "mx_gemv_dual_res": [P, P, P, P, I, P, P, P, I, P, P, I],
     "mx_ln_gemv2_i8": [P, P, P, P, F, P, L, P, P, I, I, I, P, P, I],
@@ -100,7 +108,8 @@ STATUS = {0: "ok", -1: "bad config", -2: "unsupported shape/stride", -3: "split-
 RESTYPE = {"mx_gemm_ws_elems": L, "mx_gemm_ws_counters": L, "mx_track_head_blob_elems": L,
            "mx_gemm_noalloc_max_ws": L, "mx_sdpa_tiling": None, "mx_gemm_mxfp4_tiling": None,
            "mx_kv8_sdpa_tiling": None, "mx_gemm_res_ln_stats_words": L, "mx_gemm_res_ln_sync_words": L,
-           "mx_mxfp4_code_bytes": L, "mx_mxfp4_scale_bytes": L, "mx_kv8_sdpa_ws": L}
+           "mx_mxfp4_code_bytes": L, "mx_mxfp4_scale_bytes": L, "mx_kv8_sdpa_ws": L, "mx_sdpa_prefix_ws": L,
+           "mx_sdpa_prefix_tiling": None, "mx_beam_select_ws": L}
 
 _lib = None
 

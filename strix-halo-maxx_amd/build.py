@@ -22,9 +22,9 @@ FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Xclang", "-ta
          "-packed-fp32-ops", "-Wno-unused-result", "-ffp-contract=off"]
 
 
-# Per-file extras. attn.hip: MFMA accumulators in ordinary VGPRs (the online softmax rescales and reads them with
+# Per-file extras. attn.hip, prefix_attn.hip: MFMA accumulators in ordinary VGPRs (the online softmax rescales and reads them with
 # VALU ops every key block; accumulation registers would need a copy each way).
-FILE_FLAGS = {"attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+FILE_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for f in ("attn.hip", "prefix_attn.hip")}
 
 
 def _compile(src):

@@ -1,0 +1,382 @@
+// Beam search: the selection over beams and vocabulary, and the reordering of the slots of a cache.
+//
+// Selection. Beam w of search b with score s_w offers each token v at the value
+//   s_w + x[w, v] - log sum_u exp(x[w, u]);
+// a finished beam offers eos alone, at s_w. The k largest of the W V values, in falling order, ties by the lower w V + v.
+// Two launches:
+//  * parts: a workgroup reads 4 x 64 E logits of a row once: their maximum, the sum of their exponentials, and their k largest
+//    as (logit, token) keys. Within a row the order of the values is that of the logits, so no sum is needed yet.
+//  * merge: one workgroup per search adds the parts' sums, and takes the k largest of all parts' keys by their values.
+// The sums are fp32 within a part and fp64 from there on, values are fp64 and rounded to fp32 once; where two of one beam are
+// equal in fp64, their logits decide, as they do exactly.
+#include "common.h"
+
+namespace {
+
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));  // rows start at any element
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int MAXW = 64, MAXK = 64;
+
+// Order-preserving bits of a float; -0 counts as 0. NONE: -infinity and below, no candidate.
+__device__ __forceinline__ uint32_t bits_of(float x) {
+  const uint32_t u = __float_as_uint(x + 0.f);
+  return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float float_of(uint32_t b) { return __uint_as_float(b ^ ((b >> 31) ? 0x80000000u : 0xffffffffu)); }
+constexpr uint32_t NONE = 0x007fffffu;  // bits_of(-infinity)
+
+struct SelArgs {
+  const void* x;
+  long sx_b, sx_w;  // elements
+  const float* score;
+  const uint8_t* done;  // may be null
+  int B, W, V, k, eos, segs;
+  uint64_t* keys;  // [row][seg][k]: bits << 32 | ~token, falling; 0: none
+  float* stat;     // [row][seg][2]: maximum, sum of exp(x - maximum)
+  float* o_score;
+  int *o_parent, *o_token;
+  uint8_t* o_done;  // may be null
+};
+
+// 8 logits from v0 on; -infinity past the row's end
+template <class T>
+__device__ __forceinline__ void load8(const T* row, int v0, int V, float (&f)[8]) {
+  if (v0 + 8 <= V) {
+    if constexpr (sizeof(T) == 2) {
+      const u32x4 w = *reinterpret_cast<const u32x4_any*>(row + v0);
+#pragma unroll
+      for (int e = 0; e < 4; e++) f[2 * e] = lo_bf(w[e]), f[2 * e + 1] = hi_bf(w[e]);
+    } else {
+      const u32x4 a = *reinterpret_cast<const u32x4_any*>(row + v0), b = *reinterpret_cast<const u32x4_any*>(row + v0 + 4);
+#pragma unroll
+      for (int e = 0; e < 4; e++) f[e] = __uint_as_float(a[e]), f[4 + e] = __uint_as_float(b[e]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    f[e] = -INFINITY;
+    if (v0 + e < V) {
+      if constexpr (sizeof(T) == 2) f[e] = bf2f(row[v0 + e]);
+      else f[e] = row[v0 + e];
+    }
+  }
+}
+
+// A lane holds E / 8 chunks of 8 neighbouring logits, chunk i of a wave's lanes 512 in a row. The wave's threshold is the
+// k-th largest of its lanes' maxima (found bit by bit from ballots: 32 steps whatever k is): k lanes have a logit that large,
+// so no smaller one is among the k largest, and the larger ones lie in fewer than k lanes. Those, and the first k that equal
+// the threshold, go to LDS, where every one counts the larger ones: its rank.
+template <class T, int E>
+__global__ __launch_bounds__(256) void beam_parts_kernel(SelArgs p) {
+  extern __shared__ uint64_t cand[];
+  __shared__ int count;
+  __shared__ float ms[4][2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int seg = blockIdx.x % p.segs;
+  const long row = blockIdx.x / p.segs;
+  const float score = p.score[row];
+  if ((p.done && p.done[row]) || !(fabsf(score) < INFINITY)) return;  // the merge does not look at it
+  const T* x = reinterpret_cast<const T*>(p.x) + row / p.W * p.sx_b + row % p.W * p.sx_w;
+  if (tid == 0) count = 0;
+  const int v0 = seg * 256 * E + wave * 64 * E + lane * 8;
+  float f[E];
+#pragma unroll
+  for (int i = 0; i < E / 8; i++) load8(x, v0 + 512 * i, p.V, *reinterpret_cast<float(*)[8]>(f + 8 * i));
+  float m = f[0];
+#pragma unroll
+  for (int e = 1; e < E; e++) m = fmaxf(m, f[e]);
+  const float mw = wave_max(m), mb = mw == -INFINITY ? 0.f : mw;
+  float s = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; e++) s += __builtin_amdgcn_exp2f((f[e] - mb) * LOG2E);
+  s = wave_total(s);
+  if (lane == 0) ms[wave][0] = mw, ms[wave][1] = s;
+  // ---- the wave's threshold
+  uint32_t key[E], top = 0;
+#pragma unroll
+  for (int e = 0; e < E; e++) key[e] = bits_of(f[e]), top = max(top, key[e]);
+  uint32_t t = 0;
+#pragma unroll 4
+  for (int b = 31; b >= 0; b--) {
+    const uint32_t c = t | (1u << b);
+    if (__popcll(__ballot(top >= c)) >= p.k) t = c;
+  }
+  t = max(t, NONE + 1);  // fewer than k lanes, or -infinity: every finite logit
+  __syncthreads();
+  int equal = 0;  // of the lane's logits
+  if (top >= t) {
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      if (key[e] > t) cand[atomicAdd(&count, 1)] = (uint64_t)key[e] << 32 | ~(uint32_t)(v0 + 512 * (e / 8) + e % 8);
+      equal += key[e] == t;
+    }
+  }
+  if (__any(equal != 0)) {
+    int left = p.k;  // places for logits that equal the threshold, in the order of their tokens
+#pragma unroll
+    for (int i = 0; i < E / 8; i++) {
+      int n = 0;
+#pragma unroll
+      for (int e = 0; e < 8; e++) n += key[8 * i + e] == t;
+      uint64_t who = __ballot(n != 0);
+      while (who && left > 0) {  // wave-uniform
+        const int l = __ffsll((unsigned long long)who) - 1;
+        who &= who - 1;
+        const int nl = __builtin_amdgcn_readlane(n, l);
+        if (lane == l) {
+          int free = left;
+#pragma unroll
+          for (int e = 0; e < 8; e++)
+            if (key[8 * i + e] == t && free-- > 0)
+              cand[atomicAdd(&count, 1)] = (uint64_t)t << 32 | ~(uint32_t)(v0 + 512 * i + e);
+        }
+        left -= nl;
+      }
+    }
+  }
+  __syncthreads();
+  const int n = count;
+  uint64_t* out = p.keys + (row * p.segs + seg) * p.k;
+  for (int i = tid; i < n; i += 256) {
+    const uint64_t mine = cand[i];
+    int rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; j++) rank += cand[j] > mine;
+    if (rank < p.k) out[rank] = mine;
+  }
+  if (tid >= n && tid < p.k) out[tid] = 0;
+  if (tid == 0) {
+    float M = -INFINITY, S = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) M = fmaxf(M, ms[w][0]);
+    const float Mb = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int w = 0; w < 4; w++) S += ms[w][1] * __builtin_amdgcn_exp2f((ms[w][0] == -INFINITY ? -INFINITY : ms[w][0] - Mb) * LOG2E);
+    float* st = p.stat + (row * p.segs + seg) * 2;
+    st[0] = M, st[1] = S;
+  }
+}
+
+struct Cand {
+  double v;
+  uint64_t key;  // ~bits of the logit << 32 | token
+  uint32_t w;
+};
+__device__ __forceinline__ bool before(const Cand& a, const Cand& b) {
+  return a.v > b.v || (a.v == b.v && (a.w < b.w || (a.w == b.w && a.key < b.key)));
+}
+
+// A list is a part's keys; a finished beam's is its one continuation. The k-th largest head of the lists bounds what can be
+// selected, and a key at place i of a list whose head has rank r has i + r larger ones.
+__global__ __launch_bounds__(256) void beam_merge_kernel(SelArgs p) {
+  extern __shared__ Cand sh[];  // heads [W segs], candidates [k (k + 1) / 2]
+  __shared__ double base[MAXW];  // score - log of the sum
+  __shared__ float big[MAXW];    // largest logit
+  __shared__ int state[MAXW];  // 0: offers nothing, 1: its logits, 2: eos
+  __shared__ int count;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nl = p.W * p.segs;
+  const long b = blockIdx.x;
+  Cand *head = sh, *cand = sh + nl;
+  if (tid == 0) count = 0;
+  for (int w = wave; w < p.W; w += 4) {
+    const long row = b * p.W + w;
+    const float score = p.score[row];
+    const bool alive = fabsf(score) < INFINITY, fin = p.done && p.done[row];
+    double c = score;
+    float M = -INFINITY;
+    int st = alive ? (fin ? 2 : 1) : 0;
+    if (st == 1) {
+      const float* s = p.stat + row * p.segs * 2;
+      for (int i = lane; i < p.segs; i += 64) M = fmaxf(M, s[2 * i]);
+      M = wave_max(M);
+      double sum = 0.;
+      for (int i = lane; i < p.segs; i += 64)
+        sum += s[2 * i] == -INFINITY ? (double)s[2 * i + 1] : (double)s[2 * i + 1] * exp((double)s[2 * i] - (double)M);
+#pragma unroll
+      for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
+      c = (double)score - log(sum);
+      if (!(fabs(c) < INFINITY && fabsf(M) < INFINITY)) st = 0;  // NaN or +infinity among the logits, or nothing above -infinity
+    }
+    if (lane == 0) base[w] = c, big[w] = M, state[w] = st;
+  }
+  __syncthreads();
+  auto key_of = [&](int l, int i) { return p.keys[(b * nl + l) * p.k + i]; };
+  auto value = [&](int w, uint64_t key) {
+    return Cand{((double)float_of((uint32_t)(key >> 32)) - (double)big[w]) + base[w], ~key, (uint32_t)w};
+  };
+  for (int l = tid; l < nl; l += 256) {
+    const int w = l / p.segs;
+    Cand c = {-INFINITY, ~0ull, ~0u};
+    if (state[w] == 2) {
+      if (l % p.segs == 0) c = Cand{base[w], (uint64_t)p.eos, (uint32_t)w};
+    } else if (state[w] == 1) {
+      const uint64_t key = key_of(l, 0);
+      if (key) c = value(w, key);
+    }
+    head[l] = c;
+  }
+  __syncthreads();
+  for (int l = tid; l < nl; l += 256) {
+    const Cand c = head[l];
+    if (c.v == -INFINITY) continue;
+    int rank = 0;
+#pragma unroll 4
+    for (int i = 0; i < nl; i++) rank += before(head[i], c);
+    if (rank >= p.k) continue;
+    cand[atomicAdd(&count, 1)] = c;
+    const int w = l / p.segs;
+    if (state[w] == 2) continue;
+    for (int i = 1; i + rank < p.k; i++) {
+      const uint64_t key = key_of(l, i);
+      if (!key) break;
+      cand[atomicAdd(&count, 1)] = value(w, key);
+    }
+  }
+  __syncthreads();
+  const int n = count;
+  const long o = b * p.k;
+  for (int i = tid; i < n; i += 256) {
+    const Cand c = cand[i];
+    int rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; j++) rank += before(cand[j], c);
+    if (rank >= p.k) continue;
+    const int token = (int)(uint32_t)c.key;
+    p.o_score[o + rank] = (float)c.v;
+    p.o_parent[o + rank] = (int)c.w;
+    p.o_token[o + rank] = token;
+    if (p.o_done) p.o_done[o + rank] = token == p.eos;
+  }
+  if (tid >= n && tid < p.k) {  // fewer candidates than places
+    p.o_score[o + tid] = -INFINITY;
+    p.o_parent[o + tid] = 0;
+    p.o_token[o + tid] = max(p.eos, 0);
+    if (p.o_done) p.o_done[o + tid] = 1;
+  }
+}
+
+// Logits per lane: few where that is needed to fill the CUs.
+int per_lane(long rows, int V, int k) { return k <= 32 && rows * ((V + 8191) / 8192) >= 512 ? 32 : 8; }
+int segments(long rows, int V, int k) { return (V + 256 * per_lane(rows, V, k) - 1) / (256 * per_lane(rows, V, k)); }
+
+// ---------------------------------------------------------------------------------------------- slots
+struct MoveArgs {
+  uint8_t* x;
+  long s_n, s_s, s_h, s_t;  // bytes
+  const int* parent;
+  long sp_g, sp_w;
+  const int* len;  // may be null: base
+  long len_s;
+  int base, unit, first, T, G, W, H, cpr;  // cpr: pieces per row
+  unsigned nblk;
+};
+
+// x[n, g W + w, h, t] = x[n, g W + parent[g, w], h, t] for first <= t < rows of the parent. A thread owns one piece (16, 4 or 1
+// bytes) of a row in every slot of a group, loads what moves and then stores it, so the copy is in place in any order and no
+// two threads meet. Bound by the bytes: slots that do not change are not touched.
+template <class U, int WM>
+__global__ __launch_bounds__(256) void move_kernel(MoveArgs p) {
+  __shared__ long from[WM];  // byte offset of slot w's parent; the rows that it takes from it
+  __shared__ int rows[WM];
+  const unsigned blk = blockIdx.x % p.nblk;
+  long c = blockIdx.x / p.nblk;
+  const int h = (int)(c % p.H), g = (int)(c / p.H % p.G);
+  const long n = c / p.H / p.G;
+  if (threadIdx.x < WM) {
+    const int w = threadIdx.x, src = w < p.W ? p.parent[g * p.sp_g + w * p.sp_w] : w;
+    int r = 0;
+    if (src != w && src >= 0 && src < p.W) {
+      const long len = (long)p.base + (p.len ? p.len[(g * p.W + src) * p.len_s] : 0);
+      r = (int)min((max(len, 0L) + p.unit - 1) / p.unit, (long)p.T);
+    }
+    rows[w] = r;
+    from[w] = (long)src * p.s_s;
+  }
+  __syncthreads();
+  const long q = (long)blk * 256 + threadIdx.x;
+  const long t = p.first + q / p.cpr;
+  uint8_t* at = p.x + n * p.s_n + (long)g * p.W * p.s_s + h * p.s_h + t * p.s_t + q % p.cpr * sizeof(U);
+  U v[WM] = {};
+#pragma unroll
+  for (int w = 0; w < WM; w++)
+    if (t < rows[w]) v[w] = *reinterpret_cast<const U*>(at + from[w]);
+  asm volatile("" ::: "memory");  // two separate runs of branches: merged, every combination would get its own code
+#pragma unroll
+  for (int w = 0; w < WM; w++)
+    if (t < rows[w]) *reinterpret_cast<U*>(at + w * p.s_s) = v[w];
+}
+
+template <class U>
+void move(hipStream_t st, const MoveArgs& a, unsigned grid) {
+  const auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(grid), dim3(256), 0, st, a); };
+  if (a.W <= 4) go(move_kernel<U, 4>);
+  else if (a.W <= 8) go(move_kernel<U, 8>);
+  else if (a.W <= 16) go(move_kernel<U, 16>);
+  else if (a.W <= 32) go(move_kernel<U, 32>);
+  else go(move_kernel<U, 64>);
+}
+
+bool select_ok(int B, int W, int V, int k) {
+  return B >= 1 && W >= 1 && W <= MAXW && V >= 1 && V <= 0x7fff0000 && k >= 1 && k <= MAXK && (long)B * W <= 0x7fffffL &&
+         (long)B * W * segments((long)B * W, V, k) <= 0x7fffffL;
+}
+// the merge's LDS: heads and candidates
+long merge_lds(int W, int segs, int k) { return ((long)W * segs + k * (k + 1) / 2) * (long)sizeof(Cand); }
+
+}  // namespace
+
+// Bytes of workspace of mx_beam_select.
+extern "C" long mx_beam_select_ws(int B, int W, int V, int k) {
+  if (!select_ok(B, W, V, k)) return 0;
+  return (long)B * W * segments((long)B * W, V, k) * (8L * k + 8);
+}
+
+extern "C" int mx_beam_select(hipStream_t st, const void* x, int fp32, long sx_b, long sx_w, const float* score,
+                              const uint8_t* done, int eos, int B, int W, int V, int k, float* o_score, int* o_parent,
+                              int* o_token, uint8_t* o_done, void* ws, long ws_bytes) {
+  if (!x || !score || !o_score || !o_parent || !o_token) return MX_ENULL;
+  if (!select_ok(B, W, V, k)) return MX_ESHAPE;
+  if (eos >= V || (eos < 0 && done)) return MX_ESHAPE;
+  if (((uintptr_t)x & (fp32 ? 3 : 1)) || (((uintptr_t)score | (uintptr_t)o_score | (uintptr_t)o_parent | (uintptr_t)o_token) & 3))
+    return MX_ELAYOUT;
+  const long rows = (long)B * W;
+  const int segs = segments(rows, V, k), E = per_lane(rows, V, k);
+  const long lds = merge_lds(W, segs, k);
+  if (lds > 64000) return MX_ESHAPE;
+  if (!ws || ws_bytes < mx_beam_select_ws(B, W, V, k) || ((uintptr_t)ws & 7)) return MX_ESPLIT;
+  uint64_t* keys = reinterpret_cast<uint64_t*>(ws);
+  const SelArgs a{x, sx_b, sx_w, score, done, B, W, V, k, eos, segs, keys, reinterpret_cast<float*>(keys + rows * segs * k),
+                  o_score, o_parent, o_token, o_done};
+  const dim3 grid((unsigned)(rows * segs));
+  const auto go = [&](auto kern) {
+    const size_t sh = 4 * ((k - 1) * (size_t)E + k) * 8;  // what four waves can hand over
+    hipLaunchKernelGGL(kern, grid, dim3(256), sh, st, a);
+  };
+  if (fp32) E == 32 ? go(beam_parts_kernel<float, 32>) : go(beam_parts_kernel<float, 8>);
+  else E == 32 ? go(beam_parts_kernel<uint16_t, 32>) : go(beam_parts_kernel<uint16_t, 8>);
+  if (hipGetLastError() != hipSuccess) return MX_ELAUNCH;
+  hipLaunchKernelGGL(beam_merge_kernel, dim3((unsigned)B), dim3(256), (size_t)lds, st, a);
+  return hipGetLastError() == hipSuccess ? MX_OK : MX_ELAUNCH;
+}
+
+extern "C" int mx_reorder_slots(hipStream_t st, void* x, long s_n, long s_s, long s_h, long s_t, int N, int G, int W, int H, int T,
+                                int row_bytes, const int* parent, long sp_g, long sp_w, const int* len, long len_s, int base,
+                                int unit, int first) {
+  if (!x || !parent) return MX_ENULL;
+  if (N < 1 || G < 1 || W < 1 || W > 64 || H < 1 || T < 1 || row_bytes < 1 || unit < 1 || first < 0) return MX_ESHAPE;
+  if (((uintptr_t)parent & 3) || ((uintptr_t)len & 3)) return MX_ELAYOUT;
+  if (W == 1 || first >= T) return MX_OK;
+  const uintptr_t bits = (uintptr_t)x | (uintptr_t)s_n | (uintptr_t)s_s | (uintptr_t)s_h | (uintptr_t)s_t | (uintptr_t)row_bytes;
+  const int size = bits & 3 ? 1 : bits & 15 ? 4 : 16;
+  const int cpr = row_bytes / size;
+  const double blocks = ((double)(T - first) * cpr + 255) / 256 * N * G * H;
+  if (blocks > 0x7fffff) return MX_ESHAPE;  // 2^32 threads in a grid
+  const unsigned nblk = (unsigned)(((long)(T - first) * cpr + 255) / 256);
+  const MoveArgs a{(uint8_t*)x, s_n, s_s, s_h, s_t, parent, sp_g, sp_w, len, len_s, base, unit, first, T, G, W, H, cpr, nblk};
+  const unsigned grid = nblk * (unsigned)(N * G * H);
+  if (size == 16) move<u32x4>(st, a, grid);
+  else if (size == 4) move<uint32_t>(st, a, grid);
+  else move<uint8_t>(st, a, grid);
+  return hipGetLastError() == hipSuccess ? MX_OK : MX_ELAUNCH;
+}

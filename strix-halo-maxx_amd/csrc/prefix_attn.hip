@@ -1,0 +1,811 @@
+// Attention of sequences that share a prefix, head dims 64 and 128, G query heads per key head. Sequence b = n S + j of
+// prefix n has the prefix's keys (one copy for its S sequences) and keys of its own:
+//   O[b, i, h] = sum softmax(scale <Q[b, h, i], key>) value   over the prefix's first plen_n keys and its own keys that it sees
+//   own key t is visible to query i iff t < len_b and (not causal or t <= len_b - Tq + i); a query without a key gets zeros.
+// A row is a (sequence, query, head of the group) of one key head h: row = (j Tq + i) G + g of the S Tq G that share K and V.
+//
+// Three ways to cut it (plan()):
+//  * rows: 16 rows per workgroup, from any sequences; its waves go through one list of 32-key blocks: the prefix's, then
+//    those of each sequence in the tile, which the rows of the others do not see. Few rows: everything is read once.
+//  * both: tiles of 32 - 128 rows over the prefix, which is so read once for all of them, and in the same launch 16-row
+//    tiles over the sequences' own keys. Many sequences of few rows each.
+//  * tiles: tiles of 32 - 128 rows of one sequence through the prefix and then its own keys. Prompts.
+// Each may cut its list of blocks into runs ("splits"): a run's share (maximum, sum, unnormalised output in fp32) goes to
+// memory and the join adds the shares of a row in a fixed order. The host knows capacities only (lengths may be on the
+// device), so it fixes the number of runs and the device cuts each list evenly.
+//
+// Numerics: fp32 scores, sums and outputs; weights are rounded to bf16 before their product and the sums are taken over the
+// rounded weights, so numerator and denominator use the same ones. A masked key reaches no result: blocks that need a mask
+// are searched for infinities and NaN among the values, and where there is one (never in ordinary data) it is cleared and two
+// products of indicators with the visibility find the outputs that it belongs to.
+#include "common.h"
+
+namespace {
+
+struct Seg {  // K or V of one segment: element strides
+  const uint16_t* p;
+  long s_b, s_h;
+  int s_t;
+};
+
+struct Args {
+  const uint16_t* q;
+  long sq_b, sq_h, sq_t;
+  Seg pk, pv, k, v;
+  uint16_t* o;
+  long so_b, so_t;
+  const int *plen, *len;  // null: pbase, base alone
+  long plen_s, len_s;
+  int pbase, base, P, T;
+  int N, S, H, G, Tq, causal;
+  float sl2;
+  // the shares of the tile kernel (a) and of the 16-row kernel (b): rows per tile, tiles per cell, runs, first float of
+  // the outputs and of the (maximum, sum) pairs in part
+  int rwa, nta, spa, rwb, ntb, spb;
+  long na;  // workgroups of the tile kernel
+  float *oa, *ma, *ob, *mb;
+};
+
+__device__ __forceinline__ int prefix_len(const Args& p, int n) {
+  const long l = (long)p.pbase + (p.plen ? p.plen[n * p.plen_s] : 0);
+  return (int)min(max(l, 0L), (long)p.P);
+}
+__device__ __forceinline__ int own_len(const Args& p, int b) {
+  const long l = (long)p.base + (p.len ? p.len[b * p.len_s] : 0);
+  return (int)min(max(l, 0L), (long)p.T);
+}
+// own keys that query i of a sequence of len sees
+__device__ __forceinline__ int limit(const Args& p, int len, int i) {
+  return p.causal ? min(max(len - p.Tq + 1 + i, 0), len) : len;
+}
+
+// The order of the 16-byte slots of a key's row in LDS: slot s of key lies at s ^ swz(key). 64 banks hold one row of 128 or
+// two of 64 columns; with these bits both the operand reads of K (one slot of 16 keys) and the transposed reads of V (two
+// slots of 8 keys, or four of 4) meet every bank once.
+template <int D>
+__device__ __forceinline__ int swz(int key) {
+  const int lo = ((key >> 2) & 1) * 2 + ((key >> 3) & 1);
+  return D == 128 ? ((key >> 1) & 1) * 8 + (key & 1) * 4 + lo : ((key >> 1) & 1) * 4 + lo;
+}
+
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
+}
+__device__ __forceinline__ float quarters_max(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return halves_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float quarters_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return halves_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// bit 15 of each bf16 of a pair: infinity or NaN; with them, 1.0 where it is +infinity (neg: -infinity) or NaN; cleared
+__device__ __forceinline__ uint32_t odd(uint32_t w) {
+  return ~(((w & 0x7f807f80u) ^ 0x7f807f80u) + 0x7fff7fffu) & 0x80008000u;
+}
+__device__ __forceinline__ uint32_t odd(u32x4 v) { return odd(v.x) | odd(v.y) | odd(v.z) | odd(v.w); }
+__device__ __forceinline__ uint32_t mark(uint32_t w, uint32_t neg) {  // neg: 0 or ~0
+  const uint32_t nan = (w & 0x007f007fu) + 0x7fff7fffu;
+  return ((odd(w) & (nan | (w ^ ~neg))) >> 15) * 0x3f80u;
+}
+__device__ __forceinline__ u32x4 mark(u32x4 v, uint32_t neg) {
+  return u32x4{mark(v.x, neg), mark(v.y, neg), mark(v.z, neg), mark(v.w, neg)};
+}
+__device__ __forceinline__ uint32_t finite(uint32_t w) { return w & ~((odd(w) >> 15) * 0xffffu); }
+__device__ __forceinline__ u32x4 finite(u32x4 v) { return u32x4{finite(v.x), finite(v.y), finite(v.z), finite(v.w)}; }
+// 1.0 for the two keys from `key` on that lie below lim
+__device__ __forceinline__ uint32_t seen2(int key, int lim) { return (key < lim ? 0x3f80u : 0u) | (key + 1 < lim ? 0x3f800000u : 0u); }
+
+// 2^x of the distance to a maximum that may still be -infinity.
+__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
+
+// Where the result of a row goes: bf16, or (runs > 1) the share of its record.
+struct Out {
+  uint16_t* o;
+  float *po, *pm;
+  float inv;
+};
+__device__ __forceinline__ uint16_t* out_row(const Args& p, int n, int h, int row, int D) {
+  const int M = p.G * p.Tq, j = row / M, r = row % M;
+  return p.o + (long)(n * p.S + j) * p.so_b + (long)(r / p.G) * p.so_t + (long)(h * p.G + r % p.G) * D;
+}
+__device__ __forceinline__ void put4(const Out& t, int d, float a, float b, float c, float e) {
+  if (t.po)
+    *reinterpret_cast<f32x4*>(t.po + d) = f32x4{a, b, c, e};
+  else
+    *reinterpret_cast<u32x2*>(t.o + d) = u32x2{pack2(a * t.inv, b * t.inv), pack2(c * t.inv, e * t.inv)};
+}
+
+// ---------------------------------------------------------------------------------------------- 16 rows
+template <int D, int NW>
+constexpr int rows_lds() {
+  return NW * (32 + 16 * D) * 4 > NW * 64 * D ? NW * (32 + 16 * D) * 4 : NW * 64 * D;
+}
+
+// Item = (prefix and key head, run, 16 rows). The NW waves take the 32-key blocks of the run in turn: K from memory into
+// the 16x16x32 MFMA's registers, V through a piece of LDS of the wave's own for the transposed read; the next block is in
+// flight through this one's softmax and product. S^T leaves keys 16 t + 4 (lane / 16) + r of row lane % 16 in a lane, and the
+// product with V takes its keys in that order.
+template <int D, int NW, bool PREFIX>
+__device__ __forceinline__ void rows_body(const Args& p, long item, uint8_t* smem) {
+  constexpr int NS = D / 32, NT = D / 16, NV = D / 16, CPR = D / 8;
+  const int lane = threadIdx.x & 63, kw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int rt = (int)(item % p.ntb), s = (int)(item / p.ntb % p.spb), cell = (int)(item / p.ntb / p.spb);
+  const int n = cell / p.H, h = cell % p.H;
+  const int M = p.G * p.Tq, R = p.S * M, row = rt * 16 + c, rc = min(row, R - 1), rl = min(rt * 16 + 15, R - 1);
+  const int j = rc / M, i = rc % M / p.G;
+  const int j0 = rt * 16 / M, jl = rl / M;  // the tile's sequences
+  // lane u of 16: sequence j0 + u, the keys that any / every row of it in this tile sees, blocks up to and with it
+  const int ju = min(j0 + c, jl), lenu = own_len(p, n * p.S + ju);
+  const int kendu = limit(p, lenu, min(rl - ju * M, M - 1) / p.G);
+  const int kallu = limit(p, lenu, max(rt * 16 - ju * M, 0) / p.G);
+  const int plen = PREFIX ? prefix_len(p, n) : 0, npb = (plen + 31) / 32;
+  int cum = j0 + c <= jl ? (kendu + 31) / 32 : 0;
+#pragma unroll
+  for (int d = 1; d < 16; d *= 2) {
+    const int o = __shfl_up(cum, d, 16);
+    cum += c >= d ? o : 0;
+  }
+  cum += npb;
+  const long total = __builtin_amdgcn_readlane(cum, 15);
+  const int x0 = (int)(total * s / p.spb), x1 = (int)(total * (s + 1) / p.spb);
+  const int lim_own = limit(p, own_len(p, n * p.S + j), i);
+
+  struct Blk {
+    const uint16_t *k, *v;
+    int sk, sv, key0, kend, lim;
+    bool masked;
+  } b;
+  int u = 0;
+  auto locate = [&](int x) {
+    if (PREFIX && x < npb) {
+      b.key0 = 32 * x, b.kend = b.lim = plen, b.masked = b.key0 + 32 > plen;
+      b.k = p.pk.p + n * p.pk.s_b + h * p.pk.s_h, b.sk = p.pk.s_t;
+      b.v = p.pv.p + n * p.pv.s_b + h * p.pv.s_h, b.sv = p.pv.s_t;
+      return;
+    }
+    while (x >= __builtin_amdgcn_readlane(cum, u)) u++;
+    const int first = u ? __builtin_amdgcn_readlane(cum, u - 1) : npb;
+    const long seq = n * p.S + j0 + u;
+    b.key0 = 32 * (x - first), b.kend = __builtin_amdgcn_readlane(kendu, u);
+    b.lim = j == j0 + u ? lim_own : 0;
+    b.masked = jl > j0 || b.key0 + 32 > __builtin_amdgcn_readlane(kallu, u);
+    b.k = p.k.p + seq * p.k.s_b + h * p.k.s_h, b.sk = p.k.s_t;
+    b.v = p.v.p + seq * p.v.s_b + h * p.v.s_h, b.sv = p.v.s_t;
+  };
+  u32x4 k[2][NS], v[NV];
+  auto get = [&]() {  // keys past the last are the last one again (masked)
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      const uint16_t* kr = b.k + (long)min(b.key0 + 16 * t + c, b.kend - 1) * b.sk + 8 * g;
+#pragma unroll
+      for (int e = 0; e < NS; e++) k[t][e] = *reinterpret_cast<const u32x4*>(kr + 32 * e);
+    }
+#pragma unroll
+    for (int e = 0; e < NV; e++) {
+      const int ch = lane + 64 * e;
+      v[e] = *reinterpret_cast<const u32x4*>(b.v + (long)min(b.key0 + ch / CPR, b.kend - 1) * b.sv + ch % CPR * 8);
+    }
+  };
+  f32x4 o[NT];
+#pragma unroll
+  for (int t = 0; t < NT; t++) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  uint8_t* vst = smem + kw * 64 * D;
+  auto stage = [&](const u32x4(&x)[NV]) {
+#pragma unroll
+    for (int e = 0; e < NV; e++) {
+      const int ch = lane + 64 * e, key = ch / CPR;
+      *reinterpret_cast<u32x4*>(vst + key * 2 * D + ((ch % CPR) ^ swz<D>(key)) * 16) = x[e];
+    }
+  };
+  auto operand = [&](int t) {
+    const int r0 = 4 * g + (c >> 2), slot = 2 * t + ((c & 3) >> 1), sub = (c & 1) * 8;
+    const u32x2 lo = lds_read_tr16(reinterpret_cast<const uint16_t*>(vst + r0 * 2 * D + (slot ^ swz<D>(r0)) * 16 + sub));
+    const u32x2 hi = lds_read_tr16(reinterpret_cast<const uint16_t*>(vst + (r0 + 16) * 2 * D + (slot ^ swz<D>(r0 + 16)) * 16 + sub));
+    return u32x4{lo.x, lo.y, hi.x, hi.y};
+  };
+  int x = x0 + kw;
+  if (x < x1) {
+    locate(x);
+    u32x4 qf[NS];
+    const uint16_t* qrow = p.q + (long)(n * p.S + j) * p.sq_b + (long)(h * p.G + rc % p.G) * p.sq_h + (long)i * p.sq_t + 8 * g;
+#pragma unroll
+    for (int e = 0; e < NS; e++) qf[e] = *reinterpret_cast<const u32x4*>(qrow + 32 * e);
+    get();
+    for (;;) {
+      f32x4 st[2];
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        st[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < NS; e++) st[t] = mfma16(k[t][e], qf[e], st[t]);
+      }
+      const int key = b.key0 + 4 * g, lim = b.lim;
+      if (b.masked) {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int e = 0; e < NV; e++) bad |= odd(v[e]);
+        if (__any(bad != 0)) {
+          const u32x4 vis = {seen2(key, lim), seen2(key + 2, lim), seen2(key + 16, lim), seen2(key + 18, lim)};
+          stage(v);
+#pragma unroll
+          for (int t = 0; t < NT; t++) {
+            __builtin_amdgcn_sched_barrier(0);  // one at a time: few registers for what never happens
+            const u32x4 a = operand(t);
+            const f32x4 none = {0.f, 0.f, 0.f, 0.f};
+            const f32x4 up = mfma16(mark(a, 0u), vis, none), dn = mfma16(mark(a, ~0u), vis, none);
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+              o[t][r] += up[r] > 0.f ? INFINITY : 0.f;
+              o[t][r] -= dn[r] > 0.f ? INFINITY : 0.f;
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < NV; e++) v[e] = finite(v[e]);
+        }
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) st[t][r] = key + 16 * t + r < lim ? st[t][r] : -INFINITY;
+      }
+      stage(v);
+      x += NW;
+      const bool more = x < x1;
+      if (more) {
+        locate(x);
+        get();
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) mx = fmaxf(mx, st[t][r]);
+      mx = quarters_max(mx) * p.sl2;
+      const bool grow = mx > m;
+      if (__any(grow)) {
+        // (before a row's first key its outputs are 0, or the infinities found above)
+        const float al = grow && m != -INFINITY ? __builtin_amdgcn_exp2f(m - mx) : 1.f;
+        l *= al;
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) o[t][r] *= al;
+        m = grow ? mx : m;
+      }
+      const float mb = base_of(m);
+      u32x4 w;
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+          const uint32_t pr = pack2(__builtin_amdgcn_exp2f(__builtin_fmaf(st[t][r], p.sl2, -mb)),
+                                    __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][r + 1], p.sl2, -mb)));
+          l += lo_bf(pr) + hi_bf(pr);
+          w[2 * t + r / 2] = pr;
+        }
+#pragma unroll
+      for (int t = 0; t < NT; t++) o[t] = mfma16(operand(t), w, o[t]);
+      if (!more) break;
+    }
+  }
+  l = quarters_sum(l);
+  // ---- the waves' shares meet in LDS, added in wave order; wave kw finishes the tiles t with t % NW = kw
+  __syncthreads();
+  float* cm = reinterpret_cast<float*>(smem);
+  f32x4* co = reinterpret_cast<f32x4*>(cm + NW * 32);
+  if (g == 0) {
+    cm[kw * 32 + c] = m;
+    cm[kw * 32 + 16 + c] = l;
+  }
+#pragma unroll
+  for (int t = 0; t < NT; t++) co[(kw * NT + t) * 64 + lane] = o[t];
+  __syncthreads();
+  if (row >= R) return;
+  float top = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < NW; w++) top = fmaxf(top, cm[w * 32 + c]);
+  const float tb = base_of(top);
+  float L = 0.f, f[NW];
+#pragma unroll
+  for (int w = 0; w < NW; w++) {
+    f[w] = __builtin_amdgcn_exp2f(cm[w * 32 + c] - tb);
+    L += cm[w * 32 + 16 + c] * f[w];
+  }
+  Out t;
+  t.o = out_row(p, n, h, row, D);
+  t.po = p.ob ? p.ob + (item * 16 + c) * D : nullptr;
+  t.inv = L == 0.f ? 0.f : 1.f / L;
+  if (t.po && kw == 0 && g == 0) {
+    p.mb[item * 32 + c] = top;
+    p.mb[item * 32 + 16 + c] = L;
+  }
+  for (int e = kw; e < NT; e += NW) {
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+      const f32x4 y = co[(w * NT + e) * 64 + lane];
+#pragma unroll
+      for (int r = 0; r < 4; r++) a[r] += y[r] * f[w];
+    }
+    put4(t, 16 * e + 4 * g, a[0], a[1], a[2], a[3]);
+  }
+}
+
+template <int D, int NW>
+__global__ __launch_bounds__(64 * NW) void prefix_rows_kernel(Args p) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[rows_lds<D, NW>()];
+  rows_body<D, NW, true>(p, blockIdx.x, smem);
+}
+
+// ---------------------------------------------------------------------------------------------- many rows
+template <int D, int NQW, int NKW, int KB, int S>
+struct Tile {
+  static constexpr int CPR = D / 8, KBW = KB / NKW, NST = KBW / 32, NW = NQW * NKW, DT = D / 32;
+  static constexpr int STAGE_B = 4 * KB * D;             // K and V of a block
+  static constexpr int NIW = STAGE_B / 1024 / NW;        // load instructions per wave and block
+  static constexpr int RING_B = S * STAGE_B;
+  static constexpr int COMB_B = NKW > 1 ? NW * 64 * (2 + D / 2) * 4 : 0;
+  static constexpr int BYTES = RING_B > COMB_B ? RING_B : COMB_B;
+  static_assert(KBW % 32 == 0 && STAGE_B % (1024 * NW) == 0 && BYTES <= 160 * 1024, "ring");
+};
+
+// Item = (cell, run, 32 NQW rows) on the 32x32x16 MFMA; a cell is a prefix and a key head, and (SEQ) one of its sequences.
+// NQW query waves x NKW key waves; blocks of KB keys go through an LDS ring of S stages by the asynchronous load, the
+// block's keys shared among the key waves, whose shares are added at the end. S^T = K Q^T leaves a lane the scores of one
+// row, in the key order that the product with V (transposed reads) takes.
+template <int D, int NQW, int NKW, int KB, int S, bool SEQ>
+__device__ __forceinline__ void tile_body(const Args& p, long item, uint8_t* smem) {
+  using C = Tile<D, NQW, NKW, KB, S>;
+  constexpr int CPR = C::CPR, KBW = C::KBW, NST = C::NST, DT = C::DT, RB = 2 * D;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int qg = wave % NQW, kw = wave / NQW, c = lane & 31, hk = lane >> 5;
+  const int M = p.G * p.Tq, R = SEQ ? M : p.S * M;
+  const int rt = (int)(item % p.nta), s = (int)(item / p.nta % p.spa);
+  const long cell = item / p.nta / p.spa;
+  const int j0 = SEQ ? (int)(cell % p.S) : 0;
+  const int nh = SEQ ? (int)(cell / p.S) : (int)cell, n = nh / p.H, h = nh % p.H;
+  const int r0 = rt * 32 * NQW, row = r0 + 32 * qg + c, rc = min(row, R - 1);
+  const int plen = prefix_len(p, n), npb = (plen + KB - 1) / KB;
+  int lim_own = 0, kend = 0, wend = 0, kall = 0;  // own keys that the row, any row, any / every row of this wave sees
+  if (SEQ) {
+    const int len = own_len(p, n * p.S + j0);
+    lim_own = limit(p, len, rc / p.G);
+    kend = limit(p, len, min(r0 + 32 * NQW - 1, R - 1) / p.G);
+    wend = limit(p, len, min(r0 + 32 * qg + 31, R - 1) / p.G);
+    kall = limit(p, len, min(r0 + 32 * qg, R - 1) / p.G);
+  }
+  const long total = npb + (kend + KB - 1) / KB;
+  const int x0 = (int)(total * s / p.spa), x1 = (int)(total * (s + 1) / p.spa);
+  const uint32_t sbase = lds_off(smem);
+  const uint16_t *pkb = p.pk.p + n * p.pk.s_b + h * p.pk.s_h, *pvb = p.pv.p + n * p.pv.s_b + h * p.pv.s_h;
+  const uint16_t *kb = p.k.p + (long)(n * p.S + j0) * p.k.s_b + h * p.k.s_h, *vb = p.v.p + (long)(n * p.S + j0) * p.v.s_b + h * p.v.s_h;
+  const int spk = p.pk.s_t, spv = p.pv.s_t, sok = p.k.s_t, sov = p.v.s_t;
+  // instruction q of a block brings 1 KB of the K part, then of the V part, in LDS order; keys past the last are it again
+  auto issue = [&](int x) {
+    const bool pre = !SEQ || x < npb;
+    const int first = (pre ? x : x - npb) * KB, last = (pre ? plen : kend) - 1 - first;
+    const uint32_t dst = sbase + (uint32_t)((x - x0) % S) * C::STAGE_B;
+    int stk = spk, stv = spv;
+    const uint16_t *kf = pkb, *vf = pvb;
+    if (!pre) stk = sok, stv = sov, kf = kb, vf = vb;
+    kf += (long)first * stk, vf += (long)first * stv;
+#pragma unroll
+    for (int e = 0; e < C::NIW; e++) {
+      const int q = wave * C::NIW + e;
+      const bool isv = q >= KB * CPR / 64;
+      const int ch = (q * 64 + lane) % (KB * CPR), key = ch / CPR, slot = (ch % CPR) ^ swz<D>(key);
+      dma16s(isv ? vf : kf, (uint32_t)min(key, last) * (uint32_t)(2 * (isv ? stv : stk)) + slot * 16, dst + q * 1024);
+    }
+  };
+  f32x16 o[DT];
+#pragma unroll
+  for (int t = 0; t < DT; t++)
+#pragma unroll
+    for (int e = 0; e < 16; e++) o[t][e] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  bf16x8 qf[D / 16];
+  if (x0 < x1) issue(x0);
+  {
+    const int j = SEQ ? j0 : rc / M, r = rc % M;
+    const uint16_t* qrow = p.q + (long)(n * p.S + j) * p.sq_b + (long)(h * p.G + r % p.G) * p.sq_h + (long)(r / p.G) * p.sq_t + 8 * hk;
+#pragma unroll
+    for (int e = 0; e < D / 16; e++) qf[e] = as_bf16x8(*reinterpret_cast<const u32x4*>(qrow + 16 * e));
+  }
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the compiler does not count the LDS-DMA loads, so nothing of its own may
+                                       // be in flight beside them (gfx9 encoding; expcnt, lgkmcnt not waited)
+#pragma unroll
+  for (int e = 1; e < S - 1; e++)
+    if (x0 + e < x1) issue(x0 + e);
+
+  for (int x = x0; x < x1; x++) {
+    wait_stages<C::NIW, S - 2>(x1 - 1 - x);
+    __syncthreads();
+    if (x + S - 1 < x1) issue(x + S - 1);
+    const bool pre = !SEQ || x < npb;
+    const int k0 = (pre ? x : x - npb) * KB + kw * KBW;  // first key of this wave's share
+    if (k0 >= (pre ? plen : wend)) continue;
+    const uint8_t* kst = smem + ((x - x0) % S) * C::STAGE_B + kw * KBW * RB;
+    const uint8_t* vst = kst + KB * RB;
+    f32x16 st[NST];
+#pragma unroll
+    for (int t = 0; t < NST; t++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) st[t][e] = 0.f;
+#pragma unroll
+    for (int e = 0; e < D / 16; e++)
+#pragma unroll
+      for (int t = 0; t < NST; t++) {
+        const int key = 32 * t + c;  // the swizzle depends on key % 16 only
+        const u32x4 a = *reinterpret_cast<const u32x4*>(kst + key * RB + ((2 * e + hk) ^ swz<D>(key)) * 16);
+        st[t] = mfma32(as_bf16x8(a), qf[e], st[t]);
+      }
+    const bool masked = k0 + KBW > (pre ? plen : kall);
+    const int lim = pre ? plen : lim_own, key0 = k0 + 4 * hk;
+    float mx = -INFINITY;
+    if (masked) {
+      asm volatile("");  // keeps the branch: as selects the mask would be computed for every block
+#pragma unroll
+      for (int t = 0; t < NST; t++)
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+          st[t][r] = key0 + 32 * t + 8 * (r >> 2) + (r & 3) < lim ? st[t][r] : -INFINITY;
+    }
+#pragma unroll
+    for (int t = 0; t < NST; t++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) mx = fmaxf(mx, st[t][r]);
+    // the running maximum is raised when a row's block maximum passes it by more than 8: weights stay below 2^8, and what
+    // they are relative to cancels in the end
+    mx = halves_max(mx) * p.sl2;
+    const bool grow = mx > m + 8.f;
+    if (__any(grow)) {
+      const float al = grow ? __builtin_amdgcn_exp2f(m - mx) : 1.f;
+      l *= al;
+#pragma unroll
+      for (int t = 0; t < DT; t++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[t][e] *= al;
+      m = grow ? mx : m;
+    }
+    const float mb = base_of(m);
+    uint32_t w[NST][8];
+#pragma unroll
+    for (int t = 0; t < NST; t++)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        const uint32_t pr = pack2(__builtin_amdgcn_exp2f(__builtin_fmaf(st[t][r], p.sl2, -mb)),
+                                  __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][r + 1], p.sl2, -mb)));
+        l += lo_bf(pr) + hi_bf(pr);
+        w[t][r >> 1] = pr;
+      }
+    // ---- O^T += V^T P^T: step (t, e) takes keys 32 t + 16 e + {4 hk .. 4 hk + 3, 8 + 4 hk ..}
+    const int jr = (lane & 15) >> 2, jc = 4 * (lane & 3) + 16 * ((lane >> 4) & 1);
+    auto operand = [&](int t, int e, int dt) {
+      const int r1 = 32 * t + 16 * e + 4 * hk + jr, slot = (32 * dt + jc) >> 3, sub = (jc & 7) * 2;
+      const u32x2 lo = lds_read_tr16(reinterpret_cast<const uint16_t*>(vst + r1 * RB + (slot ^ swz<D>(r1)) * 16 + sub));
+      const u32x2 hi = lds_read_tr16(reinterpret_cast<const uint16_t*>(vst + (r1 + 8) * RB + (slot ^ swz<D>(r1 + 8)) * 16 + sub));
+      return u32x4{lo.x, lo.y, hi.x, hi.y};
+    };
+    if (masked) {
+      uint32_t bad = 0;
+#pragma unroll
+      for (int t = 0; t < NST; t++)
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+          for (int dt = 0; dt < DT; dt++) bad |= odd(operand(t, e, dt));
+      if (__any(bad != 0)) {
+#pragma unroll
+        for (int t = 0; t < NST; t++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const int k1 = key0 + 32 * t + 16 * e;
+            const u32x4 pb = {w[t][4 * e], w[t][4 * e + 1], w[t][4 * e + 2], w[t][4 * e + 3]};
+            const u32x4 vis = {seen2(k1, lim), seen2(k1 + 2, lim), seen2(k1 + 8, lim), seen2(k1 + 10, lim)};
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) {
+              const u32x4 a = operand(t, e, dt);
+              o[dt] = mfma32(as_bf16x8(finite(a)), as_bf16x8(pb), o[dt]);
+#pragma unroll 1
+              for (int neg = 0; neg < 2; neg++) {
+                f32x16 hit;
+#pragma unroll
+                for (int r = 0; r < 16; r++) hit[r] = 0.f;
+                hit = mfma32(as_bf16x8(mark(a, neg ? ~0u : 0u)), as_bf16x8(vis), hit);
+                const float add = neg ? -INFINITY : INFINITY;
+#pragma unroll
+                for (int r = 0; r < 16; r++) o[dt][r] += hit[r] > 0.f ? add : 0.f;
+              }
+            }
+          }
+        continue;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < NST; t++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const u32x4 pb = {w[t][4 * e], w[t][4 * e + 1], w[t][4 * e + 2], w[t][4 * e + 3]};
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) o[dt] = mfma32(as_bf16x8(operand(t, e, dt)), as_bf16x8(pb), o[dt]);
+      }
+  }
+
+  float L = halves_sum(l);
+  Out t;
+  auto aim = [&]() {
+    t.o = out_row(p, n, h, SEQ ? j0 * M + row : row, D);
+    t.po = p.oa ? p.oa + (item * p.rwa + 32 * qg + c) * D : nullptr;
+    t.inv = L == 0.f ? 0.f : 1.f / L;
+    if (t.po && kw == 0 && hk == 0) {
+      p.ma[item * 2 * p.rwa + 32 * qg + c] = m;
+      p.ma[item * 2 * p.rwa + p.rwa + 32 * qg + c] = L;
+    }
+  };
+  if constexpr (NKW > 1) {
+    // ---- the key waves' shares, added in wave order; wave kw finishes the register groups u with u % NKW = kw
+    float* cm = reinterpret_cast<float*>(smem);
+    f32x4* co = reinterpret_cast<f32x4*>(cm + C::NW * 128);
+    wait_vm<0>();
+    __syncthreads();
+    cm[wave * 128 + lane] = m;
+    cm[wave * 128 + 64 + lane] = L;
+#pragma unroll
+    for (int u = 0; u < 4 * DT; u++)
+      co[(wave * 4 * DT + u) * 64 + lane] =
+          f32x4{o[u / 4][4 * (u % 4)], o[u / 4][4 * (u % 4) + 1], o[u / 4][4 * (u % 4) + 2], o[u / 4][4 * (u % 4) + 3]};
+    __syncthreads();
+    m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NKW; w++) m = fmaxf(m, cm[(w * NQW + qg) * 128 + lane]);
+    const float mb = base_of(m);
+    float f[NKW];
+    L = 0.f;
+#pragma unroll
+    for (int w = 0; w < NKW; w++) {
+      f[w] = __builtin_amdgcn_exp2f(cm[(w * NQW + qg) * 128 + lane] - mb);
+      L += cm[(w * NQW + qg) * 128 + 64 + lane] * f[w];
+    }
+    if (row >= R) return;
+    aim();
+    for (int u = kw; u < 4 * DT; u += NKW) {
+      f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < NKW; w++) {
+        const f32x4 y = co[((w * NQW + qg) * 4 * DT + u) * 64 + lane];
+#pragma unroll
+        for (int r = 0; r < 4; r++) a[r] += y[r] * f[w];
+      }
+      put4(t, 8 * u + 4 * hk, a[0], a[1], a[2], a[3]);
+    }
+  } else {
+    if (row >= R) return;
+    aim();
+#pragma unroll
+    for (int u = 0; u < 4 * DT; u++)
+      put4(t, 8 * u + 4 * hk, o[u / 4][4 * (u % 4)], o[u / 4][4 * (u % 4) + 1], o[u / 4][4 * (u % 4) + 2],
+           o[u / 4][4 * (u % 4) + 3]);
+  }
+}
+
+// The dispatcher sends workgroup i to XCD i % 8; neighbouring items (the row tiles over the same keys) go to one XCD, whose
+// L2 then holds those keys once.
+__device__ __forceinline__ long on_xcd(long i, long n) {
+  const long per = n / 8, rem = n % 8, x = i % 8, idx = i / 8;
+  return x < rem ? x * (per + 1) + idx : rem * (per + 1) + (x - rem) * per + idx;
+}
+
+template <int D, int NQW, int NKW, int KB, int S>
+__global__ __launch_bounds__(64 * NQW * NKW) void prefix_tile_kernel(Args p) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[Tile<D, NQW, NKW, KB, S>::BYTES];
+  tile_body<D, NQW, NKW, KB, S, true>(p, on_xcd(blockIdx.x, p.na), smem);
+}
+template <int D, int NQW, int NKW, int KB, int S>
+__global__ __launch_bounds__(64 * NQW * NKW) void prefix_both_kernel(Args p) {
+  constexpr int A = Tile<D, NQW, NKW, KB, S>::BYTES, B = rows_lds<D, NQW * NKW>();
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[A > B ? A : B];
+  if (blockIdx.x < p.na) tile_body<D, NQW, NKW, KB, S, false>(p, on_xcd(blockIdx.x, p.na), smem);
+  else rows_body<D, NQW * NKW, false>(p, blockIdx.x - p.na, smem);
+}
+
+// The shares of one row: 256 / WPR threads... one workgroup has 4 / WPR rows of WPR waves; D / 4 threads with 4 columns each
+// form a group, and the groups take the shares in turn, in a fixed order.
+template <int D, int WPR>
+__global__ __launch_bounds__(256) void prefix_join_kernel(Args p, long rows) {
+  constexpr int TD = D / 4, NT = 64 * WPR, NG = NT / TD, RPB = 256 / NT;
+  __shared__ f32x4 so[RPB][NG][TD];
+  __shared__ float red[RPB][2][WPR];
+  const int tid = threadIdx.x % NT, rb = threadIdx.x / NT, wave = tid >> 6, d = tid % TD, grp = tid / TD;
+  const long at = (long)blockIdx.x * RPB + rb;  // (prefix and key head, row); rows beyond the last do the last again
+  const int M = p.G * p.Tq, R = p.S * M;
+  const long ic = min(at, rows - 1);
+  const int cell = (int)(ic / R), row = (int)(ic % R), n = cell / p.H, h = cell % p.H;
+  // the row's shares: spa of the tile kernel (if any), then spb of the 16-row kernel
+  const bool seq = p.oa && !p.ob;  // tiles of one sequence
+  const long ca = seq ? (long)cell * p.S + row / M : cell;
+  const int ra = seq ? row % M : row;
+  const int na = p.oa ? p.spa : 0, nr = na + (p.ob ? p.spb : 0);
+  auto rec_a = [&](int s) { return (ca * p.spa + s) * p.nta + ra / p.rwa; };
+  auto rec_b = [&](int s) { return ((long)cell * p.spb + s - na) * p.ntb + row / 16; };
+  auto stat = [&](int s, int which) {
+    return s < na ? p.ma[rec_a(s) * 2 * p.rwa + which * p.rwa + ra % p.rwa] : p.mb[rec_b(s) * 32 + which * 16 + row % 16];
+  };
+  float m = -INFINITY;
+  for (int s = tid; s < nr; s += NT) m = fmaxf(m, stat(s, 0));
+  m = wave_max(m);
+  if (WPR > 1) {
+    if ((tid & 63) == 0) red[rb][0][wave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WPR; w++) m = fmaxf(m, red[rb][0][w]);
+  }
+  const float mb = base_of(m);
+  float l = 0.f;
+  for (int s = tid; s < nr; s += NT) l += stat(s, 1) * __builtin_amdgcn_exp2f(stat(s, 0) - mb);
+  l = wave_total(l);
+  if (WPR > 1) {
+    if ((tid & 63) == 0) red[rb][1][wave] = l;
+    __syncthreads();
+    l = 0.f;
+#pragma unroll
+    for (int w = 0; w < WPR; w++) l += red[rb][1][w];
+  }
+  f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = grp; s < nr; s += NG) {
+    const float f = __builtin_amdgcn_exp2f(stat(s, 0) - mb);
+    const float* src = s < na ? p.oa + (rec_a(s) * p.rwa + ra % p.rwa) * D : p.ob + (rec_b(s) * 16 + row % 16) * D;
+    const f32x4 y = *reinterpret_cast<const f32x4*>(src + 4 * d);
+#pragma unroll
+    for (int e = 0; e < 4; e++) a[e] += y[e] * f;
+  }
+  so[rb][grp][d] = a;
+  __syncthreads();
+  if (grp || at >= rows) return;
+#pragma unroll
+  for (int u = 1; u < NG; u++) a += so[rb][u][d];
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  *reinterpret_cast<u32x2*>(out_row(p, n, h, row, D) + 4 * d) = u32x2{pack2(a[0] * inv, a[1] * inv), pack2(a[2] * inv, a[3] * inv)};
+}
+
+// How a problem is cut. kind 0: rows, 1: both, 2: tiles.
+struct Plan {
+  int kind, nqw, nkw, nta, spa, nwb, ntb, spb;
+  long na, nb;  // workgroups
+};
+long cdiv(long a, long b) { return (a + b - 1) / b; }
+Plan plan(int N, int S, int H, int G, int Tq, int P, int T, int D) {
+  Plan q = {};
+  const long M = (long)G * Tq, R = S * M, cells = (long)N * H;
+  const auto clampl = [](long v, long lo, long hi) { return v < lo ? lo : v > hi ? hi : v; };
+  q.spa = q.spb = 1;
+  const long seqs = clampl(cdiv(16, M), 1, S);  // in a 16-row tile, nearly
+  if (M >= 32) {
+    q.kind = 2;
+    const auto wgs = [&](int rw) { return cells * S * cdiv(M, rw); };
+    if (wgs(128) >= 512) q.nqw = 4, q.nkw = 1;
+    else if (wgs(128) >= 192) q.nqw = 4, q.nkw = 2;
+    else if (wgs(64) >= 192) q.nqw = 2, q.nkw = 4;
+    else q.nqw = 1, q.nkw = 4;
+    q.nta = (int)cdiv(M, 32 * q.nqw);
+    const long w = cells * S * q.nta, nb = cdiv(P, 64) + cdiv(T, 64);
+    q.spa = (int)clampl(w <= 128 ? 256 / w : 1, 1, clampl(nb / 16, 1, 1024));
+    q.na = w * q.spa;
+    return q;
+  }
+  q.ntb = (int)cdiv(R, 16);
+  const long wb = cells * q.ntb;
+  if (R <= 32 || P <= 64) {
+    q.kind = 0;
+    const long nb = cdiv(P, 32) + seqs * cdiv(T, 32);
+    q.spb = (int)clampl(512 / wb, 1, clampl(nb / 16, 1, 1024));
+    q.nwb = wb * q.spb <= 256 ? 8 : 4;
+    q.nb = wb * q.spb;
+    return q;
+  }
+  q.kind = 1;
+  q.nqw = R <= 64 ? 2 : 4, q.nkw = R <= 64 ? 4 : 2;
+  q.nta = (int)cdiv(R, 32 * q.nqw);
+  const long wa = cells * q.nta;
+  q.spa = (int)clampl(256 / wa, 1, clampl(cdiv(P, 64) / 8, 1, 1024));
+  q.na = wa * q.spa;
+  const long nb = seqs * cdiv(T, 32);
+  q.spb = (int)clampl(256 / wb, 1, clampl(nb / 16, 1, 1024));
+  q.nwb = 8;
+  q.nb = wb * q.spb;
+  return q;
+}
+bool shares(const Plan& q) { return q.kind == 1 || q.spa > 1 || q.spb > 1; }
+long ws_floats(const Plan& q, int D) {
+  return shares(q) ? q.na * 32 * q.nqw * (D + 2) + q.nb * 16 * (D + 2) : 0;
+}
+
+template <int D>
+hipError_t launch(hipStream_t st, const Args& a, const Plan& q) {
+  const auto go = [&](auto kern, int waves) {
+    hipLaunchKernelGGL(kern, dim3((unsigned)(q.na + q.nb)), dim3(64 * waves), 0, st, a);
+  };
+  if (q.kind == 0) {
+    if (q.nwb == 8) go(prefix_rows_kernel<D, 8>, 8);
+    else go(prefix_rows_kernel<D, 4>, 4);
+  } else if (q.kind == 1) {
+    if (q.nqw == 4) go(prefix_both_kernel<D, 4, 2, 64, 2>, 8);
+    else go(prefix_both_kernel<D, 2, 4, 128, 2>, 8);
+  } else if (q.nqw == 4) {
+    if (q.nkw == 1) go(prefix_tile_kernel<D, 4, 1, 64, 2>, 4);
+    else go(prefix_tile_kernel<D, 4, 2, 64, 2>, 8);
+  } else if (q.nqw == 2) {
+    go(prefix_tile_kernel<D, 2, 4, 128, 2>, 8);
+  } else {
+    go(prefix_tile_kernel<D, 1, 4, 128, 2>, 4);
+  }
+  hipError_t e = hipGetLastError();
+  if (e == hipSuccess && shares(q)) {
+    const long rows = (long)a.N * a.S * a.H * a.G * a.Tq;
+    if (q.spa + q.spb > 16)
+      hipLaunchKernelGGL((prefix_join_kernel<D, 4>), dim3((unsigned)rows), dim3(256), 0, st, a, rows);
+    else
+      hipLaunchKernelGGL((prefix_join_kernel<D, 1>), dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, st, a, rows);
+    e = hipGetLastError();
+  }
+  return e;
+}
+
+bool sizes_ok(int N, int S, int H, int G, int Tq, int P, int T) {
+  return N >= 1 && S >= 1 && H >= 1 && G >= 1 && Tq >= 1 && P >= 0 && T >= 0 && P <= 0x7fffff00 && T <= 0x7fffff00 &&
+         (long)N * S <= 0x7fffff && (long)N * S * H <= 0x7fffff && (long)G * Tq <= 0x7fffff00L &&
+         (long)S * G * Tq <= 0x7fffff00L && (double)N * S * H * G * Tq <= 16777215.0 * 4;
+}
+
+}  // namespace
+
+extern "C" long mx_sdpa_prefix_ws(int N, int S, int H, int G, int Tq, int P, int T, int D) {
+  if (!sizes_ok(N, S, H, G, Tq, P, T) || (D != 64 && D != 128)) return 0;
+  return ws_floats(plan(N, S, H, G, Tq, P, T, D), D);
+}
+
+// t: 0 rows, 1 both, 2 tiles; query and key waves of the tile kernel; its runs; waves and runs of the 16-row kernel.
+extern "C" void mx_sdpa_prefix_tiling(int N, int S, int H, int G, int Tq, int P, int T, int D, int* t) {
+  for (int i = 0; i < 6; i++) t[i] = 0;
+  if (!sizes_ok(N, S, H, G, Tq, P, T) || (D != 64 && D != 128)) return;
+  const Plan q = plan(N, S, H, G, Tq, P, T, D);
+  t[0] = q.kind, t[1] = q.nqw, t[2] = q.nkw, t[3] = q.kind ? q.spa : 0, t[4] = q.nwb, t[5] = q.kind < 2 ? q.spb : 0;
+}
+
+extern "C" int mx_sdpa_prefix(hipStream_t st, const uint16_t* q, long sq_b, long sq_h, long sq_t, const uint16_t* pk, long spk_n,
+                              long spk_h, long spk_t, const uint16_t* pv, long spv_n, long spv_h, long spv_t, const uint16_t* k,
+                              long sk_b, long sk_h, long sk_t, const uint16_t* v, long sv_b, long sv_h, long sv_t, uint16_t* o,
+                              long so_b, long so_t, int N, int S, int H, int G, int Tq, int D, int P, int T, const int* plen,
+                              long plen_s, int pbase, const int* len, long len_s, int base, int causal, float scale,
+                              float* part, long part_elems) {
+  if (!q || !o || (P > 0 && (!pk || !pv)) || (T > 0 && (!k || !v))) return MX_ENULL;
+  if (D != 64 && D != 128) return MX_EBADCFG;
+  if (!sizes_ok(N, S, H, G, Tq, P, T)) return MX_ESHAPE;
+  if (!(scale > 0.f) || !(scale * 1.4426950408889634f < INFINITY)) return MX_ESHAPE;
+  if ((sq_b | sq_h | sq_t | spk_n | spk_h | spk_t | spv_n | spv_h | spv_t | sk_b | sk_h | sk_t | sv_b | sv_h | sv_t) % 8 ||
+      (so_b | so_t) % 4)
+    return MX_ESHAPE;
+  // a block's rows are addressed by 32-bit byte offsets from its first
+  const long far = 0x7fffffL;
+  if (spk_t < 0 || spv_t < 0 || sk_t < 0 || sv_t < 0 || spk_t > far || spv_t > far || sk_t > far || sv_t > far) return MX_ESHAPE;
+  if (((uintptr_t)q | (uintptr_t)pk | (uintptr_t)pv | (uintptr_t)k | (uintptr_t)v) & 15 || ((uintptr_t)o & 7) ||
+      ((uintptr_t)plen & 3) || ((uintptr_t)len & 3))
+    return MX_ELAYOUT;
+  const Plan pl = plan(N, S, H, G, Tq, P, T, D);
+  if (pl.na + pl.nb > 0x7fffffL) return MX_ESHAPE;  // 2^32 threads in a grid
+  const long need = ws_floats(pl, D);
+  if (need && (!part || part_elems < need || ((uintptr_t)part & 15))) return MX_ESPLIT;
+  Args a{q, sq_b, sq_h, sq_t, {pk, spk_n, spk_h, (int)spk_t}, {pv, spv_n, spv_h, (int)spv_t}, {k, sk_b, sk_h, (int)sk_t}, {v, sv_b, sv_h, (int)sv_t},
+         o, so_b, so_t, plen, len, plen_s, len_s, pbase, base, P, T, N, S, H, G, Tq, causal, scale * 1.4426950408889634f,
+         32 * pl.nqw, pl.nta, pl.spa, 16, pl.ntb, pl.spb, pl.na, nullptr, nullptr, nullptr, nullptr};
+  if (need) {
+    const long fa = pl.na * a.rwa, fb = pl.nb * 16;
+    if (pl.na) a.oa = part, a.ma = part + fa * D + fb * D;
+    if (pl.nb) a.ob = part + fa * D, a.mb = part + fa * D + fb * D + 2 * fa;
+  }
+  const hipError_t e = D == 64 ? launch<64>(st, a, pl) : launch<128>(st, a, pl);
+  return e == hipSuccess ? MX_OK : MX_ELAUNCH;
+}

@@ -21,16 +21,26 @@ __device__ __forceinline__ void rot_pair(float a, float b, float c, float s, flo
 // head's q, k and v (dims 16u .. 16u + 15 of the output): units 0 and 1 rotate the pairs j = 8u .. 8u + 7
 // (a = x[j] from input chunk u, b = x[16 + j] from chunk u + 2), units 2 and 3 pass dims 32 .. 63 through. Every load
 // of a thread is issued before its arithmetic, so a row is one memory round trip.
+// AT: the cache rows of sequence b start at pos0 + at[b * at_s], read here, and the row's position is rot0 more than that; rows
+// outside the cache or the table write nothing to it.
+template <bool AT>
 __global__ __launch_bounds__(128) void rope_kv_kernel(const uint16_t* __restrict__ qkv, long ldq,
                                                       const float* __restrict__ cs, uint16_t* __restrict__ q_out,
                                                       uint16_t* __restrict__ kc, uint16_t* __restrict__ vc, int n,
-                                                      int H, int ctx, int pos0, int nslots, int bcast) {
+                                                      int H, int ctx, int pos0, int nslots, int bcast,
+                                                      const int* __restrict__ at, long at_s, int rot0, int ncs) {
   const int row = blockIdx.x;  // b * n + t
   const int b = row / n, t = row % n;
-  const int pos = pos0 + t;
+  int pos = pos0 + t, rot = pos;
   const uint16_t* src = qkv + (long)row * ldq;
-  const float* cp = cs + (long)pos * 32;  // (cos, sin) interleaved per frequency: [16][2]
-  const int s0 = bcast ? 0 : b, s1 = bcast ? nslots : b + 1;
+  int s0 = bcast ? 0 : b, s1 = bcast ? nslots : b + 1;
+  if constexpr (AT) {
+    const long p = (long)pos0 + at[b * at_s] + t, r = p + rot0;
+    if (p < 0 || p >= ctx || r < 0 || r >= ncs) s1 = s0;
+    pos = (int)min(max(p, 0L), ctx - 1L);
+    rot = (int)min(max(r, 0L), ncs - 1L);
+  }
+  const float* cp = cs + (long)rot * 32;  // (cos, sin) interleaved per frequency: [16][2]
   for (int i = threadIdx.x; i < H * 4; i += 128) {
     const int h = i >> 2, u = i & 3;
     const uint16_t* qh = src + h * 64;
@@ -90,7 +100,21 @@ extern "C" int mx_rope_kv(hipStream_t st, const uint16_t* qkv, long ldq, const f
   if (bcast ? (B != 1 || nslots < 1) : (nslots < B)) return MX_ESHAPE;
   if (((uintptr_t)qkv | (uintptr_t)cs | (uintptr_t)q_out | (uintptr_t)kc | (uintptr_t)vc) & 15 || ldq % 8)
     return MX_ELAYOUT;
-  hipLaunchKernelGGL(rope_kv_kernel, dim3(B * n), dim3(128), 0, st, qkv, ldq, cs, q_out, kc, vc, n, H, ctx, pos0,
-                     nslots, bcast);
+  hipLaunchKernelGGL(rope_kv_kernel<false>, dim3(B * n), dim3(128), 0, st, qkv, ldq, cs, q_out, kc, vc, n, H, ctx, pos0,
+                     nslots, bcast, nullptr, 0L, 0, 0);
+  return hipGetLastError() == hipSuccess ? MX_OK : MX_ELAUNCH;
+}
+
+// The same for B sequences whose rows start at cache row at[b * at_s] (device memory), at rotary position rot0 + the row; cs
+// has ncs positions, the caches [B][H][ctx][64]. Rows outside the cache or the table are dropped (their q takes the nearest
+// position of the table).
+extern "C" int mx_rope_kv_at(hipStream_t st, const uint16_t* qkv, long ldq, const float* cs, int ncs, uint16_t* q_out,
+                             uint16_t* kc, uint16_t* vc, int B, int n, int H, int ctx, const int* at, long at_s, int rot0) {
+  if (!qkv || !cs || !q_out || !kc || !vc || !at) return MX_ENULL;
+  if (B < 1 || n < 1 || H < 1 || H > 65535 || ctx < 1 || ncs < 1 || ldq < 3L * H * 64 || (long)B * n > 0xffffffL) return MX_ESHAPE;
+  if (((uintptr_t)qkv | (uintptr_t)cs | (uintptr_t)q_out | (uintptr_t)kc | (uintptr_t)vc) & 15 || ldq % 8 || ((uintptr_t)at & 3))
+    return MX_ELAYOUT;
+  hipLaunchKernelGGL(rope_kv_kernel<true>, dim3(B * n), dim3(128), 0, st, qkv, ldq, cs, q_out, kc, vc, n, H, ctx, 0, B, 0, at,
+                     at_s, rot0, ncs);
   return hipGetLastError() == hipSuccess ? MX_OK : MX_ELAUNCH;
 }

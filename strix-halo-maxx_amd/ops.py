@@ -1015,6 +1015,12 @@ class KV8Cache:
                      0 if cs is None else cs.shape[0], *qa)
         return q_out
 
+    def reorder(self, parent, n=None, first=0):
+        """Slot g W + w becomes a copy of slot g W + parent[g, w] (reorder_slots), over the blocks of 64 tokens that tokens first ..
+        n - 1 lie in."""
+        for t in (self.kc, self.vc, self.ks, self.vs):
+            reorder_slots(t[None], parent, n, first, self.BLOCK)
+
     def read(self, n=None):
         """(k, v), each (slots, heads, n, hd) bf16: what positions 0 .. n - 1 (default: all) hold, exact."""
         n = self.ctx if n is None else int(n)
@@ -1091,6 +1097,207 @@ def sdpa_kv8_tiling(B, heads, G, Tq, ctx, hd):
     t = (ctypes.c_int * 4)()
     _lib.load().mx_kv8_sdpa_tiling(B, heads, G, Tq, ctx, hd, ctypes.cast(t, ctypes.c_void_p))
     return tuple(t)
+
+
+# ------------------------------------------------------------------------------------------------ shared prefixes, beams
+def _keys4(t, name, dev, B, H, D):
+    """k or v (B, H, T, D) as the kernel takes it (copied if its rows are not 16-byte aligned), and its strides."""
+    if t.dim() != 4 or t.shape[0] != B or t.shape[1] != H or t.shape[3] != D:
+        raise ValueError(f"{name} must be ({B}, {H}, keys, {D}), got {tuple(t.shape)}")
+    _need(t, name, dev)
+    s = t.stride()
+    if s[3] != 1 or (s[0] | s[1] | s[2]) % 8 or s[2] >= 0x800000 or t.data_ptr() % 16:
+        s = _steps(t)
+        if s[3] != 1 or (s[0] | s[1] | s[2]) % 8 or s[2] >= 0x800000 or t.data_ptr() % 16:
+            t = t.clone(memory_format=torch.contiguous_format)
+            s = t.stride()
+    return t, (t.data_ptr() if t.shape[2] else None), s
+
+
+_PREFIX_WS = {}  # floats of workspace of a shape (a few integers per shape a program runs)
+
+
+def sdpa_prefix(q, pk, pv, k, v, kv_len=None, prefix_len=None, out=None, scale=None, causal=True):
+    """Attention of sequences that share prefixes: q (B, Hq, Tq, D), prefixes pk, pv (N, H, P, D), own keys k, v (B, H, T, D); D 64
+    or 128, Hq a multiple of H (query head h reads key head h / (Hq / H)), B of N: sequence b has prefix b // (B / N), which is
+    stored and read once for all of them. Returns out (B, Tq, Hq * D).
+
+    Query i sees keys 0 .. prefix_len_n - 1 of its prefix and, of its own first kv_len_b keys, those up to its own: the queries
+    are the sequence's last Tq tokens, key t is visible iff t <= kv_len_b - Tq + i (causal=False: all kv_len_b). A row that sees
+    no key is 0. kv_len, prefix_len: an int, or an int32 tensor (B,) / (N,) read on the device (clamped to 0 .. T / 0 .. P);
+    None: all. out may lie in q's memory. Scores (times scale) have to stay below 2^29 in size."""
+    if q.dim() != 4 or pk.dim() != 4 or pk.shape != pv.shape or k.shape != v.shape:
+        raise ValueError(f"q, pk, pv, k, v: {tuple(q.shape)}, {tuple(pk.shape)}, {tuple(pv.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    B, Hq, Tq, D = q.shape
+    N, H, P = pk.shape[:3]
+    if D not in (64, 128) or N < 1 or H < 1 or B % N or Hq % H or Hq < 1:
+        raise ValueError(f"{B} sequences of {Hq} heads of dim {D} over {N} prefixes of {H} heads")
+    dev = q.device
+    _need(q, "q", dev)
+    pk, pkp, spk = _keys4(pk, "pk", dev, N, H, D)
+    pv, pvp, spv = _keys4(pv, "pv", dev, N, H, D)
+    k, kp, sk = _keys4(k, "k", dev, B, H, D)
+    v, vp, sv = _keys4(v, "v", dev, B, H, D)
+    T = k.shape[2]
+    lp, ls, l0 = _where(T if kv_len is None else kv_len, B, dev, "kv_len")
+    pp, ps, p0 = _where(P if prefix_len is None else prefix_len, N, dev, "prefix_len")
+    if not 0 <= l0 <= T or not 0 <= p0 <= P:
+        raise ValueError(f"kv_len {l0} of {T} keys, prefix_len {p0} of {P}")
+    sc = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < sc <= 2.0 ** 127:  # the kernel multiplies by scale log2(e), a float
+        raise ValueError(f"scale {sc} must be positive and finite, at most 2^127")
+    given = out is not None
+    if not given:
+        out = torch.empty(B, Tq, Hq * D, device=dev, dtype=BF)
+        so = out.stride()
+    else:
+        _need(out, "out", dev)
+        so = _steps(out)
+        if out.shape != (B, Tq, Hq * D) or so[2] != 1 or (so[0] | so[1]) % 4 or out.data_ptr() % 8:
+            raise ValueError(f"out must be ({B}, {Tq}, {Hq * D}) with 8-byte aligned rows of unit stride")
+    if not out.numel():
+        return out
+    if given and not _apart(q, out):
+        q = q.clone()  # a row's output may lie over another's query
+    s = _steps(q)
+    if s[3] != 1 or (s[0] | s[1] | s[2]) % 8 or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+        s = q.stride()
+    shape = (N, B // N, H, Hq // H, Tq, P, T, D)
+    need = _PREFIX_WS.get(shape)
+    if need is None:
+        need = _PREFIX_WS[shape] = _lib.load().mx_sdpa_prefix_ws(*shape)
+    part = torch.empty(need, device=dev, dtype=torch.float32) if need else None
+    _call_on(dev, "mx_sdpa_prefix", q.data_ptr(), s[0], s[1], s[2], pkp, spk[0], spk[1], spk[2], pvp, spv[0], spv[1], spv[2],
+             kp, sk[0], sk[1], sk[2], vp, sv[0], sv[1], sv[2], out.data_ptr(), so[0], so[1], N, B // N, H, Hq // H, Tq, D, P, T,
+             pp, ps, p0, lp, ls, l0, int(causal), sc, ptr(part), need)
+    return out
+
+
+def sdpa_prefix_tiling(N, S, heads, G, Tq, P, T, hd):
+    """How sdpa_prefix cuts N prefixes of S sequences each, G query heads per key head: (0 rows / 1 both / 2 tiles, query and key
+    waves and runs of the tile kernel, waves and runs of the 16-row kernel)."""
+    import ctypes
+    t = (ctypes.c_int * 6)()
+    _lib.load().mx_sdpa_prefix_tiling(N, S, heads, G, Tq, P, T, hd, ctypes.cast(t, ctypes.c_void_p))
+    return tuple(t)
+
+
+def beam_select(logits, scores, k=None, done=None, eos=None):
+    """Beam search's selection: logits (B, W, V) bf16 or fp32 of W beams with scores (B, W) fp32. Returns (score, parent, token,
+    done), each (B, k) (k: default W): the k largest of scores[b, w] + log_softmax(logits[b, w])[v] in falling order, equal ones
+    by the lowest beam, then the lowest token; parent = w, token = v (int32).
+
+    A finished beam (done (B, W) bool) offers eos alone, at its score; the returned done says which hypotheses end in eos (None
+    without eos). A beam whose score is not finite, or whose logits hold NaN or +infinity or nothing above -infinity, offers
+    nothing, and neither does a logit of -infinity (a score of -infinity, say, keeps the copies of a first beam out). Places that
+    are left hold score -infinity, parent 0, token eos (0 without), done. W and k at most 64."""
+    if logits.dim() != 3 or logits.dtype not in (BF, torch.float32):
+        raise ValueError(f"logits must be (B, W, V) in bf16 or fp32, got {tuple(logits.shape)} {logits.dtype}")
+    B, W, V = logits.shape
+    dev = logits.device
+    k = W if k is None else int(k)
+    if not (1 <= W <= 64 and 1 <= k <= 64 and V >= 1):
+        raise ValueError(f"{W} beams over {V} tokens, {k} to select: at most 64 of each, at least 1")
+    _need(scores, "scores", dev, torch.float32)
+    if scores.shape != (B, W):
+        raise ValueError(f"scores must be ({B}, {W}), got {tuple(scores.shape)}")
+    e = -1 if eos is None else int(eos)
+    if eos is not None and not 0 <= e < V:
+        raise ValueError(f"eos {e} outside the {V} tokens")
+    if done is not None:
+        if eos is None:
+            raise ValueError("done goes with eos")
+        _need(done, "done", dev, torch.bool)
+        if done.shape != (B, W):
+            raise ValueError(f"done must be ({B}, {W}), got {tuple(done.shape)}")
+        done = done.contiguous()
+    scores = scores.contiguous()
+    if logits.stride(2) != 1 and V > 1:
+        logits = logits.contiguous()
+    o = torch.empty(3, B, k, device=dev, dtype=torch.int32)
+    od = None if eos is None else torch.empty(B, k, device=dev, dtype=torch.bool)
+    score, parent, token = o.unbind()
+    score = score.view(torch.float32)
+    if B:
+        n = _lib.load().mx_beam_select_ws(B, W, V, k)
+        ws = torch.empty(n, device=dev, dtype=torch.uint8)
+        p, step = o.data_ptr(), 4 * B * k
+        _call_on(dev, "mx_beam_select", logits.data_ptr(), int(logits.dtype != BF), logits.stride(0), logits.stride(1),
+                 scores.data_ptr(), ptr(done), e, B, W, V, k, p, p + step, p + 2 * step, ptr(od), ws.data_ptr(), n)
+    return score, parent, token, od
+
+
+def _disjoint(t):
+    """Whether no two elements of t share memory (by its strides, largest last; sufficient)."""
+    end = 1
+    for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if s < end:
+            return False
+        end = s * (n - 1) + end
+    return True
+
+
+def reorder_slots(x, parent, n=None, first=0, unit=1):
+    """Reorders the slots of a cache in place: x (L, slots, H, T, ...), whose rows x[l, s, h, t] are contiguous, any type; parent
+    (G, W) int32, G W = slots (or (slots,)): slot g W + w becomes a copy of slot g W + parent[g, w], which may be any of its group,
+    several times the same; values outside 0 .. W - 1 leave their slot. Only rows first .. n - 1 move, n an int or an int32 tensor
+    (slots,) of the rows that each slot holds (a slot takes as many as its parent has; None: all T); every other row stays. unit:
+    tokens per row (first and n count tokens; the row that token `first` lies in moves). W at most 64. Returns x."""
+    if x.dim() < 4:
+        raise ValueError(f"x must be (L, slots, H, T, ...), got {tuple(x.shape)}")
+    N, S, H, T = x.shape[:4]
+    dev = x.device
+    _need(parent, "parent", dev, torch.int32)
+    if parent.dim() == 1:
+        parent = parent[None]
+    if parent.dim() != 2 or parent.numel() != S or not 1 <= parent.shape[1] <= 64:
+        raise ValueError(f"parent must be (G, W) with G W = {S} and W at most 64, got {tuple(parent.shape)}")
+    G, W = parent.shape
+    first, unit = int(first), int(unit)
+    if first < 0 or unit < 1:
+        raise ValueError(f"first {first} must not be negative, unit {unit} at least 1")
+    lp, ls, l0 = _where(T * unit if n is None else n, S, dev, "n")
+    if not 0 <= l0 <= T * unit:
+        raise ValueError(f"n {l0} outside 0 .. {T * unit}")
+    if not x.is_contiguous():
+        if not _disjoint(x) or (x.dim() > 4 and not x[0, 0, 0, 0].is_contiguous()):
+            raise ValueError("x must not overlap itself, and its rows must be contiguous")
+    if x.numel():
+        es, s = x.element_size(), _steps(x)
+        _call_on(dev, "mx_reorder_slots", x.data_ptr(), s[0] * es, s[1] * es, s[2] * es, s[3] * es, N, G, W, H, T,
+                 x[0, 0, 0, 0].numel() * es, parent.data_ptr(), *parent.stride(), lp, ls, _int32(l0, "n"), unit, first // unit)
+    return x
+
+
+def rope_kv_at(qkv, cs, kc, vc, at, rot0=0):
+    """The text decoder's rotary embedding and K / V write for rows whose place is on the device: qkv (B, n, >= 3 H 64) fused rows
+    (q | k | v), cs the (positions, 16, 2) table, caches kc, vc (B, H, ctx, 64). Row t of sequence b is written at cache row
+    at[b] + t (int32) and rotated for position rot0 + at[b] + t; rows outside the cache or the table are dropped. Returns the
+    rotated q (B, H, n, 64)."""
+    if kc.dim() != 4 or kc.shape != vc.shape or kc.shape[3] != 64 or qkv.dim() != 3 or qkv.shape[0] != kc.shape[0]:
+        raise ValueError(f"qkv {tuple(qkv.shape)}, caches {tuple(kc.shape)}, {tuple(vc.shape)}: need (B, n, 3 H 64), (B, H, ctx, 64)")
+    B, H, ctx = kc.shape[:3]
+    n, dev = qkv.shape[1], qkv.device
+    _need(qkv, "qkv", dev)
+    _need(kc, "kc", dev)
+    _need(vc, "vc", dev)
+    _need(cs, "cs", dev, torch.float32)
+    _need(at, "at", dev, torch.int32)
+    if cs.dim() != 3 or cs.shape[1:] != (16, 2) or cs.shape[0] < 1 or not cs.is_contiguous():
+        raise ValueError("cs must be a contiguous (positions, 16, 2) table")
+    if at.shape != (B,) or not kc.is_contiguous() or not vc.is_contiguous() or qkv.shape[2] < 3 * H * 64:
+        raise ValueError(f"at must be ({B},), the caches contiguous, qkv rows {3 * H * 64} wide")
+    q = torch.empty(B, H, n, 64, device=dev, dtype=BF)
+    if q.numel():
+        s = _steps(qkv)
+        if s[2] != 1 or s[1] % 8 or (B > 1 and n > 1 and s[0] != n * s[1]) or qkv.data_ptr() % 16:
+            qkv = qkv.clone(memory_format=torch.contiguous_format)
+            s = _steps(qkv)
+        ldq = s[1] if n > 1 else s[0] if B > 1 else qkv.shape[2]
+        _call_on(dev, "mx_rope_kv_at", qkv.data_ptr(), ldq, cs.data_ptr(), cs.shape[0], q.data_ptr(), kc.data_ptr(), vc.data_ptr(),
+                 B, n, H, ctx, at.data_ptr(), at.stride(0), int(rot0))
+    return q
 
 
 def gemm_tile(cfg):
