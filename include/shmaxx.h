@@ -388,27 +388,26 @@ int mx_decode_mk_layer_bytes(void);
  * sequences) and, of its own T rows, the first len_b; own key t is visible to query i iff not causal or t <= len_b - Tq + i:
  *   O[b, i, h] = sum softmax(scale <q, key>) value over the keys that the query sees, 0 where there are none.
  * Head dims D 64 and 128; G query heads per key head (query head h G + g reads key head h). q [N S][H G][Tq][D], pk / pv
- * [N][H][P][D], k / v [N S][H][T][D] by element strides (multiples of 8, unit stride along D, 16-byte aligned; row strides of
- * keys and values 0 .. 2^23 - 1), o [N S][Tq][H G D] (strides multiples of 4, 8-byte aligned). plen / len: device int32 with
+ * [N][H][P][D], k / v [N S][H][T][D] by element strides, strides[15] = {b, h, t} of q, pk, pv, k, v in turn (host memory;
+ * multiples of 8, unit stride along D, 16-byte aligned; row strides of keys and values 0 .. 2^23 - 1), o [N S][Tq][H G D] (strides multiples of 4, 8-byte aligned). plen / len: device int32 with
  * strides plen_s / len_s, added to pbase / base, or null; what lies outside 0 .. P / 0 .. T is clamped. P = 0 or T = 0: pk, pv
  * or k, v are not read. fp32 sums, weights rounded to bf16; scores (times scale) must stay below 2^29 in size. part: at least
  * mx_sdpa_prefix_ws floats, 16-byte aligned, one for each call that may run at the same time; not read from call to call.
- * N S H < 2^23, N S H G Tq < 2^26. mx_sdpa_prefix_tiling: t[6] = 0 rows, 1 both, 2 tiles; query and key waves and runs of the
- * tile kernel; waves and runs of the 16-row kernel. */
+ * N S H < 2^23, N S H G Tq < 2^24. mx_sdpa_prefix_tiling: t[6] = 0 rows, 1 both, 2 tiles; query and key waves and runs of the
+ * tile kernel; rows per workgroup and runs of the few-row kernel. */
 long mx_sdpa_prefix_ws(int N, int S, int H, int G, int Tq, int P, int T, int D);
 void mx_sdpa_prefix_tiling(int N, int S, int H, int G, int Tq, int P, int T, int D, int* t);
-int mx_sdpa_prefix(hipStream_t st, const uint16_t* q, long sq_b, long sq_h, long sq_t, const uint16_t* pk, long spk_n,
-                   long spk_h, long spk_t, const uint16_t* pv, long spv_n, long spv_h, long spv_t, const uint16_t* k, long sk_b,
-                   long sk_h, long sk_t, const uint16_t* v, long sv_b, long sv_h, long sv_t, uint16_t* o, long so_b, long so_t,
-                   int N, int S, int H, int G, int Tq, int D, int P, int T, const int* plen, long plen_s, int pbase,
-                   const int* len, long len_s, int base, int causal, float scale, float* part, long part_elems);
+int mx_sdpa_prefix(hipStream_t st, const uint16_t* q, const uint16_t* pk, const uint16_t* pv, const uint16_t* k,
+                   const uint16_t* v, uint16_t* o, const long* strides, long so_b, long so_t, int N, int S, int H, int G, int Tq,
+                   int D, int P, int T, const int* plen, long plen_s, int pbase, const int* len, long len_s, int base, int causal,
+                   float scale, float* part, long part_elems);
 /* Beam search's selection: of the values score[b, w] + x[b, w, v] - logsumexp(x[b, w, :]) of search b, the k largest in falling
  * order (equal ones: lowest w, then lowest v). A finished beam (done[b, w] != 0; done may be null) offers eos alone, at its
  * score. A beam whose score is not finite, or whose logits hold NaN or +infinity or nothing above -infinity, offers nothing;
  * neither does a logit of -infinity. x: bf16 or (fp32 != 0) float [B][W][V] by element strides sx_b, sx_w, unit stride along V;
  * score [B][W] float, done [B][W] bytes. Outputs [B][k]: o_score, o_parent (w), o_token (v), o_done (may be null: v == eos).
  * Places without a candidate: score -infinity, parent 0, token max(eos, 0), done 1. eos < 0: none (done must be null).
- * W <= 64, k <= 64, 24 (W ceil(V / 2048 or 8192) + k (k + 1) / 2) <= 64000. ws: mx_beam_select_ws bytes, 8-byte aligned, one
+ * W <= 64, k <= 64, 20 W ceil(V / 2048 or 8192) + 12 k (k + 1) < 64000. ws: mx_beam_select_ws bytes, 8-byte aligned, one
  * for each call that may run at the same time. */
 long mx_beam_select_ws(int B, int W, int V, int k);
 int mx_beam_select(hipStream_t st, const void* x, int fp32, long sx_b, long sx_w, const float* score, const uint8_t* done,

@@ -65,8 +65,7 @@ SIGNATURES = {
     "mx_rope_kv_at": [P, P, L, P, I, P, P, P, I, I, I, I, P, L, I],
     "mx_sdpa_prefix_ws": [I, I, I, I, I, I, I, I],
     "mx_sdpa_prefix_tiling": [I, I, I, I, I, I, I, I, P],
-    "mx_sdpa_prefix": [P, P, L, L, L, P, L, L, L, P, L, L, L, P, L, L, L, P, L, L, L, P, L, L, I, I, I, I, I, I, I, I, P, L, I, P, L,
-                       I, I, F, P, L],
+    "mx_sdpa_prefix": [P, P, P, P, P, P, P, P, L, L, I, I, I, I, I, I, I, I, P, L, I, P, L, I, I, F, P, L],
     "mx_beam_select_ws": [I, I, I, I],
     "mx_beam_select": [P, P, I, L, L, P, P, I, I, I, I, I, P, P, P, P, P, L],
     "mx_reorder_slots": [P, P, L, L, L, L, I, I, I, I, I, I, P, L, L, P, L, I, I, I],

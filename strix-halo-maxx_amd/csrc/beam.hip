@@ -15,7 +15,7 @@ namespace {
 
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));  // rows start at any element
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int MAXW = 64, MAXK = 64;
+constexpr int MAXW = 64, MAXK = 64, MT = 1024;  // MT: threads of the merge
 
 // Order-preserving bits of a float; -0 counts as 0. NONE: -infinity and below, no candidate.
 __device__ __forceinline__ uint32_t bits_of(float x) {
@@ -69,7 +69,7 @@ __device__ __forceinline__ void load8(const T* row, int v0, int V, float (&f)[8]
 // the threshold, go to LDS, where every one counts the larger ones: its rank.
 template <class T, int E>
 __global__ __launch_bounds__(256) void beam_parts_kernel(SelArgs p) {
-  extern __shared__ uint64_t cand[];
+  extern __shared__ uint64_t cand[];  // 4 ((k - 1) E + k)
   __shared__ int count;
   __shared__ float ms[4][2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -92,45 +92,41 @@ __global__ __launch_bounds__(256) void beam_parts_kernel(SelArgs p) {
   for (int e = 0; e < E; e++) s += __builtin_amdgcn_exp2f((f[e] - mb) * LOG2E);
   s = wave_total(s);
   if (lane == 0) ms[wave][0] = mw, ms[wave][1] = s;
-  // ---- the wave's threshold
-  uint32_t key[E], top = 0;
-#pragma unroll
-  for (int e = 0; e < E; e++) key[e] = bits_of(f[e]), top = max(top, key[e]);
+  // ---- the wave's threshold, from the lanes' maxima (bf16 logits: their upper half is all there is)
+  constexpr int LOW = sizeof(T) == 2 ? 16 : 0;
+  const uint32_t top = m > -INFINITY ? bits_of(m) >> LOW : 0u;  // (NaN is no maximum)
   uint32_t t = 0;
 #pragma unroll 4
-  for (int b = 31; b >= 0; b--) {
+  for (int b = 31 - LOW; b >= 0; b--) {
     const uint32_t c = t | (1u << b);
     if (__popcll(__ballot(top >= c)) >= p.k) t = c;
   }
-  t = max(t, NONE + 1);  // fewer than k lanes, or -infinity: every finite logit
+  // fewer than k lanes, or -infinity: every finite logit
+  const bool all = t <= NONE >> LOW;
+  const float tf = all ? -INFINITY : float_of(t << LOW | (LOW && !(t >> 15) ? 0xffffu : 0u));
   __syncthreads();
-  int equal = 0;  // of the lane's logits
-  if (top >= t) {
+  uint32_t eq = 0;  // of the lane's logits, a bit for each
+  if (m >= tf && m > -INFINITY) {
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      if (key[e] > t) cand[atomicAdd(&count, 1)] = (uint64_t)key[e] << 32 | ~(uint32_t)(v0 + 512 * (e / 8) + e % 8);
-      equal += key[e] == t;
+      if (f[e] > tf) cand[atomicAdd(&count, 1)] = (uint64_t)bits_of(f[e]) << 32 | ~(uint32_t)(v0 + 512 * (e / 8) + e % 8);
+      eq |= f[e] == tf ? 1u << e : 0u;
     }
   }
-  if (__any(equal != 0)) {
+  if (!all) {
     int left = p.k;  // places for logits that equal the threshold, in the order of their tokens
 #pragma unroll
     for (int i = 0; i < E / 8; i++) {
-      int n = 0;
-#pragma unroll
-      for (int e = 0; e < 8; e++) n += key[8 * i + e] == t;
-      uint64_t who = __ballot(n != 0);
+      const uint32_t mine = eq >> (8 * i) & 0xffu;
+      uint64_t who = __ballot(mine != 0);
       while (who && left > 0) {  // wave-uniform
         const int l = __ffsll((unsigned long long)who) - 1;
         who &= who - 1;
-        const int nl = __builtin_amdgcn_readlane(n, l);
-        if (lane == l) {
-          int free = left;
-#pragma unroll
-          for (int e = 0; e < 8; e++)
-            if (key[8 * i + e] == t && free-- > 0)
-              cand[atomicAdd(&count, 1)] = (uint64_t)t << 32 | ~(uint32_t)(v0 + 512 * i + e);
-        }
+        uint32_t bits = __builtin_amdgcn_readlane(mine, l);
+        const int nl = __popc(bits);
+        if (lane == l)
+          for (int j = left; bits && j > 0; j--, bits &= bits - 1)
+            cand[atomicAdd(&count, 1)] = (uint64_t)bits_of(tf) << 32 | ~(uint32_t)(v0 + 512 * i + __ffs(bits) - 1);
         left -= nl;
       }
     }
@@ -158,95 +154,137 @@ __global__ __launch_bounds__(256) void beam_parts_kernel(SelArgs p) {
   }
 }
 
-struct Cand {
-  double v;
-  uint64_t key;  // ~bits of the logit << 32 | token
-  uint32_t w;
-};
-__device__ __forceinline__ bool before(const Cand& a, const Cand& b) {
-  return a.v > b.v || (a.v == b.v && (a.w < b.w || (a.w == b.w && a.key < b.key)));
+// Order-preserving bits of a double (not NaN); 0 stands for no candidate.
+__device__ __forceinline__ uint64_t bits_of(double x) {
+  const uint64_t u = (uint64_t)__double_as_longlong(x + 0.);
+  return u ^ ((uint64_t)((int64_t)u >> 63) | 0x8000000000000000ull);
 }
+__device__ __forceinline__ double double_of(uint64_t b) {
+  return __longlong_as_double((int64_t)(b ^ ((b >> 63) ? 0x8000000000000000ull : ~0ull)));
+}
+typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
 
 // A list is a part's keys; a finished beam's is its one continuation. The k-th largest head of the lists bounds what can be
-// selected, and a key at place i of a list whose head has rank r has i + r larger ones.
-__global__ __launch_bounds__(256) void beam_merge_kernel(SelArgs p) {
-  extern __shared__ Cand sh[];  // heads [W segs], candidates [k (k + 1) / 2]
+// selected, and a key at place i of a list whose head has rank r has i + r larger ones: few keys are left to be ranked. What
+// takes the time is three rounds to memory, one after the other: the sums, the heads, the keys behind them.
+__global__ __launch_bounds__(MT) void beam_merge_kernel(SelArgs p) {
+  extern __shared__ u64x2 sh[];  // (value, key), key = ~logit's bits << 32 | token: the lists' heads [nl], then candidates, by rank of list
   __shared__ double base[MAXW];  // score - log of the sum
   __shared__ float big[MAXW];    // largest logit
-  __shared__ int state[MAXW];  // 0: offers nothing, 1: its logits, 2: eos
-  __shared__ int count;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nl = p.W * p.segs;
+  __shared__ int state[MAXW];    // 0: offers nothing, 1: its logits, 2: eos
+  __shared__ int best[MAXK], count;
+  const int tid = threadIdx.x, nl = p.W * p.segs;
   const long b = blockIdx.x;
-  Cand *head = sh, *cand = sh + nl;
+  u64x2 *head = sh, *cand = head + nl;
+  int* rank = reinterpret_cast<int*>(cand + p.k * (p.k + 1) / 2);  // of the heads, then the candidates' beams and ranks
+  int *cw = rank, *cr = rank + p.k * (p.k + 1) / 2;
   if (tid == 0) count = 0;
-  for (int w = wave; w < p.W; w += 4) {
-    const long row = b * p.W + w;
+  if (tid < p.k) best[tid] = -1;
+  const uint64_t* keys = p.keys + b * nl * p.k;
+  const uint64_t first = tid < nl ? keys[(long)tid * p.k] : 0;
+  int per = 64;  // threads of a row
+  while (per * p.W > MT) per /= 2;
+  const int w0 = tid / per, in = tid % per;
+  if (w0 < p.W) {
+    const long row = b * p.W + w0;
     const float score = p.score[row];
-    const bool alive = fabsf(score) < INFINITY, fin = p.done && p.done[row];
+    int st = fabsf(score) < INFINITY ? (p.done && p.done[row] ? 2 : 1) : 0;
     double c = score;
     float M = -INFINITY;
-    int st = alive ? (fin ? 2 : 1) : 0;
-    if (st == 1) {
+    if (st == 1) {  // the same for all threads of the row
       const float* s = p.stat + row * p.segs * 2;
-      for (int i = lane; i < p.segs; i += 64) M = fmaxf(M, s[2 * i]);
-      M = wave_max(M);
-      double sum = 0.;
-      for (int i = lane; i < p.segs; i += 64)
-        sum += s[2 * i] == -INFINITY ? (double)s[2 * i + 1] : (double)s[2 * i + 1] * exp((double)s[2 * i] - (double)M);
-#pragma unroll
-      for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
+      double sum = 0.;  // NaN stays: the comparisons leave the maximum alone
+      for (int i = in; i < p.segs; i += per) {
+        const float m = s[2 * i], x = s[2 * i + 1];
+        if (m > M) sum *= M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((M - m) * LOG2E), M = m;
+        sum += m == -INFINITY ? x : x * __builtin_amdgcn_exp2f((m - M) * LOG2E);
+      }
+      for (int d = per / 2; d; d >>= 1) {
+        const float m = __shfl_xor(M, d, 64);
+        const double x = __shfl_xor(sum, d, 64);
+        const float top = fmaxf(M, m), tb = top == -INFINITY ? 0.f : top;
+        sum = (M == -INFINITY ? sum : sum * __builtin_amdgcn_exp2f((M - tb) * LOG2E)) +
+              (m == -INFINITY ? x : x * __builtin_amdgcn_exp2f((m - tb) * LOG2E));
+        M = top;
+      }
       c = (double)score - log(sum);
       if (!(fabs(c) < INFINITY && fabsf(M) < INFINITY)) st = 0;  // NaN or +infinity among the logits, or nothing above -infinity
     }
-    if (lane == 0) base[w] = c, big[w] = M, state[w] = st;
+    if (in == 0) base[w0] = c, big[w0] = M, state[w0] = st;
   }
   __syncthreads();
-  auto key_of = [&](int l, int i) { return p.keys[(b * nl + l) * p.k + i]; };
-  auto value = [&](int w, uint64_t key) {
-    return Cand{((double)float_of((uint32_t)(key >> 32)) - (double)big[w]) + base[w], ~key, (uint32_t)w};
+  const auto value = [&](int w, uint64_t key) {
+    return u64x2{bits_of(((double)float_of((uint32_t)(key >> 32)) - (double)big[w]) + base[w]), ~key};
   };
-  for (int l = tid; l < nl; l += 256) {
+  for (int l = tid; l < nl; l += MT) {
     const int w = l / p.segs;
-    Cand c = {-INFINITY, ~0ull, ~0u};
-    if (state[w] == 2) {
-      if (l % p.segs == 0) c = Cand{base[w], (uint64_t)p.eos, (uint32_t)w};
-    } else if (state[w] == 1) {
-      const uint64_t key = key_of(l, 0);
-      if (key) c = value(w, key);
-    }
+    u64x2 c = {0, 0};
+    const uint64_t key = l < MT ? first : keys[(long)l * p.k];
+    if (state[w] == 2 && l == w * p.segs) c = u64x2{bits_of(base[w]), (uint64_t)p.eos};
+    if (state[w] == 1 && key) c = value(w, key);
     head[l] = c;
+    rank[l] = 0;
   }
   __syncthreads();
-  for (int l = tid; l < nl; l += 256) {
-    const Cand c = head[l];
-    if (c.v == -INFINITY) continue;
-    int rank = 0;
+  // ranks of the heads: every thread compares one with a share of the others
+  const int ways = nl < MT ? MT / nl : 1, share = (nl + ways - 1) / ways;
+  for (int e = tid; e < nl * ways; e += MT) {
+    const int l = e % nl, i0 = e / nl * share, i1 = min(i0 + share, nl), w = l / p.segs, l0 = w * p.segs, l1 = l0 + p.segs;
+    const u64x2 c = head[l];
+    if (!c.x) continue;
+    int r = 0;
 #pragma unroll 4
-    for (int i = 0; i < nl; i++) rank += before(head[i], c);
-    if (rank >= p.k) continue;
-    cand[atomicAdd(&count, 1)] = c;
-    const int w = l / p.segs;
-    if (state[w] == 2) continue;
-    for (int i = 1; i + rank < p.k; i++) {
-      const uint64_t key = key_of(l, i);
-      if (!key) break;
-      cand[atomicAdd(&count, 1)] = value(w, key);
+    for (int i = i0; i < i1; i++) {
+      const u64x2 y = head[i];
+      r += y.x > c.x || (y.x == c.x && (i < l0 || (i < l1 && y.y < c.y)));
     }
+    if (ways > 1) atomicAdd(rank + l, r);
+    else rank[l] = r;
+  }
+  __syncthreads();
+  for (int l = tid; l < nl; l += MT)
+    if (head[l].x && rank[l] < p.k) best[rank[l]] = l;
+  __syncthreads();
+  const uint64_t least = best[p.k - 1] < 0 ? 0 : head[best[p.k - 1]].x;
+#pragma unroll 2
+  for (int q = tid; q < p.k * p.k; q += MT) {
+    const int r = q / p.k, i = q % p.k, l = best[r];
+    if (l < 0 || i + r >= p.k) continue;
+    const int w = l / p.segs;
+    u64x2 c = head[l];
+    if (i) {
+      const uint64_t key = state[w] == 1 ? keys[(long)l * p.k + i] : 0;
+      if (!key) continue;
+      c = value(w, key);
+    }
+    if (c.x < least) continue;
+    const int at = atomicAdd(&count, 1);
+    cand[at] = c, cw[at] = w, cr[at] = 0;
   }
   __syncthreads();
   const int n = count;
+  const int cways = n && n < MT ? MT / n : 1, cshare = (n + cways - 1) / cways;
+  for (int e = tid; e < n * cways; e += MT) {
+    const int a = e % n, i0 = e / n * cshare, i1 = min(i0 + cshare, n), w = cw[a];
+    const u64x2 c = cand[a];
+    int r = 0;
+#pragma unroll 2
+    for (int i = i0; i < i1; i++) {
+      const u64x2 y = cand[i];
+      const int wi = cw[i];
+      r += y.x > c.x || (y.x == c.x && (wi < w || (wi == w && y.y < c.y)));
+    }
+    atomicAdd(cr + a, r);
+  }
+  __syncthreads();
   const long o = b * p.k;
-  for (int i = tid; i < n; i += 256) {
-    const Cand c = cand[i];
-    int rank = 0;
-#pragma unroll 4
-    for (int j = 0; j < n; j++) rank += before(cand[j], c);
-    if (rank >= p.k) continue;
-    const int token = (int)(uint32_t)c.key;
-    p.o_score[o + rank] = (float)c.v;
-    p.o_parent[o + rank] = (int)c.w;
-    p.o_token[o + rank] = token;
-    if (p.o_done) p.o_done[o + rank] = token == p.eos;
+  for (int i = tid; i < n; i += MT) {
+    const int r = cr[i], token = (int)(uint32_t)cand[i].y;
+    if (r >= p.k) continue;
+    p.o_score[o + r] = (float)double_of(cand[i].x);
+    p.o_parent[o + r] = cw[i];
+    p.o_token[o + r] = token;
+    if (p.o_done) p.o_done[o + r] = token == p.eos;
   }
   if (tid >= n && tid < p.k) {  // fewer candidates than places
     p.o_score[o + tid] = -INFINITY;
@@ -294,14 +332,19 @@ __global__ __launch_bounds__(256) void move_kernel(MoveArgs p) {
     from[w] = (long)src * p.s_s;
   }
   __syncthreads();
-  const long q = (long)blk * 256 + threadIdx.x;
-  const long t = p.first + q / p.cpr;
-  uint8_t* at = p.x + n * p.s_n + (long)g * p.W * p.s_s + h * p.s_h + t * p.s_t + q % p.cpr * sizeof(U);
-  U v[WM] = {};
+  int most = 0;
+  long spare = 0;
 #pragma unroll
   for (int w = 0; w < WM; w++)
-    if (t < rows[w]) v[w] = *reinterpret_cast<const U*>(at + from[w]);
-  asm volatile("" ::: "memory");  // two separate runs of branches: merged, every combination would get its own code
+    if (rows[w] > most) most = rows[w], spare = from[w];
+  const long q = (long)blk * 256 + threadIdx.x;
+  const long t = p.first + q / p.cpr;
+  if (t >= most) return;
+  uint8_t* at = p.x + n * p.s_n + (long)g * p.W * p.s_s + h * p.s_h + t * p.s_t + q % p.cpr * sizeof(U);
+  U v[WM];
+#pragma unroll
+  for (int w = 0; w < WM; w++)  // what does not move loads what the slot that moves most does: one run of loads, no branches
+    v[w] = *reinterpret_cast<const U*>(at + (t < rows[w] ? from[w] : spare));
 #pragma unroll
   for (int w = 0; w < WM; w++)
     if (t < rows[w]) *reinterpret_cast<U*>(at + w * p.s_s) = v[w];
@@ -321,8 +364,11 @@ bool select_ok(int B, int W, int V, int k) {
   return B >= 1 && W >= 1 && W <= MAXW && V >= 1 && V <= 0x7fff0000 && k >= 1 && k <= MAXK && (long)B * W <= 0x7fffffL &&
          (long)B * W * segments((long)B * W, V, k) <= 0x7fffffL;
 }
-// the merge's LDS: heads and candidates
-long merge_lds(int W, int segs, int k) { return ((long)W * segs + k * (k + 1) / 2) * (long)sizeof(Cand); }
+// the merge's LDS: values and keys of heads and candidates; ranks of the heads, and in the same place beams and ranks of candidates
+long merge_lds(int W, int segs, int k) {
+  const long nl = (long)W * segs, nc = k * (k + 1) / 2;
+  return 16 * (nl + nc) + 4 * (nl > 2 * nc ? nl : 2 * nc);
+}
 
 }  // namespace
 
@@ -356,7 +402,7 @@ extern "C" int mx_beam_select(hipStream_t st, const void* x, int fp32, long sx_b
   if (fp32) E == 32 ? go(beam_parts_kernel<float, 32>) : go(beam_parts_kernel<float, 8>);
   else E == 32 ? go(beam_parts_kernel<uint16_t, 32>) : go(beam_parts_kernel<uint16_t, 8>);
   if (hipGetLastError() != hipSuccess) return MX_ELAUNCH;
-  hipLaunchKernelGGL(beam_merge_kernel, dim3((unsigned)B), dim3(256), (size_t)lds, st, a);
+  hipLaunchKernelGGL(beam_merge_kernel, dim3((unsigned)B), dim3(MT), (size_t)lds, st, a);
   return hipGetLastError() == hipSuccess ? MX_OK : MX_ELAUNCH;
 }
 

@@ -1100,21 +1100,36 @@ def sdpa_kv8_tiling(B, heads, G, Tq, ctx, hd):
 
 
 # ------------------------------------------------------------------------------------------------ shared prefixes, beams
-def _keys4(t, name, dev, B, H, D):
-    """k or v (B, H, T, D) as the kernel takes it (copied if its rows are not 16-byte aligned), and its strides."""
-    if t.dim() != 4 or t.shape[0] != B or t.shape[1] != H or t.shape[3] != D:
-        raise ValueError(f"{name} must be ({B}, {H}, keys, {D}), got {tuple(t.shape)}")
-    _need(t, name, dev)
-    s = t.stride()
-    if s[3] != 1 or (s[0] | s[1] | s[2]) % 8 or s[2] >= 0x800000 or t.data_ptr() % 16:
-        s = _steps(t)
-        if s[3] != 1 or (s[0] | s[1] | s[2]) % 8 or s[2] >= 0x800000 or t.data_ptr() % 16:
-            t = t.clone(memory_format=torch.contiguous_format)
-            s = t.stride()
-    return t, (t.data_ptr() if t.shape[2] else None), s
+class _PrefixCall:
+    """A checked geometry of sdpa_prefix (shapes, strides and a device; nothing of the data)."""
+
+    def __init__(self, q, pk, pv, k, v):
+        if q.dim() != 4 or pk.dim() != 4 or pk.shape != pv.shape or k.dim() != 4 or k.shape != v.shape:
+            raise ValueError(f"q, pk, pv, k, v: {tuple(q.shape)}, {tuple(pk.shape)}, {tuple(pv.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+        B, Hq, Tq, D = q.shape
+        N, H, P = pk.shape[:3]
+        if D not in (64, 128) or N < 1 or H < 1 or B % N or Hq % H or Hq < 1:
+            raise ValueError(f"{B} sequences of {Hq} heads of dim {D} over {N} prefixes of {H} heads")
+        if pk.shape[3] != D or k.shape[0] != B or k.shape[1] != H or k.shape[3] != D:
+            raise ValueError(f"keys must be ({N}, {H}, P, {D}) and ({B}, {H}, T, {D}), got {tuple(pk.shape)}, {tuple(k.shape)}")
+        for t, name in ((q, "q"), (pk, "pk"), (pv, "pv"), (k, "k"), (v, "v")):
+            _need(t, name, q.device)
+        self.dev, self.N, self.P, self.T, self.B = q.device, N, P, k.shape[2], B
+        self.out = (B, Tq, Hq * D)
+        self.sizes = (N, B // N, H, Hq // H, Tq, D, P, self.T)
+        self.work = B * Tq > 0
+        self.scale = D ** -0.5
+        # what has to be copied before the kernel takes it: rows that are not of unit stride, 16-byte steps and 31-bit offsets
+        steps = [_steps(t) for t in (q, pk, pv, k, v)]
+        self.copy = any(s[3] != 1 or (s[0] | s[1] | s[2]) % 8 for s in steps) or any(not 0 <= s[2] < 0x800000 for s in steps[1:])
+        self.need = 0
+        if self.work:
+            import ctypes
+            self.strides = (ctypes.c_long * 15)(*(x for s in steps for x in s[:3]))
+            self.need = _lib.load().mx_sdpa_prefix_ws(N, B // N, H, Hq // H, Tq, P, self.T, D)
 
 
-_PREFIX_WS = {}  # floats of workspace of a shape (a few integers per shape a program runs)
+_PREFIX_CALLS = {}
 
 
 def sdpa_prefix(q, pk, pv, k, v, kv_len=None, prefix_len=None, out=None, scale=None, causal=True):
@@ -1126,61 +1141,82 @@ def sdpa_prefix(q, pk, pv, k, v, kv_len=None, prefix_len=None, out=None, scale=N
     are the sequence's last Tq tokens, key t is visible iff t <= kv_len_b - Tq + i (causal=False: all kv_len_b). A row that sees
     no key is 0. kv_len, prefix_len: an int, or an int32 tensor (B,) / (N,) read on the device (clamped to 0 .. T / 0 .. P);
     None: all. out may lie in q's memory. Scores (times scale) have to stay below 2^29 in size."""
-    if q.dim() != 4 or pk.dim() != 4 or pk.shape != pv.shape or k.shape != v.shape:
-        raise ValueError(f"q, pk, pv, k, v: {tuple(q.shape)}, {tuple(pk.shape)}, {tuple(pv.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    B, Hq, Tq, D = q.shape
-    N, H, P = pk.shape[:3]
-    if D not in (64, 128) or N < 1 or H < 1 or B % N or Hq % H or Hq < 1:
-        raise ValueError(f"{B} sequences of {Hq} heads of dim {D} over {N} prefixes of {H} heads")
-    dev = q.device
-    _need(q, "q", dev)
-    pk, pkp, spk = _keys4(pk, "pk", dev, N, H, D)
-    pv, pvp, spv = _keys4(pv, "pv", dev, N, H, D)
-    k, kp, sk = _keys4(k, "k", dev, B, H, D)
-    v, vp, sv = _keys4(v, "v", dev, B, H, D)
-    T = k.shape[2]
-    lp, ls, l0 = _where(T if kv_len is None else kv_len, B, dev, "kv_len")
-    pp, ps, p0 = _where(P if prefix_len is None else prefix_len, N, dev, "prefix_len")
-    if not 0 <= l0 <= T or not 0 <= p0 <= P:
-        raise ValueError(f"kv_len {l0} of {T} keys, prefix_len {p0} of {P}")
-    sc = D ** -0.5 if scale is None else float(scale)
-    if not 0.0 < sc <= 2.0 ** 127:  # the kernel multiplies by scale log2(e), a float
-        raise ValueError(f"scale {sc} must be positive and finite, at most 2^127")
+    key = (q.shape, q.stride(), pk.shape, pk.stride(), pv.shape, pv.stride(), k.shape, k.stride(), v.shape, v.stride(), q.device)
+    c = _PREFIX_CALLS.get(key)
+    if c is None or not (q.dtype is BF and pk.dtype is BF and pv.dtype is BF and k.dtype is BF and v.dtype is BF and
+                         q.device == pk.device == pv.device == k.device == v.device):
+        c = _PrefixCall(q, pk, pv, k, v)
+        if len(_PREFIX_CALLS) >= 4096:  # a program of ever new lengths
+            _PREFIX_CALLS.clear()
+        _PREFIX_CALLS[key] = c
+    dev = c.dev
+    lp, ls, l0 = (None, 0, c.T) if kv_len is None else _where(kv_len, c.B, dev, "kv_len")
+    pp, ps, p0 = (None, 0, c.P) if prefix_len is None else _where(prefix_len, c.N, dev, "prefix_len")
+    if not 0 <= l0 <= c.T or not 0 <= p0 <= c.P:
+        raise ValueError(f"kv_len {l0} of {c.T} keys, prefix_len {p0} of {c.P}")
+    sc = c.scale
+    if scale is not None:
+        sc = float(scale)
+        if not 0.0 < sc <= 2.0 ** 127:  # the kernel multiplies by scale log2(e), a float
+            raise ValueError(f"scale {sc} must be positive and finite, at most 2^127")
     given = out is not None
     if not given:
-        out = torch.empty(B, Tq, Hq * D, device=dev, dtype=BF)
-        so = out.stride()
+        out = torch.empty(c.out, device=dev, dtype=BF)
+        so = c.out[1] * c.out[2], c.out[2]
     else:
         _need(out, "out", dev)
         so = _steps(out)
-        if out.shape != (B, Tq, Hq * D) or so[2] != 1 or (so[0] | so[1]) % 4 or out.data_ptr() % 8:
-            raise ValueError(f"out must be ({B}, {Tq}, {Hq * D}) with 8-byte aligned rows of unit stride")
-    if not out.numel():
+        if out.shape != c.out or so[2] != 1 or (so[0] | so[1]) % 4 or out.data_ptr() % 8:
+            raise ValueError(f"out must be {c.out} with 8-byte aligned rows of unit stride")
+    if not c.work:
         return out
     if given and not _apart(q, out):
-        q = q.clone()  # a row's output may lie over another's query
-    s = _steps(q)
-    if s[3] != 1 or (s[0] | s[1] | s[2]) % 8 or q.data_ptr() % 16:
-        q = q.clone(memory_format=torch.contiguous_format)
-        s = q.stride()
-    shape = (N, B // N, H, Hq // H, Tq, P, T, D)
-    need = _PREFIX_WS.get(shape)
-    if need is None:
-        need = _PREFIX_WS[shape] = _lib.load().mx_sdpa_prefix_ws(*shape)
+        q = q.clone(memory_format=torch.contiguous_format)  # a row's output may lie over another's query
+        return sdpa_prefix(q, pk, pv, k, v, kv_len, prefix_len, out, scale, causal)
+    qp, pkp, pvp, kp, vp = q.data_ptr(), pk.data_ptr(), pv.data_ptr(), k.data_ptr(), v.data_ptr()
+    if c.copy or (qp | pkp | pvp | kp | vp) & 15:
+        q, pk, pv, k, v = (t.clone(memory_format=torch.contiguous_format) for t in (q, pk, pv, k, v))
+        return sdpa_prefix(q, pk, pv, k, v, kv_len, prefix_len, out, scale, causal)
+    need = c.need
     part = torch.empty(need, device=dev, dtype=torch.float32) if need else None
-    _call_on(dev, "mx_sdpa_prefix", q.data_ptr(), s[0], s[1], s[2], pkp, spk[0], spk[1], spk[2], pvp, spv[0], spv[1], spv[2],
-             kp, sk[0], sk[1], sk[2], vp, sv[0], sv[1], sv[2], out.data_ptr(), so[0], so[1], N, B // N, H, Hq // H, Tq, D, P, T,
-             pp, ps, p0, lp, ls, l0, int(causal), sc, ptr(part), need)
+    _call_on(dev, "mx_sdpa_prefix", qp, pkp or None, pvp or None, kp or None, vp or None, out.data_ptr(), c.strides, so[0], so[1],
+             *c.sizes, pp, ps, p0, lp, ls, l0, 1 if causal else 0, sc, part.data_ptr() if need else None, need)
     return out
 
 
 def sdpa_prefix_tiling(N, S, heads, G, Tq, P, T, hd):
     """How sdpa_prefix cuts N prefixes of S sequences each, G query heads per key head: (0 rows / 1 both / 2 tiles, query and key
-    waves and runs of the tile kernel, waves and runs of the 16-row kernel)."""
+    waves and runs of the tile kernel, rows per workgroup and runs of the few-row kernel)."""
     import ctypes
     t = (ctypes.c_int * 6)()
     _lib.load().mx_sdpa_prefix_tiling(N, S, heads, G, Tq, P, T, hd, ctypes.cast(t, ctypes.c_void_p))
     return tuple(t)
+
+
+_SELECT_CALLS = {}
+
+
+def _select_call(logits, scores, k, done, eos):
+    """(k, eos or -1, bytes of workspace, whether the logits' columns have to be gathered) of a checked geometry."""
+    if logits.dim() != 3 or logits.dtype not in (BF, torch.float32):
+        raise ValueError(f"logits must be (B, W, V) in bf16 or fp32, got {tuple(logits.shape)} {logits.dtype}")
+    B, W, V = logits.shape
+    k = W if k is None else int(k)
+    if not (1 <= W <= 64 and 1 <= k <= 64 and V >= 1):
+        raise ValueError(f"{W} beams over {V} tokens, {k} to select: at most 64 of each, at least 1")
+    _need(scores, "scores", logits.device, torch.float32)
+    if scores.shape != (B, W):
+        raise ValueError(f"scores must be ({B}, {W}), got {tuple(scores.shape)}")
+    e = -1 if eos is None else int(eos)
+    if eos is not None and not 0 <= e < V:
+        raise ValueError(f"eos {e} outside the {V} tokens")
+    if done is not None:
+        if eos is None:
+            raise ValueError("done goes with eos")
+        _need(done, "done", logits.device, torch.bool)
+        if done.shape != (B, W):
+            raise ValueError(f"done must be ({B}, {W}), got {tuple(done.shape)}")
+    return k, e, _lib.load().mx_beam_select_ws(B, W, V, k) if B else 0, logits.stride(2) != 1 and V > 1
 
 
 def beam_select(logits, scores, k=None, done=None, eos=None):
@@ -1192,39 +1228,32 @@ def beam_select(logits, scores, k=None, done=None, eos=None):
     without eos). A beam whose score is not finite, or whose logits hold NaN or +infinity or nothing above -infinity, offers
     nothing, and neither does a logit of -infinity (a score of -infinity, say, keeps the copies of a first beam out). Places that
     are left hold score -infinity, parent 0, token eos (0 without), done. W and k at most 64."""
-    if logits.dim() != 3 or logits.dtype not in (BF, torch.float32):
-        raise ValueError(f"logits must be (B, W, V) in bf16 or fp32, got {tuple(logits.shape)} {logits.dtype}")
+    key = (logits.shape, logits.stride(), logits.dtype, logits.device, scores.shape, scores.dtype, scores.device, k, eos,
+           None if done is None else (done.shape, done.dtype, done.device))
+    c = _SELECT_CALLS.get(key)
+    if c is None:
+        c = _select_call(logits, scores, k, done, eos)
+        if len(_SELECT_CALLS) >= 4096:
+            _SELECT_CALLS.clear()
+        _SELECT_CALLS[key] = c
+    k, e, n, gather = c
     B, W, V = logits.shape
     dev = logits.device
-    k = W if k is None else int(k)
-    if not (1 <= W <= 64 and 1 <= k <= 64 and V >= 1):
-        raise ValueError(f"{W} beams over {V} tokens, {k} to select: at most 64 of each, at least 1")
-    _need(scores, "scores", dev, torch.float32)
-    if scores.shape != (B, W):
-        raise ValueError(f"scores must be ({B}, {W}), got {tuple(scores.shape)}")
-    e = -1 if eos is None else int(eos)
-    if eos is not None and not 0 <= e < V:
-        raise ValueError(f"eos {e} outside the {V} tokens")
-    if done is not None:
-        if eos is None:
-            raise ValueError("done goes with eos")
-        _need(done, "done", dev, torch.bool)
-        if done.shape != (B, W):
-            raise ValueError(f"done must be ({B}, {W}), got {tuple(done.shape)}")
-        done = done.contiguous()
-    scores = scores.contiguous()
-    if logits.stride(2) != 1 and V > 1:
+    if gather:
         logits = logits.contiguous()
-    o = torch.empty(3, B, k, device=dev, dtype=torch.int32)
-    od = None if eos is None else torch.empty(B, k, device=dev, dtype=torch.bool)
-    score, parent, token = o.unbind()
-    score = score.view(torch.float32)
+    score = torch.empty((B, k), device=dev, dtype=torch.float32)
+    parent = torch.empty((B, k), device=dev, dtype=torch.int32)
+    token = torch.empty((B, k), device=dev, dtype=torch.int32)
+    od = None if e < 0 else torch.empty((B, k), device=dev, dtype=torch.bool)
     if B:
-        n = _lib.load().mx_beam_select_ws(B, W, V, k)
         ws = torch.empty(n, device=dev, dtype=torch.uint8)
-        p, step = o.data_ptr(), 4 * B * k
-        _call_on(dev, "mx_beam_select", logits.data_ptr(), int(logits.dtype != BF), logits.stride(0), logits.stride(1),
-                 scores.data_ptr(), ptr(done), e, B, W, V, k, p, p + step, p + 2 * step, ptr(od), ws.data_ptr(), n)
+        scores = scores.contiguous()
+        if done is not None:
+            done = done.contiguous()
+        s = logits.stride()
+        _call_on(dev, "mx_beam_select", logits.data_ptr(), 0 if logits.dtype is BF else 1, s[0], s[1], scores.data_ptr(),
+                 None if done is None else done.data_ptr(), e, B, W, V, k, score.data_ptr(), parent.data_ptr(), token.data_ptr(),
+                 None if od is None else od.data_ptr(), ws.data_ptr(), n)
     return score, parent, token, od
 
 
@@ -1263,10 +1292,11 @@ def reorder_slots(x, parent, n=None, first=0, unit=1):
     if not x.is_contiguous():
         if not _disjoint(x) or (x.dim() > 4 and not x[0, 0, 0, 0].is_contiguous()):
             raise ValueError("x must not overlap itself, and its rows must be contiguous")
-    if x.numel():
-        es, s = x.element_size(), _steps(x)
+    cells = N * S * H * T
+    if cells and x.numel():
+        es, s = x.element_size(), x.stride()
         _call_on(dev, "mx_reorder_slots", x.data_ptr(), s[0] * es, s[1] * es, s[2] * es, s[3] * es, N, G, W, H, T,
-                 x[0, 0, 0, 0].numel() * es, parent.data_ptr(), *parent.stride(), lp, ls, _int32(l0, "n"), unit, first // unit)
+                 x.numel() // cells * es, parent.data_ptr(), *parent.stride(), lp, ls, _int32(l0, "n"), unit, first // unit)
     return x
 
 

@@ -7,6 +7,7 @@ import torch
 
 import oracle.beams as ob
 import strix_halo_maxx_amd.ops as ops
+from beam_cases import ATTENTION, MASKED
 from strix_halo_maxx_amd import _lib
 
 A16 = 0x10000  # fake device addresses: validation never dereferences them
@@ -44,16 +45,20 @@ def test_oracle_reorder_by_hand():
     assert r(1, 1, 1, n=5, first=5, unit=4) == [0, 3, 2, 3, 4, 3]
 
 
-def prefix(**kw):
+def prefix(strides=None, **kw):
+    import ctypes
+    st = {**{n: 64 for n in ("qb", "qh", "qt", "pkn", "pkh", "pkt", "pvn", "pvh", "pvt", "kb", "kh", "kt", "vb", "vh", "vt")}, **(strides or {})}
     return _lib.load().mx_sdpa_prefix(*{**dict(
-        st=None, q=A16, qb=64, qh=64, qt=64, pk=A16, pkn=64, pkh=64, pkt=64, pv=A16, pvn=64, pvh=64, pvt=64, k=A16, kb=64, kh=64,
-        kt=64, v=A16, vb=64, vh=64, vt=64, o=A16, ob=64, ot=64, N=1, S=100, H=1, G=1, Tq=1, D=64, P=500, T=9, plen=None, ps=0,
-        pbase=500, len=None, ls=0, base=9, causal=1, scale=1.0, part=A16, pe=10 ** 9), **kw}.values())
+        st=None, q=A16, pk=A16, pv=A16, k=A16, v=A16, o=A16, strides=(ctypes.c_long * 15)(*st.values()), ob=64, ot=64, N=1, S=100, H=1,
+        G=1, Tq=1, D=64, P=500, T=9, plen=None, ps=0, pbase=500, len=None, ls=0, base=9, causal=1, scale=1.0, part=A16,
+        pe=10 ** 9), **kw}.values())
 
 
 def test_prefix_refusals():
     for n in ("q", "o", "pk", "pv", "k", "v"):
         assert prefix(**{n: None}) == -6
+    assert _lib.load().mx_sdpa_prefix(None, A16, A16, A16, A16, A16, A16, None, 64, 64, 1, 1, 1, 1, 1, 64, 1, 1, None, 0, 1, None, 0, 1, 1,
+                                      1.0, A16, 10 ** 9) == -6
     assert prefix(D=72) == -1
     for n in ("N", "S", "H", "G", "Tq"):
         assert prefix(**{n: 0}) == -2 and prefix(**{n: 2 ** 31 - 1}) == -2
@@ -61,15 +66,35 @@ def test_prefix_refusals():
     for s in (0.0, -1.0, INF, math.nan, 3e38):
         assert prefix(scale=s) == -2
     for n in ("qb", "qh", "qt", "pkn", "pkh", "pkt", "pvn", "pvh", "pvt", "kb", "kh", "kt", "vb", "vh", "vt"):
-        assert prefix(**{n: 68}) == -2
+        assert prefix({n: 68}) == -2
     for n in ("pkt", "pvt", "kt", "vt"):
-        assert prefix(**{n: -8}) == -2 and prefix(**{n: 2 ** 23}) == -2
+        assert prefix({n: -8}) == -2 and prefix({n: 2 ** 23}) == -2
     assert prefix(ob=62) == -2 and prefix(ot=62) == -2
     for n in ("q", "pk", "pv", "k", "v"):
         assert prefix(**{n: A16 + 8}) == -4
     assert prefix(o=A16 + 4) == -4 and prefix(plen=A16 + 2) == -4 and prefix(len=A16 + 1) == -4
     need = _lib.load().mx_sdpa_prefix_ws(1, 100, 1, 1, 1, 500, 9, 64)
     assert need > 0 and prefix(pe=need - 1) == -3 and prefix(part=None) == -3 and prefix(part=A16 + 8) == -3
+
+
+def test_prefix_cases_take_every_kernel():
+    """The GPU tests' shapes: each kernel of each head dim, with one run of keys and with several where it can have them, and each
+    under masks."""
+    def kernel(N, S, H, G, D, Tq, P, T):
+        kind, q, k, ra, rows, rb = ops.sdpa_prefix_tiling(N, S, H, G, Tq, P, T, D)
+        return (D, kind) + ((rows,) if kind == 0 else (q, k))
+
+    def runs(N, S, H, G, D, Tq, P, T):
+        t = ops.sdpa_prefix_tiling(N, S, H, G, Tq, P, T, D)
+        return max(t[3], t[5]) > 1
+    forms = [(0, 16), (0, 32), (1, 2, 4), (1, 4, 1), (2, 1, 4), (2, 2, 4), (2, 4, 1), (2, 4, 2), (2, 8, 1)]
+    want = {(D, *f) for D in (64, 128) for f in forms}
+    assert {kernel(*c) for c, _, _ in ATTENTION} == want
+    assert {kernel(*c) for c in MASKED} == want
+    split = {kernel(*c) for c, _, _ in ATTENTION if runs(*c)}
+    assert split >= {(D, *f) for D in (64, 128) for f in forms if f not in ((2, 4, 1), (2, 1, 4))}
+    whole = {kernel(*c)[1:] for c, _, _ in ATTENTION if not runs(*c)}
+    assert whole >= {f for f in forms if f[0] != 1}
 
 
 def test_prefix_workspace():
