@@ -13,6 +13,8 @@ rebuilt for batch-1 HBM streaming:
     a layer, still one HIP graph);
   * the LM head GEMV carries the argmax, and the next step's embedding lookup reduces it on the device, so one HIP
     graph replays a whole step with the token and position kept in device memory (no host round trip per token).
+  * several sequences at once: `answer` (every question of the batch) and `generate_beams` decode them together, by beam
+    search, behind one copy of the K/V that they share (ops.sdpa_prefix, beam_select, reorder_slots); a step is one HIP graph.
 The yes/no query is the reference's own fast path (FastMD2._encode / _query / decide, md2fast.py:201-212, 266-279):
 nq questions share the image prefix, whose K/V the prefix prefill writes into every question's cache slot; the
 questions, zero-padded to L tokens, run as one batch of nq * L rows under the prefix + causal mask; the last real
@@ -32,21 +34,25 @@ BOS = 50256  # moondream2's tokenizer bos_id (the Phi / GPT-2 <|endoftext|> id)
 
 class TextDecoder:
     def __init__(self, weights, lin_cls=ops.MxLin, device="cuda", ctx=1024, attn_splits=1, w8a8=False, nq=1, L=32,
-                 yes_ids=(), no_ids=(), mxfp4=False, kv8=False):
+                 yes_ids=(), no_ids=(), mxfp4=False, kv8=False, shared_prefix=False):
         """w8a8: the four text Linears of every layer run the reference's W8A8 path (its default text linear class,
         HI8Lin, moondream/gpu/bench.py:20) in prefill and decode; the LM head stays bf16 (md2fast.py:115).
         nq, L: questions per query and tokens per question (the reference's NQ, L, md2fast.py:71-86); the KV cache
         holds nq slots (decode uses slot 0). yes_ids / no_ids: the token ids the yes/no head keeps (the reference
         derives them from its tokenizer, md2fast.py:138-142; there is no tokenizer here, the caller passes them).
         mxfp4 (or lin_cls=ops.MxFp4Lin): the four text Linears in MXFP4, weights and activations; the LM head stays bf16.
-        kv8: the cache as ops.KV8Cache, one per layer (self.kv), in place of the bf16 kc / vc."""
+        kv8: the cache as ops.KV8Cache, one per layer (self.kv), in place of the bf16 kc / vc.
+        shared_prefix: the prefix's K/V go into slot 0 alone and the questions attend to that copy (ops.sdpa_prefix) instead
+        of one copy per slot; the query's logits are the same up to roundings. Not with kv8."""
         c = TXT
         mxfp4 = mxfp4 or lin_cls is ops.MxFp4Lin
         if mxfp4 and w8a8:
             raise ValueError("the Linears are either W8A8 or MXFP4")
         if mxfp4 and lin_cls not in (ops.MxLin, ops.MxFp4Lin):
             raise ValueError("mxfp4 chooses the Linear class itself")
-        self.mxfp4, self.kv8 = mxfp4, kv8
+        if shared_prefix and kv8:
+            raise ValueError("the 8-bit cache holds a copy of the prefix per slot")
+        self.mxfp4, self.kv8, self.shared_prefix = mxfp4, kv8, shared_prefix
         self.dev = torch.device(device)
         self.D, self.H, self.hd, self.eps = c["dim"], c["heads"], c["hd"], c["ln_eps"]
         self.ctx = ctx
@@ -175,6 +181,7 @@ class TextDecoder:
                 and torch.cuda.get_device_properties(dev).multi_processor_count >= lib.mx_decode_mk_grid()):
             self._init_mk()
         self.use_mk = self.mk_layers is not None and ctx <= 1024
+        self.beam_states = {}  # (searches, beams, own rows, prefix) -> buffers and the step's graph
         self.mk_fallbacks = 0  # generations redone on the per-layer kernels after a one-launch step timed out
 
     def _init_mk(self):
@@ -205,13 +212,14 @@ class TextDecoder:
             self.mk_ep.zero_()
 
     # ------------------------------------------------------------------ prefill (md2fast.py:169-212)
-    def _text_layers(self, x, pos0, causal_from, B=1, bcast=False, count=None, prefix=None):
+    def _text_layers(self, x, pos0, causal_from, B=1, bcast=False, count=None, prefix=None, attend=None):
         """x (B * n, D) bf16: B sequences (cache slots 0 .. B - 1) of n tokens at positions pos0 .. pos0 + n - 1;
         attends to keys 0 .. pos0 + n - 1 of its own slot (key j visible to query i iff j < causal_from or
         j <= pos0 + i; causal_from=None: all). bcast (B = 1): the K/V rows go to every cache slot (the shared image
         prefix, md2fast.py:177 rope_cache(..., bcast=(pos0 == 0))). count (int32 (B,), 8-bit cache only): rows of each
         sequence that go into the cache; the rest is padding, whose size would raise the exponents of the blocks. prefix
-        (8-bit cache only): keep the block that the first `prefix` rows end in as those rows alone give it."""
+        (8-bit cache only): keep the block that the first `prefix` rows end in as those rows alone give it. attend(i, qkv, out):
+        layer i's rotary embedding, cache write and attention in place of the above (out: where it goes, or None)."""
         n = x.shape[0] // B
         H, hd = self.H, self.hd
         Tk = pos0 + n
@@ -237,13 +245,20 @@ class TextDecoder:
                 qkv, f = y[:, :b["nq"]], y[:, b["nq"]:]
             else:
                 qkv, f = b["qkv"](h, pre=pre), None
-            if self.kv8:
+            if attend is not None:
+                a = attend(i, qkv, a)
+            elif self.kv8:
                 a = self._attend_kv8(i, qkv, pos0, Tk, causal_from, B, bcast, a, count, prefix)
             else:
                 q = torch.empty(B, H, n, hd, device=self.dev, dtype=BF)
                 call("mx_rope_kv", stream(), qkv.data_ptr(), qkv.stride(0), self.cs.data_ptr(), q.data_ptr(),
                      self.kc[i].data_ptr(), self.vc[i].data_ptr(), B, n, H, self.ctx, pos0, self.nq, int(bcast))
-                a = ops.sdpa(q, self.kc[i][:B, :, :Tk], self.vc[i][:B, :, :Tk], out=a, qpos0=pos0, causal_from=causal_from)
+                if self.shared_prefix and pos0 and causal_from == pos0:  # questions behind the prefix
+                    k, v = self.kc[i], self.vc[i]
+                    a = ops.sdpa_prefix(q, k[:1, :, :pos0], v[:1, :, :pos0], k[:B, :, pos0:Tk], v[:B, :, pos0:Tk], out=a)
+                else:
+                    a = ops.sdpa(q, self.kc[i][:B, :, :Tk], self.vc[i][:B, :, :Tk], out=a, qpos0=pos0,
+                                 causal_from=causal_from)
             if self.mxfp4:
                 x, h = b["out"](y[:, b["nq"]:], res=x), None
                 continue
@@ -322,7 +337,7 @@ class TextDecoder:
         x = torch.cat([self.wte[BOS:BOS + 1], img_emb.to(self.dev, BF), self.wte[prompt_ids.to(self.dev)]], dim=0)
         if x.shape[0] > self.ctx:
             raise ValueError(f"prefill of {x.shape[0]} tokens exceeds the cache ({self.ctx})")
-        xp = self._text_layers(x, 0, P, bcast=True, prefix=P if self.kv8 else None)[P:]
+        xp = self._text_layers(x, 0, P, bcast=not self.shared_prefix, prefix=P if self.kv8 else None)[P:]
         self.prefix = P
         self.pos_base = x.shape[0]
         self.lm_argmax(xp[-1], logits=True)
@@ -358,7 +373,7 @@ class TextDecoder:
         Returns the prefix length."""
         self._check_prefix(img_emb.shape[0])
         x = torch.cat([self.wte[BOS:BOS + 1], img_emb.to(self.dev, BF)], dim=0)
-        self._text_layers(x, 0, None, bcast=True)
+        self._text_layers(x, 0, None, bcast=not self.shared_prefix)
         self.prefix = x.shape[0]
         self._save_prefix_end()
         return self.prefix
@@ -383,18 +398,26 @@ class TextDecoder:
         self.last_idx.copy_(last)
         self.q_len.copy_(last - torch.arange(self.nq) * self.L + 1)
 
-    def _query(self):
+    def _question_rows(self):
+        """The questions through the layers: the normalised hidden state of each one's last row (nq, D)."""
         if self.prefix is None:
             raise RuntimeError("encode() the image prefix before querying")
         P = self.prefix
         self._restore_prefix_end()
         x = self.wte[self.tok_buf.view(-1)]                                   # (nq * L, D)
         x = self._text_layers(x, P, P, B=self.nq, count=self.q_len)
-        h = ops.layernorm(x.index_select(0, self.last_idx), *self.post_ln, eps=self.eps)  # (nq, D)
+        return ops.layernorm(x.index_select(0, self.last_idx), *self.post_ln, eps=self.eps)
+
+    def _lm(self, h):
+        """All logits of normalised rows h."""
+        if self.lm_full is None:
+            self.lm_full = ops.MxLin(self.w_lm, self.b_lm, BF, self.dev)  # shares the LM-head storage
+        return self.lm_full(h)
+
+    def _query(self):
+        h = self._question_rows()
         if self.full_logits:
-            if self.lm_full is None:
-                self.lm_full = ops.MxLin(self.w_lm, self.b_lm, BF, self.dev)  # shares the LM-head storage
-            return self.lm_full(h)
+            return self._lm(h)
         if self.lm_small is None:
             raise RuntimeError("no yes/no ids were given: set full_logits or pass yes_ids / no_ids")
         return self.lm_small(h)[:, :len(self.yn_ids)]
@@ -603,3 +626,161 @@ class TextDecoder:
         else:
             for _ in range(n_tokens - 1):
                 self.decode_step()
+
+    # ------------------------------------------------------------------ several sequences at once
+    def answer(self, n_tokens, beams=1, eos=None, length_penalty=0.0, use_graph=True):
+        """Answers every question of set_questions() about the encoded image: n_tokens each, by beam search (beams=1: greedy),
+        all nq * beams sequences in one step per token, over one copy of the image's K/V. eos: the token that ends an answer
+        (the rest of it is eos too). Returns (tokens (nq, beams, n_tokens) int32, scores (nq, beams)): sums of log
+        probabilities, best first, divided by (tokens up to eos) ** length_penalty for the order and the score."""
+        st = self._beam_state(self.nq, beams, n_tokens, self.L, self.prefix, eos)
+        h = self._question_rows()
+        P, n = self.prefix, min(self.L, st.T)
+        if self.kv8:
+            self._fork_kv8(st, torch.arange(self.nq, device=self.dev), P + n)
+        else:
+            own = st.own.view(len(self.blocks), 2, self.nq, beams, self.H, st.T, self.hd)
+            for i in range(len(self.blocks)):
+                for o, c in ((own[i, 0], self.kc[i]), (own[i, 1], self.vc[i])):
+                    o[..., :n, :].copy_(c[:, None, :, P:P + n])
+        st.rows.copy_(self.q_len.repeat_interleave(beams))
+        return self._beam_search(st, self._lm(h), n_tokens, eos, length_penalty, use_graph)
+
+    def generate_beams(self, img_emb, prompt_ids, n_tokens, beams=4, eos=None, length_penalty=0.0, use_graph=True):
+        """Prefill + beam search: n_tokens by `beams` hypotheses behind one copy of the image's and the prompt's K/V. Returns
+        (tokens (beams, n_tokens) int32, scores (beams,)) as answer() does."""
+        P = 1 + img_emb.shape[0] + prompt_ids.shape[0]
+        st = self._beam_state(1, beams, n_tokens, 0, P, eos)
+        self.prefill(img_emb, prompt_ids)
+        if self.kv8:
+            self._fork_kv8(st, torch.zeros(1, device=self.dev, dtype=torch.int64), P)
+        st.rows.zero_()
+        tokens, scores = self._beam_search(st, self.logits[None], n_tokens, eos, length_penalty, use_graph)
+        return tokens[0], scores[0]
+
+    def _beam_state(self, groups, beams, n_tokens, rows, prefix, eos):
+        """Buffers for `groups` searches whose sequences hold `rows` rows of their own behind `prefix` shared ones at first; kept
+        for the next search of the same sizes (a step's graph reads them)."""
+        if prefix is None:
+            raise RuntimeError("encode() the image prefix first")
+        if not 1 <= beams <= 64 or n_tokens < 1:
+            raise ValueError(f"{beams} beams, {n_tokens} tokens: need 1 .. 64 and at least 1")
+        if eos is not None and not 0 <= eos < self.V:
+            raise ValueError(f"eos {eos} outside [0, {self.V})")
+        T = max(rows + n_tokens - 1, 1)
+        if prefix + T > self.cs.shape[0]:
+            raise ValueError(f"{prefix} + {T} positions exceed the rotary table ({self.cs.shape[0]})")
+        key = (groups, beams, T, prefix)
+        st = self.beam_states.get(key)
+        if st is None:
+            if len(self.beam_states) >= 4:
+                self.beam_states.clear()
+            st = self.beam_states[key] = _BeamState(self, groups, beams, T, prefix, n_tokens)
+        elif st.hist.shape[1] < n_tokens:
+            st.hist, st.graph = st.history(n_tokens), None
+        return st
+
+    def _fork_kv8(self, st, slots, rows):
+        """The first `rows` rows of the given slots into every beam's slot, whole blocks as they are."""
+        nb = -(-rows // ops.KV8Cache.BLOCK)
+        for new, old in zip(st.kv, self.kv):
+            for a, b in ((new.kc, old.kc), (new.vc, old.vc), (new.ks, old.ks), (new.vs, old.vs)):
+                a.view(st.B, st.W, *a.shape[1:])[:, :, :, :nb].copy_(b[slots][:, None, :, :nb])
+
+    def _beam_attend(self, st, i, qkv, out):
+        qkv = qkv[:, None, :3 * self.D]
+        if self.kv8:
+            q, k, v = qkv.unflatten(2, (3, self.H, self.hd)).permute(2, 0, 3, 1, 4)
+            q = st.kv[i].append(k, v, st.rows, base=st.prefix, cs=self.cs, q=q)
+            return ops.sdpa_kv8(q, st.kv[i], st.rows, base=st.prefix + 1, out=out)
+        k, v = st.own[2 * i], st.own[2 * i + 1]
+        q = ops.rope_kv_at(qkv, self.cs, k, v, st.rows, st.prefix)
+        return ops.sdpa_prefix(q, self.kc[i][:1, :, :st.prefix], self.vc[i][:1, :, :st.prefix], k, v, st.lens, out=out)
+
+    def _beam_choose(self, st, logits, beams, eos):
+        """The next tokens of the searches from logits (groups, beams, V) of their hypotheses."""
+        score, parent, token, done = ops.beam_select(logits, st.scores[:, :beams], st.W, None if eos is None else st.done[:, :beams], eos)
+        st.scores.copy_(score)
+        if eos is not None:
+            st.done.copy_(done)
+        st.token.copy_(token)
+        st.hist.index_copy_(1, st.step, torch.stack((parent, token))[:, None])
+        st.step.add_(1)
+        return parent
+
+    def _beam_step(self, st, eos):
+        """One token for every hypothesis: its row through the layers, the selection, and the rows of each new hypothesis's
+        parent moved to its slot. Graph-capturable (no host reads)."""
+        st.lens.copy_(st.rows).add_(1)
+        x = self.wte.index_select(0, st.token.view(-1))
+        x = self._text_layers(x, 0, None, B=st.B * st.W, attend=lambda i, qkv, out: self._beam_attend(st, i, qkv, out))
+        h = ops.layernorm(x, *self.post_ln, eps=self.eps)
+        parent = self._beam_choose(st, self._lm(h).view(st.B, st.W, -1), st.W, eos)
+        if st.W > 1:
+            if self.kv8:
+                n = st.lens + st.prefix
+                for c in st.kv:
+                    c.reorder(parent, n, first=st.prefix)
+            else:
+                ops.reorder_slots(st.own, parent, st.lens)
+        st.rows.add_(1)
+
+    def _beam_search(self, st, logits, n_tokens, eos, length_penalty, use_graph):
+        st.scores.zero_()
+        st.done.zero_()
+        st.step.zero_()
+        self._beam_choose(st, logits.view(st.B, 1, -1), 1, eos)
+        for t in range(1, n_tokens):
+            # the first step runs eagerly: it picks every Linear's tiles outside the capture
+            if t > 1 and use_graph:
+                if st.graph is None or st.graph[1] != eos:
+                    g = torch.cuda.CUDAGraph()
+                    with torch.cuda.graph(g):
+                        self._beam_step(st, eos)
+                    st.graph = g, eos
+                st.graph[0].replay()
+            else:
+                self._beam_step(st, eos)
+            if eos is not None and t % 8 == 0 and bool(st.done.all()):
+                n_tokens, full = t + 1, n_tokens
+                break
+        else:
+            full = n_tokens
+        return self._beam_result(st, n_tokens, full, eos, length_penalty)
+
+    def _beam_result(self, st, n, full, eos, length_penalty):
+        """Every hypothesis from its last token back along the parents; past an early end eos goes on."""
+        parent, token = st.hist[:, :n].cpu().long()
+        out = torch.full((st.B, st.W, full), 0 if eos is None else eos, dtype=torch.int32)
+        at = torch.arange(st.W).expand(st.B, st.W)
+        for t in range(n - 1, -1, -1):
+            out[:, :, t] = token[t].gather(1, at)
+            at = parent[t].gather(1, at)
+        score = st.scores.cpu()
+        if length_penalty:
+            length = torch.full((st.B, st.W), full) if eos is None else ((out != eos).sum(2) + 1).clamp(max=full)
+            score = score / length.float() ** length_penalty
+            score, order = score.sort(dim=1, descending=True, stable=True)
+            out = out.gather(1, order[:, :, None].expand_as(out))
+        return out.to(self.dev), score.to(self.dev)
+
+
+class _BeamState:
+    """What a beam search of a TextDecoder keeps on the device: the hypotheses' own K/V rows, their scores, last tokens and
+    history (parent and token of every step)."""
+
+    def __init__(self, dec, B, W, T, prefix, n_tokens):
+        self.B, self.W, self.T, self.prefix, self.dev = B, W, T, prefix, dec.dev
+        z = lambda *s, dtype=torch.int32: torch.zeros(*s, device=dec.dev, dtype=dtype)
+        n, H, hd = len(dec.blocks), dec.H, dec.hd
+        if dec.kv8:
+            self.kv = [ops.KV8Cache(B * W, H, prefix + T, hd, device=dec.dev) for _ in range(n)]
+        else:
+            self.own = z(2 * n, B * W, H, T, hd, dtype=BF)  # K and V of each layer
+        self.rows, self.lens, self.token = z(B * W), z(B * W), z(B, W)  # own rows before and with the step's token
+        self.scores, self.done, self.step = z(B, W, dtype=torch.float32), z(B, W, dtype=torch.bool), z(1, dtype=torch.int64)
+        self.hist = self.history(n_tokens)
+        self.graph = None
+
+    def history(self, n_tokens):
+        return torch.zeros(2, n_tokens, self.B, self.W, device=self.dev, dtype=torch.int32)

@@ -1321,10 +1321,10 @@ def rope_kv_at(qkv, cs, kc, vc, at, rot0=0):
     q = torch.empty(B, H, n, 64, device=dev, dtype=BF)
     if q.numel():
         s = _steps(qkv)
-        if s[2] != 1 or s[1] % 8 or (B > 1 and n > 1 and s[0] != n * s[1]) or qkv.data_ptr() % 16:
-            qkv = qkv.clone(memory_format=torch.contiguous_format)
+        if s[2] != 1 or (s[0] | s[1]) % 8 or (B > 1 and n > 1 and s[0] != n * s[1]) or qkv.data_ptr() % 16:
+            qkv = qkv[..., :3 * H * 64].clone(memory_format=torch.contiguous_format)
             s = _steps(qkv)
-        ldq = s[1] if n > 1 else s[0] if B > 1 else qkv.shape[2]
+        ldq = s[1] if n > 1 else s[0] if B > 1 else 3 * H * 64
         _call_on(dev, "mx_rope_kv_at", qkv.data_ptr(), ldq, cs.data_ptr(), cs.shape[0], q.data_ptr(), kc.data_ptr(), vc.data_ptr(),
                  B, n, H, ctx, at.data_ptr(), at.stride(0), int(rot0))
     return q
