@@ -787,18 +787,20 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(Args p, uint32_t rows)
 
 // How a problem is cut, by its capacities. M rows of a sequence, R of the sequences of a prefix; us on one MI355X (HIP-graph
 // replays; prefixes x sequences x key heads x group, head dim, queries, prefix + own keys):
-//  * M < 32 and R <= 32 or R P < 2^20: rows, in 256 workgroups where runs of 128 keys give that many (1 x 4 x 32 x 1, 64, 1, 794 +
-//    64: 9.4, in one run 10.7; 1 x 8 x 8 x 4, 128, 1, 2000 + 200 12.3, in 128 workgroups 13.4). 32 rows per workgroup instead of
-//    16 where the keys would be read again too often, from R P = 400000 on (6 x 8 x 8 x 4, 128, 1, 16000 + 200 60, 16 rows 88; 1 x
-//    8 x 8 x 4, 128, 1, 2000 + 200 14.0, 16 rows 12.6);
+//  * M < 32 and R <= 32 or R P < 2^20: rows. Up to 24 blocks of keys (1536 keys of 64 values, 768 of 128) in one run: one launch
+//    and no workspace (1 x 4 x 32 x 1, 64, 1, 794 + 64 10.8 in a graph and, bound by the host, 11.5 called eagerly; 8 runs and the
+//    join 9.2 and 15.5). More of them in 256 workgroups where runs of 128 keys give that many (1 x 8 x 8 x 4, 128, 1, 2000 + 200
+//    12.3, in 128 workgroups 13.4). 32 rows per workgroup instead of 16 where the keys would be read again too often, from R P =
+//    400000 on (6 x 8 x 8 x 4, 128, 1, 16000 + 200 60, 16 rows 88; 1 x 8 x 8 x 4, 128, 1, 2000 + 200 14.0, 16 rows 12.6);
 //  * more rows of M < 32: both. Up to 64 rows 2 x 4 waves (1 x 16 x 8 x 4, 128, 1, 131071 + 512 109, 4 x 1 112), else 4 x 1 (1 x
 //    64 x 8 x 4, 128, 1, 65536 + 200 99, 2 x 2 111; rows of 32 175). Below, rows (5 x 48 x 4 x 7, 128, 1, 2000 + 500 53, both 60;
 //    1 x 16 x 8 x 4, 128, 1, 2000 + 1000 19.1, both 21.6);
-//  * M >= 32: tiles of no more than twice M's rows, 8 x 1 waves where 256-row tiles give two workgroups per CU (2 x 2 x 8 x 4, 128, 1024, 8001 + 1500 565, 4 x 1
-//    595), 4 x 1 where 128-row ones do, 4 x 2 down to three quarters of one per CU (1 x 4 x 8 x 4, 128, 200, 3000 + 300 63, 4 x 1
-//    73, 2 x 4 79), 2 x 4 with 64-row tiles down to the same, 1 x 4 below (1 x 4 x 8 x 4, 128, 64, 2000 + 100 26, 2 x 4 29, 4 x 1
-//    in runs 37; 1 x 8 x 32 x 1, 64, 32, 730 + 32 12.2). Over 8192 keys or more instead of those two as many rows as M has, and runs (1 x 1 x 8 x 4, 128, 256, 16000 +
-//    256 8 x 1 in 8 runs 82, 4 x 2 in 4 90, 1 x 4 in one 141).
+//  * M >= 32: tiles of no more than twice M's rows, 8 x 1 waves where 256-row tiles give two workgroups per CU (2 x 2 x 8 x 4,
+//    128, 1024, 8001 + 1500 565, 4 x 1 595), 4 x 1 where 128-row ones do, 4 x 2 down to three quarters of one per CU (1 x 4 x 8 x
+//    4, 128, 200, 3000 + 300 63, 4 x 1 73, 2 x 4 79), 2 x 4 with 64-row tiles down to the same, 1 x 4 below (1 x 4 x 8 x 4, 128,
+//    64, 2000 + 100 26, 2 x 4 29, 4 x 1 in runs 37; 1 x 8 x 32 x 1, 64, 32, 730 + 32 12.2). Over 8192 keys or more instead of
+//    those two as many rows as M has, and runs (1 x 1 x 8 x 4, 128, 256, 16000 + 256 8 x 1 in 8 runs 82, 4 x 2 in 4 90, 1 x 4 in
+//    one 141).
 struct Plan {
   int kind, nqw, nkw, nta, spa, rtb, ntb, spb;  // kind 0: rows, 1: both, 2: tiles
   long na, nb;                                  // workgroups of the tile kernel and of the 16-row kernel
@@ -832,6 +834,7 @@ Plan plan(int N, int S, int H, int G, int Tq, int P, int T, int D) {
   const long wb = cells * q.ntb, seqs = clamped(cdiv(16 * q.rtb, M), 1, S);  // sequences in a tile, nearly
   const long kb = 4096 / D, nb = (q.kind == 0 ? cdiv(P, kb) : 0) + seqs * cdiv(T, kb);
   q.spb = (int)clamped(256 / wb, 1, clamped(nb * kb / (q.kind == 0 ? 128 : 512), 1, 1024));
+  if (q.kind == 0 && nb <= 24) q.spb = 1;
   q.nb = wb * q.spb;
   if (q.kind == 0) return q;
   q.nqw = R <= 64 ? 2 : 4, q.nkw = R <= 64 ? 4 : 1;

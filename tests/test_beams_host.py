@@ -73,8 +73,8 @@ def test_prefix_refusals():
     for n in ("q", "pk", "pv", "k", "v"):
         assert prefix(**{n: A16 + 8}) == -4
     assert prefix(o=A16 + 4) == -4 and prefix(plen=A16 + 2) == -4 and prefix(len=A16 + 1) == -4
-    need = _lib.load().mx_sdpa_prefix_ws(1, 100, 1, 1, 1, 500, 9, 64)
-    assert need > 0 and prefix(pe=need - 1) == -3 and prefix(part=None) == -3 and prefix(part=A16 + 8) == -3
+    need = _lib.load().mx_sdpa_prefix_ws(1, 100, 1, 1, 1, 5000, 9, 64)
+    assert need > 0 and prefix(P=5000, pe=need - 1) == -3 and prefix(P=5000, part=None) == -3 and prefix(P=5000, part=A16 + 8) == -3
 
 
 def test_prefix_cases_take_every_kernel():
@@ -100,7 +100,7 @@ def test_prefix_cases_take_every_kernel():
 def test_prefix_workspace():
     ws = _lib.load().mx_sdpa_prefix_ws
     assert ws(1, 1, 1, 1, 1, 0, 1, 72) == 0 and ws(0, 1, 1, 1, 1, 0, 1, 64) == 0 and ws(1, 1, 1, 1, 1, -1, 1, 64) == 0
-    assert ws(1, 1, 1, 1, 1, 64, 64, 64) == 0  # one run
+    assert ws(1, 1, 1, 1, 1, 64, 64, 64) == 0 and ws(1, 4, 32, 1, 1, 794, 64, 64) == 0  # one run
     assert ws(1, 64, 8, 4, 1, 2 ** 31 - 256, 2 ** 31 - 256, 128) > 0
 
 
