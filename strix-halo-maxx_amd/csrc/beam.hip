@@ -232,12 +232,15 @@ __global__ __launch_bounds__(MT) void beam_merge_kernel(SelArgs p) {
     const int l = e % nl, i0 = e / nl * share, i1 = min(i0 + share, nl), w = l / p.segs, l0 = w * p.segs, l1 = l0 + p.segs;
     const u64x2 c = head[l];
     if (!c.x) continue;
-    int r = 0;
-#pragma unroll 4
+    int r = 0, same = l >= i0 && l < i1 ? -1 : 0;
+#pragma unroll 8
     for (int i = i0; i < i1; i++) {
-      const u64x2 y = head[i];
-      r += y.x > c.x || (y.x == c.x && (i < l0 || (i < l1 && y.y < c.y)));
+      const uint64_t y = head[i].x;
+      r += y > c.x;
+      same += y == c.x;
     }
+    if (same)  // rare, so that the loop above is two comparisons a head
+      for (int i = i0; i < i1; i++) r += head[i].x == c.x && (i < l0 || (i < l1 && head[i].y < c.y));
     if (ways > 1) atomicAdd(rank + l, r);
     else rank[l] = r;
   }
