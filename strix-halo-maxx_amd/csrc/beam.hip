@@ -9,13 +9,15 @@
 //  * merge: one workgroup per search adds the parts' sums, and takes the k largest of all parts' keys by their values.
 // The sums are fp32 within a part and fp64 from there on, values are fp64 and rounded to fp32 once; where two of one beam are
 // equal in fp64, their logits decide, as they do exactly.
+#include <float.h>
+
 #include "common.h"
 
 namespace {
 
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));  // rows start at any element
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int MAXW = 64, MAXK = 64, MT = 1024;  // MT: threads of the merge
+constexpr int MAXW = 64, MAXK = 64, MT = 1024, MAXL = 8192;  // MT, MAXL: threads and lists of the merge
 
 // Order-preserving bits of a float; -0 counts as 0. NONE: -infinity and below, no candidate.
 __device__ __forceinline__ uint32_t bits_of(float x) {
@@ -65,13 +67,14 @@ __device__ __forceinline__ void load8(const T* row, int v0, int V, float (&f)[8]
 
 // A lane holds E / 8 chunks of 8 neighbouring logits, chunk i of a wave's lanes 512 in a row. The wave's threshold is the
 // k-th largest of its lanes' maxima (found bit by bit from ballots: 32 steps whatever k is): k lanes have a logit that large,
-// so no smaller one is among the k largest, and the larger ones lie in fewer than k lanes. Those, and the first k that equal
-// the threshold, go to LDS, where every one counts the larger ones: its rank.
+// so no smaller one is among the k largest, and the larger ones lie in fewer than k lanes. What passes the largest of the four
+// waves' thresholds, and the first k of a wave that equal it, go to LDS, where every one counts the larger ones: its rank.
 template <class T, int E>
 __global__ __launch_bounds__(256) void beam_parts_kernel(SelArgs p) {
   extern __shared__ uint64_t cand[];  // 4 ((k - 1) E + k)
   __shared__ int count;
   __shared__ float ms[4][2];
+  __shared__ uint32_t bound[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int seg = blockIdx.x % p.segs;
   const long row = blockIdx.x / p.segs;
@@ -101,17 +104,38 @@ __global__ __launch_bounds__(256) void beam_parts_kernel(SelArgs p) {
     const uint32_t c = t | (1u << b);
     if (__popcll(__ballot(top >= c)) >= p.k) t = c;
   }
-  // fewer than k lanes, or -infinity: every finite logit
-  const bool all = t <= NONE >> LOW;
-  const float tf = all ? -INFINITY : float_of(t << LOW | (LOW && !(t >> 15) ? 0xffffu : 0u));
-  __syncthreads();
-  uint32_t eq = 0;  // of the lane's logits, a bit for each
-  if (m >= tf && m > -INFINITY) {
+  if (E <= 16 && p.k > 32) {  // (never more of E then) many lanes' smallest maximum is a poor bound: the k-th largest logit itself
+    uint32_t u[E];
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-      if (f[e] > tf) cand[atomicAdd(&count, 1)] = (uint64_t)bits_of(f[e]) << 32 | ~(uint32_t)(v0 + 512 * (e / 8) + e % 8);
-      eq |= f[e] == tf ? 1u << e : 0u;
+    for (int e = 0; e < E; e++) u[e] = f[e] > -INFINITY ? bits_of(f[e]) >> LOW : 0u;
+    uint32_t c0 = 0;
+#pragma unroll 1
+    for (int b = 31 - LOW; b >= 0; b--) {
+      const uint32_t c = c0 | (1u << b);
+      int n = 0;
+#pragma unroll
+      for (int e = 0; e < E; e++) n += __popcll(__ballot(u[e] >= c));
+      if (n >= p.k) c0 = c;
     }
+    t = c0;
+  }
+  if (lane == 0) bound[wave] = t;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 4; w++) t = max(t, bound[w]);  // the largest of the waves' thresholds serves them all
+  // fewer than k lanes in each, or -infinity: every finite logit
+  const bool all = t <= NONE >> LOW;
+  const float tf = all ? -INFINITY : float_of(t << LOW | (LOW && !(t >> 15) ? 0xffffu : 0u)), least = all ? -FLT_MAX : tf;
+  uint32_t ge = 0, eq = 0;  // of the lane's logits, a bit for each
+#pragma unroll
+  for (int e = 0; e < E; e++) ge |= f[e] >= least ? 1u << e : 0u;
+  for (; ge; ge &= ge - 1) {  // a few logits in a few lanes: read again, which costs less than 64 lanes' work on each of E registers
+    const int e = __ffs(ge) - 1, v = v0 + 512 * (e / 8) + e % 8;
+    float g;
+    if constexpr (sizeof(T) == 2) g = bf2f(x[v]);
+    else g = x[v];
+    if (g > tf) cand[atomicAdd(&count, 1)] = (uint64_t)bits_of(g) << 32 | ~(uint32_t)v;
+    else eq |= 1u << e;
   }
   if (!all) {
     int left = p.k;  // places for logits that equal the threshold, in the order of their tokens
@@ -173,17 +197,19 @@ __global__ __launch_bounds__(MT) void beam_merge_kernel(SelArgs p) {
   __shared__ float big[MAXW];    // largest logit
   __shared__ int state[MAXW];    // 0: offers nothing, 1: its logits, 2: eos
   __shared__ int best[MAXK], count;
+  __shared__ int above[2][31];
   const int tid = threadIdx.x, nl = p.W * p.segs;
   const long b = blockIdx.x;
   u64x2 *head = sh, *cand = head + nl;
-  int* rank = reinterpret_cast<int*>(cand + p.k * (p.k + 1) / 2);  // of the heads, then the candidates' beams and ranks
+  int* rank = reinterpret_cast<int*>(cand + p.k * (p.k + 1) / 2);  // heads and their ranks, then the candidates' beams and ranks
   int *cw = rank, *cr = rank + p.k * (p.k + 1) / 2;
   if (tid == 0) count = 0;
   if (tid < p.k) best[tid] = -1;
+  if (tid < 62) above[tid / 31][tid % 31] = 0;
   const uint64_t* keys = p.keys + b * nl * p.k;
   const uint64_t first = tid < nl ? keys[(long)tid * p.k] : 0;
-  int per = 64;  // threads of a row
-  while (per * p.W > MT) per /= 2;
+  int per = 1;  // threads of a row: no more than it has parts, a wave with few rows spends long on their fp64 functions
+  while (per < p.segs && per < 64 && 2 * per * p.W <= MT) per *= 2;
   const int w0 = tid / per, in = tid % per;
   if (w0 < p.W) {
     const long row = b * p.W + w0;
@@ -217,36 +243,72 @@ __global__ __launch_bounds__(MT) void beam_merge_kernel(SelArgs p) {
     return u64x2{bits_of(((double)float_of((uint32_t)(key >> 32)) - (double)big[w]) + base[w]), ~key};
   };
   for (int l = tid; l < nl; l += MT) {
-    const int w = l / p.segs;
+    const int w = (int)((uint32_t)l / (uint32_t)p.segs);
     u64x2 c = {0, 0};
     const uint64_t key = l < MT ? first : keys[(long)l * p.k];
     if (state[w] == 2 && l == w * p.segs) c = u64x2{bits_of(base[w]), (uint64_t)p.eos};
     if (state[w] == 1 && key) c = value(w, key);
     head[l] = c;
-    rank[l] = 0;
   }
   __syncthreads();
-  // ranks of the heads: every thread compares one with a share of the others
-  const int ways = nl < MT ? MT / nl : 1, share = (nl + ways - 1) / ways;
-  for (int e = tid; e < nl * ways; e += MT) {
-    const int l = e % nl, i0 = e / nl * share, i1 = min(i0 + share, nl), w = l / p.segs, l0 = w * p.segs, l1 = l0 + p.segs;
-    const u64x2 c = head[l];
-    if (!c.x) continue;
-    int r = 0, same = l >= i0 && l < i1 ? -1 : 0;
-#pragma unroll 8
-    for (int i = i0; i < i1; i++) {
-      const uint64_t y = head[i].x;
-      r += y > c.x;
-      same += y == c.x;
+  // The ranks of those of n values that can be among the k largest: place[i] = which << 16 | rank. Returns how many they are
+  const auto ranks = [&](int n, const u64x2* v, int* place, int (&above)[31], auto beam) {
+    int nc = n;
+    if (n > 512) {  // those whose upper 20 bits are no less than the k-th largest's (0 without so many), two bits at a time
+      uint32_t top[MAXL / MT], t = 0;
+#pragma unroll
+      for (int j = 0; j < MAXL / MT; j++) top[j] = tid + j * MT < n ? (uint32_t)(v[tid + j * MT].x >> 32) : 0u;
+      for (int bit = 0; bit < 20; bit += 2) {
+        const uint32_t d = 0x40000000u >> bit;
+        int* cnt = above + 1 + 3 * bit / 2;
+        int some[3] = {0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < MAXL / MT; j++) {
+#pragma unroll
+          for (int i = 0; i < 3; i++) some[i] += __popcll(__ballot(top[j] >= t + (i + 1) * d));
+          if (n <= (j + 1) * MT) break;
+        }
+        if ((tid & 63) < 3) atomicAdd(cnt + (tid & 63), (tid & 63) == 0 ? some[0] : (tid & 63) == 1 ? some[1] : some[2]);
+        __syncthreads();
+        t += cnt[2] >= p.k ? 3 * d : cnt[1] >= p.k ? 2 * d : cnt[0] >= p.k ? d : 0u;
+      }
+      for (int i = tid; i < n; i += MT)
+        if (v[i].x && (uint32_t)(v[i].x >> 32) >= t) place[atomicAdd(above, 1)] = i << 16;
+      __syncthreads();
+      nc = above[0];
+    } else {
+      for (int i = tid; i < n; i += MT) place[i] = i << 16;
+      __syncthreads();
     }
-    if (same)  // rare, so that the loop above is two comparisons a head
-      for (int i = i0; i < i1; i++) r += head[i].x == c.x && (i < l0 || (i < l1 && head[i].y < c.y));
-    if (ways > 1) atomicAdd(rank + l, r);
-    else rank[l] = r;
+    // every thread compares one with a share of all
+    const int ways = nc && nc < MT ? MT / nc : 1, share = (n + ways - 1) / ways;
+    for (int e = tid; e < nc * ways; e += MT) {
+      const int at = (int)((uint32_t)e % (uint32_t)nc), i0 = (int)((uint32_t)e / (uint32_t)nc) * share, i1 = min(i0 + share, n);
+      const int a = place[at] >> 16;
+      const u64x2 c = v[a];
+      if (!c.x) continue;
+      int r = 0, same = a >= i0 && a < i1 ? -1 : 0;
+#pragma unroll 8
+      for (int i = i0; i < i1; i++) {
+        const uint64_t y = v[i].x;
+        r += y > c.x;
+        same += y == c.x;
+      }
+      if (same) {  // rare, so that the loop above is two comparisons a value
+        const int w = beam(a);
+        for (int i = i0; i < i1; i++)
+          if (v[i].x == c.x) r += beam(i) < w || (beam(i) == w && v[i].y < c.y);
+      }
+      atomicAdd(place + at, r);
+    }
+    __syncthreads();
+    return nc;
+  };
+  const int nh = ranks(nl, head, rank, above[0], [&](int l) { return l / p.segs; });
+  for (int a = tid; a < nh; a += MT) {
+    const int r = rank[a] & 0xffff, l = rank[a] >> 16;
+    if (r < p.k && head[l].x) best[r] = l;
   }
-  __syncthreads();
-  for (int l = tid; l < nl; l += MT)
-    if (head[l].x && rank[l] < p.k) best[rank[l]] = l;
   __syncthreads();
   const uint64_t least = best[p.k - 1] < 0 ? 0 : head[best[p.k - 1]].x;
 #pragma unroll 2
@@ -262,30 +324,16 @@ __global__ __launch_bounds__(MT) void beam_merge_kernel(SelArgs p) {
     }
     if (c.x < least) continue;
     const int at = atomicAdd(&count, 1);
-    cand[at] = c, cw[at] = w, cr[at] = 0;
+    cand[at] = c, cw[at] = w;
   }
   __syncthreads();
-  const int n = count;
-  const int cways = n && n < MT ? MT / n : 1, cshare = (n + cways - 1) / cways;
-  for (int e = tid; e < n * cways; e += MT) {
-    const int a = e % n, i0 = e / n * cshare, i1 = min(i0 + cshare, n), w = cw[a];
-    const u64x2 c = cand[a];
-    int r = 0;
-#pragma unroll 2
-    for (int i = i0; i < i1; i++) {
-      const u64x2 y = cand[i];
-      const int wi = cw[i];
-      r += y.x > c.x || (y.x == c.x && (wi < w || (wi == w && y.y < c.y)));
-    }
-    atomicAdd(cr + a, r);
-  }
-  __syncthreads();
+  const int n = count, nc = ranks(n, cand, cr, above[1], [&](int i) { return cw[i]; });
   const long o = b * p.k;
-  for (int i = tid; i < n; i += MT) {
-    const int r = cr[i], token = (int)(uint32_t)cand[i].y;
+  for (int i = tid; i < nc; i += MT) {
+    const int r = cr[i] & 0xffff, a = cr[i] >> 16, token = (int)(uint32_t)cand[a].y;
     if (r >= p.k) continue;
-    p.o_score[o + r] = (float)double_of(cand[i].x);
-    p.o_parent[o + r] = cw[i];
+    p.o_score[o + r] = (float)double_of(cand[a].x);
+    p.o_parent[o + r] = cw[a];
     p.o_token[o + r] = token;
     if (p.o_done) p.o_done[o + r] = token == p.eos;
   }
@@ -297,8 +345,11 @@ __global__ __launch_bounds__(MT) void beam_merge_kernel(SelArgs p) {
   }
 }
 
-// Logits per lane: few where that is needed to fill the CUs.
-int per_lane(long rows, int V, int k) { return k <= 32 && rows * ((V + 8191) / 8192) >= 512 ? 32 : 8; }
+// Logits per lane: few where that is needed to fill the CUs. (More than 32 to select: 16 at most, for the LDS of what is handed over.)
+int per_lane(long rows, int V, int k) {
+  const int most = k <= 32 ? 32 : 16;
+  return rows * ((V + 256L * most - 1) / (256 * most)) >= 512 ? most : 8;
+}
 int segments(long rows, int V, int k) { return (V + 256 * per_lane(rows, V, k) - 1) / (256 * per_lane(rows, V, k)); }
 
 // ---------------------------------------------------------------------------------------------- slots
@@ -363,19 +414,20 @@ void move(hipStream_t st, const MoveArgs& a, unsigned grid) {
   else go(move_kernel<U, 64>);
 }
 
-bool select_ok(int B, int W, int V, int k) {
-  return B >= 1 && W >= 1 && W <= MAXW && V >= 1 && V <= 0x7fff0000 && k >= 1 && k <= MAXK && (long)B * W <= 0x7fffffL &&
-         (long)B * W * segments((long)B * W, V, k) <= 0x7fffffL;
-}
-// the merge's LDS: values and keys of heads and candidates; ranks of the heads, and in the same place beams and ranks of candidates
+// the merge's LDS: values and keys of heads and candidates; heads and their ranks, and in the same place beams and ranks of candidates
 long merge_lds(int W, int segs, int k) {
   const long nl = (long)W * segs, nc = k * (k + 1) / 2;
   return 16 * (nl + nc) + 4 * (nl > 2 * nc ? nl : 2 * nc);
 }
+bool select_ok(int B, int W, int V, int k) {
+  if (B < 1 || W < 1 || W > MAXW || V < 1 || V > 0x7fff0000 || k < 1 || k > MAXK || (long)B * W > 0x7fffffL) return false;
+  const long rows = (long)B * W, segs = segments(rows, V, k);
+  return rows * segs <= 0x7fffffL && W * segs <= MAXL && merge_lds(W, (int)segs, k) <= 160 * 1024 - 2048;  // (2048: what the merge has beside them)
+}
 
 }  // namespace
 
-// Bytes of workspace of mx_beam_select.
+// Bytes of workspace of mx_beam_select; 0 for what it refuses.
 extern "C" long mx_beam_select_ws(int B, int W, int V, int k) {
   if (!select_ok(B, W, V, k)) return 0;
   return (long)B * W * segments((long)B * W, V, k) * (8L * k + 8);
@@ -392,7 +444,6 @@ extern "C" int mx_beam_select(hipStream_t st, const void* x, int fp32, long sx_b
   const long rows = (long)B * W;
   const int segs = segments(rows, V, k), E = per_lane(rows, V, k);
   const long lds = merge_lds(W, segs, k);
-  if (lds > 64000) return MX_ESHAPE;
   if (!ws || ws_bytes < mx_beam_select_ws(B, W, V, k) || ((uintptr_t)ws & 7)) return MX_ESPLIT;
   uint64_t* keys = reinterpret_cast<uint64_t*>(ws);
   const SelArgs a{x, sx_b, sx_w, score, done, B, W, V, k, eos, segs, keys, reinterpret_cast<float*>(keys + rows * segs * k),
@@ -402,8 +453,8 @@ extern "C" int mx_beam_select(hipStream_t st, const void* x, int fp32, long sx_b
     const size_t sh = 4 * ((k - 1) * (size_t)E + k) * 8;  // what four waves can hand over
     hipLaunchKernelGGL(kern, grid, dim3(256), sh, st, a);
   };
-  if (fp32) E == 32 ? go(beam_parts_kernel<float, 32>) : go(beam_parts_kernel<float, 8>);
-  else E == 32 ? go(beam_parts_kernel<uint16_t, 32>) : go(beam_parts_kernel<uint16_t, 8>);
+  if (fp32) E == 32 ? go(beam_parts_kernel<float, 32>) : E == 16 ? go(beam_parts_kernel<float, 16>) : go(beam_parts_kernel<float, 8>);
+  else E == 32 ? go(beam_parts_kernel<uint16_t, 32>) : E == 16 ? go(beam_parts_kernel<uint16_t, 16>) : go(beam_parts_kernel<uint16_t, 8>);
   if (hipGetLastError() != hipSuccess) return MX_ELAUNCH;
   hipLaunchKernelGGL(beam_merge_kernel, dim3((unsigned)B), dim3(MT), (size_t)lds, st, a);
   return hipGetLastError() == hipSuccess ? MX_OK : MX_ELAUNCH;

@@ -1216,7 +1216,10 @@ def _select_call(logits, scores, k, done, eos):
         _need(done, "done", logits.device, torch.bool)
         if done.shape != (B, W):
             raise ValueError(f"done must be ({B}, {W}), got {tuple(done.shape)}")
-    return k, e, _lib.load().mx_beam_select_ws(B, W, V, k) if B else 0, logits.stride(2) != 1 and V > 1
+    need = _lib.load().mx_beam_select_ws(max(B, 1), W, V, k)
+    if not need:
+        raise ValueError(f"{B} x {W} beams over {V} tokens, {k} to select: too many")
+    return k, e, need, logits.stride(2) != 1 and V > 1
 
 
 def beam_select(logits, scores, k=None, done=None, eos=None):
@@ -1227,7 +1230,10 @@ def beam_select(logits, scores, k=None, done=None, eos=None):
     A finished beam (done (B, W) bool) offers eos alone, at its score; the returned done says which hypotheses end in eos (None
     without eos). A beam whose score is not finite, or whose logits hold NaN or +infinity or nothing above -infinity, offers
     nothing, and neither does a logit of -infinity (a score of -infinity, say, keeps the copies of a first beam out). Places that
-    are left hold score -infinity, parent 0, token eos (0 without), done. W and k at most 64."""
+    are left hold score -infinity, parent 0, token eos (0 without), done. W and k at most 64, V as far as a search's lists of
+    candidates fit the LDS (350000 for the largest W and k, millions for the usual ones)."""
+    if eos is not None:
+        eos = int(eos)
     key = (logits.shape, logits.stride(), logits.dtype, logits.device, scores.shape, scores.dtype, scores.device, k, eos,
            None if done is None else (done.shape, done.dtype, done.device))
     c = _SELECT_CALLS.get(key)
@@ -1241,10 +1247,10 @@ def beam_select(logits, scores, k=None, done=None, eos=None):
     dev = logits.device
     if gather:
         logits = logits.contiguous()
-    score = torch.empty((B, k), device=dev, dtype=torch.float32)
-    parent = torch.empty((B, k), device=dev, dtype=torch.int32)
-    token = torch.empty((B, k), device=dev, dtype=torch.int32)
-    od = None if e < 0 else torch.empty((B, k), device=dev, dtype=torch.bool)
+    score = torch.empty(B, k, device=dev, dtype=torch.float32)
+    parent = torch.empty(B, k, device=dev, dtype=torch.int32)
+    token = torch.empty(B, k, device=dev, dtype=torch.int32)
+    od = None if e < 0 else torch.empty(B, k, device=dev, dtype=torch.bool)
     if B:
         ws = torch.empty(n, device=dev, dtype=torch.uint8)
         scores = scores.contiguous()

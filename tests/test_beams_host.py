@@ -172,7 +172,8 @@ def test_python_refusals_select():
     ok = dict(logits=z(2, 3, 10), scores=z(2, 3, dtype=torch.float32), k=3, done=z(2, 3, dtype=torch.bool), eos=1)
     bad = [dict(logits=z(2, 3)), dict(logits=z(2, 3, 10, dtype=torch.float16)), dict(scores=z(2, 3)), dict(scores=z(2, 4, dtype=torch.float32)),
            dict(k=0), dict(k=65), dict(eos=10), dict(eos=-1), dict(eos=None), dict(done=z(2, 3, dtype=torch.uint8)),
-           dict(done=z(3, dtype=torch.bool)), dict(logits=z(1, 65, 10), scores=z(1, 65, dtype=torch.float32), done=None), dict(logits=z(2, 3, 0))]
+           dict(done=z(3, dtype=torch.bool)), dict(logits=z(1, 65, 10), scores=z(1, 65, dtype=torch.float32), done=None), dict(logits=z(2, 3, 0)),
+           dict(logits=z(1, 1, 1).expand(1, 64, 4 * 10 ** 8), scores=z(1, 64, dtype=torch.float32), done=None)]
     for b in bad:
         with pytest.raises(ValueError):
             ops.beam_select(**{**ok, **b})

@@ -84,6 +84,22 @@ def test_select_large_ties(dev):
     check(dev, torch.arange(9000).expand(40, 16, 9000).float().contiguous(), torch.zeros(40, 16), 20)
 
 
+def test_select_many_lists(dev):
+    """More parts of rows than can all be ranked: ties among them, beams of one part's weight, most of them empty."""
+    g = gen(3)
+    for V, k in ((6200, 64), (6200, 3), (90000, 64)):
+        W = 64 if V < 9000 else 20
+        check(dev, torch.zeros(1, W, V, dtype=BF), torch.zeros(1, W), k)
+        check(dev, torch.randint(-1, 2, (1, W, V), generator=g).to(BF), torch.zeros(1, W), k)
+        check(dev, torch.arange(V).expand(1, W, V).float().contiguous(), -torch.arange(W).float()[None] / 2, k)
+        s = torch.full((1, W), -INF)
+        s[0, 5] = -1.0
+        x = model_logits(g, 1, W, V, F32)
+        check(dev, x, s, k)
+        check(dev, torch.where(torch.rand(1, W, V, generator=g) < 1e-4, x, -INF), torch.zeros(1, W), k)
+        check(dev, x, torch.zeros(1, W), k, torch.rand(1, W, generator=g) < 0.9, eos=2)
+
+
 def test_select_nothing_to_offer(dev):
     """Scores and logits that are infinite or NaN, all finished, banned tokens, fewer candidates than places."""
     g = gen(4)
