@@ -34,7 +34,8 @@ class Workspace:
     Grown on demand outside graph capture (call reserve() before capturing); counters start at zero and every
     kernel that uses them leaves them at zero. Kernels on one stream serialise, so one buffer serves all layers (as
     the reference's single split-K workspace, moondream/gpu/hgemm.py:78-83); concurrent GEMMs on two streams would
-    race on it.
+    race on it. A buffer that was outgrown stays: graphs captured before write to it when they are replayed. (Each is at
+    least a quarter larger than the one before, so all of them hold less than five times the last.)
     """
     _by_dev = {}
 
@@ -42,6 +43,7 @@ class Workspace:
         self.dev = device
         self.ws = torch.empty(0, device=device, dtype=torch.float32)
         self.cnt = torch.zeros(0, device=device, dtype=torch.int32)
+        self.outgrown = []
 
     @classmethod
     def get(cls, device):
@@ -55,11 +57,13 @@ class Workspace:
         if elems > self.ws.numel():
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("split-K workspace must be reserved before graph capture")
+            self.outgrown.append(self.ws)
             self.ws = torch.empty(int(elems * 1.25) + 1024, device=self.dev, dtype=torch.float32)
         if counters > self.cnt.numel():
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("split-K counters must be reserved before graph capture")
             torch.cuda.synchronize(self.dev)
+            self.outgrown.append(self.cnt)
             self.cnt = torch.zeros(int(counters * 1.25) + 64, device=self.dev, dtype=torch.int32)
 
 

@@ -202,3 +202,14 @@ def test_python_refusals_rope():
             ops.rope_kv_at(**{**ok, **kw})
     with pytest.raises(ValueError, match="GPU"):
         ops.rope_kv_at(**ok)
+
+
+def test_outgrown_workspace_stays(monkeypatch):
+    """A search of many beams follows a captured query, and needs more split-K scratch: what the graph writes to stays its own."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    ws = ops.Workspace(torch.device("cpu"))
+    sizes = []
+    for n in (100, 50, 2000, 9000):
+        ws.reserve(n, 0)
+        sizes.append(ws.ws)
+    assert sizes[0] is sizes[1] and sizes[3] is ws.ws and all(any(t is o for o in ws.outgrown) for t in sizes[:3])

@@ -189,6 +189,24 @@ def test_shared_prefix_query(dev):
     one.query()
 
 
+def test_captured_query_after_a_wide_search(dev):
+    """A captured query and a captured step stay what they were when wider products have come between, replayed over again."""
+    w, dec = decoder({}, nq=2, L=12)
+    img = image(dev)
+    dec.full_logits = True
+    dec.encode(img)
+    dec.set_questions([S.prompt_ids(20, 9).tolist(), S.prompt_ids(21, 12).tolist()])
+    dec.capture_query()
+    first = dec.query().clone()
+    few = dec.answer(6, beams=2)
+    for beams in (16, 64):
+        dec.answer(4, beams=beams)
+        mine = [torch.full((1 << e,), 7.0, device=dev) for e in range(10, 23)]  # memory that something else holds now
+        again = dec.answer(6, beams=2)
+        assert torch.equal(dec.query(), first) and all(torch.equal(a, b) for a, b in zip(again, few))
+        assert all(bool((t == 7.0).all()) for t in mine)
+
+
 def test_refusals(dev):
     w, dec = decoder({}, nq=2, L=8)
     img, ids = image(dev), S.prompt_ids(8, 25)
