@@ -389,9 +389,9 @@ int mx_decode_mk_layer_bytes(void);
  *   O[b, i, h] = sum softmax(scale <q, key>) value over the keys that the query sees, 0 where there are none.
  * Head dims D 64 and 128; G query heads per key head (query head h G + g reads key head h). q [N S][H G][Tq][D], pk / pv
  * [N][H][P][D], k / v [N S][H][T][D] by element strides, strides[15] = {b, h, t} of q, pk, pv, k, v in turn (host memory;
- * multiples of 8, unit stride along D, 16-byte aligned; row strides of keys and values 0 .. 2^23 - 1), o [N S][Tq][H G D] (strides multiples of 4, 8-byte aligned). plen / len: device int32 with
- * strides plen_s / len_s, added to pbase / base, or null; what lies outside 0 .. P / 0 .. T is clamped. P = 0 or T = 0: pk, pv
- * or k, v are not read. fp32 sums, weights rounded to bf16; scores (times scale) must stay below 2^29 in size. part: at least
+ * multiples of 8, unit stride along D, 16-byte aligned; row strides of keys and values 0 .. 2^23 - 1), o [N S][Tq][H G D]
+ * (strides multiples of 4, 8-byte aligned). plen / len: device int32 with strides plen_s / len_s, added to pbase / base, or null;
+ * what lies outside 0 .. P / 0 .. T is clamped. P = 0 or T = 0: pk, pv or k, v are not read. fp32 sums, weights rounded to bf16; scores (times scale) must stay below 2^29 in size. part: at least
  * mx_sdpa_prefix_ws floats, 16-byte aligned, one for each call that may run at the same time; not read from call to call.
  * N S H < 2^23, N S H G Tq < 2^24. mx_sdpa_prefix_tiling: t[6] = 0 rows, 1 both, 2 tiles; query and key waves and runs of the
  * tile kernel; rows per workgroup and runs of the few-row kernel. */
@@ -407,8 +407,8 @@ int mx_sdpa_prefix(hipStream_t st, const uint16_t* q, const uint16_t* pk, const 
  * neither does a logit of -infinity. x: bf16 or (fp32 != 0) float [B][W][V] by element strides sx_b, sx_w, unit stride along V;
  * score [B][W] float, done [B][W] bytes. Outputs [B][k]: o_score, o_parent (w), o_token (v), o_done (may be null: v == eos).
  * Places without a candidate: score -infinity, parent 0, token max(eos, 0), done 1. eos < 0: none (done must be null).
- * W <= 64, k <= 64, 20 W ceil(V / 2048 or 8192) + 12 k (k + 1) < 64000. ws: mx_beam_select_ws bytes, 8-byte aligned, one
- * for each call that may run at the same time. */
+ * W <= 64, k <= 64, and the lists that a search's rows are cut into have to fit the merge's LDS (V up to 350000 for W = k = 64).
+ * ws: mx_beam_select_ws bytes (0 for sizes that are refused), 8-byte aligned, one for each call that may run at the same time. */
 long mx_beam_select_ws(int B, int W, int V, int k);
 int mx_beam_select(hipStream_t st, const void* x, int fp32, long sx_b, long sx_w, const float* score, const uint8_t* done,
                    int eos, int B, int W, int V, int k, float* o_score, int* o_parent, int* o_token, uint8_t* o_done, void* ws,

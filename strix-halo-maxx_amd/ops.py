@@ -1293,7 +1293,7 @@ def reorder_slots(x, parent, n=None, first=0, unit=1):
     if parent.dim() != 2 or parent.numel() != S or not 1 <= parent.shape[1] <= 64:
         raise ValueError(f"parent must be (G, W) with G W = {S} and W at most 64, got {tuple(parent.shape)}")
     G, W = parent.shape
-    first, unit = int(first), int(unit)
+    first, unit = int(first), _int32(unit, "unit")
     if first < 0 or unit < 1:
         raise ValueError(f"first {first} must not be negative, unit {unit} at least 1")
     lp, ls, l0 = _where(T * unit if n is None else n, S, dev, "n")
@@ -1306,7 +1306,7 @@ def reorder_slots(x, parent, n=None, first=0, unit=1):
     if cells and x.numel():
         es, s = x.element_size(), x.stride()
         _call_on(dev, "mx_reorder_slots", x.data_ptr(), s[0] * es, s[1] * es, s[2] * es, s[3] * es, N, G, W, H, T,
-                 x.numel() // cells * es, parent.data_ptr(), *parent.stride(), lp, ls, _int32(l0, "n"), unit, first // unit)
+                 x.numel() // cells * es, parent.data_ptr(), *parent.stride(), lp, ls, _int32(l0, "n"), unit, min(first // unit, T))
     return x
 
 
@@ -1336,7 +1336,7 @@ def rope_kv_at(qkv, cs, kc, vc, at, rot0=0):
             s = _steps(qkv)
         ldq = s[1] if n > 1 else s[0] if B > 1 else 3 * H * 64
         _call_on(dev, "mx_rope_kv_at", qkv.data_ptr(), ldq, cs.data_ptr(), cs.shape[0], q.data_ptr(), kc.data_ptr(), vc.data_ptr(),
-                 B, n, H, ctx, at.data_ptr(), at.stride(0), int(rot0))
+                 B, n, H, ctx, at.data_ptr(), at.stride(0), _int32(rot0, "rot0"))
     return q
 
 

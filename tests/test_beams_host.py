@@ -184,7 +184,7 @@ def test_python_refusals_select():
 def test_python_refusals_reorder():
     x, p = z(1, 4, 2, 5, 8), z(2, 2, dtype=torch.int32)
     for kw in (dict(x=z(4, 2, 5)), dict(parent=p.long()), dict(parent=z(3, dtype=torch.int32)), dict(parent=z(2, 2, 1, dtype=torch.int32)),
-               dict(n=6), dict(n=-1), dict(n=z(2, dtype=torch.int32)), dict(first=-1), dict(unit=0),
+               dict(n=6), dict(n=-1), dict(n=z(2, dtype=torch.int32)), dict(first=-1), dict(unit=0), dict(unit=2 ** 31, n=3),
                dict(x=z(1, 1, 2, 5, 8).expand(1, 4, 2, 5, 8)), dict(x=z(1, 4, 2, 8, 5).transpose(3, 4)),
                dict(x=z(1, 65, 1, 1, 8), parent=z(65, dtype=torch.int32))):
         with pytest.raises(ValueError):
@@ -195,7 +195,7 @@ def test_python_refusals_reorder():
 
 def test_python_refusals_rope():
     ok = dict(qkv=z(2, 1, 192), cs=z(9, 16, 2, dtype=torch.float32), kc=z(2, 1, 5, 64), vc=z(2, 1, 5, 64), at=z(2, dtype=torch.int32))
-    for kw in (dict(qkv=z(1, 1, 192)), dict(qkv=z(2, 1, 191)), dict(cs=z(9, 16, 2)), dict(cs=z(9, 32, dtype=torch.float32)),
+    for kw in (dict(rot0=2 ** 31), dict(qkv=z(1, 1, 192)), dict(qkv=z(2, 1, 191)), dict(cs=z(9, 16, 2)), dict(cs=z(9, 32, dtype=torch.float32)),
                dict(kc=z(2, 1, 5, 128)), dict(vc=z(2, 1, 6, 64)), dict(at=z(1, dtype=torch.int32)), dict(at=z(2, dtype=torch.int64)),
                dict(kc=z(2, 5, 1, 64).transpose(1, 2)[:, :, ::2], vc=z(2, 5, 1, 64).transpose(1, 2)[:, :, ::2])):
         with pytest.raises(ValueError):

@@ -213,6 +213,7 @@ def test_reorder_types_and_units(dev, shape, dtype):
     for first, n in ((0, 3 * 7), (8, [0, 1, 7, 400]), (13, [14, 7, 8, 15])):
         moved(dev, x, parent, n, first, unit=7) if not isinstance(n, int) or n <= 7 * shape[3] else None
     moved(dev, x, parent, first=10 ** 6)
+    moved(dev, x, parent, first=2 ** 32)
 
 
 def test_reorder_views(dev):
