@@ -69,6 +69,8 @@ __device__ __forceinline__ void load8(const T* row, int v0, int V, float (&f)[8]
 // k-th largest of its lanes' maxima (found bit by bit from ballots: 32 steps whatever k is): k lanes have a logit that large,
 // so no smaller one is among the k largest, and the larger ones lie in fewer than k lanes. What passes the largest of the four
 // waves' thresholds, and the first k of a wave that equal it, go to LDS, where every one counts the larger ones: its rank.
+// Bound by the vector ALU's work per logit (maximum, subtraction, scaling, exponential, sum, comparison) and, in fp32, nearly by
+// memory: 16 x 16 rows of 131071 fp32 logits 26.9 us = 5.0 TB/s; 32 x 8 of 51200 bf16 11.8.
 template <class T, int E>
 __global__ __launch_bounds__(256) void beam_parts_kernel(SelArgs p) {
   extern __shared__ uint64_t cand[];  // 4 ((k - 1) E + k)
@@ -104,7 +106,7 @@ __global__ __launch_bounds__(256) void beam_parts_kernel(SelArgs p) {
     const uint32_t c = t | (1u << b);
     if (__popcll(__ballot(top >= c)) >= p.k) t = c;
   }
-  if (E <= 16 && p.k > 32) {  // (never more of E then) many lanes' smallest maximum is a poor bound: the k-th largest logit itself
+  if constexpr (E == 16) {  // more than 32 to select: many lanes' smallest maximum is a poor bound: the k-th largest logit itself
     uint32_t u[E];
 #pragma unroll
     for (int e = 0; e < E; e++) u[e] = f[e] > -INFINITY ? bits_of(f[e]) >> LOW : 0u;
@@ -129,7 +131,7 @@ __global__ __launch_bounds__(256) void beam_parts_kernel(SelArgs p) {
   uint32_t ge = 0, eq = 0;  // of the lane's logits, a bit for each
 #pragma unroll
   for (int e = 0; e < E; e++) ge |= f[e] >= least ? 1u << e : 0u;
-  for (; ge; ge &= ge - 1) {  // a few logits in a few lanes: read again, which costs less than 64 lanes' work on each of E registers
+  for (; ge; ge &= ge - 1) {  // a few logits in a few lanes: read again, which costs less than work on each of the E registers
     const int e = __ffs(ge) - 1, v = v0 + 512 * (e / 8) + e % 8;
     float g;
     if constexpr (sizeof(T) == 2) g = bf2f(x[v]);
@@ -190,9 +192,10 @@ typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
 
 // A list is a part's keys; a finished beam's is its one continuation. The k-th largest head of the lists bounds what can be
 // selected, and a key at place i of a list whose head has rank r has i + r larger ones: few keys are left to be ranked. What
-// takes the time is three rounds to memory, one after the other: the sums, the heads, the keys behind them.
+// takes the time is three rounds to memory, one after the other: the sums, the heads, the keys behind them (32 searches of 8 beams
+// of 7 parts 6.2 us, 16 of 16 of 16 9.2).
 __global__ __launch_bounds__(MT) void beam_merge_kernel(SelArgs p) {
-  extern __shared__ u64x2 sh[];  // (value, key), key = ~logit's bits << 32 | token: the lists' heads [nl], then candidates, by rank of list
+  extern __shared__ u64x2 sh[];  // (value, key), key = ~logit's bits << 32 | token: the lists' heads [nl], then candidates
   __shared__ double base[MAXW];  // score - log of the sum
   __shared__ float big[MAXW];    // largest logit
   __shared__ int state[MAXW];    // 0: offers nothing, 1: its logits, 2: eos
@@ -254,7 +257,8 @@ __global__ __launch_bounds__(MT) void beam_merge_kernel(SelArgs p) {
   // The ranks of those of n values that can be among the k largest: place[i] = which << 16 | rank. Returns how many they are
   const auto ranks = [&](int n, const u64x2* v, int* place, int (&above)[31], auto beam) {
     int nc = n;
-    if (n > 512) {  // those whose upper 20 bits are no less than the k-th largest's (0 without so many), two bits at a time
+    if (n > 128) {  // those whose upper 20 bits are no less than the k-th largest's (0 without so many), two bits at a time. Two
+                    // searches of 400 and of 224 lists: 20 and 23 us, all ranked 40 and 31; 256 by 16 waves: 38.1 and 37.7
       uint32_t top[MAXL / MT], t = 0;
 #pragma unroll
       for (int j = 0; j < MAXL / MT; j++) top[j] = tid + j * MT < n ? (uint32_t)(v[tid + j * MT].x >> 32) : 0u;
@@ -345,12 +349,11 @@ __global__ __launch_bounds__(MT) void beam_merge_kernel(SelArgs p) {
   }
 }
 
-// Logits per lane: few where that is needed to fill the CUs. (More than 32 to select: 16 at most, for the LDS of what is handed over.)
-int per_lane(long rows, int V, int k) {
-  const int most = k <= 32 ? 32 : 16;
-  return rows * ((V + 256L * most - 1) / (256 * most)) >= 512 ? most : 8;
-}
-int segments(long rows, int V, int k) { return (V + 256 * per_lane(rows, V, k) - 1) / (256 * per_lane(rows, V, k)); }
+// Logits per lane. Fewer fill the CUs earlier, but leave the merge longer lists, which costs more (us for the whole selection with
+// 32, 16, 8 per lane: 1 x 4 x 51200 11.8, 11.5, 12.6; 8 x 8 x 51200 13.7, 15.3, 17.5; 32 x 8 x 51200 18.0, 21.9, 32.3; 16 x 16 x
+// 131071 fp32 38, 53, 66). More than 32 to select: 16, for the LDS of what is handed over (1 x 64 x 51200: 44, 8 per lane 52).
+int per_lane(int k) { return k <= 32 ? 32 : 16; }
+int segments(int V, int k) { return (V + 256 * per_lane(k) - 1) / (256 * per_lane(k)); }
 
 // ---------------------------------------------------------------------------------------------- slots
 struct MoveArgs {
@@ -366,7 +369,9 @@ struct MoveArgs {
 
 // x[n, g W + w, h, t] = x[n, g W + parent[g, w], h, t] for first <= t < rows of the parent. A thread owns one piece (16, 4 or 1
 // bytes) of a row in every slot of a group, loads what moves and then stores it, so the copy is in place in any order and no
-// two threads meet. Bound by the bytes: slots that do not change are not touched.
+// two threads meet. Bound by the bytes: slots that do not change are not touched. What a beam step of
+// the text decoder moves (48 K and V of 4 slots x 32 heads x 40 rows x 128 bytes) takes 10 us, 16 of 64 slots x 8 heads x 1 - 500
+// rows x 256 bytes 137.
 template <class U, int WM>
 __global__ __launch_bounds__(256) void move_kernel(MoveArgs p) {
   __shared__ long from[WM];  // byte offset of slot w's parent; the rows that it takes from it
@@ -414,15 +419,16 @@ void move(hipStream_t st, const MoveArgs& a, unsigned grid) {
   else go(move_kernel<U, 64>);
 }
 
-// the merge's LDS: values and keys of heads and candidates; heads and their ranks, and in the same place beams and ranks of candidates
+// the merge's LDS: values and keys of heads and candidates; ranks of heads, and in the same place beams and ranks of candidates
 long merge_lds(int W, int segs, int k) {
   const long nl = (long)W * segs, nc = k * (k + 1) / 2;
   return 16 * (nl + nc) + 4 * (nl > 2 * nc ? nl : 2 * nc);
 }
 bool select_ok(int B, int W, int V, int k) {
   if (B < 1 || W < 1 || W > MAXW || V < 1 || V > 0x7fff0000 || k < 1 || k > MAXK || (long)B * W > 0x7fffffL) return false;
-  const long rows = (long)B * W, segs = segments(rows, V, k);
-  return rows * segs <= 0x7fffffL && W * segs <= MAXL && merge_lds(W, (int)segs, k) <= 160 * 1024 - 2048;  // (2048: what the merge has beside them)
+  const long rows = (long)B * W, segs = segments(V, k);
+  // (2048 bytes: what the merge has beside its lists)
+  return rows * segs <= 0x7fffffL && W * segs <= MAXL && merge_lds(W, (int)segs, k) <= 160 * 1024 - 2048;
 }
 
 }  // namespace
@@ -430,7 +436,7 @@ bool select_ok(int B, int W, int V, int k) {
 // Bytes of workspace of mx_beam_select; 0 for what it refuses.
 extern "C" long mx_beam_select_ws(int B, int W, int V, int k) {
   if (!select_ok(B, W, V, k)) return 0;
-  return (long)B * W * segments((long)B * W, V, k) * (8L * k + 8);
+  return (long)B * W * segments(V, k) * (8L * k + 8);
 }
 
 extern "C" int mx_beam_select(hipStream_t st, const void* x, int fp32, long sx_b, long sx_w, const float* score,
@@ -442,7 +448,7 @@ extern "C" int mx_beam_select(hipStream_t st, const void* x, int fp32, long sx_b
   if (((uintptr_t)x & (fp32 ? 3 : 1)) || (((uintptr_t)score | (uintptr_t)o_score | (uintptr_t)o_parent | (uintptr_t)o_token) & 3))
     return MX_ELAYOUT;
   const long rows = (long)B * W;
-  const int segs = segments(rows, V, k), E = per_lane(rows, V, k);
+  const int segs = segments(V, k), E = per_lane(k);
   const long lds = merge_lds(W, segs, k);
   if (!ws || ws_bytes < mx_beam_select_ws(B, W, V, k) || ((uintptr_t)ws & 7)) return MX_ESPLIT;
   uint64_t* keys = reinterpret_cast<uint64_t*>(ws);
@@ -453,8 +459,11 @@ extern "C" int mx_beam_select(hipStream_t st, const void* x, int fp32, long sx_b
     const size_t sh = 4 * ((k - 1) * (size_t)E + k) * 8;  // what four waves can hand over
     hipLaunchKernelGGL(kern, grid, dim3(256), sh, st, a);
   };
-  if (fp32) E == 32 ? go(beam_parts_kernel<float, 32>) : E == 16 ? go(beam_parts_kernel<float, 16>) : go(beam_parts_kernel<float, 8>);
-  else E == 32 ? go(beam_parts_kernel<uint16_t, 32>) : E == 16 ? go(beam_parts_kernel<uint16_t, 16>) : go(beam_parts_kernel<uint16_t, 8>);
+  const auto parts = [&](auto t) {
+    typedef decltype(t) T;
+    E == 32 ? go(beam_parts_kernel<T, 32>) : go(beam_parts_kernel<T, 16>);
+  };
+  fp32 ? parts(0.f) : parts(uint16_t{});
   if (hipGetLastError() != hipSuccess) return MX_ELAUNCH;
   hipLaunchKernelGGL(beam_merge_kernel, dim3((unsigned)B), dim3(MT), (size_t)lds, st, a);
   return hipGetLastError() == hipSuccess ? MX_OK : MX_ELAUNCH;

@@ -15,9 +15,9 @@
 // device), so it fixes the number of runs and the device cuts each list evenly.
 //
 // Numerics: fp32 scores, sums and outputs; a weight is rounded to bf16 for its product (2^-9 of it on average), its sum takes it
-// before that. A masked key reaches no result: blocks that need a mask
-// are searched for infinities and NaN among the values, and where there is one (never in ordinary data) it is cleared and two
-// products of indicators with the visibility find the outputs that it belongs to.
+// before that. A masked key reaches no result: blocks that need a mask are searched for infinities and NaN among the values, and
+// where there is one (never in ordinary data) it is cleared and two products of indicators with the visibility find the outputs
+// that it belongs to.
 #include "common.h"
 
 namespace {
@@ -158,6 +158,11 @@ constexpr int rows_lds() {
 // keys of 64 columns, 32 of 128): K from memory into the 16x16x32 MFMA's registers, V through a piece of LDS of the wave's own
 // for the transposed read; the next block is in flight through this one's softmax and product. S^T leaves keys
 // 16 t + 4 (lane / 16) + r of row lane % 16 in a lane, and the product with V takes its keys in that order.
+// Bound by bytes: where the keys of a head are one workgroup's, by what one CU gets from beyond its L2, about 30 bytes per ns (1 x
+// 4 x 32 x 1, 64, 1, 794 + 64 as in plan(): 268 KB a workgroup in 10.3 us); where runs fill the chip, by memory (6 x 8 x 8 x 4,
+// 128, 1, 16000 + 200: 432 MB, some of them still in the 256 MB cache, in 60 us); where lengths on the device differ widely, by the
+// longest lists (the same with prefixes of 1 - 16000 keys: 55 us). 8 or 16 waves per workgroup brought nothing, nor did dealing the
+// runs out by the lengths on the device (3 - 8 us more for lists that are alike, 4 less for the most unlike).
 template <int D, int NW, int RT, bool PREFIX>
 __device__ __forceinline__ void rows_body(const Args& p, uint32_t item, uint8_t* smem) {
   constexpr int KB = 4096 / D, KT = KB / 16, NS = D / 32, NT = D / 16, NV = 8, CPR = D / 8, RW = 16 * RT;
@@ -446,6 +451,11 @@ struct Tile {
 // NQW query waves x NKW key waves; blocks of KB keys go through an LDS ring of S stages by the asynchronous load, the
 // block's keys shared among the key waves, whose shares are added at the end. S^T = K Q^T leaves a lane the scores of one
 // row, in the key order that the product with V (transposed reads) takes.
+// Prompts are bound by a SIMD's two waves issuing softmax and products by turns: 2 x 2 x 8 x 4, 128, 1024, 8001 + 1500 takes 553 us
+// = 0.88 PFLOP/s (a large library product 1.13), the matrix unit busy 37 % of the time, the vector ALU 40 %, no bank conflicts.
+// Tried and slower: the next block's scores before this one's softmax in one wave (588 - 620 us: registers), waves in two groups
+// that swap softmax and products at barriers (1217 us and more), rings of 3 and 4 stages (the same). Over a long prefix with few
+// rows it is bound by memory: 1 x 16 x 8 x 4, 128, 1, 131071 + 512 reads 540 MB in 102 us, 5.3 TB/s.
 template <int D, int NQW, int NKW, int KB, int S, bool SEQ>
 __device__ __forceinline__ void tile_body(const Args& p, uint32_t item, uint8_t* smem) {
   using C = Tile<D, NQW, NKW, KB, S>;
@@ -700,7 +710,8 @@ __global__ __launch_bounds__(64 * NQW * NKW, 2) void prefix_both_kernel(Args p) 
 }
 
 // The shares of one row: 256 / WPR threads... one workgroup has 4 / WPR rows of WPR waves; D / 4 threads with 4 columns each
-// form a group, and the groups take the shares in turn, in a fixed order.
+// form a group, and the groups take the shares in turn, in a fixed order. Bound by the latency of two trips to memory (pairs, then
+// outputs, of which the first four are asked for at once): 4.9 us for 192 rows of 48 runs, 8.7 for 1024 of 10.
 template <int D, int WPR>
 __global__ __launch_bounds__(256) void prefix_join_kernel(Args p, uint32_t rows) {
   constexpr int TD = D / 4, NT = 64 * WPR, NG = NT / TD, RPB = 256 / NT;
