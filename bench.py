@@ -600,12 +600,14 @@ DECODE_FORMS = {"bf16": {}, "w8a8": dict(w8a8=True), "mxfp4": dict(mxfp4=True), 
 
 
 def operator_case(name, passes=25):
-    """A listed case of perf/operators.py on the framework's kernels: set up, then `passes` passes one by one, for a kernel trace
-    or counters of its launches."""
+    """A listed case of perf/operators.py or perf/more_operators.py on the framework's kernels: set up, then `passes` passes one by
+    one, for a kernel trace or counters of its launches."""
     import torch
+    import perf.more_operators as pm
     import perf.operators as po
+    po, case = next((m, c) for m in (po, pm) for c in m.listed() if c["name"] == name)
     po.own = True
-    state = po.prepare(next(c for c in po.listed() if c["name"] == name), 1)
+    state = po.prepare(case, 1)
     torch.cuda.synchronize()
     for _ in range(passes):
         po.run(state)
@@ -1140,7 +1142,8 @@ def main():
     ap.add_argument("--no-cpu", action="store_true")
     ap.add_argument("--no-extra", action="store_true", help="headline tower only (no batch 13 / 256, decoder, TRecViT)")
     ap.add_argument("--decode", choices=DECODE_FORMS, help="only the text decoder (prefill, query, decode) in this form")
-    ap.add_argument("--case", help="only passes through one listed case of perf/operators.py, for a profiler")
+    ap.add_argument("--case", help="only passes through one listed case of perf/operators.py or perf/more_operators.py, for"
+                    " a profiler")
     ap.add_argument("--traffic-probe", action="store_true",
                     help="only the eager launches that rocprofv3 --pmc FETCH_SIZE / WRITE_SIZE runs count (see traffic_probe)")
     ap.add_argument("--traffic-probe-decode", action="store_true",
