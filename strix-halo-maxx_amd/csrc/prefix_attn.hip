@@ -884,7 +884,7 @@ hipError_t launch(hipStream_t st, const Args& a, const Plan& q) {
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && shares(q)) {
     const long rows = (long)a.N * a.S * a.H * a.G * a.Tq;
-    if (q.spa + q.spb > 16)
+    if (q.spa + q.spb > 32)  // (17 shares of 2048 rows: 7 us by single waves, 8.5 by four)
       hipLaunchKernelGGL((prefix_join_kernel<D, 4>), dim3((unsigned)rows), dim3(256), 0, st, a, (uint32_t)rows);
     else
       hipLaunchKernelGGL((prefix_join_kernel<D, 1>), dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, st, a, (uint32_t)rows);
