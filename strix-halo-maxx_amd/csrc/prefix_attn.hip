@@ -884,7 +884,9 @@ hipError_t launch(hipStream_t st, const Args& a, const Plan& q) {
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && shares(q)) {
     const long rows = (long)a.N * a.S * a.H * a.G * a.Tq;
-    if (q.spa + q.spb > 32)  // (17 shares of 2048 rows: 7 us by single waves, 8.5 by four)
+    // four waves a row for many shares, fewer of them where few rows leave CUs idle (24 rows of 21 shares, the whole call: 9.1 us, by
+    // single waves 10.0; 2048 rows of 17: 60.6, single 58.6)
+    if (q.spa + q.spb > (rows < 1024 ? 16 : 32))
       hipLaunchKernelGGL((prefix_join_kernel<D, 4>), dim3((unsigned)rows), dim3(256), 0, st, a, (uint32_t)rows);
     else
       hipLaunchKernelGGL((prefix_join_kernel<D, 1>), dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, st, a, (uint32_t)rows);
