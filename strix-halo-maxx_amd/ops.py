@@ -1282,7 +1282,8 @@ def reorder_slots(x, parent, n=None, first=0, unit=1):
     (G, W) int32, G W = slots (or (slots,)): slot g W + w becomes a copy of slot g W + parent[g, w], which may be any of its group,
     several times the same; values outside 0 .. W - 1 leave their slot. Only rows first .. n - 1 move, n an int or an int32 tensor
     (slots,) of the rows that each slot holds (a slot takes as many as its parent has; None: all T); every other row stays. unit:
-    tokens per row (first and n count tokens; the row that token `first` lies in moves). W at most 64. Returns x."""
+    tokens per row (first and n count tokens; the row that token `first` lies in moves). W at most 64; T, n and the bytes of a row
+    below 2^31. Returns x."""
     if x.dim() < 4:
         raise ValueError(f"x must be (L, slots, H, T, ...), got {tuple(x.shape)}")
     N, S, H, T = x.shape[:4]
@@ -1305,8 +1306,11 @@ def reorder_slots(x, parent, n=None, first=0, unit=1):
     cells = N * S * H * T
     if cells and x.numel():
         es, s = x.element_size(), x.stride()
+        row = x.numel() // cells * es
+        if max(N, S, H, T, row) > 0x7fffffff:
+            raise ValueError(f"x {tuple(x.shape)}: its sizes and a row's {row} bytes do not fit 32 bits")
         _call_on(dev, "mx_reorder_slots", x.data_ptr(), s[0] * es, s[1] * es, s[2] * es, s[3] * es, N, G, W, H, T,
-                 x.numel() // cells * es, parent.data_ptr(), *parent.stride(), lp, ls, _int32(l0, "n"), unit, min(first // unit, T))
+                 row, parent.data_ptr(), *parent.stride(), lp, ls, _int32(l0, "n"), unit, min(first // unit, T))
     return x
 
 

@@ -1,0 +1,28 @@
+"""Sizes and arguments of the shared-prefix attention, beam selection and slot reordering that no call on real memory reaches: what
+the C entries cannot hold is refused, nothing of an earlier call is taken for a later one. Without a GPU: the tensors have no
+memory, or the call stops before the library."""
+import pytest
+import torch
+
+import strix_halo_maxx_amd.ops as ops
+
+BF, F32, I32, U8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
+FAR = 2 ** 32 + 64  # 64 to whoever keeps the lower 32 bits
+
+
+def no(*s, dtype=BF):
+    """A tensor without memory."""
+    return torch.empty(*s, dtype=dtype, device="meta")
+
+
+def test_reorder_sizes_past_31_bits():
+    p, n = no(1, 2, dtype=I32), no(2, dtype=I32)
+    for x in (no(1, 2, 1, 1, FAR, dtype=U8), no(1, 2, 1, 1, 2 ** 31, dtype=U8), no(1, 2, 1, 1, 2 ** 29, dtype=F32),
+              no(1, 2, 1, FAR, 16), no(1, 2, FAR, 1, 16), no(FAR, 2, 1, 1, 16)):
+        with pytest.raises(ValueError, match="32 bits"):
+            ops.reorder_slots(x, p, n)
+    for x in (no(1, 2, 1, 1, 2 ** 31 - 16, dtype=U8), no(1, 2, 1, 2 ** 31 - 1, 16)):  # these reach the library
+        with pytest.raises(ValueError, match="GPU"):
+            ops.reorder_slots(x, p, n)
+    with pytest.raises(ValueError, match="32 bits"):
+        ops.reorder_slots(no(1, FAR, 1, 1, 16), no(FAR // 2, 2, dtype=I32))
