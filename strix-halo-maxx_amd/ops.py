@@ -1208,6 +1208,8 @@ def _select_call(logits, scores, k, done, eos):
     k = W if k is None else int(k)
     if not (1 <= W <= 64 and 1 <= k <= 64 and V >= 1):
         raise ValueError(f"{W} beams over {V} tokens, {k} to select: at most 64 of each, at least 1")
+    if max(B, V) > 0x7fffffff:
+        raise ValueError(f"logits {tuple(logits.shape)}: the sizes do not fit 32 bits")
     _need(scores, "scores", logits.device, torch.float32)
     if scores.shape != (B, W):
         raise ValueError(f"scores must be ({B}, {W}), got {tuple(scores.shape)}")

@@ -26,3 +26,9 @@ def test_reorder_sizes_past_31_bits():
             ops.reorder_slots(x, p, n)
     with pytest.raises(ValueError, match="32 bits"):
         ops.reorder_slots(no(1, FAR, 1, 1, 16), no(FAR // 2, 2, dtype=I32))
+
+
+def test_select_sizes_past_31_bits():
+    for B, V in ((1, FAR), (FAR, 10), (1, 2 ** 31)):
+        with pytest.raises(ValueError, match="32 bits"):
+            ops.beam_select(no(B, 1, V), no(B, 1, dtype=F32), 1)
