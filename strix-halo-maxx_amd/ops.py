@@ -1121,6 +1121,8 @@ class _PrefixCall:
         self.dev, self.N, self.P, self.T, self.B = q.device, N, P, k.shape[2], B
         self.out = (B, Tq, Hq * D)
         self.sizes = (N, B // N, H, Hq // H, Tq, D, P, self.T)
+        if max(self.sizes) > 0x7fffffff:
+            raise ValueError(f"q {tuple(q.shape)}, pk {tuple(pk.shape)}, k {tuple(k.shape)}: the sizes do not fit 32 bits")
         self.work = B * Tq > 0
         self.scale = D ** -0.5
         # what has to be copied before the kernel takes it: rows that are not of unit stride, 16-byte steps and 31-bit offsets
@@ -1193,7 +1195,8 @@ def sdpa_prefix_tiling(N, S, heads, G, Tq, P, T, hd):
     waves and runs of the tile kernel, rows per workgroup and runs of the few-row kernel)."""
     import ctypes
     t = (ctypes.c_int * 6)()
-    _lib.load().mx_sdpa_prefix_tiling(N, S, heads, G, Tq, P, T, hd, ctypes.cast(t, ctypes.c_void_p))
+    sizes = [_int32(v, "size") for v in (N, S, heads, G, Tq, P, T, hd)]
+    _lib.load().mx_sdpa_prefix_tiling(*sizes, ctypes.cast(t, ctypes.c_void_p))
     return tuple(t)
 
 

@@ -32,3 +32,13 @@ def test_select_sizes_past_31_bits():
     for B, V in ((1, FAR), (FAR, 10), (1, 2 ** 31)):
         with pytest.raises(ValueError, match="32 bits"):
             ops.beam_select(no(B, 1, V), no(B, 1, dtype=F32), 1)
+
+
+def test_prefix_sizes_past_31_bits():
+    for P, T, Tq, N in ((FAR, 3, 1, 1), (3, FAR, 1, 1), (3, 3, FAR, 1), (2 ** 31, 3, 1, 1), (3, 3, 1, FAR)):
+        q, pk, k = no(N, 1, Tq, 64), no(N, 1, P, 64), no(N, 1, T, 64)
+        with pytest.raises(ValueError, match="32 bits"):
+            ops.sdpa_prefix(q, pk, pk, k, k)
+    for i in range(7):
+        with pytest.raises(ValueError, match="32 bits"):
+            ops.sdpa_prefix_tiling(*(FAR if i == j else 1 for j in range(7)), 64)
