@@ -1335,6 +1335,8 @@ def rope_kv_at(qkv, cs, kc, vc, at, rot0=0):
     _need(at, "at", dev, torch.int32)
     if cs.dim() != 3 or cs.shape[1:] != (16, 2) or cs.shape[0] < 1 or not cs.is_contiguous():
         raise ValueError("cs must be a contiguous (positions, 16, 2) table")
+    if max(B, n, H, ctx, cs.shape[0]) > 0x7fffffff:
+        raise ValueError(f"qkv {tuple(qkv.shape)}, caches {tuple(kc.shape)}, {cs.shape[0]} positions: the sizes do not fit 32 bits")
     if at.shape != (B,) or not kc.is_contiguous() or not vc.is_contiguous() or qkv.shape[2] < 3 * H * 64:
         raise ValueError(f"at must be ({B},), the caches contiguous, qkv rows {3 * H * 64} wide")
     q = torch.empty(B, H, n, 64, device=dev, dtype=BF)

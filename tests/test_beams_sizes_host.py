@@ -42,3 +42,10 @@ def test_prefix_sizes_past_31_bits():
     for i in range(7):
         with pytest.raises(ValueError, match="32 bits"):
             ops.sdpa_prefix_tiling(*(FAR if i == j else 1 for j in range(7)), 64)
+
+
+def test_rope_sizes_past_31_bits():
+    for ctx, n, pos, B in ((FAR, 1, 9, 1), (5, FAR, 9, 1), (5, 1, FAR, 1), (5, 1, 9, FAR)):
+        kc = no(B, 1, ctx, 64)
+        with pytest.raises(ValueError, match="32 bits"):
+            ops.rope_kv_at(no(B, n, 192), no(pos, 16, 2, dtype=F32), kc, kc, no(B, dtype=I32))
