@@ -407,7 +407,8 @@ int mx_sdpa_prefix(hipStream_t st, const uint16_t* q, const uint16_t* pk, const 
  * neither does a logit of -infinity. x: bf16 or (fp32 != 0) float [B][W][V] by element strides sx_b, sx_w, unit stride along V;
  * score [B][W] float, done [B][W] bytes. Outputs [B][k]: o_score, o_parent (w), o_token (v), o_done (may be null: v == eos).
  * Places without a candidate: score -infinity, parent 0, token max(eos, 0), done 1. eos < 0: none (done must be null).
- * W <= 64, k <= 64, and the lists that a search's rows are cut into have to fit the merge's LDS (V up to 350000 for W = k = 64).
+ * W <= 64, k <= 64, B < 2^22, B W ceil(V / 8192) < 2^23 (4096 for k > 32), and the lists that a search's rows are cut into have to
+ * fit the merge's LDS (V up to 350000 for W = k = 64).
  * ws: mx_beam_select_ws bytes (0 for sizes that are refused), 8-byte aligned, one for each call that may run at the same time. */
 long mx_beam_select_ws(int B, int W, int V, int k);
 int mx_beam_select(hipStream_t st, const void* x, int fp32, long sx_b, long sx_w, const float* score, const uint8_t* done,

@@ -427,8 +427,9 @@ long merge_lds(int W, int segs, int k) {
 bool select_ok(int B, int W, int V, int k) {
   if (B < 1 || W < 1 || W > MAXW || V < 1 || V > 0x7fff0000 || k < 1 || k > MAXK || (long)B * W > 0x7fffffL) return false;
   const long rows = (long)B * W, segs = segments(V, k);
-  // (2048 bytes: what the merge has beside its lists)
-  return rows * segs <= 0x7fffffL && W * segs <= MAXL && merge_lds(W, (int)segs, k) <= 160 * 1024 - 2048;
+  // (2^32 threads in a grid: B workgroups of MT in the merge, one of 256 for each part. 2048 bytes: what the merge has beside its
+  // lists)
+  return (long)B * MT <= 0xffffffffL && rows * segs <= 0x7fffffL && W * segs <= MAXL && merge_lds(W, (int)segs, k) <= 160 * 1024 - 2048;
 }
 
 }  // namespace

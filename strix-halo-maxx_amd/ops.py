@@ -1239,8 +1239,8 @@ def beam_select(logits, scores, k=None, done=None, eos=None):
     A finished beam (done (B, W) bool) offers eos alone, at its score; the returned done says which hypotheses end in eos (None
     without eos). A beam whose score is not finite, or whose logits hold NaN or +infinity or nothing above -infinity, offers
     nothing, and neither does a logit of -infinity (a score of -infinity, say, keeps the copies of a first beam out). Places that
-    are left hold score -infinity, parent 0, token eos (0 without), done. W and k at most 64, V as far as a search's lists of
-    candidates fit the LDS (350000 for the largest W and k, millions for the usual ones)."""
+    are left hold score -infinity, parent 0, token eos (0 without), done. W and k at most 64, B below 2^22, V as far as a search's
+    lists of candidates fit the LDS (350000 for the largest W and k, millions for the usual ones)."""
     if eos is not None:
         eos = int(eos)
     key = (logits.shape, logits.stride(), logits.dtype, logits.device, scores.shape, scores.dtype, scores.device, k, eos,

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import strix_halo_maxx_amd.ops as ops
+from strix_halo_maxx_amd import _lib
 
 BF, F32, I32, U8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
 FAR = 2 ** 32 + 64  # 64 to whoever keeps the lower 32 bits
@@ -49,3 +50,13 @@ def test_rope_sizes_past_31_bits():
         kc = no(B, 1, ctx, 64)
         with pytest.raises(ValueError, match="32 bits"):
             ops.rope_kv_at(no(B, n, 192), no(pos, 16, 2, dtype=F32), kc, kc, no(B, dtype=I32))
+
+
+def test_select_searches_of_one_grid():
+    """The merge has 1024 threads for each search: 2^32 and more are no grid."""
+    ws = _lib.load().mx_beam_select_ws
+    assert ws(2 ** 22 - 1, 1, 10, 1) == (2 ** 22 - 1) * 16 and ws(2 ** 22, 1, 10, 1) == 0 and ws(5000000, 1, 10, 1) == 0
+    a = 0x10000  # never dereferenced: refused before any launch
+    assert _lib.load().mx_beam_select(None, a, 0, 10, 10, a, None, -1, 2 ** 22, 1, 10, 1, a, a, a, None, a, 2 ** 40) == -2
+    with pytest.raises(ValueError, match="too many"):
+        ops.beam_select(no(2 ** 22, 1, 10), no(2 ** 22, 1, dtype=F32), 1)
