@@ -1208,7 +1208,7 @@ def _select_call(logits, scores, k, done, eos):
     if logits.dim() != 3 or logits.dtype not in (BF, torch.float32):
         raise ValueError(f"logits must be (B, W, V) in bf16 or fp32, got {tuple(logits.shape)} {logits.dtype}")
     B, W, V = logits.shape
-    k = W if k is None else int(k)
+    k = W if k is None else k
     if not (1 <= W <= 64 and 1 <= k <= 64 and V >= 1):
         raise ValueError(f"{W} beams over {V} tokens, {k} to select: at most 64 of each, at least 1")
     if max(B, V) > 0x7fffffff:
@@ -1216,7 +1216,7 @@ def _select_call(logits, scores, k, done, eos):
     _need(scores, "scores", logits.device, torch.float32)
     if scores.shape != (B, W):
         raise ValueError(f"scores must be ({B}, {W}), got {tuple(scores.shape)}")
-    e = -1 if eos is None else int(eos)
+    e = -1 if eos is None else eos
     if eos is not None and not 0 <= e < V:
         raise ValueError(f"eos {e} outside the {V} tokens")
     if done is not None:
@@ -1241,8 +1241,8 @@ def beam_select(logits, scores, k=None, done=None, eos=None):
     nothing, and neither does a logit of -infinity (a score of -infinity, say, keeps the copies of a first beam out). Places that
     are left hold score -infinity, parent 0, token eos (0 without), done. W and k at most 64, B below 2^22, V as far as a search's
     lists of candidates fit the LDS (350000 for the largest W and k, millions for the usual ones)."""
-    if eos is not None:
-        eos = int(eos)
+    # (numbers, never a tensor that holds one: the geometry is kept by them)
+    k, eos = None if k is None else int(k), None if eos is None else int(eos)
     key = (logits.shape, logits.stride(), logits.dtype, logits.device, scores.shape, scores.dtype, scores.device, k, eos,
            None if done is None else (done.shape, done.dtype, done.device))
     c = _SELECT_CALLS.get(key)

@@ -60,3 +60,12 @@ def test_select_searches_of_one_grid():
     assert _lib.load().mx_beam_select(None, a, 0, 10, 10, a, None, -1, 2 ** 22, 1, 10, 1, a, a, a, None, a, 2 ** 40) == -2
     with pytest.raises(ValueError, match="too many"):
         ops.beam_select(no(2 ** 22, 1, 10), no(2 ** 22, 1, dtype=F32), 1)
+
+
+def test_select_count_in_a_tensor(monkeypatch):
+    """How many to select may be any number, also one that changes its value between calls."""
+    monkeypatch.setattr(ops, "_call_on", lambda *a: None)
+    x, s, k = torch.zeros(1, 3, 10), torch.zeros(1, 3), torch.tensor(2)
+    assert ops.beam_select(x, s, k)[0].shape == (1, 2)
+    k.fill_(3)
+    assert ops.beam_select(x, s, k)[0].shape == (1, 3)
