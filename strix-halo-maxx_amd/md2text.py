@@ -633,6 +633,7 @@ class TextDecoder:
         all nq * beams sequences in one step per token, over one copy of the image's K/V. eos: the token that ends an answer
         (the rest of it is eos too). Returns (tokens (nq, beams, n_tokens) int32, scores (nq, beams)): sums of log
         probabilities, best first, divided by (tokens up to eos) ** length_penalty for the order and the score."""
+        n_tokens, beams, eos = self._numbers(n_tokens, beams, eos)
         st = self._beam_state(self.nq, beams, n_tokens, self.L, self.prefix, eos)
         h = self._question_rows()
         P, n = self.prefix, min(self.L, st.T)
@@ -649,6 +650,7 @@ class TextDecoder:
     def generate_beams(self, img_emb, prompt_ids, n_tokens, beams=4, eos=None, length_penalty=0.0, use_graph=True):
         """Prefill + beam search: n_tokens by `beams` hypotheses behind one copy of the image's and the prompt's K/V. Returns
         (tokens (beams, n_tokens) int32, scores (beams,)) as answer() does."""
+        n_tokens, beams, eos = self._numbers(n_tokens, beams, eos)
         P = 1 + img_emb.shape[0] + prompt_ids.shape[0]
         st = self._beam_state(1, beams, n_tokens, 0, P, eos)
         self.prefill(img_emb, prompt_ids)
@@ -657,6 +659,11 @@ class TextDecoder:
         st.rows.zero_()
         tokens, scores = self._beam_search(st, self.logits[None], n_tokens, eos, length_penalty, use_graph)
         return tokens[0], scores[0]
+
+    @staticmethod
+    def _numbers(n_tokens, beams, eos):
+        """As ints: a search's buffers and its step's graph are kept by them, and a tensor can change its value."""
+        return int(n_tokens), int(beams), None if eos is None else int(eos)
 
     def _beam_state(self, groups, beams, n_tokens, rows, prefix, eos):
         """Buffers for `groups` searches whose sequences hold `rows` rows of their own behind `prefix` shared ones at first; kept
