@@ -1125,9 +1125,10 @@ class _PrefixCall:
             raise ValueError(f"q {tuple(q.shape)}, pk {tuple(pk.shape)}, k {tuple(k.shape)}: the sizes do not fit 32 bits")
         self.work = B * Tq > 0
         self.scale = D ** -0.5
-        # what has to be copied before the kernel takes it: rows that are not of unit stride, 16-byte steps and 31-bit offsets
+        # which have to be copied before the kernel takes them: rows that are not of unit stride, 16-byte steps and 31-bit offsets
         steps = [_steps(t) for t in (q, pk, pv, k, v)]
-        self.copy = any(s[3] != 1 or (s[0] | s[1] | s[2]) % 8 for s in steps) or any(not 0 <= s[2] < 0x800000 for s in steps[1:])
+        self.odd = [s[3] != 1 or (s[0] | s[1] | s[2]) % 8 != 0 or (i > 0 and not 0 <= s[2] < 0x800000) for i, s in enumerate(steps)]
+        self.copy = any(self.odd)
         self.need = 0
         if self.work:
             import ctypes
@@ -1181,7 +1182,8 @@ def sdpa_prefix(q, pk, pv, k, v, kv_len=None, prefix_len=None, out=None, scale=N
         return sdpa_prefix(q, pk, pv, k, v, kv_len, prefix_len, out, scale, causal)
     qp, pkp, pvp, kp, vp = q.data_ptr(), pk.data_ptr(), pv.data_ptr(), k.data_ptr(), v.data_ptr()
     if c.copy or (qp | pkp | pvp | kp | vp) & 15:
-        q, pk, pv, k, v = (t.clone(memory_format=torch.contiguous_format) for t in (q, pk, pv, k, v))
+        q, pk, pv, k, v = (t.clone(memory_format=torch.contiguous_format) if odd or t.data_ptr() & 15 else t
+                           for t, odd in zip((q, pk, pv, k, v), c.odd))
         return sdpa_prefix(q, pk, pv, k, v, kv_len, prefix_len, out, scale, causal)
     need = c.need
     part = torch.empty(need, device=dev, dtype=torch.float32) if need else None

@@ -69,3 +69,21 @@ def test_select_count_in_a_tensor(monkeypatch):
     assert ops.beam_select(x, s, k)[0].shape == (1, 2)
     k.fill_(3)
     assert ops.beam_select(x, s, k)[0].shape == (1, 3)
+
+
+def test_prefix_copies_what_it_has_to(monkeypatch):
+    """Where one tensor has strides or an address that the kernel does not take, that one is copied: not a prefix of gigabytes for
+    a query at an odd address."""
+    seen = []
+    monkeypatch.setattr(ops, "_call_on", lambda dev, name, *a: seen.append(a[:5]))
+    x = [torch.zeros(4, 2, 3, 64, dtype=BF)] + [torch.zeros(2, 2, 10, 64, dtype=BF) for _ in range(2)] + \
+        [torch.zeros(4, 2, 5, 64, dtype=BF) for _ in range(2)]
+    shift = lambda t: torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape)
+    wide = lambda t: torch.cat([t, t.new_zeros(*t.shape[:3], 3)], 3)[..., :t.shape[3]]
+    cols = lambda t: t.transpose(2, 3).contiguous().transpose(2, 3)
+    for f in (shift, wide, cols):
+        for i in range(5):
+            y = [f(t) if i == j else t for j, t in enumerate(x)]
+            ops.sdpa_prefix(*y)
+            assert [p != t.data_ptr() for p, t in zip(seen[-1], y)] == [i == j for j in range(5)], (f, i)
+            assert seen[-1][i] % 16 == 0
