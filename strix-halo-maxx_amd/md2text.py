@@ -29,6 +29,7 @@ from ._lib import call, ptr, stream
 from .synth import TXT, freqs_cis
 
 BF = torch.bfloat16
+BEAM_BYTES = 16 << 30  # of K/V that a decoder keeps of earlier beam searches, the one at work included (always at least that one)
 BOS = 50256  # moondream2's tokenizer bos_id (the Phi / GPT-2 <|endoftext|> id)
 
 
@@ -667,7 +668,8 @@ class TextDecoder:
 
     def _beam_state(self, groups, beams, n_tokens, rows, prefix, eos):
         """Buffers for `groups` searches whose sequences hold `rows` rows of their own behind `prefix` shared ones at first; kept
-        for the next search of the same sizes (a step's graph reads them)."""
+        for the next search of the same sizes (a step's graph reads them), until four others or BEAM_BYTES of them have been
+        used since."""
         if prefix is None:
             raise RuntimeError("encode() the image prefix first")
         if not 1 <= beams <= 64 or n_tokens < 1:
@@ -678,13 +680,16 @@ class TextDecoder:
         if prefix + T > self.cs.shape[0]:
             raise ValueError(f"{prefix} + {T} positions exceed the rotary table ({self.cs.shape[0]})")
         key = (groups, beams, T, prefix)
-        st = self.beam_states.get(key)
+        st = self.beam_states.pop(key, None)
         if st is None:
-            if len(self.beam_states) >= 4:
-                self.beam_states.clear()
-            st = self.beam_states[key] = _BeamState(self, groups, beams, T, prefix, n_tokens)
+            need = _BeamState.kv_bytes(self, groups * beams, T, prefix)
+            while self.beam_states and (len(self.beam_states) >= 4 or
+                                        need + sum(s.kept for s in self.beam_states.values()) > BEAM_BYTES):
+                del self.beam_states[next(iter(self.beam_states))]
+            st = _BeamState(self, groups, beams, T, prefix, n_tokens)
         elif st.hist.shape[1] < n_tokens:
             st.hist, st.graph = st.history(n_tokens), None
+        self.beam_states[key] = st  # the last used is the last to go
         return st
 
     def _fork_kv8(self, st, slots, rows):
@@ -778,6 +783,7 @@ class _BeamState:
 
     def __init__(self, dec, B, W, T, prefix, n_tokens):
         self.B, self.W, self.T, self.prefix, self.dev = B, W, T, prefix, dec.dev
+        self.kept = self.kv_bytes(dec, B * W, T, prefix)
         z = lambda *s, dtype=torch.int32: torch.zeros(*s, device=dec.dev, dtype=dtype)
         n, H, hd = len(dec.blocks), dec.H, dec.hd
         if dec.kv8:
@@ -788,6 +794,12 @@ class _BeamState:
         self.scores, self.done, self.step = z(B, W, dtype=torch.float32), z(B, W, dtype=torch.bool), z(1, dtype=torch.int64)
         self.hist = self.history(n_tokens)
         self.graph = None
+
+    @staticmethod
+    def kv_bytes(dec, slots, T, prefix):
+        """Of the K/V rows, which are nearly all of it: T of its own per sequence, or an 8-bit cache with the prefix too."""
+        rows = -(-(prefix + T) // ops.KV8Cache.BLOCK) * ops.KV8Cache.BLOCK if dec.kv8 else 2 * T
+        return 2 * len(dec.blocks) * slots * dec.H * rows * dec.hd
 
     def history(self, n_tokens):
         return torch.zeros(2, n_tokens, self.B, self.W, device=self.dev, dtype=torch.int32)

@@ -24,3 +24,34 @@ def test_searches_by_numbers():
     (a, *x), (b, *y) = seen
     assert x == [6, 7] and y == [9, 8] and all(type(v) is int for v in x + y)
     assert a.W == 2 and b.W == 3 and b.hist.shape[1] >= 9 and b.T == 8
+
+
+def test_the_search_in_use_stays():
+    """Searches of ever new lengths between do not take the buffers and the graph of the one that comes again."""
+    dec = decoder()
+    first = dec._beam_state(1, 4, 9, 0, 30, None)
+    for prefix in range(40, 60):
+        other = dec._beam_state(1, 4, 9, 0, prefix, None)
+        assert dec._beam_state(1, 4, 9, 0, prefix, None) is other
+        assert dec._beam_state(1, 4, 9, 0, 30, None) is first
+        assert len(dec.beam_states) <= 4
+    for prefix in range(40, 44):
+        dec._beam_state(1, 4, 9, 0, prefix, None)
+    assert dec._beam_state(1, 4, 9, 0, 30, None) is not first
+
+
+def test_bytes_of_kept_searches(monkeypatch):
+    """The buffers of earlier searches go where they would hold more than BEAM_BYTES with the new one's."""
+    for kv8 in (False, True):
+        dec = decoder(kv8=kv8)
+        a = dec._beam_state(1, 4, 9, 0, 100, None)
+        held = [a.own] if not kv8 else [t for c in a.kv for t in (c.kc, c.vc)]
+        size = sum(t.numel() * t.element_size() for t in held)
+        assert a.kept == size
+        monkeypatch.setattr(mt, "BEAM_BYTES", 2 * size)
+        b = dec._beam_state(1, 4, 9, 0, 101, None)
+        assert list(dec.beam_states.values()) == [a, b]
+        dec._beam_state(1, 4, 9, 0, 102, None)
+        assert list(dec.beam_states.values())[0] is b and len(dec.beam_states) == 2
+        big = dec._beam_state(1, 64, 9, 0, 102, None)  # more than the bound for itself
+        assert list(dec.beam_states.values()) == [big]
