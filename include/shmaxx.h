@@ -391,7 +391,9 @@ int mx_decode_mk_layer_bytes(void);
  * [N][H][P][D], k / v [N S][H][T][D] by element strides, strides[15] = {b, h, t} of q, pk, pv, k, v in turn (host memory;
  * multiples of 8, unit stride along D, 16-byte aligned; row strides of keys and values 0 .. 2^23 - 1), o [N S][Tq][H G D]
  * (strides multiples of 4, 8-byte aligned). plen / len: device int32 with strides plen_s / len_s, added to pbase / base, or null;
- * what lies outside 0 .. P / 0 .. T is clamped. P = 0 or T = 0: pk, pv or k, v are not read. fp32 sums, weights rounded to bf16; scores (times scale) must stay below 2^29 in size. part: at least
+ * what lies outside 0 .. P / 0 .. T is clamped. P = 0 or T = 0: pk, pv or k, v are not read. fp32 sums,
+ * weights rounded to bf16; scores (times scale) must stay below 2^29 in size. Infinities and NaN of keys that a row does not see reach
+ * nothing; an infinite value of a key that it sees, whose weight underflows to 0, gives infinity or NaN. part: at least
  * mx_sdpa_prefix_ws floats, 16-byte aligned, one for each call that may run at the same time; not read from call to call.
  * N S H < 2^23, N S H G Tq < 2^24. mx_sdpa_prefix_tiling: t[6] = 0 rows, 1 both, 2 tiles; query and key waves and runs of the
  * tile kernel; rows per workgroup and runs of the few-row kernel. */

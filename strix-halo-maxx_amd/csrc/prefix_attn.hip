@@ -17,7 +17,9 @@
 // Numerics: fp32 scores, sums and outputs; a weight is rounded to bf16 for its product (2^-9 of it on average), its sum takes it
 // before that. A masked key reaches no result: blocks that need a mask are searched for infinities and NaN among the values, and
 // where there is one (never in ordinary data) it is cleared and two products of indicators with the visibility find the outputs
-// that it belongs to.
+// that it belongs to. An infinite value of a key that is seen, but whose weight underflows to 0 in fp32, leaves infinity or NaN in its
+// column of that row, by which block, wave and run it lies in: 0 times it in a product or a joining factor is NaN, an indicator's
+// output infinity.
 #include "common.h"
 
 namespace {

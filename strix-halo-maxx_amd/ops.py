@@ -1147,7 +1147,9 @@ def sdpa_prefix(q, pk, pv, k, v, kv_len=None, prefix_len=None, out=None, scale=N
     Query i sees keys 0 .. prefix_len_n - 1 of its prefix and, of its own first kv_len_b keys, those up to its own: the queries
     are the sequence's last Tq tokens, key t is visible iff t <= kv_len_b - Tq + i (causal=False: all kv_len_b). A row that sees
     no key is 0. kv_len, prefix_len: an int, or an int32 tensor (B,) / (N,) read on the device (clamped to 0 .. T / 0 .. P);
-    None: all. out may lie in q's memory. Scores (times scale) have to stay below 2^29 in size."""
+    None: all. out may lie in q's memory. Scores (times scale) have to stay below 2^29 in size. Keys that a row does not see may
+    hold infinities and NaN; an infinite value of one that it sees gives the formula's infinity or NaN, and either of them where
+    its weight underflows to 0."""
     key = (q.shape, q.stride(), pk.shape, pk.stride(), pv.shape, pv.stride(), k.shape, k.stride(), v.shape, v.stride(), q.device)
     c = _PREFIX_CALLS.get(key)
     if c is None or not (q.dtype is BF and pk.dtype is BF and pv.dtype is BF and k.dtype is BF and v.dtype is BF and
