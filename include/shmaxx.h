@@ -419,7 +419,8 @@ int mx_beam_select(hipStream_t st, const void* x, int fp32, long sx_b, long sx_w
 /* Slots of a cache, in place: x[n, g W + w, h, t] = x[n, g W + parent[g, w], h, t] for first <= t < ceil(rows / unit), with
  * rows = base + len[parent's slot] (len may be null), at most T; other rows stay. parent [G][W] (strides sp_g, sp_w): a value
  * outside 0 .. W - 1 leaves its slot. Strides and row_bytes in bytes; the rows of different (n, slot, h, t) must not overlap.
- * W <= 64. */
+ * W <= 64. Rows move in pieces of 16 bytes, of 4 where x, a stride or row_bytes is no multiple of 16, or of 1:
+ * N G H ceil((T - first) row_bytes / piece / 256) < 2^23. */
 int mx_reorder_slots(hipStream_t st, void* x, long s_n, long s_s, long s_h, long s_t, int N, int G, int W, int H, int T,
                      int row_bytes, const int* parent, long sp_g, long sp_w, const int* len, long len_s, int base, int unit,
                      int first);

@@ -70,7 +70,7 @@ __device__ __forceinline__ void load8(const T* row, int v0, int V, float (&f)[8]
 // so no smaller one is among the k largest, and the larger ones lie in fewer than k lanes. What passes the largest of the four
 // waves' thresholds, and the first k of a wave that equal it, go to LDS, where every one counts the larger ones: its rank.
 // Bound by the vector ALU's work per logit (maximum, subtraction, scaling, exponential, sum, comparison) and, in fp32, nearly by
-// memory: 16 x 16 rows of 131071 fp32 logits 26.9 us = 5.0 TB/s; 32 x 8 of 51200 bf16 11.8.
+// memory: 16 x 16 rows of 131071 fp32 logits 27.6 us = 4.9 TB/s; 32 x 8 of 51200 bf16 11.
 template <class T, int E>
 __global__ __launch_bounds__(256) void beam_parts_kernel(SelArgs p) {
   extern __shared__ uint64_t cand[];  // 4 ((k - 1) E + k)
@@ -193,7 +193,7 @@ typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
 // A list is a part's keys; a finished beam's is its one continuation. The k-th largest head of the lists bounds what can be
 // selected, and a key at place i of a list whose head has rank r has i + r larger ones: few keys are left to be ranked. What
 // takes the time is three rounds to memory, one after the other: the sums, the heads, the keys behind them (32 searches of 8 beams
-// of 7 parts 6.2 us, 16 of 16 of 16 9.2).
+// of 7 parts 6.2 us, 16 of 16 of 16 9.7).
 __global__ __launch_bounds__(MT) void beam_merge_kernel(SelArgs p) {
   extern __shared__ u64x2 sh[];  // (value, key), key = ~logit's bits << 32 | token: the lists' heads [nl], then candidates
   __shared__ double base[MAXW];  // score - log of the sum
@@ -370,8 +370,9 @@ struct MoveArgs {
 // x[n, g W + w, h, t] = x[n, g W + parent[g, w], h, t] for first <= t < rows of the parent. A thread owns one piece (16, 4 or 1
 // bytes) of a row in every slot of a group, loads what moves and then stores it, so the copy is in place in any order and no
 // two threads meet. Bound by the bytes: slots that do not change are not touched. What a beam step of
-// the text decoder moves (48 K and V of 4 slots x 32 heads x 40 rows x 128 bytes) takes 10 us, 16 of 64 slots x 8 heads x 1 - 500
-// rows x 256 bytes 137.
+// the text decoder moves (48 K and V of 4 slots x 32 heads x 40 rows x 128 bytes) takes 8.4 us among others, 10.7 waited for; 16 of 64
+// slots x 8 heads x 1 - 500 rows x 256 bytes 143. The 8-bit cache's four buffers of each layer are a call each, bound by the
+// launches: 96 of them for 24 layers of 4 slots take 264 us in a graph, for some 50 MB.
 template <class U, int WM>
 __global__ __launch_bounds__(256) void move_kernel(MoveArgs p) {
   __shared__ long from[WM];  // byte offset of slot w's parent; the rows that it takes from it
@@ -481,7 +482,7 @@ extern "C" int mx_reorder_slots(hipStream_t st, void* x, long s_n, long s_s, lon
   const int size = bits & 3 ? 1 : bits & 15 ? 4 : 16;
   const int cpr = row_bytes / size;
   const double blocks = ((double)(T - first) * cpr + 255) / 256 * N * G * H;
-  if (blocks > 0x7fffff) return MX_ESHAPE;  // 2^32 threads in a grid
+  if (blocks > 0x7fffff) return MX_ESHAPE;  // 2^31 threads; a grid has less than 2^32
   const unsigned nblk = (unsigned)(((long)(T - first) * cpr + 255) / 256);
   const MoveArgs a{(uint8_t*)x, s_n, s_s, s_h, s_t, parent, sp_g, sp_w, len, len_s, base, unit, first, T, G, W, H, cpr, nblk};
   const unsigned grid = nblk * (unsigned)(N * G * H);

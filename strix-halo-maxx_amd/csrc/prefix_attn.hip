@@ -5,11 +5,12 @@
 // A row is a (sequence, query, head of the group) of one key head h: row = (j Tq + i) G + g of the S Tq G that share K and V.
 //
 // Three ways to cut it (plan()):
-//  * rows: 16 rows per workgroup, from any sequences; its waves go through one list of blocks of keys: the prefix's, then
-//    those of each sequence in the tile, which the rows of the others do not see. Few rows: everything is read once.
-//  * both: tiles of 32 - 128 rows over the prefix, which is so read once for all of them, and in the same launch 16-row
+//  * rows: 16 or 32 rows per workgroup, from any sequences; its waves go through one list of blocks of keys: the prefix's,
+//    then those of each sequence in the tile, which the rows of the others do not see. Few rows: a workgroup reads all keys
+//    of its rows once.
+//  * both: tiles of 64 or 128 rows over the prefix, which is so read once for each, and in the same launch 16-row
 //    tiles over the sequences' own keys. Many sequences of few rows each.
-//  * tiles: tiles of 32 - 128 rows of one sequence through the prefix and then its own keys. Prompts.
+//  * tiles: tiles of 32 - 256 rows of one sequence through the prefix and then its own keys. Prompts.
 // Each may cut its list of blocks into runs ("splits"): a run's share (maximum, sum, unnormalised output in fp32) goes to
 // memory and the join adds the shares of a row in a fixed order. The host knows capacities only (lengths may be on the
 // device), so it fixes the number of runs and the device cuts each list evenly.
@@ -161,10 +162,11 @@ constexpr int rows_lds() {
 // for the transposed read; the next block is in flight through this one's softmax and product. S^T leaves keys
 // 16 t + 4 (lane / 16) + r of row lane % 16 in a lane, and the product with V takes its keys in that order.
 // Bound by bytes: where the keys of a head are one workgroup's, by what one CU gets from beyond its L2, about 30 bytes per ns (1 x
-// 4 x 32 x 1, 64, 1, 794 + 64 as in plan(): 268 KB a workgroup in 10.3 us); where runs fill the chip, by memory (6 x 8 x 8 x 4,
+// 4 x 32 x 1, 64, 1, 794 + 64 as in plan(): 268 KB a workgroup in 10.4 us); where runs fill the chip, by memory (6 x 8 x 8 x 4,
 // 128, 1, 16000 + 200: 432 MB, some of them still in the 256 MB cache, in 60 us); where lengths on the device differ widely, by the
-// longest lists (the same with prefixes of 1 - 16000 keys: 55 us). 8 or 16 waves per workgroup brought nothing, nor did dealing the
-// runs out by the lengths on the device (3 - 8 us more for lists that are alike, 4 less for the most unlike).
+// longest lists, whose runs on_xcd keeps on one or two XCDs (the same with prefixes of 1 - 16000 keys: 52 us). 8 or 16 waves per
+// workgroup brought nothing, nor did dealing the runs out by the lengths on the device (3 - 8 us more for lists that are alike, 4 less
+// for the most unlike).
 template <int D, int NW, int RT, bool PREFIX>
 __device__ __forceinline__ void rows_body(const Args& p, uint32_t item, uint8_t* smem) {
   constexpr int KB = 4096 / D, KT = KB / 16, NS = D / 32, NT = D / 16, NV = 8, CPR = D / 8, RW = 16 * RT;
@@ -453,11 +455,11 @@ struct Tile {
 // NQW query waves x NKW key waves; blocks of KB keys go through an LDS ring of S stages by the asynchronous load, the
 // block's keys shared among the key waves, whose shares are added at the end. S^T = K Q^T leaves a lane the scores of one
 // row, in the key order that the product with V (transposed reads) takes.
-// Prompts are bound by a SIMD's two waves issuing softmax and products by turns: 2 x 2 x 8 x 4, 128, 1024, 8001 + 1500 takes 553 us
-// = 0.88 PFLOP/s (a large library product 1.13), the matrix unit busy 37 % of the time, the vector ALU 40 %, no bank conflicts.
+// Prompts are bound by a SIMD's two waves issuing softmax and products by turns: 2 x 2 x 8 x 4, 128, 1024, 8001 + 1500 takes 560 us
+// = 0.87 PFLOP/s (a large library product 1.13), the matrix unit busy 39 % of the time, the vector ALU 36 %, no bank conflicts.
 // Tried and slower: the next block's scores before this one's softmax in one wave (588 - 620 us: registers), waves in two groups
 // that swap softmax and products at barriers (1217 us and more), rings of 3 and 4 stages (the same). Over a long prefix with few
-// rows it is bound by memory: 1 x 16 x 8 x 4, 128, 1, 131071 + 512 reads 540 MB in 102 us, 5.3 TB/s.
+// rows it is bound by memory: 1 x 16 x 8 x 4, 128, 1, 131071 + 512 reads 557 MB in 104 us, 5.4 TB/s.
 template <int D, int NQW, int NKW, int KB, int S, bool SEQ>
 __device__ __forceinline__ void tile_body(const Args& p, uint32_t item, uint8_t* smem) {
   using C = Tile<D, NQW, NKW, KB, S>;
@@ -713,7 +715,8 @@ __global__ __launch_bounds__(64 * NQW * NKW, 2) void prefix_both_kernel(Args p) 
 
 // The shares of one row: 256 / WPR threads... one workgroup has 4 / WPR rows of WPR waves; D / 4 threads with 4 columns each
 // form a group, and the groups take the shares in turn, in a fixed order. Bound by the latency of two trips to memory (pairs, then
-// outputs, of which the first four are asked for at once): 4.9 us for 192 rows of 48 runs, 8.7 for 1024 of 10.
+// outputs, of which the first four are asked for at once): four waves a row 4.9 us for 512 rows of 36 runs, one wave 5.9 for 2048
+// of 17.
 template <int D, int WPR>
 __global__ __launch_bounds__(256) void prefix_join_kernel(Args p, uint32_t rows) {
   constexpr int TD = D / 4, NT = 64 * WPR, NG = NT / TD, RPB = 256 / NT;
@@ -802,8 +805,8 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(Args p, uint32_t rows)
 // replays; prefixes x sequences x key heads x group, head dim, queries, prefix + own keys):
 //  * M < 32 and R <= 32 or R P < 2^20: rows. Up to 24 blocks of keys (1536 keys of 64 values, 768 of 128) in one run: one launch
 //    and no workspace (1 x 4 x 32 x 1, 64, 1, 794 + 64 10.8 in a graph and, bound by the host, 11.5 called eagerly; 8 runs and the
-//    join 9.2 and 15.5). More of them in 256 workgroups where runs of 128 keys give that many (1 x 8 x 8 x 4, 128, 1, 2000 + 200
-//    12.3, in 128 workgroups 13.4). 32 rows per workgroup instead of 16 where the keys would be read again too often, from R P =
+//    join 9.2 and 15.5: a captured step, as the text decoder's, pays 1.6 a layer for it). More of them in 256 workgroups where
+//    runs of 128 keys give that many (1 x 8 x 8 x 4, 128, 1, 2000 + 200 12.3, in 128 workgroups 13.4). 32 rows per workgroup instead of 16 where the keys would be read again too often, from R P =
 //    400000 on (6 x 8 x 8 x 4, 128, 1, 16000 + 200 60, 16 rows 88; 1 x 8 x 8 x 4, 128, 1, 2000 + 200 14.0, 16 rows 12.6);
 //  * more rows of M < 32: both. Up to 64 rows 2 x 4 waves (1 x 16 x 8 x 4, 128, 1, 131071 + 512 109, 4 x 1 112), else 4 x 1 (1 x
 //    64 x 8 x 4, 128, 1, 65536 + 200 99, 2 x 2 111; rows of 32 175). Below, rows (5 x 48 x 4 x 7, 128, 1, 2000 + 500 53, both 60;

@@ -22,7 +22,8 @@ __device__ __forceinline__ void rot_pair(float a, float b, float c, float s, flo
 // (a = x[j] from input chunk u, b = x[16 + j] from chunk u + 2), units 2 and 3 pass dims 32 .. 63 through. Every load
 // of a thread is issued before its arithmetic, so a row is one memory round trip.
 // AT: the cache rows of sequence b start at pos0 + at[b * at_s], read here, and the row's position is rot0 more than that; rows
-// outside the cache or the table write nothing to it.
+// outside the cache or the table write nothing to it. One row of 4 to 64 sequences x 32 heads: 2.9 - 3.1 us in a graph (a launch and a
+// chain of three loads: place, table, row); 64 x 32 rows 9.8, 50 MB.
 template <bool AT>
 __global__ __launch_bounds__(128) void rope_kv_kernel(const uint16_t* __restrict__ qkv, long ldq,
                                                       const float* __restrict__ cs, uint16_t* __restrict__ q_out,

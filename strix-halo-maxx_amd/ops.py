@@ -1020,8 +1020,8 @@ class KV8Cache:
         return q_out
 
     def reorder(self, parent, n=None, first=0):
-        """Slot g W + w becomes a copy of slot g W + parent[g, w] (reorder_slots), over the blocks of 64 tokens that tokens first ..
-        n - 1 lie in."""
+        """Slot g W + w becomes a copy of slot g W + parent[g, w] (reorder_slots, unit 64), over blocks first // 64 .. ceil(n / 64)
+        - 1: tokens before `first` in its block go along. Four launches."""
         for t in (self.kc, self.vc, self.ks, self.vs):
             reorder_slots(t[None], parent, n, first, self.BLOCK)
 
@@ -1142,12 +1142,17 @@ _PREFIX_CALLS = {}
 def sdpa_prefix(q, pk, pv, k, v, kv_len=None, prefix_len=None, out=None, scale=None, causal=True):
     """Attention of sequences that share prefixes: q (B, Hq, Tq, D), prefixes pk, pv (N, H, P, D), own keys k, v (B, H, T, D); D 64
     or 128, Hq a multiple of H (query head h reads key head h / (Hq / H)), B of N: sequence b has prefix b // (B / N), which is
-    stored and read once for all of them. Returns out (B, Tq, Hq * D).
+    stored once for all of them. Returns out (B, Tq, Hq * D).
+
+    How often keys are read: a workgroup reads those of its rows, so the prefix goes through the caches once for every 16 to 128
+    rows (sequence, query, head of a group) where a sequence has fewer than 32 rows per key head, of any sequences of the prefix,
+    and once for every 32 to 256 rows of one sequence else (sdpa_prefix_tiling).
 
     Query i sees keys 0 .. prefix_len_n - 1 of its prefix and, of its own first kv_len_b keys, those up to its own: the queries
     are the sequence's last Tq tokens, key t is visible iff t <= kv_len_b - Tq + i (causal=False: all kv_len_b). A row that sees
     no key is 0. kv_len, prefix_len: an int, or an int32 tensor (B,) / (N,) read on the device (clamped to 0 .. T / 0 .. P);
-    None: all. out may lie in q's memory. Scores (times scale) have to stay below 2^29 in size. Keys that a row does not see may
+    None: all. out may lie in q's memory, not in the keys' or values'. Scores (times scale) have to stay below 2^29 in size, N S H
+    below 2^23 and N S H G Tq below 2^24 (S sequences of a prefix, G query heads of a key head). Keys that a row does not see may
     hold infinities and NaN; an infinite value of one that it sees gives the formula's infinity or NaN, and either of them where
     its weight underflows to 0."""
     key = (q.shape, q.stride(), pk.shape, pk.stride(), pv.shape, pv.stride(), k.shape, k.stride(), v.shape, v.stride(), q.device)
@@ -1291,8 +1296,9 @@ def reorder_slots(x, parent, n=None, first=0, unit=1):
     (G, W) int32, G W = slots (or (slots,)): slot g W + w becomes a copy of slot g W + parent[g, w], which may be any of its group,
     several times the same; values outside 0 .. W - 1 leave their slot. Only rows first .. n - 1 move, n an int or an int32 tensor
     (slots,) of the rows that each slot holds (a slot takes as many as its parent has; None: all T); every other row stays. unit:
-    tokens per row (first and n count tokens; the row that token `first` lies in moves). W at most 64; T, n and the bytes of a row
-    below 2^31. Returns x."""
+    tokens per row; first and n then count tokens, and rows first // unit .. ceil(n / unit) - 1 move. W at most 64; T, n and the
+    bytes of a row below 2^31. Rows move in pieces of 16 bytes, of 4 where an address or a stride is no multiple of 16, or of
+    1; a call takes L G H ceil(pieces of a slot's rows / 256) below 2^23. Returns x."""
     if x.dim() < 4:
         raise ValueError(f"x must be (L, slots, H, T, ...), got {tuple(x.shape)}")
     N, S, H, T = x.shape[:4]
