@@ -405,7 +405,8 @@ int mx_sdpa_prefix(hipStream_t st, const uint16_t* q, const uint16_t* pk, const 
                    float scale, float* part, long part_elems);
 /* Beam search's selection: of the values score[b, w] + x[b, w, v] - logsumexp(x[b, w, :]) of search b, the k largest in falling
  * order (equal ones: lowest w, then lowest v). A finished beam (done[b, w] != 0; done may be null) offers eos alone, at its
- * score. A beam whose score is not finite, or whose logits hold NaN or +infinity or nothing above -infinity, offers nothing;
+ * score. Within a beam the order is exact; two beams' values that lie nearer than 2^-17 (the sums are fp32 within 8192 logits) may
+ * come in either order. A beam whose score is not finite, or whose logits hold NaN or +infinity or nothing above -infinity, offers nothing;
  * neither does a logit of -infinity. x: bf16 or (fp32 != 0) float [B][W][V] by element strides sx_b, sx_w, unit stride along V;
  * score [B][W] float, done [B][W] bytes. Outputs [B][k]: o_score, o_parent (w), o_token (v), o_done (may be null: v == eos).
  * Places without a candidate: score -infinity, parent 0, token max(eos, 0), done 1. eos < 0: none (done must be null).

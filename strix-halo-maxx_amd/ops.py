@@ -1243,7 +1243,9 @@ def _select_call(logits, scores, k, done, eos):
 def beam_select(logits, scores, k=None, done=None, eos=None):
     """Beam search's selection: logits (B, W, V) bf16 or fp32 of W beams with scores (B, W) fp32. Returns (score, parent, token,
     done), each (B, k) (k: default W): the k largest of scores[b, w] + log_softmax(logits[b, w])[v] in falling order, equal ones
-    by the lowest beam, then the lowest token; parent = w, token = v (int32).
+    by the lowest beam, then the lowest token; parent = w, token = v (int32). Within a beam the order is exact; between beams it is
+    that of the computed values, whose sums of exponentials are fp32 within 8192 logits: two that lie nearer than 2^-17 may come
+    in either order.
 
     A finished beam (done (B, W) bool) offers eos alone, at its score; the returned done says which hypotheses end in eos (None
     without eos). A beam whose score is not finite, or whose logits hold NaN or +infinity or nothing above -infinity, offers
